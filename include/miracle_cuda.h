@@ -48,7 +48,7 @@ enum mr_status {
     MR_ERR_NOMEM = 5      /* device allocation failed */
 };
 
-enum mr_dtype { MR_DTYPE_F32 = 0, MR_DTYPE_F16 = 1, MR_DTYPE_BF16 = 2 };
+enum mr_dtype { MR_DTYPE_F32 = 0, MR_DTYPE_F16 = 1, MR_DTYPE_BF16 = 2, MR_DTYPE_I32 = 3 };
 
 /* config.py:9-10 FAMILIES, in order */
 enum mr_family {
@@ -85,6 +85,11 @@ MR_API int mr_device_query(int ordinal, mr_device_info *info);
 
 /* ---- context: one device + one stream (OpenCLBackend.__init__, opencl.py:136-166) */
 MR_API int mr_context_create(int device_ordinal, mr_context **out);
+/* The same on a stream that the caller owns (a cudaStream_t; NULL: the legacy
+ * default stream): every call of the context is queued there, in order with
+ * the caller's own work.  The stream has to outlive the context and all that
+ * is made on it.  No reference counterpart. */
+MR_API int mr_context_create_on_stream(int device_ordinal, void *stream, mr_context **out);
 /* Releases the caller's reference.  Buffers and models made on the context
  * hold their own references, so handles may be released in any order; the
  * stream is destroyed with the last one. */
@@ -98,6 +103,8 @@ MR_API int mr_context_finish(mr_context *ctx);
 MR_API int mr_buffer_alloc(mr_context *ctx, size_t count, mr_buffer **out);          /* empty()  */
 MR_API int mr_buffer_free(mr_buffer *buf);                                           /* Tensor.__del__ */
 MR_API int mr_buffer_count(const mr_buffer *buf, size_t *count);
+/* The buffer's device address, for the entry points that take mr_array. */
+MR_API int mr_buffer_pointer(const mr_buffer *buf, void **pointer);
 MR_API int mr_buffer_upload(mr_buffer *buf, size_t offset, const float *host, size_t count);   /* upload() */
 MR_API int mr_buffer_download(const mr_buffer *buf, size_t offset, float *host, size_t count); /* read() */
 /* copy() (opencl.py:209-217): bounds-checked; count 0 is a no-op. */
@@ -356,6 +363,83 @@ MR_API int mr_attention_static_scratch(mr_context *ctx, const float *q, const fl
                                        const float *extra_keys, const float *extra_values, float *out, int heads,
                                        int kv_heads, int dim, int capacity, int start, int length,
                                        int extra_length);
+
+/* ---- paged key / value cache and its attention -----------------------------
+ * For serving several sequences from one pool of pages.  No counterpart in the
+ * reference (one sequence, one ring per layer: model.py:104-160); head grouping,
+ * window and scale follow its attention (kernels.cl:58-107, model.py:146-160).
+ *
+ * Arrays are described by mr_array: device memory of any owner, on the
+ * context's device, shape and strides in elements.  The last of several
+ * dimensions is contiguous; rows of F32 / F16 / BF16 start on 16-byte boundaries (address and
+ * strides), so the head dim is a multiple of 4 (F32) or 8.  Head dims to 128.
+ * A pool of pages is [pages, page rows, kv heads, dim] (any strides, so head-
+ * major pages are a permuted view); page_table [batch, table pages] I32 holds
+ * page ids; row t of sequence s is row t % page rows of page page_table[s][t /
+ * page rows].  lengths [batch] I32.  The tables' values live on the device and
+ * are not read by the host: an id outside the pool hides its rows (attention
+ * does not see them, an append drops them, an eviction copies zeros), a length
+ * is cut to the table's rows (an append drops the rows past them), a negative
+ * one is 0.
+ * Calls queue work on the context's stream and return; they can be captured
+ * into a CUDA graph.  Scratch memory: calls outside a capture share the
+ * context's, in stream order; a captured call's belongs to its graph.  So two
+ * contexts, or two graphs, may run at the same time. */
+typedef struct {
+    void *data;
+    int32_t dtype;      /* enum mr_dtype */
+    int32_t ndim;       /* 1 .. 4 */
+    int64_t shape[4];
+    int64_t stride[4];  /* in elements */
+} mr_array;
+
+/* Copies new rows keys / values [tokens, kv heads, dim] into their pages.
+ * offsets [batch + 1] I32: sequence s owns the rows offsets[s] .. offsets[s + 1]
+ * - 1, which become the last of its lengths[s] rows; NULL: one row per sequence
+ * (tokens = batch).  Rows in no sequence are not read.  Two rows given the same
+ * place leave one of the two there. */
+MR_API int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_array *values, const mr_array *key_pages,
+                           const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
+                           const mr_array *offsets);
+
+/* Attention of each sequence's newest token: query [batch, heads, dim] over the
+ * sequence's rows, out [batch, heads, dim]; heads / kv heads query heads share a
+ * key / value head.  window > 0: the newest `window` rows and the first `sinks`
+ * rows are visible; 0: all.  Scores are scaled by `scale`.  A sequence that sees
+ * no row gives zeros.  weights (NULL, or F32 [batch, kv heads, table rows]):
+ * row t's softmax weight, summed over the query heads of its key / value head,
+ * is added to weights[s][kv head][t]. */
+MR_API int mr_paged_attention(mr_context *ctx, const mr_array *query, const mr_array *key_pages,
+                              const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
+                              const mr_array *weights, const mr_array *out, int window, int sinks, float scale);
+
+/* Attention of prompts packed one after the other: query [tokens, heads, dim],
+ * keys / values [rows, kv heads, dim]; sequence s owns query rows
+ * query_offsets[s] .. query_offsets[s + 1] - 1 and key rows key_offsets[s] ..
+ * (I32 [batch + 1], rising, cut to the arrays).  The last query stands at the
+ * last key: query i of n over m keys at position p = m - n + i sees key j if
+ * j <= p and (window is 0, or p - j < window, or j < sinks).  A query that sees
+ * none gives zeros.  Rows of out that belong to no sequence stay as they were. */
+MR_API int mr_window_attention(mr_context *ctx, const mr_array *query, const mr_array *keys, const mr_array *values,
+                               const mr_array *query_offsets, const mr_array *key_offsets, const mr_array *out,
+                               int window, int sinks, float scale);
+
+/* Keeps `budget` rows of every sequence and key / value head: the first `sinks`,
+ * the last `recent`, and of the others those of the largest weight (F32 [batch,
+ * kv heads, table rows]; the lower row where weights are equal; NaN counts as
+ * the lowest).  All rows of a sequence of at most `budget` rows are kept.  The
+ * kept rows are copied, in their order, to the pages of target_table [batch,
+ * target pages] in target_keys / target_values (pools of the same page rows,
+ * heads, dim and type, which may be the source pools; the pages themselves must
+ * not overlap the sequences' source pages), so shared pages stay whole.
+ * kept I32 [batch, kv heads, budget]: the rows, ascending, -1 behind;
+ * new_lengths I32 [batch]; new_weights F32 [batch, kv heads, target rows]: the
+ * kept rows' weights, zeros behind. */
+MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_array *value_pages,
+                          const mr_array *page_table, const mr_array *lengths, const mr_array *weights,
+                          const mr_array *target_keys, const mr_array *target_values, const mr_array *target_table,
+                          const mr_array *kept, const mr_array *new_lengths, const mr_array *new_weights, int budget,
+                          int sinks, int recent);
 
 #ifdef __cplusplus
 }

@@ -56,11 +56,13 @@ SIGNATURES = {
     "mr_device_count": (_I, [_IP]),
     "mr_device_query": (_I, [_I, C.POINTER(DeviceInfo)]),
     "mr_context_create": (_I, [_I, C.POINTER(_P)]),
+    "mr_context_create_on_stream": (_I, [_I, _P, C.POINTER(_P)]),
     "mr_context_destroy": (_I, [_P]),
     "mr_context_finish": (_I, [_P]),
     "mr_buffer_alloc": (_I, [_P, _SZ, C.POINTER(_P)]),
     "mr_buffer_free": (_I, [_P]),
     "mr_buffer_count": (_I, [_P, C.POINTER(_SZ)]),
+    "mr_buffer_pointer": (_I, [_P, C.POINTER(_P)]),
     "mr_buffer_upload": (_I, [_P, _SZ, _P, _SZ]),
     "mr_buffer_download": (_I, [_P, _SZ, _P, _SZ]),
     "mr_buffer_copy": (_I, [_P, _P, _SZ, _SZ, _SZ]),
@@ -103,6 +105,11 @@ SIGNATURES = {
     "mr_model_bench_decode": (_I, [_P, _I, _I, _FP]),
     "mr_model_trace_decode": (_I, [_P, _I, C.POINTER(C.c_uint64), _I, _IP, _IP]),
     "mr_attention_static_scratch": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I]),
+    # mr_array arguments are passed as the struct's bytes (arrays.describe)
+    "mr_append_pages": (_I, [_P] * 8),
+    "mr_paged_attention": (_I, [_P] * 8 + [_I, _I, _F]),
+    "mr_window_attention": (_I, [_P] * 7 + [_I, _I, _F]),
+    "mr_evict_pages": (_I, [_P] * 12 + [_I, _I, _I]),
     "mr_model_set_wait_limit": (_I, [_P, C.c_uint64]),
     "mr_model_load_file": (_I, [_P, C.c_char_p, _I, _I, C.POINTER(C.c_int64), C.c_char_p, C.c_uint64]),
     "mr_model_inject_fault": (_I, [_P, _I]),

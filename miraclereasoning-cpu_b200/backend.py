@@ -7,6 +7,10 @@ behaviour, and a ``device`` with ``max_allocation_bytes`` and ``to_dict()``.
 Tensors are float32 device buffers owned by the C library; ``run(name, ...)``
 dispatches to the kernel's ``mr_op_*`` entry point.  There is no host fallback:
 a missing library or device raises ``CUDAError``.
+
+Beyond the reference: a paged key / value cache for serving several sequences
+(``append_pages``, ``paged_attention``, ``window_attention``, ``evict_pages``),
+on arrays of any owner in float32, float16 or bfloat16 (``arrays.py``).
 """
 from __future__ import annotations
 
@@ -18,6 +22,7 @@ import numpy as np
 
 from . import _native
 from ._native import CUDAError, call
+from .arrays import DeviceArray, describe, host_type, stored, widened
 
 # kernel name -> (NDRange rank, argument kinds) in kernels.cl order
 _KERNELS = {
@@ -70,15 +75,49 @@ class Tensor:
             _native._lib.mr_buffer_free(handle)
             self.handle = None
 
+    # the accessors of an operator's array argument (arrays.py)
+    dtype = "float32"
+    stride = DeviceArray.stride
+    get_device = DeviceArray.get_device
+
+    def data_ptr(self):
+        pointer = C.c_void_p()
+        call("mr_buffer_pointer", self.handle, C.byref(pointer))
+        return pointer.value
+
+    def new_empty(self, shape):
+        return self.backend.empty(shape)
+
+
+def _counts(**values):
+    for name, value in values.items():
+        if not isinstance(value, (int, np.integer)) or isinstance(value, bool) or not 0 <= value < 2 ** 31:
+            raise ValueError(f"{name} must be a whole number from 0 on: {value!r}")
+
+
+def _window(window, sinks):
+    _counts(sinks=sinks)
+    if window is None:
+        return 0
+    _counts(window=window)
+    if window == 0:
+        raise ValueError("window must be at least 1, or None for no window")
+    return window
+
 
 class CUDABackend:
     """Float32 execution on one B200 (one context = one device + one stream).
+
+    ``stream``: a CUDA stream of the caller's (its handle as an int; 0 is the
+    legacy default stream) on which all of this backend's work is queued, in
+    order with the caller's own; it has to outlive the backend.  None: a stream
+    of its own, which the caller orders with other streams' work (``finish``).
 
     An instance must be used by a single thread at a time, as the reference
     backend requires.
     """
 
-    def __init__(self, *, device_index=0, platform_index=None, device_type="gpu"):
+    def __init__(self, *, device_index=0, platform_index=None, device_type="gpu", stream=None):
         if device_type not in ("gpu", "cuda"):
             raise ValueError("CUDABackend executes on a CUDA GPU; device_type must be 'gpu'")
         devices = list_devices()
@@ -86,7 +125,10 @@ class CUDABackend:
             raise CUDAError(f"No CUDA device {device_index} (found {len(devices)}); no automatic CPU fallback.")
         self.device = devices[device_index]
         handle = C.c_void_p()
-        call("mr_context_create", device_index, C.byref(handle))
+        if stream is None:
+            call("mr_context_create", device_index, C.byref(handle))
+        else:
+            call("mr_context_create_on_stream", device_index, stream, C.byref(handle))
         self.context = handle
 
     def __del__(self):
@@ -220,6 +262,109 @@ class CUDABackend:
                  extra_values if extra_values is not None else values, out,
                  heads, kv_heads, dim, values.shape[0], start, length, extra_length)
         return out
+
+    # arrays of other types (arrays.py) ---------------------------------------------
+    def empty_array(self, shape, dtype="float32"):
+        return DeviceArray(self, shape, dtype)
+
+    def upload_array(self, array, dtype="float32"):
+        """A host array on the device; bfloat16 rounds float values to nearest even."""
+        raw = stored(array, dtype)
+        out = DeviceArray(self, raw.shape, dtype)
+        if out.size:
+            flat = np.zeros(out.words, np.uint32)
+            flat.view(np.uint8)[:raw.nbytes] = raw.reshape(-1).view(np.uint8)
+            call("mr_buffer_upload", out.handle, 0, flat.ctypes.data, out.words)
+        return out
+
+    def read_array(self, array):
+        """A DeviceArray's values on the host (bfloat16 widened to float32)."""
+        self._owns(array)
+        flat = np.empty(array.words, np.uint32)
+        call("mr_buffer_download", array.handle, 0, flat.ctypes.data, array.words)
+        kind = host_type(array.dtype)
+        raw = flat.view(np.uint8)[:array.size * kind.itemsize].view(kind).reshape(array.shape)
+        return widened(raw, array.dtype)
+
+    # paged key / value cache (include/miracle_cuda.h: mr_array and what follows) -----
+    # Pools are [pages, page rows, kv heads, dim], page_table [batch, table pages] and lengths
+    # [batch] int32; row t of sequence s is row t % page rows of page page_table[s, t // page rows].
+
+    def append_pages(self, keys, values, key_pages, value_pages, page_table, lengths, offsets=None):
+        """New rows [tokens, kv heads, dim] into their pages.  ``lengths`` counts them already; sequence s's
+        new rows are offsets[s] .. offsets[s + 1] - 1 (``offsets`` None: one row per sequence)."""
+        device = self.device.ordinal
+        call("mr_append_pages", self.context, describe(keys, "keys", device), describe(values, "values", device),
+             describe(key_pages, "key_pages", device), describe(value_pages, "value_pages", device),
+             describe(page_table, "page_table", device), describe(lengths, "lengths", device),
+             None if offsets is None else describe(offsets, "offsets", device))
+
+    def paged_attention(self, query, key_pages, value_pages, page_table, lengths, *, window=None, sinks=0, scale=None,
+                        weights=None, out=None):
+        """Attention of every sequence's newest token, query [batch, heads, dim], over its rows; returns ``out``
+        (an array like the query).  ``window``: only the newest rows, and the first ``sinks``, are visible.
+        ``scale`` defaults to 1 / sqrt(dim).  ``weights`` float32 [batch, kv heads, table rows] has each row's
+        softmax weights, summed over the query heads that share its head, added to it."""
+        window = _window(window, sinks)
+        device = self.device.ordinal
+        q = describe(query, "query", device)
+        if out is None:
+            out = query.new_empty(query.shape)
+        call("mr_paged_attention", self.context, q, describe(key_pages, "key_pages", device),
+             describe(value_pages, "value_pages", device), describe(page_table, "page_table", device),
+             describe(lengths, "lengths", device),
+             None if weights is None else describe(weights, "weights", device), describe(out, "out", device),
+             window, sinks, query.shape[-1] ** -0.5 if scale is None else scale)
+        return out
+
+    def window_attention(self, query, keys, values, query_offsets, key_offsets=None, *, window=None, sinks=0,
+                         scale=None, out=None):
+        """Causal attention of prompts packed one after the other: query [tokens, heads, dim], keys and values
+        [rows, kv heads, dim], sequence s's rows at query_offsets[s] .. query_offsets[s + 1] - 1 and at
+        ``key_offsets`` (None: the same) alike; its last query stands at its last key.  A query sees the newest
+        ``window`` keys up to its own (None: all) and the first ``sinks``.  Returns ``out`` (an array like the
+        query; rows of no sequence are not written)."""
+        window = _window(window, sinks)
+        device = self.device.ordinal
+        q = describe(query, "query", device)
+        offsets = describe(query_offsets, "query_offsets", device)
+        if out is None:
+            out = query.new_empty(query.shape)
+        call("mr_window_attention", self.context, q, describe(keys, "keys", device),
+             describe(values, "values", device), offsets,
+             offsets if key_offsets is None else describe(key_offsets, "key_offsets", device),
+             describe(out, "out", device), window, sinks, query.shape[-1] ** -0.5 if scale is None else scale)
+        return out
+
+    def evict_pages(self, key_pages, value_pages, page_table, lengths, weights, target_table, *, budget, sinks=0,
+                    recent=0, target_keys=None, target_values=None, kept=None, new_lengths=None, new_weights=None):
+        """Keeps ``budget`` rows of each sequence and head (the first ``sinks``, the last ``recent``, and those of
+        the largest ``weights``) and copies them in order to the pages of ``target_table``, in the same pools or in
+        ``target_keys`` / ``target_values``.  The target pages must be others than the sequences' own.  Returns
+        kept (int32 [batch, kv heads, budget] rows, -1 behind), the new lengths and the kept rows' weights
+        (float32 [batch, kv heads, target rows], zeros behind)."""
+        _counts(budget=budget, sinks=sinks, recent=recent)
+        device = self.device.ordinal
+        pools = describe(key_pages, "key_pages", device), describe(value_pages, "value_pages", device)
+        if (target_keys is None) != (target_values is None):
+            raise ValueError("target_keys and target_values go together")
+        targets = pools if target_keys is None else (describe(target_keys, "target_keys", device),
+                                                     describe(target_values, "target_values", device))
+        table, old = describe(target_table, "target_table", device), describe(weights, "weights", device)
+        if len(weights.shape) != 3 or len(key_pages.shape) != 4 or len(target_table.shape) != 2:
+            raise ValueError("weights must be [batch, kv heads, rows], target_table [batch, pages], the pages 4-D")
+        batch, heads = weights.shape[:2]
+        if kept is None:
+            kept = lengths.new_empty((batch, heads, budget))
+        if new_lengths is None:
+            new_lengths = lengths.new_empty(lengths.shape)
+        if new_weights is None:
+            new_weights = weights.new_empty((batch, heads, target_table.shape[1] * key_pages.shape[1]))
+        call("mr_evict_pages", self.context, *pools, describe(page_table, "page_table", device),
+             describe(lengths, "lengths", device), old, *targets, table, describe(kept, "kept", device),
+             describe(new_lengths, "new_lengths", device), describe(new_weights, "new_weights", device), budget, sinks,
+             recent)
+        return kept, new_lengths, new_weights
 
     def finish(self):
         call("mr_context_finish", self.context)

@@ -1,0 +1,337 @@
+// Rows of a paged key / value cache: appending new ones, and eviction (the rows
+// of largest accumulated weight kept and copied to other pages).
+//
+// Both move whole rows and are bound by memory: an append reads and writes every
+// new row once; an eviction reads every weight once to choose, then reads and
+// writes the kept rows.  Rows move as 16-byte pieces, consecutive threads taking
+// consecutive pieces of a row and then the next key / value head, so that both
+// sides touch whole 32-byte sectors whatever the head dim.
+#include "cache_ops.cuh"
+
+namespace mr {
+namespace cache {
+namespace {
+
+// A pool's base and strides in bytes.
+struct Pool {
+    char *base;
+    int64_t page, row, head;
+};
+Pool make_pool(const mr_array *a) {
+    const int64_t size = dtype_bytes(a->dtype);
+    return Pool{static_cast<char *>(a->data), a->stride[0] * size, a->stride[1] * size, a->stride[2] * size};
+}
+
+// ---- append -----------------------------------------------------------------------
+struct AppendArgs {
+    const char *keys, *values;  // new rows; strides in bytes
+    int64_t key_token, key_head, value_token, value_head;
+    Pool k, v;
+    Pages pages;
+    const int *lengths, *offsets;
+    int64_t length_stride, offset_stride;
+    int tokens, batch, heads, pieces;  // pieces: 16-byte pieces of a row
+};
+
+// The sequence that owns packed row i: the last s with offsets[s] <= i; -1 if its
+// end is not behind i (offsets that do not rise own nothing twice: one s a row).
+__device__ int sequence_of(const int *offsets, int64_t stride, int batch, int i) {
+    int lo = -1, hi = batch;  // offsets[lo] <= i < offsets[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(offsets + mid * stride) <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo >= 0 && __ldg(offsets + (lo + 1) * stride) > i ? lo : -1;
+}
+
+// One warp per token: its place is found once, then its heads' pieces are copied.
+__global__ void __launch_bounds__(256) k_append(AppendArgs a) {
+    const int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (token >= a.tokens) return;
+    int s = token, behind = 1;  // rows from this one to the sequence's end
+    if (a.offsets) {
+        s = sequence_of(a.offsets, a.offset_stride, a.batch, token);
+        if (s < 0) return;
+        behind = __ldg(a.offsets + (s + 1) * a.offset_stride) - token;
+    }
+    const int t = __ldg(a.lengths + s * a.length_stride) - behind;
+    if (t < 0) return;
+    const int64_t kr = a.pages.row(s, t, a.k.page, a.k.row), vr = a.pages.row(s, t, a.v.page, a.v.row);
+    if (kr < 0) return;
+    const int n = a.heads * a.pieces;
+    for (int i = lane; i < n; i += 32) {
+        const int h = i / a.pieces, c = (i - h * a.pieces) * 16;
+        const uint4 x = *reinterpret_cast<const uint4 *>(a.keys + token * a.key_token + h * a.key_head + c);
+        const uint4 y = *reinterpret_cast<const uint4 *>(a.values + token * a.value_token + h * a.value_head + c);
+        *reinterpret_cast<uint4 *>(a.k.base + kr + h * a.k.head + c) = x;
+        *reinterpret_cast<uint4 *>(a.v.base + vr + h * a.v.head + c) = y;
+    }
+}
+
+// ---- eviction -----------------------------------------------------------------------
+struct EvictArgs {
+    Pool k, v, tk, tv;
+    Pages from, to;
+    const int *lengths;
+    int64_t length_stride;
+    const float *weights;
+    int64_t w_batch, w_head;
+    int *kept, *new_lengths;
+    int64_t kept_batch, kept_head, new_length_stride;
+    float *new_weights;
+    int64_t nw_batch, nw_head;
+    int batch, heads, capacity, target_rows, budget, sinks, recent, pieces;
+};
+
+// Weights in rising order as unsigned numbers; both zeros equal, NaN the lowest.
+__device__ __forceinline__ uint32_t rank_key(float w) {
+    if (w != w) return 0;
+    const uint32_t bits = __float_as_uint(w == 0.f ? 0.f : w);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+
+// CTA = (sequence, head).  The rows between the sinks and the recent ones compete
+// for the rest of the budget: the value of the last one kept is found by four
+// passes over 8 bits of the weights' order each (counts of the 256 digits among
+// the rows that match the digits found so far); rows above it stay, and the first
+// few equal to it.  Then each warp counts its own stretch of the rows, the counts
+// are summed over the warps, and each warp writes its kept rows in order.
+__global__ void __launch_bounds__(kSelectThreads) k_select(EvictArgs a) {
+    __shared__ int counts[256];
+    __shared__ int above[kSelectWarps], equal[kSelectWarps];
+    __shared__ uint32_t s_prefix;
+    __shared__ int s_need;
+    const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int n = sequence_rows(a.lengths, a.length_stride, s, a.capacity);
+    const float *w = a.weights + s * a.w_batch + h * a.w_head;
+    int *kept = a.kept + s * a.kept_batch + h * a.kept_head;
+    float *nw = a.new_weights + s * a.nw_batch + h * a.nw_head;
+    const int total = min(n, a.budget);
+    if (tid == 0 && h == 0) a.new_lengths[s * a.new_length_stride] = total;
+    const int first = min(a.sinks, n), last = max(n - a.recent, first);
+    uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
+    int ties = n;
+    if (n > a.budget) {
+        int need = a.budget - first - (n - last);  // rows to keep among first .. last - 1
+        uint32_t prefix = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += kSelectThreads) counts[i] = 0;
+            __syncthreads();
+            for (int t = first + tid; t < last; t += kSelectThreads) {
+                const uint32_t key = rank_key(__ldg(w + t));
+                if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&counts[(key >> shift) & 255], 1);
+            }
+            __syncthreads();
+            if (tid == 0) {
+                int left = need, digit = 255;
+                while (digit > 0 && counts[digit] < left) left -= counts[digit--];
+                s_prefix = prefix << 8 | static_cast<uint32_t>(digit);
+                s_need = left;
+            }
+            __syncthreads();
+            prefix = s_prefix;
+            need = s_need;
+        }
+        cut = prefix;
+        ties = need;
+    }
+    // 0: dropped, 1: kept, 2: equal to the cut
+    auto state = [&](int t) {
+        if (t >= n) return 0;
+        if (n <= a.budget || t < first || t >= last) return 1;
+        const uint32_t key = rank_key(__ldg(w + t));
+        return key > cut ? 1 : key == cut ? 2 : 0;
+    };
+    const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) & ~31, lo = warp * stretch;
+    int kept_here = 0, equal_here = 0;
+    for (int t = lo + lane; t < lo + stretch && t - lane < n; t += 32) {
+        const int st = state(t);
+        kept_here += __popc(__ballot_sync(0xffffffffu, st == 1));
+        equal_here += __popc(__ballot_sync(0xffffffffu, st == 2));
+    }
+    if (lane == 0) {
+        above[warp] = kept_here;
+        equal[warp] = equal_here;
+    }
+    __syncthreads();
+    int kept_before = 0, equal_before = 0;
+    for (int i = 0; i < warp; ++i) {
+        kept_before += above[i];
+        equal_before += equal[i];
+    }
+    const uint32_t below = (1u << lane) - 1;
+    for (int t = lo + lane; t < lo + stretch && t - lane < n; t += 32) {
+        const int st = state(t);
+        const uint32_t m1 = __ballot_sync(0xffffffffu, st == 1), m2 = __ballot_sync(0xffffffffu, st == 2);
+        const int eq = equal_before + __popc(m2 & below);
+        const int at = kept_before + __popc(m1 & below) + min(eq, ties);
+        if ((st == 1 || (st == 2 && eq < ties)) && at < a.budget) {
+            kept[at] = t;
+            if (at < a.target_rows) nw[at] = __ldg(w + t);
+        }
+        kept_before += __popc(m1);
+        equal_before += __popc(m2);
+    }
+    for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    for (int i = total + tid; i < a.target_rows; i += kSelectThreads) nw[i] = 0.f;
+}
+
+// Kept rows to their target pages: a thread per (row, head, piece), the head inside the row.
+__global__ void __launch_bounds__(256) k_copy_kept(EvictArgs a) {
+    const int s = blockIdx.y, per_row = a.heads * a.pieces;
+    const int total = min(sequence_rows(a.lengths, a.length_stride, s, a.capacity), min(a.budget, a.target_rows));
+    const int64_t all = static_cast<int64_t>(total) * per_row;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < all;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int at = static_cast<int>(i / per_row), rest = static_cast<int>(i - static_cast<int64_t>(at) * per_row);
+        const int h = rest / a.pieces, c = (rest - h * a.pieces) * 16;
+        const int64_t to_k = a.to.row(s, at, a.tk.page, a.tk.row), to_v = a.to.row(s, at, a.tv.page, a.tv.row);
+        if (to_k < 0) continue;
+        const int t = __ldg(a.kept + s * a.kept_batch + h * a.kept_head + at);
+        const int64_t k = a.from.row(s, t, a.k.page, a.k.row), v = a.from.row(s, t, a.v.page, a.v.row);
+        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+        if (k >= 0) {
+            x = *reinterpret_cast<const uint4 *>(a.k.base + k + h * a.k.head + c);
+            y = *reinterpret_cast<const uint4 *>(a.v.base + v + h * a.v.head + c);
+        }
+        *reinterpret_cast<uint4 *>(a.tk.base + to_k + h * a.tk.head + c) = x;
+        *reinterpret_cast<uint4 *>(a.tv.base + to_v + h * a.tv.head + c) = y;
+    }
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace mr
+
+using namespace mr::cache;
+
+extern "C" int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_array *values, const mr_array *key_pages,
+                               const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
+                               const mr_array *offsets) {
+    MR_CHECK(check_array(keys, "keys", 3, true, false));
+    MR_CHECK(check_array(values, "values", 3, true, false));
+    MR_CHECK(check_pools(key_pages, value_pages, "key_pages", "value_pages", true));
+    MR_REQUIRE(keys->dtype == key_pages->dtype && values->dtype == key_pages->dtype,
+               "keys, values and the pages must be of one type");
+    for (int i = 0; i < 3; ++i) MR_REQUIRE(keys->shape[i] == values->shape[i], "keys and values differ in shape");
+    MR_REQUIRE(keys->shape[1] == key_pages->shape[2] && keys->shape[2] == key_pages->shape[3],
+               "keys must be [tokens, %lld, %lld], as the pages' heads and dim",
+               static_cast<long long>(key_pages->shape[2]), static_cast<long long>(key_pages->shape[3]));
+    MR_CHECK(check_ints(lengths, "lengths", 1));
+    const int64_t batch = lengths->shape[0];
+    MR_CHECK(check_table(page_table, "page_table", batch, key_pages->shape[1]));
+    if (offsets) {
+        MR_CHECK(check_ints(offsets, "offsets", 1));
+        MR_REQUIRE(offsets->shape[0] == batch + 1, "offsets must have %lld values (batch + 1)",
+                   static_cast<long long>(batch + 1));
+    } else {
+        MR_REQUIRE(keys->shape[0] == batch, "without offsets, keys must have one row for each of the %lld sequences",
+                   static_cast<long long>(batch));
+    }
+    MR_REQUIRE(ctx, "ctx is NULL");
+    if (!keys->shape[0] || !batch || !key_pages->shape[0] || !page_table->shape[1]) return MR_OK;
+    DeviceGuard guard(ctx->device);
+    const int64_t size = dtype_bytes(keys->dtype);
+    AppendArgs a;
+    a.keys = static_cast<const char *>(keys->data);
+    a.values = static_cast<const char *>(values->data);
+    a.key_token = keys->stride[0] * size;
+    a.key_head = keys->stride[1] * size;
+    a.value_token = values->stride[0] * size;
+    a.value_head = values->stride[1] * size;
+    a.k = make_pool(key_pages);
+    a.v = make_pool(value_pages);
+    a.pages = make_pages(key_pages, page_table);
+    a.lengths = static_cast<const int *>(lengths->data);
+    a.length_stride = lengths->stride[0];
+    a.offsets = offsets ? static_cast<const int *>(offsets->data) : nullptr;
+    a.offset_stride = offsets ? offsets->stride[0] : 0;
+    a.tokens = static_cast<int>(keys->shape[0]);
+    a.batch = static_cast<int>(batch);
+    a.heads = static_cast<int>(keys->shape[1]);
+    a.pieces = static_cast<int>(keys->shape[2] * size / 16);
+    const int warps = a.tokens < 4 * ctx->sm_count ? 1 : 8;  // few tokens: a CTA each, over all SMs
+    k_append<<<(a.tokens - 1) / warps + 1, warps * 32, 0, ctx->stream>>>(a);
+    MR_CUDA_TRY(cudaGetLastError());
+    return MR_OK;
+}
+
+extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_array *value_pages,
+                              const mr_array *page_table, const mr_array *lengths, const mr_array *weights,
+                              const mr_array *target_keys, const mr_array *target_values, const mr_array *target_table,
+                              const mr_array *kept, const mr_array *new_lengths, const mr_array *new_weights,
+                              int budget, int sinks, int recent) {
+    MR_CHECK(check_pools(key_pages, value_pages, "key_pages", "value_pages", false));
+    MR_CHECK(check_pools(target_keys, target_values, "target_keys", "target_values", true));
+    MR_REQUIRE(target_keys->dtype == key_pages->dtype, "the target pages must be of the pages' type");
+    for (int i = 1; i < 4; ++i)
+        MR_REQUIRE(target_keys->shape[i] == key_pages->shape[i],
+                   "the target pages must have the pages' rows, heads and dim");
+    MR_CHECK(check_ints(lengths, "lengths", 1));
+    const int64_t batch = lengths->shape[0], page = key_pages->shape[1], heads = key_pages->shape[2];
+    MR_CHECK(check_table(page_table, "page_table", batch, page));
+    MR_CHECK(check_table(target_table, "target_table", batch, page));
+    MR_REQUIRE(sinks >= 0 && recent >= 0 && budget > 0, "budget must be positive, sinks and recent not negative");
+    MR_REQUIRE(static_cast<int64_t>(sinks) + recent <= budget, "budget %d is less than sinks %d and recent %d", budget,
+               sinks, recent);
+    const int64_t capacity = page_table->shape[1] * page, room = target_table->shape[1] * page;
+    MR_REQUIRE(room >= std::min<int64_t>(budget, capacity),
+               "target_table has room for %lld rows of the %lld that may be kept", static_cast<long long>(room),
+               static_cast<long long>(std::min<int64_t>(budget, capacity)));
+    MR_CHECK(check_weights(weights, "weights", batch, heads, capacity, false));
+    MR_CHECK(check_weights(new_weights, "new_weights", batch, heads, room, true));
+    MR_CHECK(check_ints(kept, "kept", 3, true));
+    MR_REQUIRE(kept->shape[0] == batch && kept->shape[1] == heads && kept->shape[2] == budget,
+               "kept must be [%lld, %lld, %d] (batch, kv heads, budget)", static_cast<long long>(batch),
+               static_cast<long long>(heads), budget);
+    MR_CHECK(check_ints(new_lengths, "new_lengths", 1, true));
+    MR_REQUIRE(new_lengths->shape[0] == batch, "new_lengths must have %lld values", static_cast<long long>(batch));
+    MR_CHECK(check_apart(weights, "weights", new_weights, "new_weights"));
+    MR_CHECK(check_apart(lengths, "lengths", new_lengths, "new_lengths"));
+    MR_REQUIRE(batch <= 65535, "more than 65535 sequences");
+    MR_REQUIRE(batch * heads <= INT32_MAX, "too many heads");
+    MR_REQUIRE(ctx, "ctx is NULL");
+    if (!batch) return MR_OK;
+    DeviceGuard guard(ctx->device);
+    EvictArgs a;
+    a.k = make_pool(key_pages);
+    a.v = make_pool(value_pages);
+    a.tk = make_pool(target_keys);
+    a.tv = make_pool(target_values);
+    a.from = make_pages(key_pages, page_table);
+    a.to = make_pages(target_keys, target_table);
+    a.lengths = static_cast<const int *>(lengths->data);
+    a.length_stride = lengths->stride[0];
+    a.weights = static_cast<const float *>(weights->data);
+    a.w_batch = weights->stride[0];
+    a.w_head = weights->stride[1];
+    a.kept = static_cast<int *>(kept->data);
+    a.kept_batch = kept->stride[0];
+    a.kept_head = kept->stride[1];
+    a.new_lengths = static_cast<int *>(new_lengths->data);
+    a.new_length_stride = new_lengths->stride[0];
+    a.new_weights = static_cast<float *>(new_weights->data);
+    a.nw_batch = new_weights->stride[0];
+    a.nw_head = new_weights->stride[1];
+    a.batch = static_cast<int>(batch);
+    a.heads = static_cast<int>(heads);
+    a.capacity = static_cast<int>(capacity);
+    a.target_rows = static_cast<int>(room);
+    a.budget = budget;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
+    k_select<<<a.batch * a.heads, kSelectThreads, 0, ctx->stream>>>(a);
+    MR_CUDA_TRY(cudaGetLastError());
+    const int64_t work = std::min<int64_t>(budget, capacity) * a.heads * a.pieces;
+    if (work) {
+        const int blocks = static_cast<int>(std::min<int64_t>((work - 1) / 256 + 1, 16 * ctx->sm_count));
+        k_copy_kept<<<dim3(blocks, a.batch), 256, 0, ctx->stream>>>(a);
+        MR_CUDA_TRY(cudaGetLastError());
+    }
+    return MR_OK;
+}

@@ -38,6 +38,9 @@ struct mr_context {
     int sm_count = 0;
     cudaStream_t stream = nullptr;
     size_t max_allocation = 0;
+    bool owns_stream = true;
+    void *scratch = nullptr;  // of the calls queued outside a capture, in stream order (context_scratch)
+    size_t scratch_bytes = 0;
     std::atomic<int> refs{1};
 };
 
@@ -45,9 +48,15 @@ namespace mr {
 inline void context_retain(mr_context *ctx) { ctx->refs.fetch_add(1, std::memory_order_relaxed); }
 inline void context_release(mr_context *ctx) {
     if (ctx->refs.fetch_sub(1, std::memory_order_acq_rel) != 1) return;
+    int current = ctx->device;
+    cudaGetDevice(&current);
     cudaSetDevice(ctx->device);
-    cudaStreamSynchronize(ctx->stream);
-    cudaStreamDestroy(ctx->stream);
+    if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
+    if (ctx->owns_stream) {
+        cudaStreamSynchronize(ctx->stream);
+        cudaStreamDestroy(ctx->stream);
+    }
+    cudaSetDevice(current);
     delete ctx;
 }
 }  // namespace mr

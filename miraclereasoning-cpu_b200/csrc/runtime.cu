@@ -62,7 +62,7 @@ int mr_device_query(int ordinal, mr_device_info *info) {
     return MR_OK;
 }
 
-int mr_context_create(int device_ordinal, mr_context **out) {
+static int new_context(int device_ordinal, bool on_stream, void *stream, mr_context **out) {
     MR_REQUIRE(out, "out is NULL");
     int count = 0;
     int rc = mr_device_count(&count);
@@ -79,13 +79,23 @@ int mr_context_create(int device_ordinal, mr_context **out) {
     ctx->device = device_ordinal;
     ctx->sm_count = prop.multiProcessorCount;
     ctx->max_allocation = prop.totalGlobalMem;
-    cudaError_t err = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
-    if (err != cudaSuccess) {
-        delete ctx;
-        return mr::cuda_error(err, "cudaStreamCreate");
+    ctx->owns_stream = !on_stream;
+    ctx->stream = static_cast<cudaStream_t>(stream);
+    if (!on_stream) {
+        cudaError_t err = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
+        if (err != cudaSuccess) {
+            delete ctx;
+            return mr::cuda_error(err, "cudaStreamCreate");
+        }
     }
     *out = ctx;
     return MR_OK;
+}
+
+int mr_context_create(int device_ordinal, mr_context **out) { return new_context(device_ordinal, false, nullptr, out); }
+
+int mr_context_create_on_stream(int device_ordinal, void *stream, mr_context **out) {
+    return new_context(device_ordinal, true, stream, out);
 }
 
 int mr_context_destroy(mr_context *ctx) {
@@ -128,6 +138,12 @@ int mr_buffer_free(mr_buffer *buf) {
 int mr_buffer_count(const mr_buffer *buf, size_t *count) {
     MR_REQUIRE(buf && count, "NULL argument");
     *count = buf->count;
+    return MR_OK;
+}
+
+int mr_buffer_pointer(const mr_buffer *buf, void **pointer) {
+    MR_REQUIRE(buf && pointer, "NULL argument");
+    *pointer = buf->ptr;
     return MR_OK;
 }
 
