@@ -4,6 +4,9 @@
 #pragma once
 
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "common.cuh"
 
@@ -151,6 +154,17 @@ struct Scratch {
         if (captured) cudaFreeAsync(data, ctx->stream);
     }
 };
+
+// Lets a kernel take more than 48 KB of shared memory; asked of the driver once a kernel and device.
+inline int allow_shared(int device, const void *kernel, int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<int, const void *>> done;
+    std::lock_guard<std::mutex> guard(lock);
+    if (done.count({device, kernel})) return MR_OK;
+    MR_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.insert({device, kernel});
+    return MR_OK;
+}
 
 // ---- device side ------------------------------------------------------------------
 // t / d and t % d for 0 <= t < 2^31 by a multiplication: floor(t m / 2^63) with

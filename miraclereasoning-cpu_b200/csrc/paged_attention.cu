@@ -10,19 +10,24 @@
 //
 // Work.  A unit is (sequence, key / value head, block of at most kHeads query
 // heads).  Its visible rows, numbered 0 .. without the gap between sinks and
-// window, form tiles; the tiles of all units, one after the other, are cut into
-// as many even stretches as the grid has CTAs (two an SM, all resident).  So a
-// batch of any lengths is balanced to a tile, one long sequence runs on the whole
-// GPU, and the host need not know the lengths.  A CTA's stretch holds the end of
-// one unit, whole units, and the start of another: whole units are written out,
-// the two ends go to scratch as softmax partials (weighted values, maximum, sum),
-// and k_join, already resident when the last CTA ends (programmatic dependent
-// launch), joins the units that were cut.
+// window, form steps of STEP rows; the steps of all units, one after the other,
+// are cut into as many even stretches as the grid has warps (eight an SM, all
+// resident).  So a batch of any lengths is balanced to a step, one long sequence
+// runs on the whole GPU, and the host need not know the lengths.  A warp's
+// stretch holds the end of one unit, whole units, and the start of another: whole
+// units are written out, the two ends go to scratch as softmax partials (weighted
+// values, maximum, sum), and k_join (launched early, waiting for this kernel's
+// end) joins the units that were cut.
 //
-// Rows.  The warps of a CTA take steps of a tile in turn, each with its own ring
-// of row copies (cp.async, 16 bytes a lane, page ids looked up a step ahead) and
-// its own running softmax, so nothing in the loop waits for another warp.  The
-// partials of the warps meet in shared memory once per unit.
+// Where no token can see more than kFewSteps steps (a window, a short table), a
+// unit is a CTA's instead, a quarter of it each warp's: there is nothing to join
+// but the four warps' partials, in shared memory, and the second launch is saved
+// (flashnano-1.7's window of 516 rows in a
+// batch of 48: 9.7 us, cut and joined 20.1).
+//
+// Rows.  Warps never wait for each other there: each has its own ring of row copies
+// (cp.async, 16 bytes a lane, page ids looked up a step ahead), which runs on
+// from one unit into the next, and its own running softmax.
 #include <cmath>
 
 #include "cache_ops.cuh"
@@ -32,6 +37,8 @@ namespace cache {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kCtasPerSm = 2;
+constexpr int64_t kMaxSteps = INT32_MAX / 2;
+constexpr int kFewSteps = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedArgs {
@@ -48,7 +55,7 @@ struct PagedArgs {
     int batch, kv_heads, group, blocks, dim, capacity, window, sinks;  // blocks: blocks of query heads a group has
     float scale;     // times log2(e): scores are kept as powers of two
     // scratch
-    float *partial;  // [CTA][2][kHeads * DP values, kHeads maxima, kHeads sums]
+    float *partial;  // [warp][2][kHeads * DP values, kHeads maxima, kHeads sums]
     float *lse;      // [unit][kHeads] of whole units, with weights: log2 of the softmax sum, the maximum in it
     float *scores;   // [unit][seen rows][heads2], with weights
     int64_t seen_max;
@@ -71,37 +78,40 @@ __device__ __forceinline__ Seen seen_of(const PagedArgs &a, int s) {
     return x;
 }
 
-// Tiles of all sequences in one row: a sequence's units follow each other, each
-// with the sequence's number of tiles.
-template <int TILE>
+// Steps of all sequences in one row: a sequence's units follow each other, each
+// with the sequence's number of steps.
+template <int STEP>
 struct Plan {
-    int64_t total;
-    int units;  // of a sequence
-    int ctas;   // that get tiles: at most one each
-    // Sum of the sequences' tiles, by every warp on its own.
+    int total, units;  // units of a sequence
+    int workers;       // warps that get steps: at most one each
+    static __device__ __forceinline__ int steps_of(const Seen &seen) { return (seen.rows + STEP - 1) / STEP; }
     __device__ void init(const PagedArgs &a) {
         const int lane = threadIdx.x % 32;
         units = a.kv_heads * a.blocks;
-        int64_t sum = 0;
-        for (int s = lane; s < a.batch; s += 32) sum += (seen_of(a, s).rows + TILE - 1) / TILE;
+        int sum = 0;
+        for (int s = lane; s < a.batch; s += 32) sum += steps_of(seen_of(a, s));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum * units;
-        ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
+        workers = min(total, static_cast<int>(gridDim.x) * kWarps);
     }
-    // First tile of CTA b <= ctas, and the CTA that has tile x: the last b with b total / ctas < x + 1.
-    __device__ int64_t start(int b) const { return b * total / ctas; }
-    __device__ int cta_of(int64_t x) const { return static_cast<int>(((x + 1) * ctas - 1) / total); }
-    // The sequence of tile x (x < total) and its first tile; whole warp.
-    __device__ void find(const PagedArgs &a, int64_t x, int &s, int64_t &base) const {
+    // First step of worker b <= workers, and the worker that has step x: the last b with b total / workers < x + 1.
+    __device__ __forceinline__ int start(int b) const {
+        return static_cast<int>(static_cast<int64_t>(b) * total / workers);
+    }
+    __device__ __forceinline__ int worker_of(int x) const {
+        return static_cast<int>((static_cast<int64_t>(x + 1) * workers - 1) / total);
+    }
+    // The sequence of step x (x < total) and its first step.
+    __device__ void find(const PagedArgs &a, int x, int &s, int &base) const {
         const int lane = threadIdx.x % 32;
         base = 0;
         for (int s0 = 0;; s0 += 32) {
-            int64_t mine = s0 + lane < a.batch ? static_cast<int64_t>((seen_of(a, s0 + lane).rows + TILE - 1) / TILE) * units : 0;
-            int64_t sum = mine;
+            const int mine = s0 + lane < a.batch ? steps_of(seen_of(a, s0 + lane)) * units : 0;
+            int sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t below = __shfl_up_sync(0xffffffffu, sum, o);
+                const int below = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += below;
             }
             const uint32_t past = __ballot_sync(0xffffffffu, base + sum > x);
@@ -116,38 +126,58 @@ struct Plan {
     }
 };
 
-// Walks a CTA's stretch of tiles unit by unit.
-template <int TILE>
-struct Walk {
-    Plan<TILE> plan;
-    int64_t x, end, base;  // next tile, end of the stretch, first tile of the sequence
-    int s, tiles;          // sequence, tiles of each of its units
+// A piece of work: steps t0 .. t1 - 1 of unit u of sequence s, whose units have `steps` steps each.
+struct Piece {
+    int s, u, t0, t1, steps;
     Seen seen;
-    __device__ bool init(const PagedArgs &a) {
-        plan.init(a);
-        if (static_cast<int>(blockIdx.x) >= plan.ctas) return false;
-        x = plan.start(blockIdx.x);
-        end = plan.start(blockIdx.x + 1);
+};
+
+// Walks a stretch of steps unit by unit.
+struct Walk : Piece {
+    int x, end, base;  // next step, end of the stretch, first step of the sequence
+    template <int STEP>
+    __device__ bool init(const PagedArgs &a, const Plan<STEP> &plan, int worker) {
+        if (worker >= plan.workers) return false;
+        x = plan.start(worker);
+        end = plan.start(worker + 1);
         plan.find(a, x, s, base);
-        load(a);
+        seen = seen_of(a, s);
+        steps = Plan<STEP>::steps_of(seen);
         return true;
     }
-    __device__ void load(const PagedArgs &a) {
-        seen = seen_of(a, s);
-        tiles = (seen.rows + TILE - 1) / TILE;
-    }
-    // The next piece: unit u of sequence s, tiles t0 .. t1 - 1.  False behind the last.
-    __device__ bool next(const PagedArgs &a, int &u, int &t0, int &t1) {
+    // The next piece; false behind the last.
+    template <int STEP>
+    __device__ __forceinline__ bool next(const PagedArgs &a, const Plan<STEP> &plan) {
         if (x >= end) return false;
-        while (x >= base + static_cast<int64_t>(tiles) * plan.units) {
-            base += static_cast<int64_t>(tiles) * plan.units;
+        while (x >= base + steps * plan.units) {
+            base += steps * plan.units;
             ++s;
-            load(a);
+            seen = seen_of(a, s);
+            steps = Plan<STEP>::steps_of(seen);
         }
-        u = static_cast<int>((x - base) / tiles);
-        t0 = static_cast<int>((x - base) - static_cast<int64_t>(u) * tiles);
-        t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - x)));
+        u = (x - base) / steps;
+        t0 = (x - base) - u * steps;
+        t1 = min(steps, t0 + (end - x));
         x += t1 - t0;
+        return true;
+    }
+};
+
+// Walks the units of a CTA, a quarter of each.
+template <int STEP>
+struct Quarters : Piece {
+    int unit;  // the next
+    __device__ __forceinline__ bool next(const PagedArgs &a) {
+        const int units = a.kv_heads * a.blocks;
+        if (unit >= a.batch * units) return false;
+        s = unit / units;
+        u = unit - s * units;
+        seen = seen_of(a, s);
+        steps = (seen.rows + STEP - 1) / STEP;
+        const int warp = threadIdx.x / 32;
+        t0 = steps * warp / kWarps;
+        t1 = steps * (warp + 1) / kWarps;
+        unit += gridDim.x;
         return true;
     }
 };
@@ -251,11 +281,9 @@ struct Math16 {
     uint32_t qf[DP / 16][2];   // Q^T fragments: head lane / 4
     float o[DP / 16][4];       // O^T: dims 16 b + lane / 4 (+ 8), heads 2 (lane % 4) and + 1
     float m[2], l[2];          // heads 2 (lane % 4), + 1; l only of this lane's rows
-    bool fine;                 // weights in two parts
 
-    __device__ __forceinline__ void begin(const PagedArgs &a, const char *q, int heads, bool two_parts) {
+    __device__ __forceinline__ void begin(const PagedArgs &a, const char *q, int heads) {
         const int lane = threadIdx.x % 32, h = lane / 4;
-        fine = two_parts;
 #pragma unroll
         for (int b = 0; b < DP / 16; ++b) {
 #pragma unroll
@@ -270,8 +298,8 @@ struct Math16 {
         l[0] = l[1] = 0.f;
     }
 
-    // One step: rows in `stage` (keys, then values), bit r of `live`: row r is seen.
-    __device__ __forceinline__ void step(const PagedArgs &a, uint32_t stage, uint32_t live, float *scores) {
+    // One step: `rows` rows in `stage` (keys, then values), bit r of `live`: row r is seen.
+    __device__ __forceinline__ void step(const PagedArgs &a, uint32_t stage, uint32_t live, int rows, float *scores) {
         const int lane = threadIdx.x % 32;
         constexpr int S = STEP / 16;
         float s[S][4];
@@ -299,7 +327,7 @@ struct Math16 {
 #pragma unroll
             for (int x = 0; x < 2 * S; ++x) {
                 const int r = x * 8 + lane / 4;
-                if (h < a.heads2 && (live >> r) & 1u)
+                if (h < a.heads2 && r < rows)
                     *reinterpret_cast<float2 *>(scores + r * a.heads2 + h) = make_float2(s[x / 2][(x & 1) * 2], s[x / 2][(x & 1) * 2 + 1]);
             }
         }
@@ -348,33 +376,62 @@ struct Math16 {
                 ldmatrix_t(v, stage + STEP * R::kRowBytes +
                                   R::offset(x * 16 + lane % 8 + (lane / 16) * 8, b * 2 + ((lane / 8) & 1)));
                 mma16(o[b], v, b0, b1, T());
-                if (fine) mma16(o[b], v, c0, c1, T());
+                mma16(o[b], v, c0, c1, T());
             }
         }
     }
 
-    // The warp's results: values [head][DP + 4], then maxima and sums.  False if a value is not finite.
-    __device__ __forceinline__ bool finish(float *values, float *maxima, float *sums) {
-        const int lane = threadIdx.x % 32, h = 2 * (lane % 4);
+    // Sums over the warp; false if a value is not finite.
+    __device__ __forceinline__ bool finish() {
         bool finite = true;
 #pragma unroll
         for (int b = 0; b < DP / 16; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                finite &= fabsf(o[b][e]) < INFINITY;
-                values[(h + (e & 1)) * (DP + 4) + b * 16 + lane / 4 + (e >> 1) * 8] = o[b][e];
-            }
+            for (int e = 0; e < 4; ++e) finite &= fabsf(o[b][e]) < INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float sum = l[e];
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-            if (lane < 4) {
-                maxima[h + e] = m[e];
-                sums[h + e] = sum;
+            for (int i = 4; i < 32; i <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], i);
+        return __all_sync(0xffffffffu, finite);
+    }
+    // Every pair of values of consecutive dims of a head, times its head's factor:
+    // put(head, dim, x, y).  Lanes whose rows are neighbours swap one of their two heads.
+    template <typename Put>
+    __device__ __forceinline__ void each(float f0, float f1, const Put &put) const {
+        const int lane = threadIdx.x % 32, h = 2 * (lane % 4);
+        const bool odd = lane & 4;
+#pragma unroll
+        for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = o[b][2 * e] * f0, y = o[b][2 * e + 1] * f1;
+                const float z = __shfl_xor_sync(0xffffffffu, odd ? x : y, 4);
+                const int dim = b * 16 + e * 8 + (lane / 4 & ~1);
+                put(odd ? h + 1 : h, dim, odd ? z : x, odd ? y : z);
             }
-        }
-        return finite;
+    }
+    __device__ __forceinline__ void put_out(const PagedArgs &a, char *out, int heads) const {
+        each(l[0] != 0.f ? 1.f / l[0] : 0.f, l[1] != 0.f ? 1.f / l[1] : 0.f, [&](int h, int dim, float x, float y) {
+            if (h < heads && dim < a.dim) *reinterpret_cast<uint32_t *>(out + h * a.o_head + dim * 2) = pack2(x, y, T());
+        });
+    }
+    __device__ __forceinline__ void put_partial(float *to, int heads) const {
+        const int lane = threadIdx.x % 32;
+        each(1.f, 1.f, [&](int h, int dim, float x, float y) {
+            if (h < heads) *reinterpret_cast<float2 *>(to + h * DP + dim) = make_float2(x, y);
+        });
+        if (lane < 4)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                to[kHeads * DP + 2 * lane + e] = m[e];
+                to[kHeads * DP + kHeads + 2 * lane + e] = l[e];
+            }
+    }
+    __device__ __forceinline__ void put_lse(float *lse) const {
+        const int lane = threadIdx.x % 32;
+        if (lane < 4)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) lse[2 * lane + e] = log_sum(m[e], l[e]);
     }
 };
 
@@ -389,7 +446,7 @@ struct Math32 {
     float4 q[4], o[4];
     float m, l;  // head lane % 4; l only of this lane's rows
 
-    __device__ __forceinline__ void begin(const PagedArgs &a, const char *src, int heads, bool) {
+    __device__ __forceinline__ void begin(const PagedArgs &a, const char *src, int heads) {
         const int j = 4 * (threadIdx.x % kLanes);
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
@@ -408,7 +465,7 @@ struct Math32 {
     }
     // Row r of the step belongs to lanes r / kEach * kLanes ..; after the fold lane i of
     // those has row r = (its part) * kEach + i / 4 and head i % 4.
-    __device__ __forceinline__ void step(const PagedArgs &a, uint32_t stage, uint32_t live, float *scores) {
+    __device__ __forceinline__ void step(const PagedArgs &a, uint32_t stage, uint32_t live, int rows, float *scores) {
         const int lane = threadIdx.x % 32, part = lane / kLanes, i = lane % kLanes;
         float s[kLanes];  // [row][head]
 #pragma unroll
@@ -429,7 +486,7 @@ struct Math32 {
         }
         const int row = part * kEach + i / 4, head = i % 4;
         const float x = (live >> row) & 1u ? s[0] * a.scale : -INFINITY;
-        if (scores && head < a.heads2 && (live >> row) & 1u) scores[row * a.heads2 + head] = x;
+        if (scores && head < a.heads2 && row < rows) scores[row * a.heads2 + head] = x;
         float top = x;
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
@@ -463,8 +520,7 @@ struct Math32 {
             }
         }
     }
-    __device__ __forceinline__ bool finish(float *values, float *maxima, float *sums) {
-        const int lane = threadIdx.x % 32;
+    __device__ __forceinline__ bool finish() {
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -474,290 +530,465 @@ struct Math32 {
                 o[h].z += __shfl_xor_sync(0xffffffffu, o[h].z, w);
                 o[h].w += __shfl_xor_sync(0xffffffffu, o[h].w, w);
             }
-        if (lane < kLanes)
 #pragma unroll
-            for (int h = 0; h < 4; ++h) *reinterpret_cast<float4 *>(values + h * (DP + 4) + 4 * lane) = o[h];
-        float sum = l;
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        if (lane < 4) {
-            maxima[lane] = m;
-            sums[lane] = sum;
-        }
+        for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
         return true;
+    }
+    __device__ __forceinline__ void put_out(const PagedArgs &a, char *out, int heads) const {
+        const int j = 4 * (threadIdx.x % 32);
+        const float f = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const float fh = __shfl_sync(0xffffffffu, f, h);
+            if (h < heads && j < min(DP, a.dim))
+                *reinterpret_cast<float4 *>(out + h * a.o_head + j * 4) =
+                    make_float4(o[h].x * fh, o[h].y * fh, o[h].z * fh, o[h].w * fh);
+        }
+    }
+    __device__ __forceinline__ void put_partial(float *to, int heads) const {
+        const int lane = threadIdx.x % 32;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+            if (h < heads && lane < kLanes) *reinterpret_cast<float4 *>(to + h * DP + 4 * lane) = o[h];
+        if (lane < 4) {
+            to[kHeads * DP + lane] = m;
+            to[kHeads * DP + kHeads + lane] = l;
+        }
+    }
+    __device__ __forceinline__ void put_lse(float *lse) const {
+        if (threadIdx.x % 32 < 4) lse[threadIdx.x % 32] = log_sum(m, l);
     }
 };
 
-// One warp's share of a piece of a unit: rows [from, to) of `seen`, in steps
-// warp, warp + kWarps, ...
-template <typename M>
-__device__ __forceinline__ void walk_rows(const PagedArgs &a, M &math, const Seen &seen, int s, const char *k,
-                                          const char *v, int from, int to, uint32_t ring, float *scores) {
+// A warp's row copies, some steps ahead of its work: the same pieces walked by
+// itself, a step's page ids read when the step before it is copied.
+template <typename M, typename Next>
+struct Feed {
     using R = typename M::R;
-    constexpr int STEP = M::STEP, STAGES = M::STAGES, kCopies = STEP * R::kPieces / 32;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int steps = (to - from + STEP - 1) / STEP;
-    const int *table = a.pages.table + s * a.pages.table_stride;
-    const int live_pieces = a.dim * static_cast<int>(R::kRowBytes / M::DP) / 16;
-    auto place = [&](int step) {  // of row `lane` of a step
-        Place p = {-1, 0};
-        const int i = from + step * STEP + lane;
-        if (lane < STEP && i < to) {
-            const int t = seen.at(i), page = a.pages.page.div(t);
-            const int id = __ldg(table + page);
-            p.row = t - page * a.pages.page.d;
-            p.id = static_cast<unsigned>(id) < static_cast<unsigned>(a.pages.pages) ? id : -1;
-        }
-        return p;
-    };
-    auto issue = [&](const Place &p, int slot) {
-        const uint32_t stage = ring + slot * R::kBytes;
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-            const int e = c * 32 + lane, row = e / R::kPieces, piece = e % R::kPieces;
-            const int id = __shfl_sync(0xffffffffu, p.id, row), r = __shfl_sync(0xffffffffu, p.row, row);
-            const bool live = id >= 0 && piece < live_pieces;
-            const uint64_t page = live ? id : 0;
-            const uint32_t to_shared = stage + R::offset(row, piece);
-            copy16(to_shared, k + (page * a.k_page + static_cast<uint64_t>(r) * a.k_row + piece * 16), live);
-            copy16(to_shared + STEP * R::kRowBytes, v + (page * a.v_page + static_cast<uint64_t>(r) * a.v_row + piece * 16), live);
-        }
-    };
-    int step = warp, ahead = warp;
-    uint32_t masks[STAGES];
-    Place next = place(ahead);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        masks[i] = __ballot_sync(0xffffffffu, next.id >= 0);
-        if (ahead < steps) issue(next, i);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ahead += kWarps;
-        next = place(ahead);
+    static constexpr int STEP = M::STEP, kCopies = STEP * R::kPieces / 32;
+    Next next;             // steps a walk on; false behind its last piece
+    int i, to;             // rows of the step looked up: i .. , and the piece's end
+    bool more;             // such a step is there
+    int id, row;           // lane's row of it: page (-1: hidden) and place there
+    int64_t k, v;          // its head's offset
+    __device__ __forceinline__ explicit Feed(const Next &n) : next(n) {}
+    __device__ __forceinline__ void piece() {
+        do {
+            more = next();
+            i = next.walk.t0 * STEP;
+            to = min(next.walk.t1 * STEP, next.walk.seen.rows);
+        } while (more && i >= to);
     }
-    while (step < steps) {
+    __device__ __forceinline__ void look(const PagedArgs &a) {
+        const int at = i + static_cast<int>(threadIdx.x % 32);
+        id = -1;
+        row = 0;
+        if (more && threadIdx.x % 32 < STEP && at < to) {
+            const int t = next.walk.seen.at(at), page = a.pages.page.div(t);
+            const int found = __ldg(a.pages.table + next.walk.s * a.pages.table_stride + page);
+            row = t - page * a.pages.page.d;
+            id = static_cast<unsigned>(found) < static_cast<unsigned>(a.pages.pages) ? found : -1;
+        }
+        const int kh = next.walk.u / a.blocks;
+        k = kh * a.k_head;
+        v = kh * a.v_head;
+    }
+    // Queues the copies of the step looked up into `stage` and looks up the next.
+    // Returns the rows that are seen, a bit each.
+    __device__ __forceinline__ uint32_t issue(const PagedArgs &a, uint32_t stage) {
+        const int lane = threadIdx.x % 32;
+        const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
+        if (more) {
+            const int pieces = a.dim * (R::kRowBytes / M::DP) / 16;
+            const char *kb = a.k + k, *vb = a.v + v;
 #pragma unroll
-        for (int i = 0; i < STAGES; ++i) {
-            if (step < steps) {
-                constexpr int kWait = STAGES - 2;
-                asm volatile("cp.async.wait_group %0;" ::"n"(kWait) : "memory");
-                __syncwarp();  // every lane's copies of this step have landed, and all are done with the slot refilled next
-                const int slot = (i + STAGES - 1) % STAGES;
-                masks[slot] = __ballot_sync(0xffffffffu, next.id >= 0);
-                if (ahead < steps) issue(next, slot);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                ahead += kWarps;
-                next = place(ahead);
-                math.step(a, ring + i * R::kBytes, masks[i],
-                          scores ? scores + static_cast<int64_t>(from + step * STEP) * a.heads2 : nullptr);
-                step += kWarps;
+            for (int c = 0; c < kCopies; ++c) {
+                const int e = c * 32 + lane, r = e / R::kPieces, p = e % R::kPieces;
+                const int page = __shfl_sync(0xffffffffu, id, r), at = __shfl_sync(0xffffffffu, row, r);
+                const bool there = page >= 0 && p < pieces;
+                const uint64_t n = there ? page : 0, t = there ? at : 0;
+                const int q = there ? p : 0;
+                const uint32_t to_shared = stage + R::offset(r, p);
+                copy16(to_shared, kb + (n * a.k_page + t * a.k_row + q * 16), there);
+                copy16(to_shared + STEP * R::kRowBytes, vb + (n * a.v_page + t * a.v_row + q * 16), there);
             }
+            i += STEP;
+            if (i >= to) piece();
+            look(a);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return live;
+    }
+};
+
+// A piece whose values are not all finite, again and row by row: an infinite value
+// meets the second part of a weight as 0 x inf or inf - inf on the tensor cores.
+template <typename T, typename M>
+__device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk, const char *q, char *out, float *partial,
+                                           int heads) {
+    constexpr int H = M::kHeads, DP = M::DP;
+    const int lane = threadIdx.x % 32, kh = walk.u / a.blocks;
+    const int from = walk.t0 * M::STEP, to = min(walk.t1 * M::STEP, walk.seen.rows);
+    auto load = [&](const char *src, float (&x)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            x[j] = 4 * lane + j < a.dim ? widen(reinterpret_cast<const T *>(src) + 4 * lane + j) : 0.f;
+    };
+    for (int h = 0; h < heads; ++h) {
+        float x[4], o[4] = {}, m = -INFINITY, l = 0.f;
+        load(q + h * a.q_head, x);
+        for (int i = from; i < to; ++i) {
+            const int t = walk.seen.at(i);
+            const int64_t kr = a.pages.row(walk.s, t, a.k_page, a.k_row), vr = a.pages.row(walk.s, t, a.v_page, a.v_row);
+            if (kr < 0) continue;
+            float k[4], v[4];
+            load(a.k + kr + kh * a.k_head, k);
+            load(a.v + vr + kh * a.v_head, v);
+            const float y = warp_sum(x[0] * k[0] + x[1] * k[1] + x[2] * k[2] + x[3] * k[3]) * a.scale;
+            const float top = fmaxf(m, y), ref = top == -INFINITY ? 0.f : top;
+            const float c = ex2(m - ref), p = ex2(y - ref);
+            l = fmaf(l, c, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(o[j], c, p * v[j]);
+            m = top;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 4 * lane + j;
+            if (out && d < a.dim) narrow(l != 0.f ? o[j] / l : 0.f, reinterpret_cast<T *>(out + h * a.o_head) + d);
+            if (partial && d < DP) partial[h * DP + d] = o[j];
+        }
+        if (partial && lane == 0) {
+            partial[H * DP + h] = m;
+            partial[H * DP + H + h] = l;
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncwarp();
 }
 
-// Results of a unit's piece: dims of the block's heads.
+// A unit's weights: rows i = from + first, + step, .. of those seen.
+template <int H>
+__device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
+                                            int to, int first, int step, const float (&lse)[H]) {
+    constexpr int kRows = 4;  // in flight
+    float *weights = a.weights + walk.s * a.w_batch + kh * a.w_head;
+    for (int i0 = from + first; i0 < to; i0 += step * kRows) {
+        float sum[kRows], was[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int i = i0 + r * step;
+            sum[r] = 0.f;
+            was[r] = i < to ? weights[walk.seen.at(i)] : 0.f;
+#pragma unroll
+            for (int h = 0; h < H; h += 2) {
+                if (h >= a.heads2 || i >= to) continue;
+                const float2 x = __ldcg(reinterpret_cast<const float2 *>(scores + static_cast<int64_t>(i) * a.heads2 + h));
+                // a hidden row's score is -inf, and adds nothing whatever the sum is
+                sum[r] += x.x == -INFINITY ? 0.f : ex2(x.x - lse[h]);
+                sum[r] += x.y == -INFINITY ? 0.f : ex2(x.y - lse[h + 1]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            const int i = i0 + r * step;
+            if (i < to) weights[walk.seen.at(i)] = was[r] + sum[r];
+        }
+    }
+}
+
+// Works through pieces; `done(math, piece, q, heads, kh, h0)` takes each one's results.
+template <typename T, typename M, typename Next, typename Done>
+__device__ __forceinline__ void work_through(const PagedArgs &a, uint32_t ring, const Next &start, const Done &done) {
+    using R = typename M::R;
+    constexpr int H = M::kHeads, STEP = M::STEP, STAGES = M::STAGES;
+    Next next(start);
+    Feed<M, Next> feed(start);
+    feed.piece();
+    feed.look(a);
+    uint32_t live[STAGES - 1];  // of the steps in flight, the oldest first
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) live[i] = feed.issue(a, ring + i * R::kBytes);
+    int slot = 0;
+    while (next()) {
+        const Piece &walk = next.walk;
+        const int kh = walk.u / a.blocks, h0 = walk.u % a.blocks * H, heads = min(H, a.group - h0);
+        const int64_t unit = static_cast<int64_t>(walk.s) * (a.kv_heads * a.blocks) + walk.u;
+        const char *q = a.q + walk.s * a.q_batch + (kh * a.group + h0) * a.q_head;
+        const int to = min(walk.t1 * STEP, walk.seen.rows);
+        M math;
+        math.begin(a, q, heads);
+        for (int i = walk.t0 * STEP; i < to; i += STEP) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();  // every lane's copies of the step have landed, and all are done with the slot filled next
+            const uint32_t seen = live[0];
+#pragma unroll
+            for (int j = 0; j + 1 < STAGES - 1; ++j) live[j] = live[j + 1];
+            live[STAGES - 2] = feed.issue(a, ring + (slot == 0 ? STAGES - 1 : slot - 1) * R::kBytes);
+            math.step(a, ring + slot * R::kBytes, seen, to - i,
+                      a.scores ? a.scores + (unit * a.seen_max + i) * a.heads2 : nullptr);
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
+        }
+        done(math, walk, q, unit, heads, kh, h0);
+    }
+}
+
+template <int STEP>
+struct NextStretch {
+    Walk walk;
+    const PagedArgs &a;
+    const Plan<STEP> &plan;
+    __device__ __forceinline__ bool operator()() { return walk.next(a, plan); }
+};
+template <int STEP>
+struct NextQuarter {
+    Quarters<STEP> walk;
+    const PagedArgs &a;
+    __device__ __forceinline__ bool operator()() { return walk.next(a); }
+};
+
 template <typename T, typename M>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged(PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged(const __grid_constant__ PagedArgs a) {
     extern __shared__ __align__(128) char smem[];
-    constexpr int H = M::kHeads, DP = M::DP, kValues = H * (DP + 4);
-    static_assert((kValues + 2 * H) * 4 <= M::R::kWarpBytes, "a warp's results fit its ring");
-    const int tid = threadIdx.x, warp = tid / 32;
+    constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, worker = blockIdx.x * kWarps + warp;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // sequences that see nothing give zeros
-    for (int s = blockIdx.x; s < a.batch; s += gridDim.x) {
+    for (int s = worker; s < a.batch; s += gridDim.x * kWarps) {
         if (seen_of(a, s).rows > 0) continue;
         const int heads = a.kv_heads * a.group;
-        for (int e = tid; e < heads * a.dim; e += kThreads)
+        for (int e = lane; e < heads * a.dim; e += 32)
             narrow(0.f, reinterpret_cast<T *>(a.out + s * a.o_batch + e / a.dim * a.o_head) + e % a.dim);
     }
-    Walk<M::STEP * kWarps> walk;
-    if (!walk.init(a)) return;
-    int u, t0, t1, slot = 0;
-    char *mine = smem + warp * M::R::kWarpBytes;
-    while (walk.next(a, u, t0, t1)) {
-        const int s = walk.s, kh = u / a.blocks, h0 = u % a.blocks * H, heads = min(H, a.group - h0);
-        const int from = t0 * M::STEP * kWarps, to = min(t1 * M::STEP * kWarps, walk.seen.rows);
-        const bool whole = t0 == 0 && t1 == walk.tiles;
-        const int64_t unit = static_cast<int64_t>(s) * walk.plan.units + u;
-        const char *q = a.q + s * a.q_batch + (kh * a.group + h0) * a.q_head;
-        float *scores = a.scores ? a.scores + unit * a.seen_max * a.heads2 : nullptr;
-        float *values = reinterpret_cast<float *>(mine);
-        // An infinite value meets a weight's second part as 0 x inf or inf - inf: such a
-        // unit is worked out again with the weights in one part.
-        for (int parts = 2; parts > 0; --parts) {
-            M math;
-            math.begin(a, q, heads, parts == 2);
-            walk_rows<M>(a, math, walk.seen, s, a.k + kh * a.k_head, a.v + kh * a.v_head, from, to,
-                         shared_address(mine), scores);
-            const bool finite = math.finish(values, values + kValues, values + kValues + H);
-            if (!__syncthreads_or(!finite)) break;
-        }
-        // the warps' partials: a column of values a thread at a time
-        auto part = [&](int w) { return reinterpret_cast<const float *>(smem + w * M::R::kWarpBytes); };
-        for (int e = tid; e < heads * DP; e += kThreads) {
-            const int h = e / DP, j = e % DP;
-            float top = -INFINITY, sum = 0.f, x = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part(w)[kValues + h]);
-            const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float c = ex2(part(w)[kValues + h] - ref);
-                sum = fmaf(part(w)[kValues + H + h], c, sum);
-                x = fmaf(part(w)[h * (DP + 4) + j], c, x);
-            }
-            if (whole) {
-                if (j < a.dim)
-                    narrow(sum != 0.f ? x / sum : 0.f,
-                           reinterpret_cast<T *>(a.out + s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j);
-                if (j == 0 && a.lse) a.lse[unit * H + h] = log_sum(ref, sum);
-            } else {
-                float *to_join = a.partial + (blockIdx.x * 2 + slot) * static_cast<int64_t>(H * (DP + 2));
-                to_join[h * DP + j] = x;
-                if (j == 0) {
-                    to_join[H * DP + h] = top;
-                    to_join[H * DP + H + h] = sum;
-                }
-            }
-        }
-        slot = 1;
-        __syncthreads();  // the rings are filled again
-    }
+    Plan<STEP> plan;
+    plan.init(a);
+    Walk walk = {};
+    if (!walk.init(a, plan, worker)) return;
+    int part = 0;
+    work_through<T, M>(a, shared_address(smem + warp * M::R::kWarpBytes), NextStretch<STEP>{walk, a, plan},
+                       [&](M &math, const Piece &piece, const char *q, int64_t unit, int heads, int kh, int h0) {
+        const bool whole = piece.t0 == 0 && piece.t1 == piece.steps;
+        char *out = whole ? a.out + piece.s * a.o_batch + (kh * a.group + h0) * a.o_head : nullptr;
+        float *partial = whole ? nullptr : a.partial + (worker * 2 + part) * static_cast<int64_t>(H * (DP + 2));
+        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, out, partial, heads);
+        else if (whole) math.put_out(a, out, heads);
+        else math.put_partial(partial, heads);
+        if (whole && a.lse) math.put_lse(a.lse + unit * H);
+        part = 1;
+    });
 }
 
-// Joins the units that were cut: the CTAs whose stretch starts inside a unit
-// share its columns.  With weights, every CTA then adds up its own stretch's rows.
+// The same with a unit a CTA.
 template <typename T, typename M>
-__global__ void __launch_bounds__(kThreads) k_join(PagedArgs a) {
-    constexpr int H = M::kHeads, DP = M::DP, TILE = M::STEP * kWarps;
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid_constant__ PagedArgs a) {
+    extern __shared__ __align__(128) char smem[];
+    constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP, kPart = H * (DP + 2);
+    const int tid = threadIdx.x, warp = tid / 32;
+    float *parts = reinterpret_cast<float *>(smem + kWarps * M::R::kWarpBytes);
+    Quarters<STEP> walk = {};
+    walk.unit = blockIdx.x;
+    work_through<T, M>(a, shared_address(smem + warp * M::R::kWarpBytes), NextQuarter<STEP>{walk, a},
+                       [&](M &math, const Piece &piece, const char *q, int64_t unit, int heads, int kh, int h0) {
+        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, nullptr, parts + warp * kPart, heads);
+        else math.put_partial(parts + warp * kPart, heads);
+        __syncthreads();
+        char *out = a.out + piece.s * a.o_batch + (kh * a.group + h0) * a.o_head;
+        for (int e = tid; e < heads * DP; e += kThreads) {
+            const int h = e / DP, j = e % DP;
+            Partial all = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float *p = parts + w * kPart;
+                all.add(p[H * DP + h], p[H * DP + H + h], p[e]);
+            }
+            if (j < a.dim)
+                narrow(all.sum != 0.f ? all.x / all.sum : 0.f, reinterpret_cast<T *>(out + h * a.o_head) + j);
+        }
+        if (a.weights) {
+            float lse[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                Partial all = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float *p = parts + w * kPart + H * DP;
+                    if (h < heads) all.add(p[h], p[H + h], 0.f);
+                }
+                lse[h] = log_sum(all.top, all.sum);
+            }
+            add_weights<H>(a, piece, a.scores + unit * a.seen_max * a.heads2, kh, 0, piece.seen.rows, tid, kThreads, lse);
+        }
+        __syncthreads();  // the partials have been read
+    });
+}
+
+// Joins the units that were cut: the warps whose stretch starts inside a unit
+// share its columns, four at a time.  With weights, every warp then adds up its
+// own stretch's rows.
+constexpr int kMaxShares = 2432;  // weights of partials a warp keeps: of all heads for few, of two heads for all there can be
+
+template <typename T, typename M>
+__global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ PagedArgs a) {
+    constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
     constexpr int64_t kPart = H * (DP + 2);
-    __shared__ float s_lse[8];
-    __shared__ Partial s_part[kThreads];
-    Walk<TILE> walk;
-    const int tid = threadIdx.x;
-    const bool work = walk.init(a);
+    __shared__ float shares[kWarps][kMaxShares];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, worker = blockIdx.x * kWarps + warp;
+    Plan<STEP> plan;
+    plan.init(a);
+    Walk walk = {};
+    const bool work = walk.init(a, plan, worker);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!work) return;
-    const int64_t x0 = walk.x;
-    // the partial of CTA b of the unit whose first tile is `first`
-    auto part = [&](int b, int64_t first) {
-        return a.partial + (b * 2 + (walk.plan.start(b) >= first ? 0 : 1)) * kPart;
+    // The partials of a unit cut between workers b0 ..: a worker's first piece is in its
+    // slot 0, so only b0's may be its last one, in slot 1.
+    struct Parts {
+        const float *at;
+        int b0, slot0;
+        __device__ __forceinline__ const float *operator()(int b) const {
+            return at + (b * 2 + (b == b0 ? slot0 : 0)) * kPart;
+        }
     };
-    {
-        const int u = static_cast<int>((x0 - walk.base) / walk.tiles);
-        const int64_t first = walk.base + static_cast<int64_t>(u) * walk.tiles;
-        if (first < x0) {
-            const int b0 = walk.plan.cta_of(first), b1 = walk.plan.cta_of(first + walk.tiles - 1);
-            const int kh = u / a.blocks, h0 = u % a.blocks * H, heads = min(H, a.group - h0);
-            // columns of four values: this CTA's share, each on kThreads / share threads
-            const int columns = heads * (DP / 4), share = b1 - b0, me = static_cast<int>(blockIdx.x) - b0 - 1;
-            for (int c = me; c < columns; c += share) {
-                const int h = c / (DP / 4), j = c % (DP / 4) * 4;
-                Partial mine = {-INFINITY, 0.f, 0.f};
-                for (int b = b0 + tid / 4; b <= b1; b += kThreads / 4) {
-                    const float *p = part(b, first);
-                    mine.add(__ldcg(p + H * DP + h), __ldcg(p + H * DP + H + h), __ldcg(p + h * DP + j + tid % 4));
+    // A cut unit's softmax over its partials: each head's maximum and sum, in every lane.
+    auto softmax_of = [&](const Parts &part, int b1, float (&top)[H], float (&sum)[H]) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            top[h] = -INFINITY;
+            sum[h] = 0.f;
+        }
+#pragma unroll 2
+        for (int b = part.b0 + lane; b <= b1; b += 32) {
+            float m[H], l[H];
+            const float *p = part(b) + H * DP;
+#pragma unroll
+            for (int h = 0; h < H; h += 4) {
+                *reinterpret_cast<float4 *>(m + h) = __ldcg(reinterpret_cast<const float4 *>(p + h));
+                *reinterpret_cast<float4 *>(l + h) = __ldcg(reinterpret_cast<const float4 *>(p + H + h));
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const float t = fmaxf(top[h], m[h]), ref = t == -INFINITY ? 0.f : t;
+                sum[h] = fmaf(sum[h], ex2(top[h] - ref), l[h] * ex2(m[h] - ref));
+                top[h] = t;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const float t = warp_max(top[h]), ref = t == -INFINITY ? 0.f : t;
+            sum[h] = warp_sum(sum[h] * ex2(top[h] - ref));
+            top[h] = t;
+        }
+    };
+    const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
+    if (first < walk.x) {
+        const int b0 = plan.worker_of(first), b1 = plan.worker_of(first + walk.steps - 1), n = b1 - b0 + 1;
+        const Parts part = {a.partial, b0, plan.start(b0) >= first ? 0 : 1};
+        const int kh = cut / a.blocks, h0 = cut % a.blocks * H, heads = min(H, a.group - h0);
+        const int columns = heads * (DP / 4), me = worker - b0 - 1;
+        const int c0 = columns * me / (n - 1), c1 = columns * (me + 1) / (n - 1);
+        if (c0 < c1) {
+            const int ha = c0 / (DP / 4), hb = (c1 - 1) / (DP / 4) + 1;  // its heads
+            float top[H], sum[H];
+            softmax_of(part, b1, top, sum);
+            float *share = shares[warp];  // [head of its][partial]: the factor of a partial's values
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                if (h >= ha && h < hb) {
+                    const float ref = top[h] == -INFINITY ? 0.f : top[h], f = sum[h] != 0.f ? 1.f / sum[h] : 0.f;
+                    for (int b = lane; b < n; b += 32)
+                        share[(h - ha) * n + b] = ex2(__ldcg(part(b0 + b) + H * DP + h) - ref) * f;
                 }
-                s_part[tid] = mine;
-                __syncthreads();
-                for (int w = kThreads / 2; w >= 4; w >>= 1) {
-                    if (tid < w) s_part[tid].add(s_part[tid + w].top, s_part[tid + w].sum, s_part[tid + w].x);
-                    __syncthreads();
+            __syncwarp();
+            int wide = 1;  // lanes side by side over the columns, the rest over the partials
+            while (wide < 32 && wide < c1 - c0) wide <<= 1;
+            for (int base = c0; base < c1; base += wide) {
+                const int c = min(base + lane % wide, c1 - 1), h = c / (DP / 4), j = c % (DP / 4) * 4;
+                const float *mine = share + (h - ha) * n;
+                float4 x = {};
+#pragma unroll 8
+                for (int b = lane / wide; b < n; b += 32 / wide) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(b0 + b) + h * DP + j));
+                    x.x = fmaf(mine[b], v.x, x.x);
+                    x.y = fmaf(mine[b], v.y, x.y);
+                    x.z = fmaf(mine[b], v.z, x.z);
+                    x.w = fmaf(mine[b], v.w, x.w);
                 }
-                if (tid < 4 && j + tid < a.dim)
-                    narrow(s_part[tid].sum != 0.f ? s_part[tid].x / s_part[tid].sum : 0.f,
-                           reinterpret_cast<T *>(a.out + walk.s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j + tid);
-                __syncthreads();
+                for (int w = 16; w >= wide; w >>= 1) {
+                    x.x += __shfl_xor_sync(0xffffffffu, x.x, w);
+                    x.y += __shfl_xor_sync(0xffffffffu, x.y, w);
+                    x.z += __shfl_xor_sync(0xffffffffu, x.z, w);
+                    x.w += __shfl_xor_sync(0xffffffffu, x.w, w);
+                }
+                if (lane < wide && base + lane < c1 && j < a.dim) {
+                    T *out = reinterpret_cast<T *>(a.out + walk.s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j;
+                    narrow(x.x, out);
+                    narrow(x.y, out + 1);
+                    narrow(x.z, out + 2);
+                    narrow(x.w, out + 3);
+                }
             }
         }
     }
     if (!a.weights) return;
-    int u, t0, t1;
-    while (walk.next(a, u, t0, t1)) {
-        if (u % a.blocks) continue;  // the group's first block of heads adds up for all of them
-        const int s = walk.s, kh = u / a.blocks;
-        const int from = t0 * TILE, to = min(t1 * TILE, walk.seen.rows);
+    while (walk.next(a, plan)) {
+        if (walk.u % a.blocks) continue;  // the group's first block of heads adds up for all of them
+        const int from = walk.t0 * STEP, to = min(walk.t1 * STEP, walk.seen.rows);
         for (int b = 0; b < a.blocks; ++b) {
-            const int64_t unit = static_cast<int64_t>(s) * walk.plan.units + u + b;
-            const int64_t first = walk.base + static_cast<int64_t>(u + b) * walk.tiles;
-            const int heads = min(H, a.group - b * H);
-            const int b0 = walk.plan.cta_of(first), b1 = walk.plan.cta_of(first + walk.tiles - 1);
-            __syncthreads();
-            for (int h = tid / 32; h < heads; h += kWarps) {
-                float lse;
-                if (b0 == b1) {
-                    lse = __ldcg(a.lse + unit * H + h);
-                } else {
-                    Partial mine = {-INFINITY, 0.f, 0.f};
-                    for (int c = b0 + tid % 32; c <= b1; c += 32) {
-                        const float *p = part(c, first);
-                        mine.add(__ldcg(p + H * DP + h), __ldcg(p + H * DP + H + h), 0.f);
-                    }
+            const int64_t unit = static_cast<int64_t>(walk.s) * plan.units + walk.u + b;
+            const int start = walk.base + (walk.u + b) * walk.steps;
+            const int b0 = plan.worker_of(start), b1 = plan.worker_of(start + walk.steps - 1);
+            float top[H], sum[H], lse[H];
+            if (b0 != b1) softmax_of({a.partial, b0, plan.start(b0) >= start ? 0 : 1}, b1, top, sum);
 #pragma unroll
-                    for (int w = 16; w > 0; w >>= 1) {
-                        const float t = __shfl_xor_sync(0xffffffffu, mine.top, w), l = __shfl_xor_sync(0xffffffffu, mine.sum, w);
-                        mine.add(t, l, 0.f);
-                    }
-                    lse = log_sum(mine.top == -INFINITY ? 0.f : mine.top, mine.sum);
-                }
-                if (tid % 32 == 0) s_lse[h] = lse;
-            }
-            __syncthreads();
-            const float *scores = a.scores + unit * a.seen_max * a.heads2;
-            float *weights = a.weights + s * a.w_batch + kh * a.w_head;
-            for (int i = from + tid; i < to; i += kThreads) {
-                const int t = walk.seen.at(i);
-                if (a.pages.row(s, t, 0, 0) < 0) continue;
-                float sum = 0.f;
-                for (int h = 0; h < heads; ++h)
-                    sum += ex2(__ldcg(scores + static_cast<int64_t>(i) * a.heads2 + h) - s_lse[h]);
-                weights[t] += sum;
-            }
+            for (int h = 0; h < H; ++h)
+                lse[h] = h >= a.group - b * H ? INFINITY : b0 == b1 ? __ldcg(a.lse + unit * H + h) : log_sum(top[h], sum[h]);
+            add_weights<H>(a, walk, a.scores + unit * a.seen_max * a.heads2, walk.u / a.blocks, from, to, lane, 32, lse);
         }
     }
 }
 
 template <typename T, typename M>
 int launch(mr_context *ctx, PagedArgs &a) {
-    constexpr int H = M::kHeads, TILE = M::STEP * kWarps;
-    constexpr int kSmem = kWarps * M::R::kWarpBytes;
+    constexpr int H = M::kHeads, STEP = M::STEP;
     a.blocks = (a.group - 1) / H + 1;
     a.heads2 = (std::min(a.group, H) + 1) / 2 * 2;
-    // the most rows a token can see, and the most tiles there can be
+    // the most rows a token can see, and the most steps there can be
     a.seen_max = a.window ? std::min<int64_t>(a.capacity, static_cast<int64_t>(a.window) + a.sinks) : a.capacity;
     const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.blocks;
-    const int64_t tiles = (a.seen_max + TILE - 1) / TILE;
-    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(units * tiles, kCtasPerSm * ctx->sm_count)));
-    const size_t partial = sizeof(float) * 2 * grid * H * (M::DP + 2);
-    const size_t lse = a.weights ? sizeof(float) * units * H : 0;
+    const int64_t steps = (a.seen_max + STEP - 1) / STEP;
+    MR_REQUIRE(units <= kMaxSteps && units * steps <= kMaxSteps, "the sequences' rows and heads are too many for one call");
+    // weights of a group in several blocks are added up by one warp, which only k_join can
+    const bool few = steps <= kFewSteps && (!a.weights || a.blocks == 1);
+    const int64_t ctas = few ? units : (units * steps + kWarps - 1) / kWarps;
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, kCtasPerSm * ctx->sm_count)));
+    const size_t partial = few ? 0 : sizeof(float) * 2 * kWarps * grid * H * (M::DP + 2);
+    const size_t lse = a.weights && !few ? sizeof(float) * units * H : 0;
     const size_t scores = a.weights ? sizeof(float) * units * a.seen_max * a.heads2 : 0;
     auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
     Scratch scratch(ctx);
-    // with a tile a unit at most, nothing can be cut
-    const bool cut = tiles > 1;
-    if (cut || a.weights) MR_CHECK(scratch.take(up(partial) + up(lse) + scores));
+    MR_CHECK(scratch.take(up(partial) + up(lse) + scores));
     char *base = static_cast<char *>(scratch.data);
     a.partial = reinterpret_cast<float *>(base);
-    a.lse = a.weights ? reinterpret_cast<float *>(base + up(partial)) : nullptr;
-    a.scores = a.weights ? reinterpret_cast<float *>(base + up(partial) + up(lse)) : nullptr;
-    auto kernel = k_paged<T, M>;
-    MR_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    kernel<<<grid, kThreads, kSmem, ctx->stream>>>(a);
-    MR_CUDA_TRY(cudaGetLastError());
-    if (cut || a.weights) {
-        cudaLaunchAttribute early;
-        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        early.val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t config = {};
-        config.gridDim = dim3(grid);
-        config.blockDim = dim3(kThreads);
-        config.stream = ctx->stream;
-        config.attrs = &early;
-        config.numAttrs = 1;
-        MR_CUDA_TRY(cudaLaunchKernelEx(&config, k_join<T, M>, a));
+    a.lse = lse ? reinterpret_cast<float *>(base + up(partial)) : nullptr;
+    a.scores = scores ? reinterpret_cast<float *>(base + up(partial) + up(lse)) : nullptr;
+    constexpr int kRings = kWarps * M::R::kWarpBytes;
+    if (few) {
+        constexpr int kSmem = kRings + kWarps * H * (M::DP + 2) * 4;
+        MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged_few<T, M>), kSmem));
+        k_paged_few<T, M><<<grid, kThreads, kSmem, ctx->stream>>>(a);
+        MR_CUDA_TRY(cudaGetLastError());
+        return MR_OK;
     }
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings));
+    k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
+    MR_CUDA_TRY(cudaGetLastError());
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(kThreads);
+    config.stream = ctx->stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    MR_CUDA_TRY(cudaLaunchKernelEx(&config, k_join<T, M>, a));
     return MR_OK;
 }
 

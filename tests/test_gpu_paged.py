@@ -116,6 +116,25 @@ def test_long_sequences_are_split_and_joined(served, dtype, lengths, window, sin
     check_paged(served, cache, queries(len(lengths), 8, 64, dtype), dtype, window, sinks, True)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv, dim, page, lengths", [(8, 2, 32, 16, [1500, 40]), (12, 4, 128, 32, [1100, 0, 690]),
+                                                           (20, 2, 96, 20, [1300]), (3, 3, 40, 7, [1200, 1200])])
+def test_cut_units_of_every_layout(served, dtype, heads, kv, dim, page, lengths):
+    for weighted in (False, True):
+        check_paged(served, Cache(lengths, page, kv, dim, dtype), queries(len(lengths), heads, dim, dtype), dtype,
+                    weighted=weighted)
+
+
+def test_an_infinite_value_in_a_cut_unit(served):
+    import torch
+    cache = Cache([3000], 16, 1, 64, "bfloat16")
+    cache.values[int(cache.table[0, 40]), 3, 0, 5] = float("-inf")
+    got = served.paged_attention(queries(1, 2, 64, "bfloat16"), cache.keys, cache.values, cache.table, cache.lengths)
+    assert torch.isinf(got[0, :, 5]).all() and torch.isfinite(got[0, :, :5]).all() and torch.isfinite(got[0, :, 6:]).all()
+    cache.values[int(cache.table[0, 40]), 3] = cache.rows[0][1][40 * 16 + 3]
+    check_paged(served, cache, queries(1, 2, 64, "bfloat16"), "bfloat16")
+
+
 def test_many_sequences(served):
     rng = np.random.default_rng(3)
     lengths = [int(n) for n in rng.integers(0, 40, 300)]
