@@ -18,6 +18,12 @@ int cuda_error(cudaError_t err, const char *what);
 
 }  // namespace mr
 
+struct mr_context;
+namespace mr {
+// MR_ERR_TIMEOUT, once, if a wait of a kernel queued on the context gave up since the last call.
+int check_waits(mr_context *ctx);
+}  // namespace mr
+
 #define MR_CUDA_TRY(call)                                                       \
     do {                                                                        \
         cudaError_t _e = (call);                                                \
@@ -41,6 +47,7 @@ struct mr_context {
     bool owns_stream = true;
     void *scratch = nullptr;  // of the calls queued outside a capture, in stream order (context_scratch)
     size_t scratch_bytes = 0;
+    int *wait_error = nullptr;  // host memory that kernels set when a bounded wait gave up (check_waits)
     std::atomic<int> refs{1};
 };
 
@@ -52,6 +59,10 @@ inline void context_release(mr_context *ctx) {
     cudaGetDevice(&current);
     cudaSetDevice(ctx->device);
     if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
+    if (ctx->wait_error) {
+        cudaStreamSynchronize(ctx->stream);
+        cudaFreeHost(ctx->wait_error);
+    }
     if (ctx->owns_stream) {
         cudaStreamSynchronize(ctx->stream);
         cudaStreamDestroy(ctx->stream);

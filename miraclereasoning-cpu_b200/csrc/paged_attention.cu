@@ -22,8 +22,7 @@
 // Where no token can see more than kFewSteps steps (a window, a short table), a
 // unit is a CTA's instead, a quarter of it each warp's: there is nothing to join
 // but the four warps' partials, in shared memory, and the second launch is saved
-// (flashnano-1.7's window of 516 rows in a
-// batch of 48: 9.7 us, cut and joined 20.1).
+// (flashnano-1.7's window of 516 rows in a batch of 48: 9.7 us, cut and joined 20.1).
 //
 // Rows.  Warps never wait for each other there: each has its own ring of row copies
 // (cp.async, 16 bytes a lane, page ids looked up a step ahead), which runs on

@@ -26,6 +26,13 @@ int cuda_error(cudaError_t err, const char *what) {
                      what, cudaGetErrorString(err), cudaGetErrorName(err));
 }
 
+int check_waits(mr_context *ctx) {
+    volatile int *gave_up = ctx->wait_error;
+    if (!*gave_up) return MR_OK;
+    *gave_up = 0;
+    return set_error(MR_ERR_TIMEOUT, "a bounded device-side wait of an earlier call gave up; its results are not valid");
+}
+
 }  // namespace mr
 
 extern "C" {
@@ -88,6 +95,15 @@ static int new_context(int device_ordinal, bool on_stream, void *stream, mr_cont
             return mr::cuda_error(err, "cudaStreamCreate");
         }
     }
+    // mapped: kernels of a captured call write it too, and the host reads it without a copy
+    cudaError_t err = cudaHostAlloc(reinterpret_cast<void **>(&ctx->wait_error), sizeof(int),
+                                    cudaHostAllocMapped | cudaHostAllocPortable);
+    if (err != cudaSuccess) {
+        if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
+        delete ctx;
+        return mr::cuda_error(err, "cudaHostAlloc");
+    }
+    *ctx->wait_error = 0;
     *out = ctx;
     return MR_OK;
 }
@@ -107,7 +123,7 @@ int mr_context_finish(mr_context *ctx) {
     MR_REQUIRE(ctx, "ctx is NULL");
     MR_CUDA_TRY(cudaSetDevice(ctx->device));
     MR_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-    return MR_OK;
+    return mr::check_waits(ctx);
 }
 
 int mr_buffer_alloc(mr_context *ctx, size_t count, mr_buffer **out) {

@@ -4,9 +4,33 @@
 //   p = m - n + i   (query i of a sequence of n queries and m keys)
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the j that query i sees:
 //           j <= p and (no window, or p - j < window, or j < sinks).
+//
+// 16-bit types run on the 5th-generation tensor cores (k_window).  A CTA works on
+// two tiles of 128 query rows (128 / group tokens x the group's heads: the heads
+// share their keys, and a tile of few tokens wastes little at the mask's edges)
+// over the 128-key tiles that any of their rows sees; tiles between the sinks and
+// the window are skipped.  Warp roles: warps 0-3 and 4-7 the softmax of one query
+// tile each (a thread a row, so a row's maximum and sum need no exchange), warp 8
+// the TMA loads, warp 9 the products.  S = Q K^T and O += P V accumulate in TMEM
+// (S of both tiles 2 x 128 columns, O of both behind); P, rounded to the operands'
+// type, goes back to TMEM over its own S and is the first operand of the second
+// product, V the second one as it lies in memory (MN-major).  While one tile is in
+// softmax the other is in the products.  The two exponentials and products of a
+// 128 x 128 tile (head dim 128) cost 1024 cycles each on an SM, so both units bound
+// the kernel together.  O is rescaled only where a row's maximum grows by more than
+// 2^8: until then the weights are taken against the old maximum, which the sum
+// shares, so nothing is lost but headroom.
+//
+// A weight is 0 where the mask hides a key, but 0 x NaN is NaN: a row whose values are
+// not all finite at the end is worked out again from the visible keys alone
+// (row_alone), so that what a mask hides, also in other sequences, never matters.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <cmath>
 
 #include "cache_ops.cuh"
+#include "tcgen05.cuh"
 
 namespace mr {
 namespace cache {
@@ -20,6 +44,7 @@ struct WindowArgs {
     int64_t qo_stride, ko_stride;
     int tokens, rows, batch, heads, kv_heads, group, dim, window, sinks;
     float scale;
+    int *gave_up;    // host word of the context
 };
 
 // Where sequence s lies, cut to the arrays: first query, queries, first key, keys.
@@ -35,26 +60,19 @@ __device__ __forceinline__ Span span_of(const WindowArgs &a, int s) {
     return x;
 }
 
-// A warp per (query row, head), four values of a row a lane.
+// One query row's attention by one warp, four values of a row a lane: row i of the
+// sequence, head h.
 template <typename T>
-__global__ void __launch_bounds__(128) k_rows(WindowArgs a) {
-    const int64_t id = blockIdx.x * static_cast<int64_t>(4) + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32, i = static_cast<int>(id / a.heads), h = static_cast<int>(id % a.heads);
-    if (i >= a.tokens) return;
-    int s = 0;
-    Span x = {};
-    for (; s < a.batch; ++s) {
-        x = span_of(a, s);
-        if (i >= x.q0 && i < x.q0 + x.n) break;
-    }
-    if (s == a.batch) return;
+__device__ void row_alone(const WindowArgs &a, const Span &x, int i, int h) {
+    const int lane = threadIdx.x % 32;
     auto load = [&](const char *row, float (&y)[4]) {
+#pragma unroll
         for (int j = 0; j < 4; ++j)
             y[j] = 4 * lane + j < a.dim ? widen(reinterpret_cast<const T *>(row) + 4 * lane + j) : 0.f;
     };
-    const int p = x.m - x.n + i - x.q0, kh = h / a.group;
+    const int p = x.m - x.n + i, kh = h / a.group;
     float q[4], o[4] = {}, m = -INFINITY, l = 0.f;
-    load(a.q + i * a.q_row + h * a.q_head, q);
+    load(a.q + (x.q0 + i) * a.q_row + h * a.q_head, q);
     for (int j = 0; j <= p; ++j) {
         if (a.window && p - j >= a.window && j >= a.sinks) {
             j = p - a.window;
@@ -64,14 +82,464 @@ __global__ void __launch_bounds__(128) k_rows(WindowArgs a) {
         load(a.k + (x.k0 + j) * a.k_row + kh * a.k_head, k);
         load(a.v + (x.k0 + j) * a.v_row + kh * a.v_head, v);
         const float y = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]) * a.scale;
-        const float m_new = fmaxf(m, y), c = expf(m - m_new), w = expf(y - m_new);
+        const float top = fmaxf(m, y), ref = top == -INFINITY ? 0.f : top, c = expf(m - ref), w = expf(y - ref);
         l = l * c + w;
+#pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = o[e] * c + w * v[e];
-        m = m_new;
+        m = top;
     }
-    T *out = reinterpret_cast<T *>(a.out + i * a.o_row + h * a.o_head);
+    T *out = reinterpret_cast<T *>(a.out + (x.q0 + i) * a.o_row + h * a.o_head);
+#pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (4 * lane + j < a.dim) narrow(l > 0.f ? o[j] / l : 0.f, out + 4 * lane + j);
+        if (4 * lane + j < a.dim) narrow(l != 0.f ? o[j] / l : 0.f, out + 4 * lane + j);
+}
+
+// A warp per (query row, head).
+template <typename T>
+__global__ void __launch_bounds__(128) k_rows(const __grid_constant__ WindowArgs a) {
+    const int64_t id = blockIdx.x * static_cast<int64_t>(4) + threadIdx.x / 32;
+    const int i = static_cast<int>(id / a.heads), h = static_cast<int>(id % a.heads);
+    if (i >= a.tokens) return;
+    int s = 0;
+    Span x = {};
+    for (; s < a.batch; ++s) {
+        x = span_of(a, s);
+        if (i >= x.q0 && i < x.q0 + x.n) break;
+    }
+    if (s < a.batch) row_alone<T>(a, x, i - x.q0, h);
+}
+
+// ---- tensor cores -----------------------------------------------------------------
+constexpr int kTile = 128;  // query rows, and keys, of a tile
+constexpr int kLoadWarp = 8, kMathWarp = 9, kTcThreads = 320;
+constexpr uint32_t kHalf = kTile * 128;  // bytes of 64 dims of a tile's rows
+
+template <int DP>
+struct Shape {
+    static constexpr int kHalves = DP / 64;
+    static constexpr uint32_t kTileBytes = kHalves * kHalf;
+    static constexpr int kStages = DP == 128 ? 5 : 8;
+    static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTileBytes + 256;
+    static constexpr uint32_t kO = 2 * kTile;  // TMEM columns: S0, S1, O0, O1
+};
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+// Shared memory behind the tiles.
+struct Barriers {
+    uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_done[2];
+    uint32_t tmem;
+    int stop;  // a wait gave up: every role leaves
+};
+
+// A bounded wait; false when it gives up, or another role has.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up) {
+    if (tc::try_wait(bar, parity)) return true;
+    const uint64_t start = tc::now();
+    for (unsigned spin = 1;; ++spin) {
+        if (tc::try_wait(bar, parity)) return true;
+        if (spin % 64 == 0) {
+            if (*reinterpret_cast<volatile int *>(&b->stop)) return false;
+            if (tc::now() - start > tc::kWaitNs) {
+                *reinterpret_cast<volatile int *>(&b->stop) = 1;
+                *reinterpret_cast<volatile int *>(gave_up) = 1;
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::saddr(bar)) : "memory");
+}
+__device__ __forceinline__ void expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::saddr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(head), "r"(row), "r"(tc::saddr(bar))
+        : "memory");
+}
+// D (+)= A B^T with A in TMEM (two 16-bit values a column).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+// An operand tile as rows of 64 contiguous values of the operand's outer (not summed)
+// dimension, 128-byte swizzle: 8-row groups 1024 bytes apart, the next 64 values a half on.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kHalf >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+// Instruction descriptor: D float32, A and B of one 16-bit type; A negated; B MN-major.
+__device__ __forceinline__ uint32_t mma_desc(bool bf16, int n, bool negate, bool b_mn) {
+    const uint32_t type = bf16 ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((negate ? 1u : 0u) << 13) | ((b_mn ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+#define MR_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define MR_I8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+// 32 columns of this thread's lane, not waited for (settle).
+__device__ __forceinline__ void tmem_get(uint32_t addr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : MR_R8(v, 0), MR_R8(v, 8), MR_R8(v, 16), MR_R8(v, 24)
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_put(uint32_t addr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MR_I8(v, 0),
+        MR_I8(v, 8), MR_I8(v, 16), MR_I8(v, 24), "r"(addr)
+        : "memory");
+}
+// Waits for the loads before it; the values may be used behind it only.
+template <int N>
+__device__ __forceinline__ void settle(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+__device__ __forceinline__ float pow2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pair_of(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pair_of(float x, float y, __half) {
+    const __half2 p = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// A CTA's work: queries t0 .. of sequence `x`, KV head `kh`, and the key tiles they see.
+struct Item {
+    Span x;
+    int kh, t0, count;         // first query and queries (of two tiles)
+    int front, first, tiles;   // tiles 0 .. front - 1, then first ..
+    __device__ __forceinline__ int tile(int j) const { return j < front ? j : first + j - front; }
+};
+// Items in falling order of their tiles' numbers, so that the longest of a causal prompt start first.
+__device__ bool item_of(const WindowArgs &a, int per, Item &it) {
+    const int lane = threadIdx.x % 32;
+    int total = 0;
+    for (int s = lane; s < a.batch; s += 32) total += (span_of(a, s).n + 2 * per - 1) / (2 * per);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(total) * a.kv_heads) return false;
+    const int pair = total - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
+    it.kh = static_cast<int>(blockIdx.x) % a.kv_heads;
+    int base = 0, s = -1;
+    for (int s0 = 0; s0 < a.batch; s0 += 32) {
+        const int mine = s0 + lane < a.batch ? (span_of(a, s0 + lane).n + 2 * per - 1) / (2 * per) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += below;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, base + sum > pair);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            s = s0 + l;
+            base += __shfl_sync(0xffffffffu, sum - mine, l);
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (s < 0) return false;  // offsets that overlap so far that their sum wraps
+    it.x = span_of(a, s);
+    it.t0 = (pair - base) * 2 * per;
+    it.count = min(2 * per, it.x.n - it.t0);
+    const int low = it.x.m - it.x.n + it.t0, high = low + it.count - 1;  // their positions
+    it.front = it.first = it.tiles = 0;
+    if (high < 0) return true;
+    const int start = a.window ? max(0, low - a.window + 1) : 0;  // the first key in a window
+    it.first = start / kTile;
+    it.front = min(it.first, (min(a.sinks, start) + kTile - 1) / kTile);
+    it.tiles = it.front + high / kTile - it.first + 1;
+    return true;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant__ WindowArgs a,
+                                                          const __grid_constant__ Maps maps) {
+    using S = Shape<DP>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    Barriers *b = reinterpret_cast<Barriers *>(tiles + (2 + S::kStages) * S::kTileBytes);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int per = kTile / a.group;  // tokens of a query tile
+    Item it;
+    if (!item_of(a, per, it)) return;
+    if (tid == 0) {
+        auto init = [](uint64_t *bar, int count) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc::saddr(bar)), "r"(count) : "memory");
+        };
+        init(&b->q_full, 1);
+        for (int i = 0; i < S::kStages; ++i) {
+            init(&b->kv_full[i], 1);
+            init(&b->kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            init(&b->s_full[i], 1);
+            init(&b->p_full[i], 128);
+            init(&b->o_done[i], 1);
+        }
+        b->stop = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMathWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::saddr(&b->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = b->tmem, q_tiles = tc::saddr(tiles), stages = q_tiles + 2 * S::kTileBytes;
+    const int n = it.tiles;
+    if (warp == kLoadWarp) {
+        if (lane == 0 && n > 0) {
+            // K0, V0, K1, V1, ... through the stages; Q first
+            expect(&b->q_full, 2 * S::kHalves * per * a.group * 128);
+            for (int w = 0; w < 2; ++w)
+                for (int h = 0; h < S::kHalves; ++h)
+                    load_box(q_tiles + w * S::kTileBytes + h * kHalf, &maps.q, h * 64, it.kh * a.group,
+                             it.x.q0 + it.t0 + w * per, &b->q_full);
+            int issued = 0;
+            for (; issued < 2 * n; ++issued) {
+                const int st = issued % S::kStages, use = issued / S::kStages;
+                if (use > 0 && !wait_for(&b->kv_empty[st], (use - 1) & 1, b, a.gave_up)) break;
+                expect(&b->kv_full[st], S::kTileBytes);
+                for (int h = 0; h < S::kHalves; ++h)
+                    load_box(stages + st * S::kTileBytes + h * kHalf, issued & 1 ? &maps.v : &maps.k, h * 64, it.kh,
+                             it.x.k0 + it.tile(issued / 2) * kTile, &b->kv_full[st]);
+            }
+            // no copy may land after the CTA has left (the last stages; those before were waited for by the products)
+            const uint64_t start = tc::now();
+            while (!tc::try_wait(&b->q_full, 0) && tc::now() - start < tc::kWaitNs) {
+            }
+            for (int i = max(0, issued - S::kStages); i < issued; ++i)
+                while (!tc::try_wait(&b->kv_full[i % S::kStages], (i / S::kStages) & 1) && tc::now() - start < tc::kWaitNs) {
+                }
+        }
+    } else if (warp == kMathWarp) {
+        if (lane == 0 && n > 0) {
+            constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+            const uint32_t qk = mma_desc(kBf16, kTile, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
+            auto scores = [&](int w, int st) {
+                const uint32_t q = q_tiles + w * S::kTileBytes, k = stages + st * S::kTileBytes;
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i)
+                    tc::mma(tmem + w * kTile, tc::sw128_desc(q + (i / 4) * kHalf + (i % 4) * 32),
+                            tc::sw128_desc(k + (i / 4) * kHalf + (i % 4) * 32), qk, i > 0);
+                tc::commit(&b->s_full[w]);
+            };
+            bool ok = wait_for(&b->q_full, 0, b, a.gave_up) && wait_for(&b->kv_full[0], 0, b, a.gave_up);
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                scores(0, 0);
+                scores(1, 0);
+                tc::commit(&b->kv_empty[0]);
+            }
+            for (int j = 0; j < n && ok; ++j) {
+                const int vi = 2 * j + 1, vs = vi % S::kStages, ki = vi + 1, ks = ki % S::kStages;
+                const bool more = j + 1 < n;
+                ok = wait_for(&b->kv_full[vs], (vi / S::kStages) & 1, b, a.gave_up);
+                if (ok && more) ok = wait_for(&b->kv_full[ks], (ki / S::kStages) & 1, b, a.gave_up);
+                for (int w = 0; w < 2 && ok; ++w) {
+                    ok = wait_for(&b->p_full[w], j & 1, b, a.gave_up);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t v = stages + vs * S::kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < kTile / 16; ++i)
+                        mma_ts(tmem + S::kO + w * DP, tmem + w * kTile + i * 8, mn_desc(v + i * 2048), pv, j > 0 || i > 0);
+                    tc::commit(&b->o_done[w]);
+                    if (more) scores(w, ks);
+                }
+                tc::commit(&b->kv_empty[vs]);
+                if (more) tc::commit(&b->kv_empty[ks]);
+            }
+        }
+    } else {
+        const int w = warp / 4, r = (warp & 3) * 32 + lane, tt = r / a.group, g = r - tt * a.group;
+        const int i = it.t0 + w * per + tt;  // query of the sequence
+        const bool live = tt < per && w * per + tt < it.count;
+        const int p = live ? it.x.m - it.x.n + i : -1;
+        // every row's position of this tile, for the tiles that need no mask
+        const int p_low = it.x.m - it.x.n + it.t0 + w * per, p_high = p_low + min(per, it.count - w * per) - 1;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + w * kTile, o_at = tmem + lanes + S::kO + w * DP;
+        const float scale = fabsf(a.scale) * 1.4426950408889634f;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n && ok; ++j) {
+            ok = __all_sync(0xffffffffu, wait_for(&b->s_full[w], j & 1, b, a.gave_up));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t s[kTile];
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) tmem_get(s_at + c, s + c);
+            settle(s);
+            const int kb = it.tile(j) * kTile;
+            if (kb + kTile - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kTile > a.sinks)) {
+                const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
+#pragma unroll
+                for (int c = 0; c < kTile; ++c)
+                    if (c > high || (c < low && c >= front)) s[c] = 0xff800000u;
+            }
+            float top = __uint_as_float(s[0]);
+#pragma unroll
+            for (int c = 1; c < kTile; ++c) top = fmaxf(top, __uint_as_float(s[c]));
+            if (__any_sync(0xffffffffu, (top - m) * scale > 8.f)) {  // also from -inf; NaN (nothing yet) is no reason
+                const float grown = fmaxf(m, top);
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (j - 1) & 1, b, a.gave_up));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const float c = m == grown ? 1.f : pow2((m - grown) * scale);
+                    l *= c;
+#pragma unroll
+                    for (int d = 0; d < DP; d += 32) {
+                        uint32_t o[32];
+                        tmem_get(o_at + d, o);
+                        settle(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                        tmem_put(o_at + d, o);
+                    }
+                }
+                m = grown;
+            }
+            const float shift = m == -INFINITY ? 0.f : -m * scale;
+            float sum[4] = {};
+            // The weights, rounded to the operands' type: half a step each, at random, of sums
+            // whose result is rounded to that type again.  The sum takes them unrounded.
+#pragma unroll
+            for (int c = 0; c < kTile; c += 2) {
+                const float x = pow2(fmaf(__uint_as_float(s[c]), scale, shift));
+                const float y = pow2(fmaf(__uint_as_float(s[c + 1]), scale, shift));
+                sum[c / 2 % 4] += x + y;
+                s[c / 2] = pair_of(x, y, T());
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_put(s_at, s);
+            tmem_put(s_at + 32, s + 32);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            arrive(&b->p_full[w]);
+        }
+        if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (n - 1) & 1, b, a.gave_up));
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int h = it.kh * a.group + g;
+            char *out = a.out + (it.x.q0 + i) * a.o_row + h * a.o_head;
+            const float f = l != 0.f ? 1.f / l : 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int d = 0; d < DP; d += 32) {
+                uint32_t o[32] = {};
+                if (n > 0) {
+                    tmem_get(o_at + d, o);
+                    settle(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint4 x;
+                    uint32_t *y = &x.x;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float u = __uint_as_float(o[e + 2 * c]) * f, v = __uint_as_float(o[e + 2 * c + 1]) * f;
+                        finite &= fabsf(u) < INFINITY && fabsf(v) < INFINITY;
+                        y[c] = pair_of(u, v, T());
+                    }
+                    if (live && d + e < a.dim) *reinterpret_cast<uint4 *>(out + (d + e) * 2) = x;
+                }
+            }
+            for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1) {
+                const int from = __ffs(again) - 1;
+                row_alone<T>(a, it.x, __shfl_sync(0xffffffffu, i, from), __shfl_sync(0xffffffffu, h, from));
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == kMathWarp) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static const auto fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// Rows [rows][heads][dim] as boxes of 64 dims x `heads_box` heads x `rows_box` rows; dims past the end read as zeros.
+int encode(CUtensorMap *map, const void *data, bool bf16, int64_t dim, int64_t heads, int64_t rows, int64_t head_stride,
+           int64_t row_stride, int heads_box, int rows_box) {
+    auto fn = map_encoder();
+    if (!fn) return set_error(MR_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t size[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    // a dimension of one element may come with any stride, also none
+    const cuuint64_t stride[2] = {static_cast<cuuint64_t>(heads == 1 ? 16 : head_stride),
+                                  static_cast<cuuint64_t>(rows == 1 ? 16 : row_stride)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads_box), static_cast<cuuint32_t>(rows_box)}, one[3] = {1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                          const_cast<void *>(data), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(MR_ERR_ARGUMENT, "the rows' layout cannot be loaded by tiles (%d)", static_cast<int>(r));
+    return MR_OK;
+}
+
+template <typename T, int DP>
+int launch(mr_context *ctx, WindowArgs &a) {
+    using S = Shape<DP>;
+    constexpr bool kBf16 = !__is_same(T, __half);
+    const int per = kTile / a.group;
+    Maps maps;
+    MR_CHECK(encode(&maps.q, a.q, kBf16, a.dim, a.heads, a.tokens, a.q_head, a.q_row, a.group, per));
+    MR_CHECK(encode(&maps.k, a.k, kBf16, a.dim, a.kv_heads, a.rows, a.k_head, a.k_row, 1, kTile));
+    MR_CHECK(encode(&maps.v, a.v, kBf16, a.dim, a.kv_heads, a.rows, a.v_head, a.v_row, 1, kTile));
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window<T, DP>), S::kSmem));
+    const int64_t pairs = a.tokens / (2 * per) + a.batch;  // no sequence has more than one that is not full
+    MR_REQUIRE(pairs * a.kv_heads <= INT32_MAX, "too many rows and heads for one call");
+    k_window<T, DP><<<static_cast<unsigned>(pairs * a.kv_heads), kTcThreads, S::kSmem, ctx->stream>>>(a, maps);
+    MR_CUDA_TRY(cudaGetLastError());
+    return MR_OK;
+}
+
+template <typename T>
+int launch_rows(mr_context *ctx, const WindowArgs &a) {
+    const int64_t warps = static_cast<int64_t>(a.tokens) * a.heads;
+    MR_REQUIRE((warps + 3) / 4 <= INT32_MAX, "too many rows and heads for one call");
+    k_rows<T><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, ctx->stream>>>(a);
+    MR_CUDA_TRY(cudaGetLastError());
+    return MR_OK;
+}
+
+template <typename T>
+int launch16(mr_context *ctx, WindowArgs &a) {
+    // a tile holds whole groups; a group of more heads than it has rows goes by rows, as no rows of keys do
+    if (a.group > kTile || a.rows == 0) return launch_rows<T>(ctx, a);
+    return a.dim <= 64 ? launch<T, 64>(ctx, a) : launch<T, 128>(ctx, a);
 }
 
 }  // namespace
@@ -109,6 +577,7 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     MR_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
     MR_REQUIRE(std::isfinite(scale), "scale must be finite");
     MR_REQUIRE(ctx, "ctx is NULL");
+    MR_CHECK(mr::check_waits(ctx));
     if (!query->shape[0] || query_offsets->shape[0] == 1) return MR_OK;
     DeviceGuard guard(ctx->device);
     const int64_t size = dtype_bytes(query->dtype);
@@ -138,12 +607,10 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     a.dim = static_cast<int>(query->shape[2]);
     a.window = window;
     a.sinks = sinks;
-    a.scale = scale;
-    auto kernel = query->dtype == MR_DTYPE_F32   ? k_rows<float>
-                  : query->dtype == MR_DTYPE_F16 ? k_rows<__half>
-                                                 : k_rows<__nv_bfloat16>;
-    const int64_t warps = static_cast<int64_t>(a.tokens) * a.heads;
-    kernel<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, ctx->stream>>>(a);
-    MR_CUDA_TRY(cudaGetLastError());
-    return MR_OK;
+    // a scale of 0 weighs all visible keys alike, and must leave the hidden ones' -inf alone
+    a.scale = scale == 0.f ? 1e-30f : scale;
+    a.gave_up = ctx->wait_error;
+    return query->dtype == MR_DTYPE_F32   ? launch_rows<float>(ctx, a)
+           : query->dtype == MR_DTYPE_F16 ? launch16<__half>(ctx, a)
+                                          : launch16<__nv_bfloat16>(ctx, a);
 }

@@ -288,20 +288,21 @@ def test_more_queries_than_keys(served, dtype):
 @pytest.mark.parametrize("bad", [NAN, float("inf"), float("-inf")])
 def test_hidden_keys_of_a_prompt_do_not_matter(served, dtype, bad):
     import torch
-    # the last rows of each sequence are bad: the rows before them keep their values
+    # the last rows of each sequence are bad, and some that fall out of the window again: the
+    # rows that do not see them are as exact as ever (worked out another way, so not the same bits)
     q, k, v = (queries(n, h, 64, dtype, seed=n) for n, h in ((300, 4), (299, 2), (298, 2)))
     k, v = torch.cat([k, k[:1]]), torch.cat([v, v[:2]])
     offsets = torch.tensor([0, 150, 300], dtype=torch.int32, device="cuda")
-    clean = served.window_attention(q, k, v, offsets, window=100, sinks=2)
-    for end in (150, 300):
-        k[end - 9:end], v[end - 9:end] = bad, bad
-    got = served.window_attention(q, k, v, offsets, window=100, sinks=2)
-    for a, b in ((0, 150), (150, 300)):
-        assert torch.equal(got[a:b - 9], clean[a:b - 9])
-    # bad rows that fall out of the window are forgotten again
-    k[2:9], v[2:9] = bad, bad
-    got = served.window_attention(q, k, v, offsets, window=100, sinks=2)
-    assert torch.equal(got[109:141], clean[109:141])
+    q64, k64, v64 = wide(q), wide(k), wide(v)
+    for x in (k, v):
+        x[141:150], x[291:300], x[2:9] = bad, bad, bad
+    got = wide(served.window_attention(q, k, v, offsets, window=100, sinks=2))
+    for a in (0, 150):
+        want, _, mixed, reach = ref.attend(q64[a:a + 150], k64[a:a + 150], v64[a:a + 150], range(150), 0.125, 100, 2)
+        bound = ref.output_bound(want, mixed, reach, 64, 150, dtype, True)
+        clean = slice(109, 141) if a == 0 else slice(0, 141)
+        assert np.all(np.abs(got[a:a + 150] - want)[clean] <= bound[clean])
+        assert not np.isfinite(got[a + 149]).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
