@@ -110,16 +110,19 @@ __global__ void __launch_bounds__(128) k_rows(const __grid_constant__ WindowArgs
 }
 
 // ---- tensor cores -----------------------------------------------------------------
-constexpr int kTile = 128;  // query rows, and keys, of a tile
-constexpr int kLoadWarp = 8, kMathWarp = 9, kTcThreads = 320;
-constexpr uint32_t kHalf = kTile * 128;  // bytes of 64 dims of a tile's rows
+constexpr int kTile = 128, kKeys = 128;  // query rows and keys of a tile
+constexpr int kLoadWarp = 8, kMathWarp = 9, kTcThreads = 384;  // warp 11 fills the third warpgroup
+// bytes of 64 dims of a tile's queries, and of its keys
+constexpr uint32_t kHalfQ = kTile * 128, kHalfK = kKeys * 128;
+
+constexpr int kPoly = 0;
 
 template <int DP>
 struct Shape {
     static constexpr int kHalves = DP / 64;
-    static constexpr uint32_t kTileBytes = kHalves * kHalf;
+    static constexpr uint32_t kQBytes = kHalves * kHalfQ, kStageBytes = kHalves * kHalfK;
     static constexpr int kStages = DP == 128 ? 5 : 8;
-    static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTileBytes + 256;
+    static constexpr uint32_t kSmem = 1024 + 2 * kQBytes + kStages * kStageBytes + 512;
     static constexpr uint32_t kO = 2 * kTile;  // TMEM columns: S0, S1, O0, O1
 };
 
@@ -129,7 +132,7 @@ struct Maps {
 
 // Shared memory behind the tiles.
 struct Barriers {
-    uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_done[2];
+    uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_done[2];
     uint32_t tmem;
     int stop;  // a wait gave up: every role leaves
 };
@@ -149,6 +152,12 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b,
             }
         }
     }
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
 }
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::saddr(bar)) : "memory");
@@ -173,7 +182,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 // An operand tile as rows of 64 contiguous values of the operand's outer (not summed)
 // dimension, 128-byte swizzle: 8-row groups 1024 bytes apart, the next 64 values a half on.
 __device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kHalf >> 4) << 16) |
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kHalfK >> 4) << 16) |
            (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 // Instruction descriptor: D float32, A and B of one 16-bit type; A negated; B MN-major.
@@ -199,6 +208,18 @@ __device__ __forceinline__ void tmem_put(uint32_t addr, const uint32_t *v) {
         MR_I8(v, 8), MR_I8(v, 16), MR_I8(v, 24), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_get16(uint32_t addr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : MR_R8(v, 0), MR_R8(v, 8)
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_put16(uint32_t addr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MR_I8(v, 0),
+        MR_I8(v, 8), "r"(addr)
+        : "memory");
+}
 // Waits for the loads before it; the values may be used behind it only.
 template <int N>
 __device__ __forceinline__ void settle(uint32_t (&v)[N]) {
@@ -210,6 +231,50 @@ __device__ __forceinline__ float pow2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two float32 operations as one instruction.
+__device__ __forceinline__ uint64_t bits_of(float2 x) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(x.x), "f"(x.y));
+    return y;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return floats_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return floats_of(d);
+}
+// 2^x of two values by float32 arithmetic: x = n + f with |f| <= 1/2 (adding 1.5 x 2^23
+// rounds to a whole number), the polynomial of least relative error for 2^f of degree 4
+// (Remez exchange; 2.6e-6, where a weight keeps 2^-9 or 2^-12), n added to its exponent.
+// Below -126 it gives 2^-126, not 0.
+__device__ __forceinline__ float2 pow2_by_fma(float2 x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+    const float2 minus = make_float2(-1.f, -1.f);
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 t = add2(x, magic), f = fma2(add2(t, back), minus, x);
+    float2 p = make_float2(0.00957010191f, 0.00957010191f);
+    p = fma2(p, f, make_float2(0.0559178603f, 0.0559178603f));
+    p = fma2(p, f, make_float2(0.240247448f, 0.240247448f));
+    p = fma2(p, f, make_float2(0.693121815f, 0.693121815f));
+    p = fma2(p, f, make_float2(0.999999261f, 0.999999261f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one is
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
 }
 __device__ __forceinline__ uint32_t pair_of(float x, float y, __nv_bfloat16) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
@@ -263,9 +328,9 @@ __device__ bool item_of(const WindowArgs &a, int per, Item &it) {
     it.front = it.first = it.tiles = 0;
     if (high < 0) return true;
     const int start = a.window ? max(0, low - a.window + 1) : 0;  // the first key in a window
-    it.first = start / kTile;
-    it.front = min(it.first, (min(a.sinks, start) + kTile - 1) / kTile);
-    it.tiles = it.front + high / kTile - it.first + 1;
+    it.first = start / kKeys;
+    it.front = min(it.first, (min(a.sinks, start) + kKeys - 1) / kKeys);
+    it.tiles = it.front + high / kKeys - it.first + 1;
     return true;
 }
 
@@ -275,7 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
     using S = Shape<DP>;
     extern __shared__ uint8_t raw[];
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    Barriers *b = reinterpret_cast<Barriers *>(tiles + (2 + S::kStages) * S::kTileBytes);
+    Barriers *b = reinterpret_cast<Barriers *>(tiles + 2 * S::kQBytes + S::kStages * S::kStageBytes);
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int per = kTile / a.group;  // tokens of a query tile
     Item it;
@@ -287,11 +352,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         init(&b->q_full, 1);
         for (int i = 0; i < S::kStages; ++i) {
             init(&b->kv_full[i], 1);
-            init(&b->kv_empty[i], 1);
+            init(&b->kv_empty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             init(&b->s_full[i], 1);
-            init(&b->p_full[i], 128);
+            init(&b->p_half[i], 4);
+            init(&b->p_full[i], 4);
             init(&b->o_done[i], 1);
         }
         b->stop = 0;
@@ -304,25 +370,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = b->tmem, q_tiles = tc::saddr(tiles), stages = q_tiles + 2 * S::kTileBytes;
+    const uint32_t tmem = b->tmem, q_tiles = tc::saddr(tiles), stages = q_tiles + 2 * S::kQBytes;
     const int n = it.tiles;
+    // 384 threads start with 168 registers each; a softmax thread holds a row of 128 scores
+    // and takes 208, of what the third warpgroup gives: 2 x 208 + 88 = 3 x 168.
+    if (warp >= kLoadWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == kLoadWarp) {
         if (lane == 0 && n > 0) {
-            // K0, V0, K1, V1, ... through the stages; Q first
             expect(&b->q_full, 2 * S::kHalves * per * a.group * 128);
             for (int w = 0; w < 2; ++w)
                 for (int h = 0; h < S::kHalves; ++h)
-                    load_box(q_tiles + w * S::kTileBytes + h * kHalf, &maps.q, h * 64, it.kh * a.group,
+                    load_box(q_tiles + w * S::kQBytes + h * kHalfQ, &maps.q, h * 64, it.kh * a.group,
                              it.x.q0 + it.t0 + w * per, &b->q_full);
+            // K0, V0, K1, V1, ... through the stages
             int issued = 0;
-            for (; issued < 2 * n; ++issued) {
+            auto load = [&](const CUtensorMap *map, int j) {
                 const int st = issued % S::kStages, use = issued / S::kStages;
-                if (use > 0 && !wait_for(&b->kv_empty[st], (use - 1) & 1, b, a.gave_up)) break;
-                expect(&b->kv_full[st], S::kTileBytes);
+                if (use > 0 && !wait_for(&b->kv_empty[st], (use - 1) & 1, b, a.gave_up)) return false;
+                expect(&b->kv_full[st], S::kStageBytes);
                 for (int h = 0; h < S::kHalves; ++h)
-                    load_box(stages + st * S::kTileBytes + h * kHalf, issued & 1 ? &maps.v : &maps.k, h * 64, it.kh,
-                             it.x.k0 + it.tile(issued / 2) * kTile, &b->kv_full[st]);
-            }
+                    load_box(stages + st * S::kStageBytes + h * kHalfK, map, h * 64, it.kh, it.x.k0 + it.tile(j) * kKeys,
+                             &b->kv_full[st]);
+                ++issued;
+                return true;
+            };
+            for (int j = 0; j < n; ++j)
+                if (!load(&maps.k, j) || !load(&maps.v, j)) break;
             // no copy may land after the CTA has left (the last stages; those before were waited for by the products)
             const uint64_t start = tc::now();
             while (!tc::try_wait(&b->q_full, 0) && tc::now() - start < tc::kWaitNs) {
@@ -331,46 +404,74 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 while (!tc::try_wait(&b->kv_full[i % S::kStages], (i / S::kStages) & 1) && tc::now() - start < tc::kWaitNs) {
                 }
         }
-    } else if (warp == kMathWarp) {
-        if (lane == 0 && n > 0) {
+    } else if (warp == kMathWarp || warp == kMathWarp + 1) {
+        // A warp for each query tile, so that one's waits do not hold up the other's products.
+        // All of it walks through them and one lane issues: descriptors stay in uniform
+        // registers, where the instruction wants them.
+        if (n > 0) {
             constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
-            const uint32_t qk = mma_desc(kBf16, kTile, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
-            auto scores = [&](int w, int st) {
-                const uint32_t q = q_tiles + w * S::kTileBytes, k = stages + st * S::kTileBytes;
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i)
-                    tc::mma(tmem + w * kTile, tc::sw128_desc(q + (i / 4) * kHalf + (i % 4) * 32),
-                            tc::sw128_desc(k + (i / 4) * kHalf + (i % 4) * 32), qk, i > 0);
-                tc::commit(&b->s_full[w]);
-            };
-            bool ok = wait_for(&b->q_full, 0, b, a.gave_up) && wait_for(&b->kv_full[0], 0, b, a.gave_up);
-            if (ok) {
+            const uint32_t qk = mma_desc(kBf16, kKeys, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
+            const int w = warp - kMathWarp;
+            const uint64_t q = tc::sw128_desc(q_tiles + w * S::kQBytes), k_desc = tc::sw128_desc(stages), v_desc = mn_desc(stages);
+            const uint32_t s_at = tmem + w * kTile, o_at = tmem + S::kO + w * DP;
+            const bool leader = elect();
+            int st = 0, round = 0;  // the next stage, and the parity of its fill
+            auto take = [&] {
+                if (!wait_for(&b->kv_full[st], round, b, a.gave_up)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                scores(0, 0);
-                scores(1, 0);
-                tc::commit(&b->kv_empty[0]);
+                return true;
+            };
+            auto leave = [&] {
+                if (leader) tc::commit(&b->kv_empty[st]);
+                __syncwarp();
+                if (++st == S::kStages) {
+                    st = 0;
+                    round ^= 1;
+                }
+            };
+            auto scores = [&] {
+                const uint64_t k = k_desc + st * (S::kStageBytes >> 4);
+                if (leader) {
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i)
+                        tc::mma(s_at, q + ((i / 4) * kHalfQ + (i % 4) * 32) / 16, k + ((i / 4) * kHalfK + (i % 4) * 32) / 16, qk,
+                                i > 0);
+                    tc::commit(&b->s_full[w]);
+                }
+                __syncwarp();
+            };
+            bool ok = wait_for(&b->q_full, 0, b, a.gave_up) && take();
+            if (ok) {
+                scores();
+                leave();
             }
             for (int j = 0; j < n && ok; ++j) {
-                const int vi = 2 * j + 1, vs = vi % S::kStages, ki = vi + 1, ks = ki % S::kStages;
-                const bool more = j + 1 < n;
-                ok = wait_for(&b->kv_full[vs], (vi / S::kStages) & 1, b, a.gave_up);
-                if (ok && more) ok = wait_for(&b->kv_full[ks], (ki / S::kStages) & 1, b, a.gave_up);
-                for (int w = 0; w < 2 && ok; ++w) {
-                    ok = wait_for(&b->p_full[w], j & 1, b, a.gave_up);
+                ok = take();
+                const uint64_t v = v_desc + st * (S::kStageBytes >> 4);
+                // P comes in two halves; the first is multiplied while the second is worked out
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && wait_for(half ? &b->p_full[w] : &b->p_half[w], j & 1, b, a.gave_up);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t v = stages + vs * S::kTileBytes;
+                    if (leader) {
 #pragma unroll
-                    for (int i = 0; i < kTile / 16; ++i)
-                        mma_ts(tmem + S::kO + w * DP, tmem + w * kTile + i * 8, mn_desc(v + i * 2048), pv, j > 0 || i > 0);
-                    tc::commit(&b->o_done[w]);
-                    if (more) scores(w, ks);
+                        for (int i = half * kKeys / 32; i < (half + 1) * kKeys / 32; ++i)
+                            mma_ts(o_at, s_at + i * 8, v + i * 128, pv, j > 0 || i > 0);
+                        if (half) tc::commit(&b->o_done[w]);
+                    }
+                    __syncwarp();
                 }
-                tc::commit(&b->kv_empty[vs]);
-                if (more) tc::commit(&b->kv_empty[ks]);
+                leave();
+                if (ok && j + 1 < n) {
+                    ok = take();
+                    if (ok) scores();
+                    leave();
+                }
             }
         }
-    } else {
+    } else if (warp < kLoadWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int w = warp / 4, r = (warp & 3) * 32 + lane, tt = r / a.group, g = r - tt * a.group;
         const int i = it.t0 + w * per + tt;  // query of the sequence
         const bool live = tt < per && w * per + tt < it.count;
@@ -380,70 +481,90 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + w * kTile, o_at = tmem + lanes + S::kO + w * DP;
         const float scale = fabsf(a.scale) * 1.4426950408889634f;
-        float m = -INFINITY, l = 0.f;
+        constexpr float kNone = -3.4028235e38f;  // no key seen yet
+        float m = kNone, l = 0.f;
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             ok = __all_sync(0xffffffffu, wait_for(&b->s_full[w], j & 1, b, a.gave_up));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[kTile];
+            uint32_t s[kKeys];
 #pragma unroll
-            for (int c = 0; c < kTile; c += 32) tmem_get(s_at + c, s + c);
+            for (int c = 0; c < kKeys; c += 32) tmem_get(s_at + c, s + c);
             settle(s);
-            const int kb = it.tile(j) * kTile;
-            if (kb + kTile - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kTile > a.sinks)) {
+            const int kb = it.tile(j) * kKeys;
+            if (kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)) {
                 const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
 #pragma unroll
-                for (int c = 0; c < kTile; ++c)
+                for (int c = 0; c < kKeys; ++c)
                     if (c > high || (c < low && c >= front)) s[c] = 0xff800000u;
             }
-            float top = __uint_as_float(s[0]);
+            float tops[8];
 #pragma unroll
-            for (int c = 1; c < kTile; ++c) top = fmaxf(top, __uint_as_float(s[c]));
-            if (__any_sync(0xffffffffu, (top - m) * scale > 8.f)) {  // also from -inf; NaN (nothing yet) is no reason
-                const float grown = fmaxf(m, top);
+            for (int c = 0; c < 8; ++c) tops[c] = __uint_as_float(s[c]);
+#pragma unroll
+            for (int c = 8; c < kKeys; ++c) tops[c % 8] = max_nan(tops[c % 8], __uint_as_float(s[c]));
+            const float top = max_nan(max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])),
+                                      max_nan(max_nan(tops[4], tops[5]), max_nan(tops[6], tops[7])));
+            if (__any_sync(0xffffffffu, !((top - m) * scale <= 8.f))) {  // a NaN goes into the maximum, and so everywhere
+                const float grown = max_nan(m, top);
                 if (j > 0) {
+                    // done already, since the scores came behind it
                     ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (j - 1) & 1, b, a.gave_up));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const float c = m == grown ? 1.f : pow2((m - grown) * scale);
                     l *= c;
 #pragma unroll
-                    for (int d = 0; d < DP; d += 32) {
-                        uint32_t o[32];
-                        tmem_get(o_at + d, o);
+                    for (int d = 0; d < DP; d += 16) {
+                        uint32_t o[16];
+                        tmem_get16(o_at + d, o);
                         settle(o);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
-                        tmem_put(o_at + d, o);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                        tmem_put16(o_at + d, o);
                     }
                 }
                 m = grown;
             }
-            const float shift = m == -INFINITY ? 0.f : -m * scale;
-            float sum[4] = {};
+            const float shift = m == kNone ? 0.f : -m * scale;
+            float2 sum[2] = {};
             // The weights, rounded to the operands' type: half a step each, at random, of sums
             // whose result is rounded to that type again.  The sum takes them unrounded.
 #pragma unroll
-            for (int c = 0; c < kTile; c += 2) {
-                const float x = pow2(fmaf(__uint_as_float(s[c]), scale, shift));
-                const float y = pow2(fmaf(__uint_as_float(s[c + 1]), scale, shift));
-                sum[c / 2 % 4] += x + y;
-                s[c / 2] = pair_of(x, y, T());
+            for (int c = 0; c < kKeys; c += 2) {
+                float2 x = fma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(scale, scale),
+                                make_float2(shift, shift));
+                if (kPoly && c / 2 % 8 >= 8 - kPoly) {
+                    x = pow2_by_fma(x);
+                } else {
+                    x.x = pow2(x.x);
+                    x.y = pow2(x.y);
+                }
+                sum[c / 2 % 2] = add2(sum[c / 2 % 2], x);
+                s[c / 2] = pair_of(x.x, x.y, T());
+                if (c == kKeys / 2 - 2) {
+                    tmem_put(s_at, s);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive(&b->p_half[w]);
+                }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_put(s_at, s);
-            tmem_put(s_at + 32, s + 32);
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            tmem_put(s_at + kKeys / 4, s + kKeys / 4);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            arrive(&b->p_full[w]);
+            __syncwarp();
+            if (lane == 0) arrive(&b->p_full[w]);
         }
         if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (n - 1) & 1, b, a.gave_up));
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int h = it.kh * a.group + g;
             char *out = a.out + (it.x.q0 + i) * a.o_row + h * a.o_head;
-            const float f = l != 0.f ? 1.f / l : 0.f;
+            const float f = m == kNone ? 0.f : 1.f / l;
             bool finite = true;
 #pragma unroll
             for (int d = 0; d < DP; d += 32) {
@@ -516,8 +637,8 @@ int launch(mr_context *ctx, WindowArgs &a) {
     const int per = kTile / a.group;
     Maps maps;
     MR_CHECK(encode(&maps.q, a.q, kBf16, a.dim, a.heads, a.tokens, a.q_head, a.q_row, a.group, per));
-    MR_CHECK(encode(&maps.k, a.k, kBf16, a.dim, a.kv_heads, a.rows, a.k_head, a.k_row, 1, kTile));
-    MR_CHECK(encode(&maps.v, a.v, kBf16, a.dim, a.kv_heads, a.rows, a.v_head, a.v_row, 1, kTile));
+    MR_CHECK(encode(&maps.k, a.k, kBf16, a.dim, a.kv_heads, a.rows, a.k_head, a.k_row, 1, kKeys));
+    MR_CHECK(encode(&maps.v, a.v, kBf16, a.dim, a.kv_heads, a.rows, a.v_head, a.v_row, 1, kKeys));
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window<T, DP>), S::kSmem));
     const int64_t pairs = a.tokens / (2 * per) + a.batch;  // no sequence has more than one that is not full
     MR_REQUIRE(pairs * a.kv_heads <= INT32_MAX, "too many rows and heads for one call");
