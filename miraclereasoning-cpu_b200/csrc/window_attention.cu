@@ -115,8 +115,6 @@ constexpr int kLoadWarp = 8, kMathWarp = 9, kTcThreads = 384;  // warp 11 fills 
 // bytes of 64 dims of a tile's queries, and of its keys
 constexpr uint32_t kHalfQ = kTile * 128, kHalfK = kKeys * 128;
 
-constexpr int kPoly = 0;
-
 template <int DP>
 struct Shape {
     static constexpr int kHalves = DP / 64;
@@ -253,24 +251,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits_of(a)), "l"(bits_of(b)));
     return floats_of(d);
 }
-// 2^x of two values by float32 arithmetic: x = n + f with |f| <= 1/2 (adding 1.5 x 2^23
-// rounds to a whole number), the polynomial of least relative error for 2^f of degree 4
-// (Remez exchange; 2.6e-6, where a weight keeps 2^-9 or 2^-12), n added to its exponent.
-// Below -126 it gives 2^-126, not 0.
-__device__ __forceinline__ float2 pow2_by_fma(float2 x) {
-    const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
-    const float2 minus = make_float2(-1.f, -1.f);
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const float2 t = add2(x, magic), f = fma2(add2(t, back), minus, x);
-    float2 p = make_float2(0.00957010191f, 0.00957010191f);
-    p = fma2(p, f, make_float2(0.0559178603f, 0.0559178603f));
-    p = fma2(p, f, make_float2(0.240247448f, 0.240247448f));
-    p = fma2(p, f, make_float2(0.693121815f, 0.693121815f));
-    p = fma2(p, f, make_float2(0.999999261f, 0.999999261f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
+// The lowest n of 32 bits.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one is
     float z;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
@@ -343,8 +325,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
     Barriers *b = reinterpret_cast<Barriers *>(tiles + 2 * S::kQBytes + S::kStages * S::kStageBytes);
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int per = kTile / a.group;  // tokens of a query tile
-    Item it;
-    if (!item_of(a, per, it)) return;
     if (tid == 0) {
         auto init = [](uint64_t *bar, int count) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc::saddr(bar)), "r"(count) : "memory");
@@ -367,6 +347,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::saddr(&b->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (warp == kLoadWarp && lane < 3)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
+    Item it = {};
+    const bool work = item_of(a, per, it);
+    if (!work) it.tiles = it.count = 0;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -496,8 +481,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             if (kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)) {
                 const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
 #pragma unroll
-                for (int c = 0; c < kKeys; ++c)
-                    if (c > high || (c < low && c >= front)) s[c] = 0xff800000u;
+                for (int c = 0; c < kKeys; c += 32) {
+                    // a bit for each key that is seen: up to `high`, and from `low` on or in the sinks
+                    const uint32_t seen = below(high + 1 - c) & (~below(low - c) | below(front - c));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen & (1u << e))) s[c + e] = 0xff800000u;
+                }
             }
             float tops[8];
 #pragma unroll
@@ -535,12 +525,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             for (int c = 0; c < kKeys; c += 2) {
                 float2 x = fma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(scale, scale),
                                 make_float2(shift, shift));
-                if (kPoly && c / 2 % 8 >= 8 - kPoly) {
-                    x = pow2_by_fma(x);
-                } else {
-                    x.x = pow2(x.x);
-                    x.y = pow2(x.y);
-                }
+                x.x = pow2(x.x);
+                x.y = pow2(x.y);
                 sum[c / 2 % 2] = add2(sum[c / 2 % 2], x);
                 s[c / 2] = pair_of(x.x, x.y, T());
                 if (c == kKeys / 2 - 2) {
