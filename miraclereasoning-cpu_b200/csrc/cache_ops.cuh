@@ -166,6 +166,23 @@ inline int allow_shared(int device, const void *kernel, int bytes) {
     return MR_OK;
 }
 
+// Launches a kernel that may start while the one before it runs (programmatic dependent
+// launch) and waits for that one's end itself (griddepcontrol.wait).
+template <typename Args>
+int launch_early(mr_context *ctx, dim3 grid, dim3 threads, void (*kernel)(Args), const Args &args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = threads;
+    config.stream = ctx->stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    MR_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args));
+    return MR_OK;
+}
+
 // ---- device side ------------------------------------------------------------------
 // t / d and t % d for 0 <= t < 2^31 by a multiplication: floor(t m / 2^63) with
 // m = floor(2^63 / d) + 1 is exact, since t (m d - 2^63) <= t d < 2^63.

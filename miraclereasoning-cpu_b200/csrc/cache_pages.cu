@@ -91,21 +91,24 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048;
 
-// CTA = (sequence, head).  The rows between the sinks and the recent ones compete
-// for the rest of the budget: the value of the last one kept is found by four
-// passes over 8 bits of the weights' order each (counts of the 256 digits among
-// the rows that match the digits found so far); rows above it stay, and the first
-// few equal to it.  Then each warp counts its own stretch of the rows, the counts
-// are summed over the warps, and each warp writes its kept rows in order.
-__global__ void __launch_bounds__(kSelectThreads) k_select(EvictArgs a) {
-    __shared__ int counts[256];
+// CTA = (sequence, head).  The rows between the sinks and the recent ones compete for the
+// rest of the budget: the value of the last one kept is found digit by digit, 11, 11 and 10
+// bits of the weights' order: counts of a digit among the rows that match the digits found
+// so far, and the highest digit that has the wanted row.  (The first 11 bits are sign, exponent and two
+// bits of the fraction, so that weights of all sizes fall on many counters; a warp whose rows
+// all fall on one counts them at once.)  Rows above that value stay, and the first few equal
+// to it.  Then each warp counts its own stretch of the rows, and writes its kept rows in order
+// behind those of the warps before it.
+__global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant__ EvictArgs a) {
+    __shared__ int counts[kBins];
     __shared__ int above[kSelectWarps], equal[kSelectWarps];
-    __shared__ uint32_t s_prefix;
+    __shared__ uint32_t s_digit;
     __shared__ int s_need;
     const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = sequence_rows(a.lengths, a.length_stride, s, a.capacity);
     const float *w = a.weights + s * a.w_batch + h * a.w_head;
     int *kept = a.kept + s * a.kept_batch + h * a.kept_head;
@@ -117,26 +120,64 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(EvictArgs a) {
     int ties = n;
     if (n > a.budget) {
         int need = a.budget - first - (n - last);  // rows to keep among first .. last - 1
-        uint32_t prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelectThreads) counts[i] = 0;
+        for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+            const int bits = shift ? 11 : 10, bins = 1 << bits;
+            for (int i = tid; i < bins; i += kSelectThreads) counts[i] = 0;
             __syncthreads();
-            for (int t = first + tid; t < last; t += kSelectThreads) {
-                const uint32_t key = rank_key(__ldg(w + t));
-                if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&counts[(key >> shift) & 255], 1);
+#pragma unroll 4
+            for (int t0 = first + warp * 32; t0 < last; t0 += kSelectThreads) {
+                const int t = t0 + lane;
+                const uint32_t key = t < last ? rank_key(__ldg(w + t)) : 0;
+                const bool counted = t < last && (shift == 21 || key >> (shift + bits) == cut);
+                const uint32_t digit = key >> shift & (bins - 1);
+                const uint32_t all = __ballot_sync(0xffffffffu, counted);
+                if (!all) continue;
+                const uint32_t one = __shfl_sync(0xffffffffu, digit, __ffs(all) - 1);
+                if (__all_sync(0xffffffffu, !counted || digit == one)) {
+                    if (lane == 0) atomicAdd(&counts[one], __popc(all));
+                } else if (counted) {
+                    atomicAdd(&counts[digit], 1);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                int left = need, digit = 255;
-                while (digit > 0 && counts[digit] < left) left -= counts[digit--];
-                s_prefix = prefix << 8 | static_cast<uint32_t>(digit);
-                s_need = left;
+            // each warp's bins summed, then the warp that has the row looks into its own
+            const int mine = bins / kSelectWarps, base = warp * mine;  // 64 or 32 bins
+            const int low = counts[base + lane], high = mine == 64 ? counts[base + 32 + lane] : 0;
+            const int sum = __reduce_add_sync(0xffffffffu, low + high);
+            if (lane == 0) above[warp] = sum;
+            __syncthreads();
+            const int over = __reduce_add_sync(0xffffffffu, lane > warp ? above[lane] : 0);  // rows of higher warps' bins
+            if (over < need && over + sum >= need) {
+                int left = need - over;
+                auto find = [&](int count, int at) {  // in 32 bins from the highest: the one that has the row
+                    int from = count;  // rows in this bin and the higher ones
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int up = __shfl_down_sync(0xffffffffu, from, o);
+                        if (lane + o < 32) from += up;
+                    }
+                    const uint32_t reach = __ballot_sync(0xffffffffu, from >= left);
+                    if (!reach) {
+                        left -= __shfl_sync(0xffffffffu, from, 0);
+                        return false;
+                    }
+                    const int bin = 31 - __clz(reach);
+                    if (lane == bin) {
+                        s_digit = at + bin;
+                        s_need = left - (from - count);
+                    }
+                    return true;
+                };
+                if (mine == 32 || !find(high, base + 32)) find(low, base);
+            }
+            if (need == 0 && tid == 0) {  // nothing to keep: above all
+                s_digit = bins - 1;
+                s_need = 0;
             }
             __syncthreads();
-            prefix = s_prefix;
+            cut = cut << bits | s_digit;
             need = s_need;
         }
-        cut = prefix;
         ties = need;
     }
     // 0: dropped, 1: kept, 2: equal to the cut
@@ -147,28 +188,31 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(EvictArgs a) {
         return key > cut ? 1 : key == cut ? 2 : 0;
     };
     const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) & ~31, lo = warp * stretch;
+    const int hi = min(lo + stretch, n);
     int kept_here = 0, equal_here = 0;
-    for (int t = lo + lane; t < lo + stretch && t - lane < n; t += 32) {
-        const int st = state(t);
-        kept_here += __popc(__ballot_sync(0xffffffffu, st == 1));
-        equal_here += __popc(__ballot_sync(0xffffffffu, st == 2));
+#pragma unroll 4
+    for (int t0 = lo; t0 < hi; t0 += 32) {
+        const int st = state(t0 + lane);
+        kept_here += st == 1;
+        equal_here += st == 2;
     }
+    kept_here = __reduce_add_sync(0xffffffffu, kept_here);
+    equal_here = __reduce_add_sync(0xffffffffu, equal_here);
+    __syncthreads();  // above[] of the last digit has been read
     if (lane == 0) {
         above[warp] = kept_here;
         equal[warp] = equal_here;
     }
     __syncthreads();
-    int kept_before = 0, equal_before = 0;
-    for (int i = 0; i < warp; ++i) {
-        kept_before += above[i];
-        equal_before += equal[i];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    for (int t = lo + lane; t < lo + stretch && t - lane < n; t += 32) {
-        const int st = state(t);
+    int kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
+    int equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
+    const uint32_t before = (1u << lane) - 1;
+#pragma unroll 4
+    for (int t0 = lo; t0 < hi; t0 += 32) {
+        const int t = t0 + lane, st = state(t);
         const uint32_t m1 = __ballot_sync(0xffffffffu, st == 1), m2 = __ballot_sync(0xffffffffu, st == 2);
-        const int eq = equal_before + __popc(m2 & below);
-        const int at = kept_before + __popc(m1 & below) + min(eq, ties);
+        const int eq = equal_before + __popc(m2 & before);
+        const int at = kept_before + __popc(m1 & before) + min(eq, ties);
         if ((st == 1 || (st == 2 && eq < ties)) && at < a.budget) {
             kept[at] = t;
             if (at < a.target_rows) nw[at] = __ldg(w + t);
@@ -180,26 +224,55 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(EvictArgs a) {
     for (int i = total + tid; i < a.target_rows; i += kSelectThreads) nw[i] = 0.f;
 }
 
-// Kept rows to their target pages: a thread per (row, head, piece), the head inside the row.
-__global__ void __launch_bounds__(256) k_copy_kept(EvictArgs a) {
-    const int s = blockIdx.y, per_row = a.heads * a.pieces;
+// Kept rows to their target pages: a warp takes 32 rows of a head, a lane looks up one row's two
+// places, and all copy the rows piece by piece, four loads of each pool in flight a lane.
+constexpr int kCopyWarps = 4;
+__global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_constant__ EvictArgs a) {
+    const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % 32;
+    const int at = (blockIdx.x * kCopyWarps + threadIdx.x / 32) * 32 + lane;
     const int total = min(sequence_rows(a.lengths, a.length_stride, s, a.capacity), min(a.budget, a.target_rows));
-    const int64_t all = static_cast<int64_t>(total) * per_row;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < all;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int at = static_cast<int>(i / per_row), rest = static_cast<int>(i - static_cast<int64_t>(at) * per_row);
-        const int h = rest / a.pieces, c = (rest - h * a.pieces) * 16;
-        const int64_t to_k = a.to.row(s, at, a.tk.page, a.tk.row), to_v = a.to.row(s, at, a.tv.page, a.tv.row);
-        if (to_k < 0) continue;
-        const int t = __ldg(a.kept + s * a.kept_batch + h * a.kept_head + at);
-        const int64_t k = a.from.row(s, t, a.k.page, a.k.row), v = a.from.row(s, t, a.v.page, a.v.row);
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (k >= 0) {
-            x = *reinterpret_cast<const uint4 *>(a.k.base + k + h * a.k.head + c);
-            y = *reinterpret_cast<const uint4 *>(a.v.base + v + h * a.v.head + c);
+    if (at - lane >= total) return;
+    // the target's page is found before the selection is waited for
+    int64_t to_k = -1, to_v = -1, k = -1, v = -1;
+    if (at < total) {
+        to_k = a.to.row(s, at, a.tk.page, a.tk.row);
+        to_v = a.to.row(s, at, a.tv.page, a.tv.row);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (at < total) {
+        const int t = __ldcg(a.kept + s * a.kept_batch + h * a.kept_head + at);
+        k = a.from.row(s, t, a.k.page, a.k.row);
+        v = a.from.row(s, t, a.v.page, a.v.row);
+    }
+    const char *kb = a.k.base + h * a.k.head, *vb = a.v.base + h * a.v.head;
+    char *tk = a.tk.base + h * a.tk.head, *tv = a.tv.base + h * a.tv.head;
+    const int n = 32 * a.pieces;
+    constexpr int kFlight = 4;
+    for (int e0 = lane; e0 < n; e0 += 32 * kFlight) {
+        uint4 x[kFlight], y[kFlight];
+        int64_t tks[kFlight], tvs[kFlight];
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i) {
+            const int e = min(e0 + 32 * i, n - 1), r = e / a.pieces, c = (e - r * a.pieces) * 16;
+            const int64_t from_k = __shfl_sync(0xffffffffu, k, r), from_v = __shfl_sync(0xffffffffu, v, r);
+            tks[i] = __shfl_sync(0xffffffffu, to_k, r);
+            tvs[i] = __shfl_sync(0xffffffffu, to_v, r);
+            if (e0 + 32 * i >= n) tks[i] = -1;
+            x[i] = y[i] = make_uint4(0, 0, 0, 0);
+            if (from_k >= 0 && tks[i] >= 0) {
+                x[i] = __ldcs(reinterpret_cast<const uint4 *>(kb + from_k + c));
+                y[i] = __ldcs(reinterpret_cast<const uint4 *>(vb + from_v + c));
+            }
+            tks[i] += c;
+            tvs[i] += c;
+            if (tks[i] < c) tks[i] = -1;
         }
-        *reinterpret_cast<uint4 *>(a.tk.base + to_k + h * a.tk.head + c) = x;
-        *reinterpret_cast<uint4 *>(a.tv.base + to_v + h * a.tv.head + c) = y;
+#pragma unroll
+        for (int i = 0; i < kFlight; ++i)
+            if (tks[i] >= 0) {
+                *reinterpret_cast<uint4 *>(tk + tks[i]) = x[i];
+                *reinterpret_cast<uint4 *>(tv + tvs[i]) = y[i];
+            }
     }
 }
 
@@ -293,7 +366,7 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     MR_CHECK(check_apart(weights, "weights", new_weights, "new_weights"));
     MR_CHECK(check_apart(lengths, "lengths", new_lengths, "new_lengths"));
     MR_REQUIRE(batch <= 65535, "more than 65535 sequences");
-    MR_REQUIRE(batch * heads <= INT32_MAX, "too many heads");
+    MR_REQUIRE(heads <= 65535 && batch * heads <= INT32_MAX, "too many heads");
     MR_REQUIRE(ctx, "ctx is NULL");
     if (!batch) return MR_OK;
     DeviceGuard guard(ctx->device);
@@ -327,11 +400,10 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
     k_select<<<a.batch * a.heads, kSelectThreads, 0, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
-    const int64_t work = std::min<int64_t>(budget, capacity) * a.heads * a.pieces;
-    if (work) {
-        const int blocks = static_cast<int>(std::min<int64_t>((work - 1) / 256 + 1, 16 * ctx->sm_count));
-        k_copy_kept<<<dim3(blocks, a.batch), 256, 0, ctx->stream>>>(a);
-        MR_CUDA_TRY(cudaGetLastError());
+    const int64_t rows = std::min<int64_t>(budget, capacity);
+    if (rows) {
+        const dim3 grid(static_cast<unsigned>((rows - 1) / (32 * kCopyWarps) + 1), a.heads, a.batch);
+        MR_CHECK(launch_early(ctx, grid, dim3(kCopyWarps * 32), k_copy_kept, a));
     }
     return MR_OK;
 }

@@ -668,7 +668,7 @@ __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk
 template <int H>
 __device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
                                             int to, int first, int step, const float (&lse)[H]) {
-    constexpr int kRows = 4;  // in flight
+    constexpr int kRows = 8;  // in flight
     float *weights = a.weights + walk.s * a.w_batch + kh * a.w_head;
     for (int i0 = from + first; i0 < to; i0 += step * kRows) {
         float sum[kRows], was[kRows];
@@ -822,13 +822,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
 // Joins the units that were cut: the warps whose stretch starts inside a unit
 // share its columns, four at a time.  With weights, every warp then adds up its
 // own stretch's rows.
-constexpr int kMaxShares = 2432;  // weights of partials a warp keeps: of all heads for few, of two heads for all there can be
+//
+// A cut unit has as many partials as warps had a part of it, n; n - 1 warps share its
+// heads x DP / 4 columns of four, at most 256.  So a warp that has columns of more than one
+// head meets at most 257 partials, and with eight heads at most two: kPairs maxima and sums
+// of (head, partial) hold for all there can be.
+constexpr int kPairs = 1216;
 
 template <typename T, typename M>
 __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ PagedArgs a) {
     constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
     constexpr int64_t kPart = H * (DP + 2);
-    __shared__ float shares[kWarps][kMaxShares];
+    __shared__ float2 pairs[kWarps][kPairs];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, worker = blockIdx.x * kWarps + warp;
     Plan<STEP> plan;
     plan.init(a);
@@ -845,6 +850,91 @@ __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Paged
             return at + (b * 2 + (b == b0 ? slot0 : 0)) * kPart;
         }
     };
+    const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
+    if (first < walk.x) {
+        const int b0 = plan.worker_of(first), b1 = plan.worker_of(first + walk.steps - 1), n = b1 - b0 + 1;
+        const Parts part = {a.partial, b0, plan.start(b0) >= first ? 0 : 1};
+        const int kh = cut / a.blocks, h0 = cut % a.blocks * H, heads = min(H, a.group - h0);
+        const int columns = heads * (DP / 4), me = worker - b0 - 1;
+        const int c0 = columns * me / (n - 1), c1 = columns * (me + 1) / (n - 1);
+        if (c0 < c1) {
+            const int ha = c0 / (DP / 4), hb = (c1 - 1) / (DP / 4) + 1;  // its heads
+            int wide = 1;  // lanes side by side over the columns, the rest over the partials
+            while (wide < 32 && wide < c1 - c0) wide <<= 1;
+            const int step = 32 / wide;
+            constexpr int kFlight = 8;
+            auto value = [&](int c, int b) {
+                return __ldcg(reinterpret_cast<const float4 *>(part(b0 + b) + 4 * c));
+            };
+            float4 v[kFlight];  // the first columns' values are under way while the factors are worked out
+            auto load = [&](int c) {
+#pragma unroll
+                for (int i = 0; i < kFlight; ++i) {
+                    const int b = lane / wide + i * step;
+                    v[i] = b < n ? value(c, b) : float4{};
+                }
+            };
+            load(min(c0 + lane % wide, c1 - 1));
+            float2 *pair = pairs[warp];  // [head][partial]: its maximum and sum, then the factor of its values
+            const int count = (hb - ha) * n;
+#pragma unroll 8
+            for (int i = lane; i < count; i += 32) {
+                const int h = i / n, b = i - h * n;
+                const float *p = part(b0 + b) + H * DP + ha + h;
+                pair[i] = make_float2(__ldcg(p), __ldcg(p + H));
+            }
+            __syncwarp();
+            for (int h = 0; h < hb - ha; ++h) {
+                float top = -INFINITY, sum = 0.f;
+                for (int b = lane; b < n; b += 32) top = fmaxf(top, pair[h * n + b].x);
+                top = warp_max(top);
+                const float ref = top == -INFINITY ? 0.f : top;
+                for (int b = lane; b < n; b += 32) {
+                    float2 x = pair[h * n + b];
+                    x.x = ex2(x.x - ref);
+                    sum = fmaf(x.x, x.y, sum);
+                    pair[h * n + b].x = x.x;
+                }
+                sum = warp_sum(sum);
+                const float f = sum != 0.f ? 1.f / sum : 0.f;
+                for (int b = lane; b < n; b += 32) pair[h * n + b].x *= f;
+            }
+            __syncwarp();
+            for (int base = c0; base < c1; base += wide) {
+                const int c = min(base + lane % wide, c1 - 1), h = c / (DP / 4), j = c % (DP / 4) * 4;
+                const float2 *mine = pair + (h - ha) * n;
+                if (base != c0) load(c);
+                float4 x = {};
+                auto mix = [&](float f, const float4 &y) {
+                    x.x = fmaf(f, y.x, x.x);
+                    x.y = fmaf(f, y.y, x.y);
+                    x.z = fmaf(f, y.z, x.z);
+                    x.w = fmaf(f, y.w, x.w);
+                };
+#pragma unroll
+                for (int i = 0; i < kFlight; ++i) {
+                    const int b = lane / wide + i * step;
+                    if (b < n) mix(mine[b].x, v[i]);
+                }
+#pragma unroll 4
+                for (int b = lane / wide + kFlight * step; b < n; b += step) mix(mine[b].x, value(c, b));
+                for (int w = 16; w >= wide; w >>= 1) {
+                    x.x += __shfl_xor_sync(0xffffffffu, x.x, w);
+                    x.y += __shfl_xor_sync(0xffffffffu, x.y, w);
+                    x.z += __shfl_xor_sync(0xffffffffu, x.z, w);
+                    x.w += __shfl_xor_sync(0xffffffffu, x.w, w);
+                }
+                if (lane < wide && base + lane < c1 && j < a.dim) {
+                    T *out = reinterpret_cast<T *>(a.out + walk.s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j;
+                    narrow(x.x, out);
+                    narrow(x.y, out + 1);
+                    narrow(x.z, out + 2);
+                    narrow(x.w, out + 3);
+                }
+            }
+        }
+    }
+    if (!a.weights) return;
     // A cut unit's softmax over its partials: each head's maximum and sum, in every lane.
     auto softmax_of = [&](const Parts &part, int b1, float (&top)[H], float (&sum)[H]) {
 #pragma unroll
@@ -875,57 +965,6 @@ __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Paged
             top[h] = t;
         }
     };
-    const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
-    if (first < walk.x) {
-        const int b0 = plan.worker_of(first), b1 = plan.worker_of(first + walk.steps - 1), n = b1 - b0 + 1;
-        const Parts part = {a.partial, b0, plan.start(b0) >= first ? 0 : 1};
-        const int kh = cut / a.blocks, h0 = cut % a.blocks * H, heads = min(H, a.group - h0);
-        const int columns = heads * (DP / 4), me = worker - b0 - 1;
-        const int c0 = columns * me / (n - 1), c1 = columns * (me + 1) / (n - 1);
-        if (c0 < c1) {
-            const int ha = c0 / (DP / 4), hb = (c1 - 1) / (DP / 4) + 1;  // its heads
-            float top[H], sum[H];
-            softmax_of(part, b1, top, sum);
-            float *share = shares[warp];  // [head of its][partial]: the factor of a partial's values
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-                if (h >= ha && h < hb) {
-                    const float ref = top[h] == -INFINITY ? 0.f : top[h], f = sum[h] != 0.f ? 1.f / sum[h] : 0.f;
-                    for (int b = lane; b < n; b += 32)
-                        share[(h - ha) * n + b] = ex2(__ldcg(part(b0 + b) + H * DP + h) - ref) * f;
-                }
-            __syncwarp();
-            int wide = 1;  // lanes side by side over the columns, the rest over the partials
-            while (wide < 32 && wide < c1 - c0) wide <<= 1;
-            for (int base = c0; base < c1; base += wide) {
-                const int c = min(base + lane % wide, c1 - 1), h = c / (DP / 4), j = c % (DP / 4) * 4;
-                const float *mine = share + (h - ha) * n;
-                float4 x = {};
-#pragma unroll 8
-                for (int b = lane / wide; b < n; b += 32 / wide) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(b0 + b) + h * DP + j));
-                    x.x = fmaf(mine[b], v.x, x.x);
-                    x.y = fmaf(mine[b], v.y, x.y);
-                    x.z = fmaf(mine[b], v.z, x.z);
-                    x.w = fmaf(mine[b], v.w, x.w);
-                }
-                for (int w = 16; w >= wide; w >>= 1) {
-                    x.x += __shfl_xor_sync(0xffffffffu, x.x, w);
-                    x.y += __shfl_xor_sync(0xffffffffu, x.y, w);
-                    x.z += __shfl_xor_sync(0xffffffffu, x.z, w);
-                    x.w += __shfl_xor_sync(0xffffffffu, x.w, w);
-                }
-                if (lane < wide && base + lane < c1 && j < a.dim) {
-                    T *out = reinterpret_cast<T *>(a.out + walk.s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j;
-                    narrow(x.x, out);
-                    narrow(x.y, out + 1);
-                    narrow(x.z, out + 2);
-                    narrow(x.w, out + 3);
-                }
-            }
-        }
-    }
-    if (!a.weights) return;
     while (walk.next(a, plan)) {
         if (walk.u % a.blocks) continue;  // the group's first block of heads adds up for all of them
         const int from = walk.t0 * STEP, to = min(walk.t1 * STEP, walk.seen.rows);
@@ -978,16 +1017,7 @@ int launch(mr_context *ctx, PagedArgs &a) {
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings));
     k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(kThreads);
-    config.stream = ctx->stream;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    MR_CUDA_TRY(cudaLaunchKernelEx(&config, k_join<T, M>, a));
+    MR_CHECK((launch_early(ctx, dim3(grid), dim3(kThreads), k_join<T, M>, a)));
     return MR_OK;
 }
 
