@@ -54,10 +54,12 @@ struct PagedArgs {
     int batch, kv_heads, group, blocks, dim, capacity, window, sinks;  // blocks: blocks of query heads a group has
     float scale;     // times log2(e): scores are kept as powers of two
     // scratch
-    float *partial;  // [warp][2][kHeads * DP values, kHeads maxima, kHeads sums]
+    float *partial;  // [warp][2][kHeads * DP values]
+    float2 *sums;    // [2][kHeads][warps]: their maxima and sums, side by side as k_join reads them
     float *lse;      // [unit][kHeads] of whole units, with weights: log2 of the softmax sum, the maximum in it
     float *scores;   // [unit][seen rows][heads2], with weights
     int64_t seen_max;
+    int warps;       // of k_paged
     int heads2;      // query heads of a block, rounded up to even
 };
 
@@ -82,7 +84,8 @@ __device__ __forceinline__ Seen seen_of(const PagedArgs &a, int s) {
 template <int STEP>
 struct Plan {
     int total, units;  // units of a sequence
-    int workers;       // warps that get steps: at most one each
+    int workers;       // warps that get steps
+    int each, more;    // steps of a worker: each + 1 for the first `more`, then each
     static __device__ __forceinline__ int steps_of(const Seen &seen) { return (seen.rows + STEP - 1) / STEP; }
     __device__ void init(const PagedArgs &a) {
         const int lane = threadIdx.x % 32;
@@ -92,14 +95,15 @@ struct Plan {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         total = sum * units;
-        workers = min(total, static_cast<int>(gridDim.x) * kWarps);
+        workers = min(total, a.warps);
+        each = total / max(workers, 1);
+        more = total - each * workers;
     }
-    // First step of worker b <= workers, and the worker that has step x: the last b with b total / workers < x + 1.
-    __device__ __forceinline__ int start(int b) const {
-        return static_cast<int>(static_cast<int64_t>(b) * total / workers);
-    }
+    // First step of worker b <= workers, and the worker that has step x.
+    __device__ __forceinline__ int start(int b) const { return b * each + min(b, more); }
     __device__ __forceinline__ int worker_of(int x) const {
-        return static_cast<int>((static_cast<int64_t>(x + 1) * workers - 1) / total);
+        const int longer = more * (each + 1);
+        return x < longer ? x / (each + 1) : more + (x - longer) / each;
     }
     // The sequence of step x (x < total) and its first step.
     __device__ void find(const PagedArgs &a, int x, int &s, int &base) const {
@@ -414,17 +418,15 @@ struct Math16 {
             if (h < heads && dim < a.dim) *reinterpret_cast<uint32_t *>(out + h * a.o_head + dim * 2) = pack2(x, y, T());
         });
     }
-    __device__ __forceinline__ void put_partial(float *to, int heads) const {
+    // values [head][DP], and the maxima and sums `stride` apart
+    __device__ __forceinline__ void put_partial(float *to, float2 *sums, int64_t stride, int heads) const {
         const int lane = threadIdx.x % 32;
         each(1.f, 1.f, [&](int h, int dim, float x, float y) {
             if (h < heads) *reinterpret_cast<float2 *>(to + h * DP + dim) = make_float2(x, y);
         });
         if (lane < 4)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                to[kHeads * DP + 2 * lane + e] = m[e];
-                to[kHeads * DP + kHeads + 2 * lane + e] = l[e];
-            }
+            for (int e = 0; e < 2; ++e) sums[(2 * lane + e) * stride] = make_float2(m[e], l[e]);
     }
     __device__ __forceinline__ void put_lse(float *lse) const {
         const int lane = threadIdx.x % 32;
@@ -544,15 +546,12 @@ struct Math32 {
                     make_float4(o[h].x * fh, o[h].y * fh, o[h].z * fh, o[h].w * fh);
         }
     }
-    __device__ __forceinline__ void put_partial(float *to, int heads) const {
+    __device__ __forceinline__ void put_partial(float *to, float2 *sums, int64_t stride, int heads) const {
         const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int h = 0; h < 4; ++h)
             if (h < heads && lane < kLanes) *reinterpret_cast<float4 *>(to + h * DP + 4 * lane) = o[h];
-        if (lane < 4) {
-            to[kHeads * DP + lane] = m;
-            to[kHeads * DP + kHeads + lane] = l;
-        }
+        if (lane < 4) sums[lane * stride] = make_float2(m, l);
     }
     __device__ __forceinline__ void put_lse(float *lse) const {
         if (threadIdx.x % 32 < 4) lse[threadIdx.x % 32] = log_sum(m, l);
@@ -624,8 +623,8 @@ struct Feed {
 // meets the second part of a weight as 0 x inf or inf - inf on the tensor cores.
 template <typename T, typename M>
 __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk, const char *q, char *out, float *partial,
-                                           int heads) {
-    constexpr int H = M::kHeads, DP = M::DP;
+                                           float2 *sums, int64_t stride, int heads) {
+    constexpr int DP = M::DP;
     const int lane = threadIdx.x % 32, kh = walk.u / a.blocks;
     const int from = walk.t0 * M::STEP, to = min(walk.t1 * M::STEP, walk.seen.rows);
     auto load = [&](const char *src, float (&x)[4]) {
@@ -657,10 +656,7 @@ __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk
             if (out && d < a.dim) narrow(l != 0.f ? o[j] / l : 0.f, reinterpret_cast<T *>(out + h * a.o_head) + d);
             if (partial && d < DP) partial[h * DP + d] = o[j];
         }
-        if (partial && lane == 0) {
-            partial[H * DP + h] = m;
-            partial[H * DP + H + h] = l;
-        }
+        if (partial && lane == 0) sums[h * stride] = make_float2(m, l);
     }
 }
 
@@ -668,7 +664,7 @@ __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk
 template <int H>
 __device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
                                             int to, int first, int step, const float (&lse)[H]) {
-    constexpr int kRows = 8;  // in flight
+    constexpr int kRows = 4;  // in flight
     float *weights = a.weights + walk.s * a.w_batch + kh * a.w_head;
     for (int i0 = from + first; i0 < to; i0 += step * kRows) {
         float sum[kRows], was[kRows];
@@ -766,10 +762,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged(const __grid_con
                        [&](M &math, const Piece &piece, const char *q, int64_t unit, int heads, int kh, int h0) {
         const bool whole = piece.t0 == 0 && piece.t1 == piece.steps;
         char *out = whole ? a.out + piece.s * a.o_batch + (kh * a.group + h0) * a.o_head : nullptr;
-        float *partial = whole ? nullptr : a.partial + (worker * 2 + part) * static_cast<int64_t>(H * (DP + 2));
-        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, out, partial, heads);
+        float *partial = whole ? nullptr : a.partial + (worker * 2 + part) * static_cast<int64_t>(H * DP);
+        const int64_t warps = a.warps;
+        float2 *sums = a.sums + part * H * warps + worker;
+        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, out, partial, sums, warps, heads);
         else if (whole) math.put_out(a, out, heads);
-        else math.put_partial(partial, heads);
+        else math.put_partial(partial, sums, warps, heads);
         if (whole && a.lse) math.put_lse(a.lse + unit * H);
         part = 1;
     });
@@ -786,8 +784,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
     walk.unit = blockIdx.x;
     work_through<T, M>(a, shared_address(smem + warp * M::R::kWarpBytes), NextQuarter<STEP>{walk, a},
                        [&](M &math, const Piece &piece, const char *q, int64_t unit, int heads, int kh, int h0) {
-        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, nullptr, parts + warp * kPart, heads);
-        else math.put_partial(parts + warp * kPart, heads);
+        float *mine = parts + warp * kPart;
+        float2 *sums = reinterpret_cast<float2 *>(mine + H * DP);
+        if (!math.finish()) piece_by_rows<T, M>(a, piece, q, nullptr, mine, sums, 1, heads);
+        else math.put_partial(mine, sums, 1, heads);
         __syncthreads();
         char *out = a.out + piece.s * a.o_batch + (kh * a.group + h0) * a.o_head;
         for (int e = tid; e < heads * DP; e += kThreads) {
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float *p = parts + w * kPart;
-                all.add(p[H * DP + h], p[H * DP + H + h], p[e]);
+                all.add(p[H * DP + 2 * h], p[H * DP + 2 * h + 1], p[e]);
             }
             if (j < a.dim)
                 narrow(all.sum != 0.f ? all.x / all.sum : 0.f, reinterpret_cast<T *>(out + h * a.o_head) + j);
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float *p = parts + w * kPart + H * DP;
-                    if (h < heads) all.add(p[h], p[H + h], 0.f);
+                    if (h < heads) all.add(p[2 * h], p[2 * h + 1], 0.f);
                 }
                 lse[h] = log_sum(all.top, all.sum);
             }
@@ -822,19 +822,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
 // Joins the units that were cut: the warps whose stretch starts inside a unit
 // share its columns, four at a time.  With weights, every warp then adds up its
 // own stretch's rows.
-//
-// A cut unit has as many partials as warps had a part of it, n; n - 1 warps share its
-// heads x DP / 4 columns of four, at most 256.  So a warp that has columns of more than one
-// head meets at most 257 partials, and with eight heads at most two: kPairs maxima and sums
-// of (head, partial) hold for all there can be.
-constexpr int kPairs = 1216;
+constexpr int kJoin = 2;  // warps for each of k_paged's, to hide the latency of the little that each reads
 
 template <typename T, typename M>
-__global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ PagedArgs a) {
     constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
-    constexpr int64_t kPart = H * (DP + 2);
-    __shared__ float2 pairs[kWarps][kPairs];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, worker = blockIdx.x * kWarps + warp;
+    constexpr int64_t kPart = H * DP;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int id = blockIdx.x * kWarps + warp, worker = id / kJoin, share = id % kJoin;
     Plan<STEP> plan;
     plan.init(a);
     Walk walk = {};
@@ -850,81 +845,67 @@ __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Paged
             return at + (b * 2 + (b == b0 ? slot0 : 0)) * kPart;
         }
     };
+    const int64_t warps = a.warps;
+    auto sums_of = [&](const Parts &part, int b, int h) {
+        return __ldcg(a.sums + ((b == part.b0 ? part.slot0 : 0) * H + h) * warps + b);
+    };
     const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
     if (first < walk.x) {
         const int b0 = plan.worker_of(first), b1 = plan.worker_of(first + walk.steps - 1), n = b1 - b0 + 1;
         const Parts part = {a.partial, b0, plan.start(b0) >= first ? 0 : 1};
         const int kh = cut / a.blocks, h0 = cut % a.blocks * H, heads = min(H, a.group - h0);
-        const int columns = heads * (DP / 4), me = worker - b0 - 1;
-        const int c0 = columns * me / (n - 1), c1 = columns * (me + 1) / (n - 1);
-        if (c0 < c1) {
-            const int ha = c0 / (DP / 4), hb = (c1 - 1) / (DP / 4) + 1;  // its heads
+        const int columns = heads * (DP / 4), sharers = (n - 1) * kJoin, me = (worker - b0 - 1) * kJoin + share;
+        const int c0 = columns * me / sharers, c1 = columns * (me + 1) / sharers;
+        // head by head of its columns
+        for (int h = c0 / (DP / 4); h * (DP / 4) < c1; ++h) {
+            const int lo = max(c0, h * (DP / 4)), hi = min(c1, (h + 1) * (DP / 4));
             int wide = 1;  // lanes side by side over the columns, the rest over the partials
-            while (wide < 32 && wide < c1 - c0) wide <<= 1;
+            while (wide < 32 && wide < hi - lo) wide <<= 1;
             const int step = 32 / wide;
-            constexpr int kFlight = 8;
-            auto value = [&](int c, int b) {
-                return __ldcg(reinterpret_cast<const float4 *>(part(b0 + b) + 4 * c));
+            constexpr int kFlight = 5;
+            float4 v[kFlight];  // the first columns' values are under way while the softmax is worked out
+            float top_of[kFlight];
+            auto load = [&](int c, int i, int b) {
+                v[i] = b < n ? __ldcg(reinterpret_cast<const float4 *>(part(b0 + b) + 4 * c)) : float4{};
+                top_of[i] = b < n ? sums_of(part, b0 + b, h).x : -INFINITY;
             };
-            float4 v[kFlight];  // the first columns' values are under way while the factors are worked out
-            auto load = [&](int c) {
 #pragma unroll
-                for (int i = 0; i < kFlight; ++i) {
-                    const int b = lane / wide + i * step;
-                    v[i] = b < n ? value(c, b) : float4{};
-                }
-            };
-            load(min(c0 + lane % wide, c1 - 1));
-            float2 *pair = pairs[warp];  // [head][partial]: its maximum and sum, then the factor of its values
-            const int count = (hb - ha) * n;
-#pragma unroll 8
-            for (int i = lane; i < count; i += 32) {
-                const int h = i / n, b = i - h * n;
-                const float *p = part(b0 + b) + H * DP + ha + h;
-                pair[i] = make_float2(__ldcg(p), __ldcg(p + H));
+            for (int i = 0; i < kFlight; ++i) load(min(lo + lane % wide, hi - 1), i, lane / wide + i * step);
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll 5
+            for (int b = lane; b < n; b += 32) {
+                const float2 x = sums_of(part, b0 + b, h);
+                const float t = fmaxf(top, x.x), ref = t == -INFINITY ? 0.f : t;
+                sum = fmaf(sum, ex2(top - ref), x.y * ex2(x.x - ref));
+                top = t;
             }
-            __syncwarp();
-            for (int h = 0; h < hb - ha; ++h) {
-                float top = -INFINITY, sum = 0.f;
-                for (int b = lane; b < n; b += 32) top = fmaxf(top, pair[h * n + b].x);
-                top = warp_max(top);
-                const float ref = top == -INFINITY ? 0.f : top;
-                for (int b = lane; b < n; b += 32) {
-                    float2 x = pair[h * n + b];
-                    x.x = ex2(x.x - ref);
-                    sum = fmaf(x.x, x.y, sum);
-                    pair[h * n + b].x = x.x;
-                }
-                sum = warp_sum(sum);
-                const float f = sum != 0.f ? 1.f / sum : 0.f;
-                for (int b = lane; b < n; b += 32) pair[h * n + b].x *= f;
-            }
-            __syncwarp();
-            for (int base = c0; base < c1; base += wide) {
-                const int c = min(base + lane % wide, c1 - 1), h = c / (DP / 4), j = c % (DP / 4) * 4;
-                const float2 *mine = pair + (h - ha) * n;
-                if (base != c0) load(c);
+            const float most = warp_max(top), ref = most == -INFINITY ? 0.f : most;
+            sum = warp_sum(sum * ex2(top - ref));
+            const float f = sum != 0.f ? 1.f / sum : 0.f;
+            for (int base = lo; base < hi; base += wide) {
+                const int c = min(base + lane % wide, hi - 1);
                 float4 x = {};
-                auto mix = [&](float f, const float4 &y) {
-                    x.x = fmaf(f, y.x, x.x);
-                    x.y = fmaf(f, y.y, x.y);
-                    x.z = fmaf(f, y.z, x.z);
-                    x.w = fmaf(f, y.w, x.w);
-                };
+                for (int b = 0; b < n; b += kFlight * step) {
+                    if (base != lo || b)
 #pragma unroll
-                for (int i = 0; i < kFlight; ++i) {
-                    const int b = lane / wide + i * step;
-                    if (b < n) mix(mine[b].x, v[i]);
+                        for (int i = 0; i < kFlight; ++i) load(c, i, b + lane / wide + i * step);
+#pragma unroll
+                    for (int i = 0; i < kFlight; ++i) {
+                        const float w = ex2(top_of[i] - ref) * f;
+                        x.x = fmaf(w, v[i].x, x.x);
+                        x.y = fmaf(w, v[i].y, x.y);
+                        x.z = fmaf(w, v[i].z, x.z);
+                        x.w = fmaf(w, v[i].w, x.w);
+                    }
                 }
-#pragma unroll 4
-                for (int b = lane / wide + kFlight * step; b < n; b += step) mix(mine[b].x, value(c, b));
                 for (int w = 16; w >= wide; w >>= 1) {
                     x.x += __shfl_xor_sync(0xffffffffu, x.x, w);
                     x.y += __shfl_xor_sync(0xffffffffu, x.y, w);
                     x.z += __shfl_xor_sync(0xffffffffu, x.z, w);
                     x.w += __shfl_xor_sync(0xffffffffu, x.w, w);
                 }
-                if (lane < wide && base + lane < c1 && j < a.dim) {
+                const int j = c % (DP / 4) * 4;
+                if (lane < wide && base + lane < hi && j < a.dim) {
                     T *out = reinterpret_cast<T *>(a.out + walk.s * a.o_batch + (kh * a.group + h0 + h) * a.o_head) + j;
                     narrow(x.x, out);
                     narrow(x.y, out + 1);
@@ -944,17 +925,13 @@ __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Paged
         }
 #pragma unroll 2
         for (int b = part.b0 + lane; b <= b1; b += 32) {
-            float m[H], l[H];
-            const float *p = part(b) + H * DP;
+            float2 x[H];
 #pragma unroll
-            for (int h = 0; h < H; h += 4) {
-                *reinterpret_cast<float4 *>(m + h) = __ldcg(reinterpret_cast<const float4 *>(p + h));
-                *reinterpret_cast<float4 *>(l + h) = __ldcg(reinterpret_cast<const float4 *>(p + H + h));
-            }
+            for (int h = 0; h < H; ++h) x[h] = sums_of(part, b, h);
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const float t = fmaxf(top[h], m[h]), ref = t == -INFINITY ? 0.f : t;
-                sum[h] = fmaf(sum[h], ex2(top[h] - ref), l[h] * ex2(m[h] - ref));
+                const float t = fmaxf(top[h], x[h].x), ref = t == -INFINITY ? 0.f : t;
+                sum[h] = fmaf(sum[h], ex2(top[h] - ref), x[h].y * ex2(x[h].x - ref));
                 top[h] = t;
             }
         }
@@ -967,7 +944,8 @@ __global__ void __launch_bounds__(kThreads) k_join(const __grid_constant__ Paged
     };
     while (walk.next(a, plan)) {
         if (walk.u % a.blocks) continue;  // the group's first block of heads adds up for all of them
-        const int from = walk.t0 * STEP, to = min(walk.t1 * STEP, walk.seen.rows);
+        const int lo = walk.t0 * STEP, rows = min(walk.t1 * STEP, walk.seen.rows) - lo;
+        const int from = lo + rows * share / kJoin, to = lo + rows * (share + 1) / kJoin;
         for (int b = 0; b < a.blocks; ++b) {
             const int64_t unit = static_cast<int64_t>(walk.s) * plan.units + walk.u + b;
             const int start = walk.base + (walk.u + b) * walk.steps;
@@ -996,16 +974,21 @@ int launch(mr_context *ctx, PagedArgs &a) {
     const bool few = steps <= kFewSteps && (!a.weights || a.blocks == 1);
     const int64_t ctas = few ? units : (units * steps + kWarps - 1) / kWarps;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, kCtasPerSm * ctx->sm_count)));
-    const size_t partial = few ? 0 : sizeof(float) * 2 * kWarps * grid * H * (M::DP + 2);
+    a.warps = grid * kWarps;
+    const size_t partial = few ? 0 : sizeof(float) * 2 * kWarps * grid * H * M::DP;
+    const size_t sums = few ? 0 : sizeof(float2) * 2 * kWarps * grid * H;
     const size_t lse = a.weights && !few ? sizeof(float) * units * H : 0;
     const size_t scores = a.weights ? sizeof(float) * units * a.seen_max * a.heads2 : 0;
     auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
     Scratch scratch(ctx);
-    MR_CHECK(scratch.take(up(partial) + up(lse) + scores));
+    MR_CHECK(scratch.take(up(partial) + up(sums) + up(lse) + scores));
     char *base = static_cast<char *>(scratch.data);
     a.partial = reinterpret_cast<float *>(base);
-    a.lse = lse ? reinterpret_cast<float *>(base + up(partial)) : nullptr;
-    a.scores = scores ? reinterpret_cast<float *>(base + up(partial) + up(lse)) : nullptr;
+    base += up(partial);
+    a.sums = reinterpret_cast<float2 *>(base);
+    base += up(sums);
+    a.lse = lse ? reinterpret_cast<float *>(base) : nullptr;
+    a.scores = scores ? reinterpret_cast<float *>(base + up(lse)) : nullptr;
     constexpr int kRings = kWarps * M::R::kWarpBytes;
     if (few) {
         constexpr int kSmem = kRings + kWarps * H * (M::DP + 2) * 4;
@@ -1017,7 +1000,7 @@ int launch(mr_context *ctx, PagedArgs &a) {
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings));
     k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
-    MR_CHECK((launch_early(ctx, dim3(grid), dim3(kThreads), k_join<T, M>, a)));
+    MR_CHECK((launch_early(ctx, dim3(grid * kJoin), dim3(kThreads), k_join<T, M>, a)));
     return MR_OK;
 }
 
