@@ -143,4 +143,6 @@ def check(code, what=""):
 
 
 def call(name, *args):
-    check(getattr(library(), name)(*args), name)
+    code = getattr(_lib or library(), name)(*args)
+    if code != MR_OK:
+        check(code, name)

@@ -19,33 +19,35 @@ from .weights import float32_to_bf16_bits
 TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 3}   # enum mr_dtype
 _ITEM = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4}
 _CODES = {}    # a dtype object -> its code, as its name says
-_PACK = {n: struct.Struct("<Qii" + f"{n}q{4 - n}q{n}q{4 - n}q").pack for n in range(1, 5)}   # mr_array
-_PAD = {n: (0,) * (4 - n) for n in range(1, 5)}
-
-
-def _code(dtype):
-    code = _CODES.get(dtype)
-    if code is None:
-        code = TYPES.get(str(dtype).rsplit(".", 1)[-1])
-        if code is None:
-            raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16 or int32 is needed")
-        _CODES[dtype] = code
-    return code
+_PACK = {n: struct.Struct(f"<Qii{n}q{8 * (4 - n)}x{n}q{8 * (4 - n)}x").pack for n in range(1, 5)}   # mr_array
 
 
 def describe(array, name, device):
     """The mr_array of an operator's argument, as bytes."""
     try:
-        where, shape, strides = array.get_device(), array.shape, array.stride()
-        n = len(shape)
-        if where == device and 0 < n < 5:
-            pad = _PAD[n]
-            return _PACK[n](array.data_ptr(), _code(array.dtype), n, *shape, *pad, *strides, *pad)
-    except AttributeError:
-        raise ValueError(f"{name} must be a device array, not {type(array).__name__}") from None
+        if array.get_device() == device:
+            shape = array.shape
+            n = len(shape)
+            return _PACK[n](array.data_ptr(), _CODES[array.dtype], n, *shape, *array.stride())
+    except (AttributeError, KeyError):   # a type not met before, or no such array
+        pass
+    return _described(array, name, device)
+
+
+def _described(array, name, device):
+    for accessor in ("get_device", "data_ptr", "stride", "shape", "dtype"):
+        if not hasattr(array, accessor):
+            raise ValueError(f"{name} must be a device array, not {type(array).__name__}")
+    where, shape, dtype = array.get_device(), array.shape, array.dtype
     if where != device:
         raise ValueError(f"{name} must be on device {device}, not {where if where >= 0 else 'the host'}")
-    raise ValueError(f"{name} must have 1 to 4 dimensions, not {n}")
+    if not 0 < len(shape) < 5:
+        raise ValueError(f"{name} must have 1 to 4 dimensions, not {len(shape)}")
+    code = TYPES.get(str(dtype).rsplit(".", 1)[-1])
+    if code is None:
+        raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16 or int32 is needed")
+    _CODES[dtype] = code
+    return _PACK[len(shape)](array.data_ptr(), code, len(shape), *shape, *array.stride())
 
 
 class DeviceArray:

@@ -89,20 +89,12 @@ class Tensor:
         return self.backend.empty(shape)
 
 
-def _counts(**values):
-    for name, value in values.items():
-        if not isinstance(value, (int, np.integer)) or isinstance(value, bool) or not 0 <= value < 2 ** 31:
-            raise ValueError(f"{name} must be a whole number from 0 on: {value!r}")
-
-
-def _window(window, sinks):
-    _counts(sinks=sinks)
-    if window is None:
-        return 0
-    _counts(window=window)
-    if window == 0:
-        raise ValueError("window must be at least 1, or None for no window")
-    return window
+def _count(value, name, least=0):
+    if type(value) is int and least <= value < 2 ** 31:
+        return value
+    if isinstance(value, np.integer) and least <= value < 2 ** 31:
+        return int(value)
+    raise ValueError(f"{name} must be a whole number from {least} on{', or None' if least else ''}: {value!r}")
 
 
 class CUDABackend:
@@ -305,16 +297,16 @@ class CUDABackend:
         (an array like the query).  ``window``: only the newest rows, and the first ``sinks``, are visible.
         ``scale`` defaults to 1 / sqrt(dim).  ``weights`` float32 [batch, kv heads, table rows] has each row's
         softmax weights, summed over the query heads that share its head, added to it."""
-        window = _window(window, sinks)
+        window = 0 if window is None else _count(window, "window", 1)
         device = self.device.ordinal
-        q = describe(query, "query", device)
+        q, shape = describe(query, "query", device), query.shape
         if out is None:
-            out = query.new_empty(query.shape)
+            out = query.new_empty(shape)
         call("mr_paged_attention", self.context, q, describe(key_pages, "key_pages", device),
              describe(value_pages, "value_pages", device), describe(page_table, "page_table", device),
              describe(lengths, "lengths", device),
              None if weights is None else describe(weights, "weights", device), describe(out, "out", device),
-             window, sinks, query.shape[-1] ** -0.5 if scale is None else scale)
+             window, _count(sinks, "sinks"), shape[-1] ** -0.5 if scale is None else scale)
         return out
 
     def window_attention(self, query, keys, values, query_offsets, key_offsets=None, *, window=None, sinks=0,
@@ -324,16 +316,16 @@ class CUDABackend:
         ``key_offsets`` (None: the same) alike; its last query stands at its last key.  A query sees the newest
         ``window`` keys up to its own (None: all) and the first ``sinks``.  Returns ``out`` (an array like the
         query; rows of no sequence are not written)."""
-        window = _window(window, sinks)
+        window = 0 if window is None else _count(window, "window", 1)
         device = self.device.ordinal
-        q = describe(query, "query", device)
+        q, shape = describe(query, "query", device), query.shape
         offsets = describe(query_offsets, "query_offsets", device)
         if out is None:
-            out = query.new_empty(query.shape)
+            out = query.new_empty(shape)
         call("mr_window_attention", self.context, q, describe(keys, "keys", device),
              describe(values, "values", device), offsets,
              offsets if key_offsets is None else describe(key_offsets, "key_offsets", device),
-             describe(out, "out", device), window, sinks, query.shape[-1] ** -0.5 if scale is None else scale)
+             describe(out, "out", device), window, _count(sinks, "sinks"), shape[-1] ** -0.5 if scale is None else scale)
         return out
 
     def evict_pages(self, key_pages, value_pages, page_table, lengths, weights, target_table, *, budget, sinks=0,
@@ -343,7 +335,7 @@ class CUDABackend:
         ``target_keys`` / ``target_values``.  The target pages must be others than the sequences' own.  Returns
         kept (int32 [batch, kv heads, budget] rows, -1 behind), the new lengths and the kept rows' weights
         (float32 [batch, kv heads, target rows], zeros behind)."""
-        _counts(budget=budget, sinks=sinks, recent=recent)
+        budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
         device = self.device.ordinal
         pools = describe(key_pages, "key_pages", device), describe(value_pages, "value_pages", device)
         if (target_keys is None) != (target_values is None):
