@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048;
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048, kCached = 48 << 10;
 
 // CTA = (sequence, head).  The rows between the sinks and the recent ones compete for the
 // rest of the budget: the value of the last one kept is found digit by digit, 11, 11 and 10
@@ -101,6 +101,10 @@ constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins =
 // all fall on one counts them at once.)  Rows above that value stay, and the first few equal
 // to it.  Then each warp counts its own stretch of the rows, and writes its kept rows in order
 // behind those of the warps before it.
+//
+// The weights' order is kept in shared memory after the first read where it fits.  Every
+// instruction here runs a few times at most, and a warp waits hundreds of cycles for code that
+// it meets first: the loops stay rolled (unrolled by eight, 12000 weights took 40 us).
 __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant__ EvictArgs a) {
     __shared__ int counts[kBins];
     __shared__ int above[kSelectWarps], equal[kSelectWarps];
@@ -111,6 +115,9 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = sequence_rows(a.lengths, a.length_stride, s, a.capacity);
     const float *w = a.weights + s * a.w_batch + h * a.w_head;
+    extern __shared__ uint32_t cached[];
+    const bool in_shared = a.capacity <= kCached;
+    auto key_of = [&](int t) { return in_shared ? cached[t] : rank_key(__ldg(w + t)); };
     int *kept = a.kept + s * a.kept_batch + h * a.kept_head;
     float *nw = a.new_weights + s * a.nw_batch + h * a.nw_head;
     const int total = min(n, a.budget);
@@ -118,16 +125,21 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     const int first = min(a.sinks, n), last = max(n - a.recent, first);
     uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
     int ties = n;
+    if (in_shared) {
+#pragma unroll 4
+        for (int t = tid; t < n; t += kSelectThreads) cached[t] = rank_key(__ldg(w + t));
+        __syncthreads();
+    }
     if (n > a.budget) {
         int need = a.budget - first - (n - last);  // rows to keep among first .. last - 1
+#pragma unroll 1
         for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
             const int bits = shift ? 11 : 10, bins = 1 << bits;
             for (int i = tid; i < bins; i += kSelectThreads) counts[i] = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int t0 = first + warp * 32; t0 < last; t0 += kSelectThreads) {
-                const int t = t0 + lane;
-                const uint32_t key = t < last ? rank_key(__ldg(w + t)) : 0;
+#pragma unroll 1
+            for (int t = first + tid; t - lane < last; t += kSelectThreads) {
+                const uint32_t key = t < last ? key_of(t) : 0;
                 const bool counted = t < last && (shift == 21 || key >> (shift + bits) == cut);
                 const uint32_t digit = key >> shift & (bins - 1);
                 const uint32_t all = __ballot_sync(0xffffffffu, counted);
@@ -181,18 +193,17 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
         ties = need;
     }
     // 0: dropped, 1: kept, 2: equal to the cut
-    auto state = [&](int t) {
+    auto state = [&](int t, uint32_t key) {
         if (t >= n) return 0;
         if (n <= a.budget || t < first || t >= last) return 1;
-        const uint32_t key = rank_key(__ldg(w + t));
         return key > cut ? 1 : key == cut ? 2 : 0;
     };
     const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) & ~31, lo = warp * stretch;
     const int hi = min(lo + stretch, n);
     int kept_here = 0, equal_here = 0;
-#pragma unroll 4
-    for (int t0 = lo; t0 < hi; t0 += 32) {
-        const int st = state(t0 + lane);
+#pragma unroll 1
+    for (int t = lo + lane; t < hi; t += 32) {
+        const int st = state(t, key_of(t));
         kept_here += st == 1;
         equal_here += st == 2;
     }
@@ -207,9 +218,9 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     int kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
     int equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
     const uint32_t before = (1u << lane) - 1;
-#pragma unroll 4
-    for (int t0 = lo; t0 < hi; t0 += 32) {
-        const int t = t0 + lane, st = state(t);
+#pragma unroll 1
+    for (int t = lo + lane; t - lane < hi; t += 32) {
+        const int st = t < hi ? state(t, key_of(t)) : 0;
         const uint32_t m1 = __ballot_sync(0xffffffffu, st == 1), m2 = __ballot_sync(0xffffffffu, st == 2);
         const int eq = equal_before + __popc(m2 & before);
         const int at = kept_before + __popc(m1 & before) + min(eq, ties);
@@ -220,7 +231,9 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
         kept_before += __popc(m1);
         equal_before += __popc(m2);
     }
+#pragma unroll 1
     for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+#pragma unroll 1
     for (int i = total + tid; i < a.target_rows; i += kSelectThreads) nw[i] = 0.f;
 }
 
@@ -398,7 +411,9 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     a.sinks = sinks;
     a.recent = recent;
     a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
-    k_select<<<a.batch * a.heads, kSelectThreads, 0, ctx->stream>>>(a);
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_select), kCached * 4));
+    const int cached = capacity <= kCached ? static_cast<int>(capacity) * 4 : 0;
+    k_select<<<a.batch * a.heads, kSelectThreads, cached, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     const int64_t rows = std::min<int64_t>(budget, capacity);
     if (rows) {
