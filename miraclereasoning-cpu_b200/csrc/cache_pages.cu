@@ -93,63 +93,73 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048, kCached = 48 << 10;
 
-// CTA = (sequence, head).  The rows between the sinks and the recent ones compete for the
-// rest of the budget: the value of the last one kept is found digit by digit, 11, 11 and 10
-// bits of the weights' order: counts of a digit among the rows that match the digits found
-// so far, and the highest digit that has the wanted row.  (The first 11 bits are sign, exponent and two
-// bits of the fraction, so that weights of all sizes fall on many counters; a warp whose rows
-// all fall on one counts them at once.)  Rows above that value stay, and the first few equal
-// to it.  Then each warp counts its own stretch of the rows, and writes its kept rows in order
-// behind those of the warps before it.
+// CTA = (sequence, head).  The sinks and the recent rows take part as the largest of all, so
+// the `budget` largest stay: the value of the last of them is found digit by digit, 11, 11
+// and 10 bits of the weights' order: counts of a digit among the rows that match the digits
+// found so far, and the highest digit that has the wanted row.  (The first 11 bits are sign,
+// exponent and two bits of the fraction, so that weights of all sizes fall on many counters; 128
+// rows that all fall on one, as after a reset, are counted at once.)  Rows above that value
+// stay, and the first few equal to it.  Then each warp counts its own stretch of the rows,
+// and writes its kept rows in order behind those of the warps before it.
 //
-// The weights' order is kept in shared memory after the first read where it fits.  Every
-// instruction here runs a few times at most, and a warp waits hundreds of cycles for code that
-// it meets first: the loops stay rolled (unrolled by eight, 12000 weights took 40 us).
+// The weights' order is kept in shared memory after the first read where it fits, four rows a
+// lane and access.  Every instruction here runs a few times at most, and a warp waits hundreds of
+// cycles for code that it meets first: the loops stay rolled (unrolled by eight, 12000 weights
+// took 40 us).
 __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant__ EvictArgs a) {
     __shared__ int counts[kBins];
     __shared__ int above[kSelectWarps], equal[kSelectWarps];
     __shared__ uint32_t s_digit;
     __shared__ int s_need;
+    extern __shared__ __align__(16) uint32_t cached[];
     const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = sequence_rows(a.lengths, a.length_stride, s, a.capacity);
     const float *w = a.weights + s * a.w_batch + h * a.w_head;
-    extern __shared__ uint32_t cached[];
-    const bool in_shared = a.capacity <= kCached;
-    auto key_of = [&](int t) { return in_shared ? cached[t] : rank_key(__ldg(w + t)); };
     int *kept = a.kept + s * a.kept_batch + h * a.kept_head;
     float *nw = a.new_weights + s * a.nw_batch + h * a.nw_head;
     const int total = min(n, a.budget);
     if (tid == 0 && h == 0) a.new_lengths[s * a.new_length_stride] = total;
-    const int first = min(a.sinks, n), last = max(n - a.recent, first);
-    uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
-    int ties = n;
+    auto read = [&](int t) {  // rows past the end: 0, and told apart by their number
+        if (t >= n) return 0u;
+        return t < a.sinks || t >= n - a.recent ? 0xffffffffu : rank_key(__ldg(w + t));
+    };
+    const bool in_shared = a.capacity <= kCached;
+    auto four = [&](int t) {
+        return in_shared ? *reinterpret_cast<const uint4 *>(cached + t)
+                         : make_uint4(read(t), read(t + 1), read(t + 2), read(t + 3));
+    };
     if (in_shared) {
-#pragma unroll 4
-        for (int t = tid; t < n; t += kSelectThreads) cached[t] = rank_key(__ldg(w + t));
+        const int end = (n + 3) & ~3;
+#pragma unroll 8
+        for (int t = tid; t < end; t += kSelectThreads) cached[t] = read(t);
         __syncthreads();
     }
+    uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
+    int ties = n;
     if (n > a.budget) {
-        int need = a.budget - first - (n - last);  // rows to keep among first .. last - 1
+        int need = a.budget;
 #pragma unroll 1
         for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
             const int bits = shift ? 11 : 10, bins = 1 << bits;
             for (int i = tid; i < bins; i += kSelectThreads) counts[i] = 0;
             __syncthreads();
 #pragma unroll 1
-            for (int t = first + tid; t - lane < last; t += kSelectThreads) {
-                const uint32_t key = t < last ? key_of(t) : 0;
-                const bool counted = t < last && (shift == 21 || key >> (shift + bits) == cut);
-                const uint32_t digit = key >> shift & (bins - 1);
-                const uint32_t all = __ballot_sync(0xffffffffu, counted);
-                if (!all) continue;
-                const uint32_t one = __shfl_sync(0xffffffffu, digit, __ffs(all) - 1);
-                if (__all_sync(0xffffffffu, !counted || digit == one)) {
-                    if (lane == 0) atomicAdd(&counts[one], __popc(all));
-                } else if (counted) {
-                    atomicAdd(&counts[digit], 1);
+            for (int t = 4 * tid; t - 4 * lane < n; t += 4 * kSelectThreads) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (t < n) x = four(t);
+                const uint32_t key[4] = {x.x, x.y, x.z, x.w};
+                const uint32_t one = __shfl_sync(0xffffffffu, x.x >> shift, 0);
+                if (__all_sync(0xffffffffu, t + 3 < n && x.x >> shift == one && x.y >> shift == one &&
+                                                x.z >> shift == one && x.w >> shift == one)) {
+                    if (lane == 0 && (shift == 21 || one >> bits == cut)) atomicAdd(&counts[one & (bins - 1)], 128);
+                    continue;
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + i < n && (shift == 21 || key[i] >> (shift + bits) == cut))
+                        atomicAdd(&counts[key[i] >> shift & (bins - 1)], 1);
             }
             __syncthreads();
             // each warp's bins summed, then the warp that has the row looks into its own
@@ -182,54 +192,66 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
                 };
                 if (mine == 32 || !find(high, base + 32)) find(low, base);
             }
-            if (need == 0 && tid == 0) {  // nothing to keep: above all
-                s_digit = bins - 1;
-                s_need = 0;
-            }
             __syncthreads();
             cut = cut << bits | s_digit;
             need = s_need;
         }
         ties = need;
     }
-    // 0: dropped, 1: kept, 2: equal to the cut
-    auto state = [&](int t, uint32_t key) {
-        if (t >= n) return 0;
-        if (n <= a.budget || t < first || t >= last) return 1;
-        return key > cut ? 1 : key == cut ? 2 : 0;
+    // a warp's stretch: rows to keep, and rows equal to the cut (in the upper half of a count), four a lane
+    auto marks = [&](int t, uint4 &x) {
+        x = t < n ? four(t) : make_uint4(0, 0, 0, 0);
+        const uint32_t key[4] = {x.x, x.y, x.z, x.w};
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) count += (key[i] > cut ? 1 : 0) + (key[i] == cut && t + i < n ? 1 << 16 : 0);
+        return count;
     };
-    const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) & ~31, lo = warp * stretch;
-    const int hi = min(lo + stretch, n);
-    int kept_here = 0, equal_here = 0;
+    const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 127) & ~127, lo = warp * stretch, hi = min(lo + stretch, n);
+    int kept_before = 0, equal_before = 0;
 #pragma unroll 1
-    for (int t = lo + lane; t < hi; t += 32) {
-        const int st = state(t, key_of(t));
-        kept_here += st == 1;
-        equal_here += st == 2;
+    for (int t = lo + 4 * lane; t < hi; t += 128) {
+        uint4 x;
+        const int count = marks(t, x);
+        kept_before += count & 0xffff;
+        equal_before += count >> 16;
     }
-    kept_here = __reduce_add_sync(0xffffffffu, kept_here);
-    equal_here = __reduce_add_sync(0xffffffffu, equal_here);
+    kept_before = __reduce_add_sync(0xffffffffu, kept_before);
+    equal_before = __reduce_add_sync(0xffffffffu, equal_before);
     __syncthreads();  // above[] of the last digit has been read
     if (lane == 0) {
-        above[warp] = kept_here;
-        equal[warp] = equal_here;
+        above[warp] = kept_before;
+        equal[warp] = equal_before;
     }
     __syncthreads();
-    int kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
-    int equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
-    const uint32_t before = (1u << lane) - 1;
+    kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
+    equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
 #pragma unroll 1
-    for (int t = lo + lane; t - lane < hi; t += 32) {
-        const int st = t < hi ? state(t, key_of(t)) : 0;
-        const uint32_t m1 = __ballot_sync(0xffffffffu, st == 1), m2 = __ballot_sync(0xffffffffu, st == 2);
-        const int eq = equal_before + __popc(m2 & before);
-        const int at = kept_before + __popc(m1 & before) + min(eq, ties);
-        if ((st == 1 || (st == 2 && eq < ties)) && at < a.budget) {
-            kept[at] = t;
-            if (at < a.target_rows) nw[at] = __ldg(w + t);
+    for (int t = lo + 4 * lane; t - 4 * lane < hi; t += 128) {
+        uint4 x;
+        const int count = marks(t, x);
+        int sum = count;  // of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += below;
         }
-        kept_before += __popc(m1);
-        equal_before += __popc(m2);
+        int over = kept_before + ((sum - count) & 0xffff), eq = equal_before + ((sum - count) >> 16);
+        const uint32_t key[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool same = key[i] == cut && t + i < n, more = key[i] > cut;
+            const int at = over + min(eq, ties);
+            if ((more || (same && eq < ties)) && at < a.budget) {
+                kept[at] = t + i;
+                if (at < a.target_rows) nw[at] = __ldg(w + t + i);
+            }
+            over += more;
+            eq += same;
+        }
+        const int all = __shfl_sync(0xffffffffu, sum, 31);
+        kept_before += all & 0xffff;
+        equal_before += all >> 16;
     }
 #pragma unroll 1
     for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
@@ -412,7 +434,7 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     a.recent = recent;
     a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_select), kCached * 4));
-    const int cached = capacity <= kCached ? static_cast<int>(capacity) * 4 : 0;
+    const int cached = capacity <= kCached ? (static_cast<int>(capacity) + 3) / 4 * 16 : 0;
     k_select<<<a.batch * a.heads, kSelectThreads, cached, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     const int64_t rows = std::min<int64_t>(budget, capacity);
