@@ -121,10 +121,10 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     float *nw = a.new_weights + s * a.nw_batch + h * a.nw_head;
     const int total = min(n, a.budget);
     if (tid == 0 && h == 0) a.new_lengths[s * a.new_length_stride] = total;
-    auto read = [&](int t) {  // rows past the end: 0, and told apart by their number
-        if (t >= n) return 0u;
-        return t < a.sinks || t >= n - a.recent ? 0xffffffffu : rank_key(__ldg(w + t));
+    auto order = [&](int t, float x) {  // rows past the end: 0, and told apart by their number
+        return t >= n ? 0u : t < a.sinks || t >= n - a.recent ? 0xffffffffu : rank_key(x);
     };
+    auto read = [&](int t) { return t < n ? order(t, __ldg(w + t)) : 0u; };
     const bool in_shared = a.capacity <= kCached;
     auto four = [&](int t) {
         return in_shared ? *reinterpret_cast<const uint4 *>(cached + t)
@@ -132,8 +132,16 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     };
     if (in_shared) {
         const int end = (n + 3) & ~3;
-#pragma unroll 8
-        for (int t = tid; t < end; t += kSelectThreads) cached[t] = read(t);
+        constexpr int kFlight = 8;
+#pragma unroll 1
+        for (int t = tid; t < end; t += kSelectThreads * kFlight) {
+            float x[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i) x[i] = __ldg(w + min(t + i * kSelectThreads, n - 1));
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i)
+                if (t + i * kSelectThreads < end) cached[t + i * kSelectThreads] = order(t + i * kSelectThreads, x[i]);
+        }
         __syncthreads();
     }
     uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
@@ -242,10 +250,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
         for (int i = 0; i < 4; ++i) {
             const bool same = key[i] == cut && t + i < n, more = key[i] > cut;
             const int at = over + min(eq, ties);
-            if ((more || (same && eq < ties)) && at < a.budget) {
-                kept[at] = t + i;
-                if (at < a.target_rows) nw[at] = __ldg(w + t + i);
-            }
+            if ((more || (same && eq < ties)) && at < a.budget) kept[at] = t + i;
             over += more;
             eq += same;
         }
@@ -255,8 +260,20 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     }
 #pragma unroll 1
     for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    __syncthreads();
+    constexpr int kFlight = 4;
 #pragma unroll 1
-    for (int i = total + tid; i < a.target_rows; i += kSelectThreads) nw[i] = 0.f;
+    for (int i = tid; i < a.target_rows; i += kSelectThreads * kFlight) {
+        int t[kFlight];
+        float x[kFlight];
+#pragma unroll
+        for (int e = 0; e < kFlight; ++e) t[e] = i + e * kSelectThreads < total ? __ldcg(kept + i + e * kSelectThreads) : -1;
+#pragma unroll
+        for (int e = 0; e < kFlight; ++e) x[e] = t[e] >= 0 ? __ldg(w + t[e]) : 0.f;
+#pragma unroll
+        for (int e = 0; e < kFlight; ++e)
+            if (i + e * kSelectThreads < a.target_rows) nw[i + e * kSelectThreads] = x[e];
+    }
 }
 
 // Kept rows to their target pages: a warp takes 32 rows of a head, a lane looks up one row's two
