@@ -4,9 +4,7 @@
 #pragma once
 
 #include <algorithm>
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -155,14 +153,13 @@ struct Scratch {
     }
 };
 
-// Lets a kernel take more than 48 KB of shared memory; asked of the driver once a kernel and device.
-inline int allow_shared(int device, const void *kernel, int bytes) {
-    static std::mutex lock;
-    static std::set<std::pair<int, const void *>> done;
-    std::lock_guard<std::mutex> guard(lock);
-    if (done.count({device, kernel})) return MR_OK;
+// Lets a kernel take more than 48 KB of shared memory; asked of the driver once a device
+// (`done`: a bit each, of the kernel's own).
+inline int allow_shared(int device, const void *kernel, int bytes, std::atomic<uint64_t> &done) {
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return MR_OK;
     MR_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.insert({device, kernel});
+    done.fetch_or(bit, std::memory_order_relaxed);
     return MR_OK;
 }
 

@@ -450,7 +450,8 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     a.sinks = sinks;
     a.recent = recent;
     a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_select), kCached * 4));
+    static std::atomic<uint64_t> allowed{0};
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_select), kCached * 4, allowed));
     const int cached = capacity <= kCached ? (static_cast<int>(capacity) + 3) / 4 * 16 : 0;
     k_select<<<a.batch * a.heads, kSelectThreads, cached, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());

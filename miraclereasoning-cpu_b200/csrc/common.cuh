@@ -47,7 +47,7 @@ struct mr_context {
     bool owns_stream = true;
     void *scratch = nullptr;  // of the calls queued outside a capture, in stream order (context_scratch)
     size_t scratch_bytes = 0;
-    int *wait_error = nullptr;  // host memory that kernels set when a bounded wait gave up (check_waits)
+    int *wait_error = nullptr;  // host word that kernels set when a bounded wait gave up (check_waits)
     std::atomic<int> refs{1};
 };
 
@@ -59,10 +59,6 @@ inline void context_release(mr_context *ctx) {
     cudaGetDevice(&current);
     cudaSetDevice(ctx->device);
     if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
-    if (ctx->wait_error) {
-        cudaStreamSynchronize(ctx->stream);
-        cudaFreeHost(ctx->wait_error);
-    }
     if (ctx->owns_stream) {
         cudaStreamSynchronize(ctx->stream);
         cudaStreamDestroy(ctx->stream);

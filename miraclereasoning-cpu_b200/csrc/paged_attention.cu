@@ -992,12 +992,14 @@ int launch(mr_context *ctx, PagedArgs &a) {
     constexpr int kRings = kWarps * M::R::kWarpBytes;
     if (few) {
         constexpr int kSmem = kRings + kWarps * H * (M::DP + 2) * 4;
-        MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged_few<T, M>), kSmem));
+        static std::atomic<uint64_t> allowed{0};
+        MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged_few<T, M>), kSmem, allowed));
         k_paged_few<T, M><<<grid, kThreads, kSmem, ctx->stream>>>(a);
         MR_CUDA_TRY(cudaGetLastError());
         return MR_OK;
     }
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings));
+    static std::atomic<uint64_t> allowed{0};
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings, allowed));
     k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     MR_CHECK((launch_early(ctx, dim3(grid * kJoin), dim3(kThreads), k_join<T, M>, a)));

@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -24,6 +25,26 @@ int set_error(int code, const char *fmt, ...) {
 int cuda_error(cudaError_t err, const char *what) {
     return set_error(err == cudaErrorMemoryAllocation ? MR_ERR_NOMEM : MR_ERR_CUDA, "%s failed: %s (%s)",
                      what, cudaGetErrorString(err), cudaGetErrorName(err));
+}
+
+// A context's word, of a page-locked block that stays until the process ends: a captured graph
+// may still write it when the context is gone.  (Contexts past the first 1024 share words, so
+// that one may report another's wait.)
+static int wait_word(int **out) {
+    constexpr unsigned kWords = 1024;
+    static std::mutex lock;
+    static int *block = nullptr;
+    static unsigned next = 0;
+    lock.lock();
+    cudaError_t err = cudaSuccess;
+    if (!block) {
+        err = cudaHostAlloc(reinterpret_cast<void **>(&block), kWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        if (err == cudaSuccess) memset(block, 0, kWords * sizeof(int));
+        else block = nullptr;
+    }
+    if (block) *out = block + next++ % kWords;
+    lock.unlock();
+    return err == cudaSuccess ? MR_OK : cuda_error(err, "cudaHostAlloc");
 }
 
 int check_waits(mr_context *ctx) {
@@ -95,15 +116,12 @@ static int new_context(int device_ordinal, bool on_stream, void *stream, mr_cont
             return mr::cuda_error(err, "cudaStreamCreate");
         }
     }
-    // mapped: kernels of a captured call write it too, and the host reads it without a copy
-    cudaError_t err = cudaHostAlloc(reinterpret_cast<void **>(&ctx->wait_error), sizeof(int),
-                                    cudaHostAllocMapped | cudaHostAllocPortable);
-    if (err != cudaSuccess) {
+    rc = mr::wait_word(&ctx->wait_error);
+    if (rc) {
         if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
         delete ctx;
-        return mr::cuda_error(err, "cudaHostAlloc");
+        return rc;
     }
-    *ctx->wait_error = 0;
     *out = ctx;
     return MR_OK;
 }

@@ -808,7 +808,8 @@ int launch(mr_context *ctx, WindowArgs &a) {
     MR_CHECK(encode(&maps.q, a.q, kBf16, a.dim, a.heads, a.tokens, a.q_head, a.q_row, a.group, per));
     MR_CHECK(encode(&maps.k, a.k, kBf16, a.dim, a.kv_heads, a.rows, a.k_head, a.k_row, 1, kKeys));
     MR_CHECK(encode(&maps.v, a.v, kBf16, a.dim, a.kv_heads, a.rows, a.v_head, a.v_row, 1, kKeys));
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window<T, DP>), S::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window<T, DP>), S::kSmem, allowed));
     const int64_t pairs = a.tokens / (2 * per) + static_cast<int64_t>(a.batch);  // no sequence has more than one that is not full
     MR_REQUIRE(pairs * a.kv_heads <= INT32_MAX, "too many rows and heads for one call");
     k_window<T, DP><<<static_cast<unsigned>(pairs * a.kv_heads), kTcThreads, S::kSmem, ctx->stream>>>(a, maps);
@@ -830,7 +831,8 @@ int launch32(mr_context *ctx, const WindowArgs &a) {
     const int per = kRows32 / a.group;
     const int64_t items = (a.tokens / per + static_cast<int64_t>(a.batch)) * a.kv_heads;
     MR_REQUIRE(items <= INT32_MAX, "too many rows and heads for one call");
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window32<DP>), sizeof(Shared32<DP>)));
+    static std::atomic<uint64_t> allowed{0};
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window32<DP>), sizeof(Shared32<DP>), allowed));
     k_window32<DP><<<static_cast<unsigned>(items), kThreads32, sizeof(Shared32<DP>), ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     return MR_OK;

@@ -320,6 +320,31 @@ def test_prompt_scales_and_strides(served, dtype):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 104])
+def test_prompts_in_other_layouts(served, dtype, dim):
+    # head-major rows, keys broadcast to all heads, rows of a longer buffer read backwards in heads
+    import torch
+    q, k, v = (queries(130, h, dim, dtype, seed=h) for h in (4, 2, 2))
+    offsets = torch.tensor([0, 60, 130], dtype=torch.int32, device="cuda")
+    want = served.window_attention(q, k, v, offsets, window=50, sinks=3)
+    major = [x.permute(1, 0, 2).contiguous().permute(1, 0, 2) for x in (q, k, v)]
+    assert torch.equal(served.window_attention(*major, offsets, window=50, sinks=3), want)
+    same = k[:, :1].expand(-1, 2, -1)
+    got = served.window_attention(q, same, same, offsets, window=50, sinks=3)
+    assert torch.equal(got, served.window_attention(q, same.contiguous(), same.contiguous(), offsets, window=50, sinks=3))
+    row = k[7:8].expand(130, -1, -1)
+    got = served.window_attention(q, row, row, offsets)
+    assert torch.equal(got, served.window_attention(q, row.contiguous(), row.contiguous(), offsets))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads", [70, 128, 130])
+def test_groups_of_many_heads(served, dtype, heads):
+    check_window(served, dtype, heads, 1, 16, [9, 14], [3, 0], 5, 2)
+    check_paged(served, Cache([40, 17], 8, 1, 16, dtype), queries(2, heads, 16, dtype), dtype, weighted=True)
+
+
 def test_offsets_that_do_not_rise_stay_inside(served):
     import torch
     q, k = queries(20, 2, 64, "bfloat16"), queries(20, 2, 64, "bfloat16", seed=2)
