@@ -19,26 +19,15 @@ from .weights import float32_to_bf16_bits
 TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 3}   # enum mr_dtype
 _ITEM = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4}
 _CODES = {}    # a dtype object -> its code, as its name says
-_PACK = {n: struct.Struct(f"<Qii{n}q{8 * (4 - n)}x{n}q{8 * (4 - n)}x").pack for n in range(1, 5)}   # mr_array
 
 
-def describe(array, name, device):
-    """The mr_array of an operator's argument, as bytes."""
-    try:
-        if array.get_device() == device:
-            shape = array.shape
-            n = len(shape)
-            return _PACK[n](array.data_ptr(), _CODES[array.dtype], n, *shape, *array.stride())
-    except (AttributeError, KeyError):   # a type not met before, or no such array
-        pass
-    return _described(array, name, device)
-
-
-def _described(array, name, device):
+def described(array, name, device):
+    """The mr_array of an operator's argument, as bytes; ValueError if it is none on the device.  (_pycall reads
+    the usual ones itself and comes here for a type's first array, and for those that are wrong.)"""
     for accessor in ("get_device", "data_ptr", "stride", "shape", "dtype"):
         if not hasattr(array, accessor):
             raise ValueError(f"{name} must be a device array, not {type(array).__name__}")
-    where, shape, dtype = array.get_device(), array.shape, array.dtype
+    where, shape, dtype = array.get_device(), tuple(array.shape), array.dtype
     if where != device:
         raise ValueError(f"{name} must be on device {device}, not {where if where >= 0 else 'the host'}")
     if not 0 < len(shape) < 5:
@@ -47,7 +36,32 @@ def _described(array, name, device):
     if code is None:
         raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16 or int32 is needed")
     _CODES[dtype] = code
-    return _PACK[len(shape)](array.data_ptr(), code, len(shape), *shape, *array.stride())
+    pad = (0,) * (4 - len(shape))
+    return struct.pack("<Qii8q", array.data_ptr(), code, len(shape), *shape, *pad, *array.stride(), *pad)
+
+
+try:
+    from . import _pycall
+except ImportError as missing:
+    raise _native.CUDAError(f"{_native.LIBRARY_PATH.with_name('_pycall.so')} is missing or unusable ({missing}): build it "
+                            f"with 'python miraclereasoning-cpu_b200/build.py'") from None
+_pycall.types(_CODES, described)
+describe = _pycall.describe
+APPEND, PAGED, WINDOW, EVICT = _pycall.APPEND, _pycall.PAGED, _pycall.WINDOW, _pycall.EVICT
+_NAMES = ("mr_append_pages", "mr_paged_attention", "mr_window_attention", "mr_evict_pages")
+
+
+def bind():
+    """Hands the library's operators over to ``invoke``."""
+    lib = _native.library()
+    _pycall.bind(*[C.cast(getattr(lib, name), C.c_void_p).value for name in _NAMES])
+
+
+def invoke(which, *args):
+    """An operator: its context's address, the device, arrays (None: left out) and scalars."""
+    status = _pycall.call(which, *args)
+    if status:
+        _native.check(status, _NAMES[which])
 
 
 class DeviceArray:

@@ -20,9 +20,9 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from . import _native
+from . import _native, arrays
 from ._native import CUDAError, call
-from .arrays import DeviceArray, describe, host_type, stored, widened
+from .arrays import DeviceArray, host_type, invoke, stored, widened
 
 # kernel name -> (NDRange rank, argument kinds) in kernels.cl order
 _KERNELS = {
@@ -97,6 +97,13 @@ def _count(value, name, least=0):
     raise ValueError(f"{name} must be a whole number from {least} on{', or None' if least else ''}: {value!r}")
 
 
+def _like(array, name):
+    try:
+        return array.new_empty(array.shape)
+    except AttributeError:
+        raise ValueError(f"{name} must be a device array, not {type(array).__name__}") from None
+
+
 class CUDABackend:
     """Float32 execution on one B200 (one context = one device + one stream).
 
@@ -122,6 +129,8 @@ class CUDABackend:
         else:
             call("mr_context_create_on_stream", device_index, stream, C.byref(handle))
         self.context = handle
+        self._where = handle.value, device_index   # of every array operator's call
+        arrays.bind()
 
     def __del__(self):
         ctx = getattr(self, "context", None)
@@ -285,11 +294,7 @@ class CUDABackend:
     def append_pages(self, keys, values, key_pages, value_pages, page_table, lengths, offsets=None):
         """New rows [tokens, kv heads, dim] into their pages.  ``lengths`` counts them already; sequence s's
         new rows are offsets[s] .. offsets[s + 1] - 1 (``offsets`` None: one row per sequence)."""
-        device = self.device.ordinal
-        call("mr_append_pages", self.context, describe(keys, "keys", device), describe(values, "values", device),
-             describe(key_pages, "key_pages", device), describe(value_pages, "value_pages", device),
-             describe(page_table, "page_table", device), describe(lengths, "lengths", device),
-             None if offsets is None else describe(offsets, "offsets", device))
+        invoke(arrays.APPEND, *self._where, keys, values, key_pages, value_pages, page_table, lengths, offsets)
 
     def paged_attention(self, query, key_pages, value_pages, page_table, lengths, *, window=None, sinks=0, scale=None,
                         weights=None, out=None):
@@ -298,15 +303,10 @@ class CUDABackend:
         ``scale`` defaults to 1 / sqrt(dim).  ``weights`` float32 [batch, kv heads, table rows] has each row's
         softmax weights, summed over the query heads that share its head, added to it."""
         window = 0 if window is None else _count(window, "window", 1)
-        device = self.device.ordinal
-        q, shape = describe(query, "query", device), query.shape
         if out is None:
-            out = query.new_empty(shape)
-        call("mr_paged_attention", self.context, q, describe(key_pages, "key_pages", device),
-             describe(value_pages, "value_pages", device), describe(page_table, "page_table", device),
-             describe(lengths, "lengths", device),
-             None if weights is None else describe(weights, "weights", device), describe(out, "out", device),
-             window, _count(sinks, "sinks"), shape[-1] ** -0.5 if scale is None else scale)
+            out = _like(query, "query")
+        invoke(arrays.PAGED, *self._where, query, key_pages, value_pages, page_table, lengths, weights, out, window,
+               _count(sinks, "sinks"), query.shape[-1] ** -0.5 if scale is None else scale)
         return out
 
     def window_attention(self, query, keys, values, query_offsets, key_offsets=None, *, window=None, sinks=0,
@@ -317,15 +317,11 @@ class CUDABackend:
         ``window`` keys up to its own (None: all) and the first ``sinks``.  Returns ``out`` (an array like the
         query; rows of no sequence are not written)."""
         window = 0 if window is None else _count(window, "window", 1)
-        device = self.device.ordinal
-        q, shape = describe(query, "query", device), query.shape
-        offsets = describe(query_offsets, "query_offsets", device)
         if out is None:
-            out = query.new_empty(shape)
-        call("mr_window_attention", self.context, q, describe(keys, "keys", device),
-             describe(values, "values", device), offsets,
-             offsets if key_offsets is None else describe(key_offsets, "key_offsets", device),
-             describe(out, "out", device), window, _count(sinks, "sinks"), shape[-1] ** -0.5 if scale is None else scale)
+            out = _like(query, "query")
+        invoke(arrays.WINDOW, *self._where, query, keys, values, query_offsets,
+               query_offsets if key_offsets is None else key_offsets, out, window, _count(sinks, "sinks"),
+               query.shape[-1] ** -0.5 if scale is None else scale)
         return out
 
     def evict_pages(self, key_pages, value_pages, page_table, lengths, weights, target_table, *, budget, sinks=0,
@@ -336,14 +332,11 @@ class CUDABackend:
         kept (int32 [batch, kv heads, budget] rows, -1 behind), the new lengths and the kept rows' weights
         (float32 [batch, kv heads, target rows], zeros behind)."""
         budget, sinks, recent = _count(budget, "budget"), _count(sinks, "sinks"), _count(recent, "recent")
-        device = self.device.ordinal
-        pools = describe(key_pages, "key_pages", device), describe(value_pages, "value_pages", device)
         if (target_keys is None) != (target_values is None):
             raise ValueError("target_keys and target_values go together")
-        targets = pools if target_keys is None else (describe(target_keys, "target_keys", device),
-                                                     describe(target_values, "target_values", device))
-        table, old = describe(target_table, "target_table", device), describe(weights, "weights", device)
-        if len(weights.shape) != 3 or len(key_pages.shape) != 4 or len(target_table.shape) != 2:
+        if target_keys is None:
+            target_keys, target_values = key_pages, value_pages
+        if not (len(weights.shape) == 3 and len(key_pages.shape) == 4 and len(target_table.shape) == 2):
             raise ValueError("weights must be [batch, kv heads, rows], target_table [batch, pages], the pages 4-D")
         batch, heads = weights.shape[:2]
         if kept is None:
@@ -352,10 +345,8 @@ class CUDABackend:
             new_lengths = lengths.new_empty(lengths.shape)
         if new_weights is None:
             new_weights = weights.new_empty((batch, heads, target_table.shape[1] * key_pages.shape[1]))
-        call("mr_evict_pages", self.context, *pools, describe(page_table, "page_table", device),
-             describe(lengths, "lengths", device), old, *targets, table, describe(kept, "kept", device),
-             describe(new_lengths, "new_lengths", device), describe(new_weights, "new_weights", device), budget, sinks,
-             recent)
+        invoke(arrays.EVICT, *self._where, key_pages, value_pages, page_table, lengths, weights, target_keys, target_values,
+               target_table, kept, new_lengths, new_weights, budget, sinks, recent)
         return kept, new_lengths, new_weights
 
     def finish(self):

@@ -3,8 +3,9 @@
     python miraclereasoning-cpu_b200/build.py [--force] [--verbose] [--ptxas-verbose]
 
 nvcc compiles every csrc/*.cu with ``-gencode arch=compute_100a,code=sm_100a``
-and links one shared library next to this file.  The build is incremental on
-source timestamps.  No GPU is needed to build.
+and links one shared library next to this file; the C compiler builds the
+array operators' calls from Python (csrc/pycall.c) as the module ``_pycall``.
+The build is incremental on source timestamps.  No GPU is needed to build.
 """
 from __future__ import annotations
 
@@ -13,11 +14,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 SRC = HERE / "csrc"
 OUT = HERE / "libmiracle_cuda.so"
+PYCALL = HERE / "_pycall.so"
 OBJ = HERE / "_build"
 HEADER = HERE.parent / "include" / "miracle_cuda.h"
 
@@ -61,7 +64,21 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
         os.replace(tmp, OUT)
+    build_pycall(force, verbose)
     return OUT
+
+
+def build_pycall(force: bool = False, verbose: bool = False) -> Path:
+    src = SRC / "pycall.c"
+    if force or _stale(PYCALL, [src, HEADER]):
+        tmp = PYCALL.with_suffix(".so.tmp")
+        cmd = [shutil.which("gcc") or "cc", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+               f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, PYCALL)
+    return PYCALL
 
 
 def main(argv=None) -> int:
