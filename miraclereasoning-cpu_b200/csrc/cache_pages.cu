@@ -45,7 +45,8 @@ __device__ int sequence_of(const int *offsets, int64_t stride, int batch, int i)
     return lo >= 0 && __ldg(offsets + (lo + 1) * stride) > i ? lo : -1;
 }
 
-// One warp per token: its place is found once, then its heads' pieces are copied.
+// One warp per token: its place is found once, then its heads' pieces are copied, four of the
+// keys and four of the values in flight a lane.
 __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     const int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
     if (token >= a.tokens) return;
@@ -60,12 +61,25 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a) {
     const int64_t kr = a.pages.row(s, t, a.k.page, a.k.row), vr = a.pages.row(s, t, a.v.page, a.v.row);
     if (kr < 0) return;
     const int n = a.heads * a.pieces;
-    for (int i = lane; i < n; i += 32) {
-        const int h = i / a.pieces, c = (i - h * a.pieces) * 16;
-        const uint4 x = *reinterpret_cast<const uint4 *>(a.keys + token * a.key_token + h * a.key_head + c);
-        const uint4 y = *reinterpret_cast<const uint4 *>(a.values + token * a.value_token + h * a.value_head + c);
-        *reinterpret_cast<uint4 *>(a.k.base + kr + h * a.k.head + c) = x;
-        *reinterpret_cast<uint4 *>(a.v.base + vr + h * a.v.head + c) = y;
+    constexpr int kFlight = 4;
+    const char *keys = a.keys + token * a.key_token, *values = a.values + token * a.value_token;
+    for (int i0 = lane; i0 < n; i0 += 32 * kFlight) {
+        uint4 x[kFlight], y[kFlight];
+        int64_t at[kFlight];
+#pragma unroll
+        for (int e = 0; e < kFlight; ++e) {
+            const int i = min(i0 + 32 * e, n - 1), h = i / a.pieces, c = (i - h * a.pieces) * 16;
+            x[e] = *reinterpret_cast<const uint4 *>(keys + h * a.key_head + c);
+            y[e] = *reinterpret_cast<const uint4 *>(values + h * a.value_head + c);
+            at[e] = static_cast<int64_t>(h) << 32 | c;
+        }
+#pragma unroll
+        for (int e = 0; e < kFlight; ++e)
+            if (i0 + 32 * e < n) {
+                const int64_t h = at[e] >> 32, c = at[e] & 0xffffffff;
+                *reinterpret_cast<uint4 *>(a.k.base + kr + h * a.k.head + c) = x[e];
+                *reinterpret_cast<uint4 *>(a.v.base + vr + h * a.v.head + c) = y[e];
+            }
     }
 }
 
