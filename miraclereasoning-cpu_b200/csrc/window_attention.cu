@@ -320,29 +320,34 @@ __device__ bool item_of(const WindowArgs &a, int most, Item &it) {
 
 // ---- float32 ------------------------------------------------------------------------
 // On the CUDA cores, in float32 throughout (the tensor cores would need three parts of
-// every operand): a CTA takes 64 query rows (64 / group tokens x the group's heads) over
-// tiles of 32 keys.  A thread has 8 rows x 2 keys of the scores, and 8 rows x DP / 16
-// dims of the values, so that a 16-byte read of shared memory feeds at least 8 products;
-// the weights pass through shared memory between the two.  A tile's values arrive while
-// its scores are worked out, the next keys while the values are mixed.
-constexpr int kRows32 = 64, kKeys32 = 32, kThreads32 = 128;
+// every operand): a CTA takes ROWS query rows (ROWS / group tokens x the group's heads) over
+// tiles of 32 keys.  A thread has ROWS / 8 rows x 2 keys of the scores, and as many rows x
+// DP / 16 dims of the values; the weights pass through shared memory between the two.  A
+// tile's values arrive while its scores are worked out, the next keys while the values are
+// mixed.  64 rows read shared memory least often for a product; where they would leave SMs
+// without a CTA, 32 rows, with the next keys asked for a tile earlier (two buffers).
+// Rows ty, ty + 8, ..: the two rows that a warp reads at once lie in different banks.
+constexpr int kKeys32 = 32, kThreads32 = 128;
 
 __device__ __forceinline__ void copy16(void *dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::saddr(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-template <int DP>
+template <int DP, int ROWS>
 struct Shared32 {
-    float q[kRows32][DP + 4], k[kKeys32][DP + 4], v[kKeys32][DP], p[kKeys32][kRows32 + 4];
+    static constexpr int kBuffers = ROWS == 32 ? 2 : 1;
+    float q[ROWS][DP + 4], k[kBuffers][kKeys32][DP + 4], v[kKeys32][DP], p[kKeys32][ROWS + 4];
 };
 
-template <int DP>
-__global__ void __launch_bounds__(kThreads32) k_window32(const __grid_constant__ WindowArgs a) {
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constant__ WindowArgs a) {
     extern __shared__ __align__(16) char raw32[];
-    Shared32<DP> &sm = *reinterpret_cast<Shared32<DP> *>(raw32);
+    using Shared = Shared32<DP, ROWS>;
+    Shared &sm = *reinterpret_cast<Shared *>(raw32);
+    constexpr int kMine = ROWS / 8, kAhead = Shared::kBuffers - 1;  // a thread's rows; tiles the keys run ahead
     constexpr int kVec = DP >= 64 ? 4 : 2, kVecs = DP / 16 / kVec;  // a thread's dims: kVecs pieces of kVec
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    const int per = kRows32 / a.group;
+    const int per = ROWS / a.group;
     Item it;
     if (!item_of<kKeys32>(a, per, it)) return;
     auto rows_in = [&](auto &to, const char *base, int64_t stride, int tile) {  // a tile's keys or values; zeros past the end
@@ -354,52 +359,60 @@ __global__ void __launch_bounds__(kThreads32) k_window32(const __grid_constant__
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     const char *kb = a.k + it.kh * a.k_head, *vb = a.v + it.kh * a.v_head;
-    for (int e = tid; e < kRows32 * DP / 4; e += kThreads32) {
+    for (int e = tid; e < ROWS * DP / 4; e += kThreads32) {
         const int r = e / (DP / 4), c = e % (DP / 4), t = r / a.group, g = r - t * a.group;
         const bool live = t < per && t < it.count && 4 * c < a.dim;
         copy16(&sm.q[r][4 * c],
                live ? a.q + (it.x.q0 + it.t0 + t) * a.q_row + (it.kh * a.group + g) * a.q_head + c * 16 : a.q, live);
     }
-    if (it.tiles > 0) rows_in(sm.k, kb, a.k_row, 0);
+    if (it.tiles > 0) rows_in(sm.k[0], kb, a.k_row, 0);
     const float scale = a.scale * 1.4426950408889634f;
-    float m[8], l[8], o[8][DP / 16];
-    int pos[8];  // the rows' positions; -1: no row
+    float m[kMine], l[kMine];
+    float2 o[kMine][DP / 32];
+    int pos[kMine];  // the rows' positions; -1: no row
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = ty * 8 + i, t = r / a.group;
+    for (int i = 0; i < kMine; ++i) {
+        const int r = ty + 8 * i, t = r / a.group;
         pos[i] = t < per && t < it.count ? it.x.m - it.x.n + it.t0 + t : -1;
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) o[i][d] = 0.f;
+        for (int d = 0; d < DP / 32; ++d) o[i][d] = make_float2(0.f, 0.f);
     }
     for (int j = 0; j < it.tiles; ++j) {
         rows_in(sm.v, vb, a.v_row, j);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (kAhead) {
+            if (j + 1 < it.tiles) rows_in(sm.k[(j + 1) % Shared::kBuffers], kb, a.k_row, j + 1);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(1 + kAhead) : "memory");
         __syncthreads();  // the keys are there
-        float s[8][2] = {};
-#pragma unroll 4
+        const auto &keys = sm.k[j % Shared::kBuffers];
+        float2 dot[kMine][2] = {};  // of the even and the odd pairs' dims
+#pragma unroll 2
         for (int d = 0; d < DP; d += 4) {
             float4 k[2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) k[y] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * y][d]);
+            for (int y = 0; y < 2; ++y) k[y] = *reinterpret_cast<const float4 *>(&keys[tx + 16 * y][d]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 q = *reinterpret_cast<const float4 *>(&sm.q[ty * 8 + i][d]);
+            for (int i = 0; i < kMine; ++i) {
+                const float4 q = *reinterpret_cast<const float4 *>(&sm.q[ty + 8 * i][d]);
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
-                    s[i][y] = fmaf(q.x, k[y].x, fmaf(q.y, k[y].y, fmaf(q.z, k[y].z, fmaf(q.w, k[y].w, s[i][y]))));
+                    dot[i][y] = fma2(make_float2(q.z, q.w), make_float2(k[y].z, k[y].w),
+                                     fma2(make_float2(q.x, q.y), make_float2(k[y].x, k[y].y), dot[i][y]));
             }
         }
+        float s[kMine][2];
         const int first = it.tile(j) * kKeys32 + tx;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kMine; ++i) {
             float top = -INFINITY;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int key = first + 16 * y;
                 const bool seen = key <= pos[i] && (a.window == 0 || pos[i] - key < a.window || key < a.sinks);
-                s[i][y] = seen ? s[i][y] * scale : -INFINITY;
+                s[i][y] = seen ? (dot[i][y].x + dot[i][y].y) * scale : -INFINITY;
                 top = fmaxf(top, s[i][y]);
             }
 #pragma unroll
@@ -411,40 +424,47 @@ __global__ void __launch_bounds__(kThreads32) k_window32(const __grid_constant__
             for (int y = 0; y < 2; ++y) s[i][y] = pow2(s[i][y] - ref);
             l[i] = fmaf(l[i], c, s[i][0] + s[i][1]);
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) o[i][d] *= c;
+            for (int d = 0; d < DP / 32; ++d) o[i][d] = make_float2(o[i][d].x * c, o[i][d].y * c);
         }
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<float4 *>(&sm.p[tx + 16 * y][ty * 8 + i]) = make_float4(s[i][y], s[i + 1][y], s[i + 2][y], s[i + 3][y]);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+            for (int i = 0; i < kMine; i += 4)
+                *reinterpret_cast<float4 *>(&sm.p[tx + 16 * y][ty * kMine + i]) = make_float4(s[i][y], s[i + 1][y], s[i + 2][y], s[i + 3][y]);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncthreads();  // the values and all weights are there, the keys are done with
-        if (j + 1 < it.tiles) rows_in(sm.k, kb, a.k_row, j + 1);
+        if (!kAhead && j + 1 < it.tiles) rows_in(sm.k[0], kb, a.k_row, j + 1);
 #pragma unroll 4
         for (int key = 0; key < kKeys32; ++key) {
-            float p[8], v[DP / 16];
+            float p[kMine];
+            float2 v[DP / 32];
 #pragma unroll
-            for (int i = 0; i < 8; i += 4) *reinterpret_cast<float4 *>(p + i) = *reinterpret_cast<const float4 *>(&sm.p[key][ty * 8 + i]);
+            for (int i = 0; i < kMine; i += 4)
+                *reinterpret_cast<float4 *>(p + i) = *reinterpret_cast<const float4 *>(&sm.p[key][ty * kMine + i]);
 #pragma unroll
-            for (int d = 0; d < kVecs; ++d)
+            for (int d = 0; d < kVecs; ++d) {
+                const float *at = &sm.v[key][d * 16 * kVec + tx * kVec];
+                if (kVec == 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(at);
+                    v[2 * d] = make_float2(x.x, x.y);
+                    v[2 * d + 1] = make_float2(x.z, x.w);
+                } else {
+                    v[d] = *reinterpret_cast<const float2 *>(at);
+                }
+            }
 #pragma unroll
-                for (int e = 0; e < kVec; e += 2)
-                    *reinterpret_cast<float2 *>(v + d * kVec + e) =
-                        *reinterpret_cast<const float2 *>(&sm.v[key][d * 16 * kVec + tx * kVec + e]);
+            for (int i = 0; i < kMine; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) o[i][d] = fmaf(p[i], v[d], o[i][d]);
+                for (int d = 0; d < DP / 32; ++d) o[i][d] = fma2(make_float2(p[i], p[i]), v[d], o[i][d]);
         }
         __syncthreads();  // the values and weights are done with
     }
     uint32_t again = 0;  // rows with values that are not finite
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kMine; ++i) {
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-        const int r = ty * 8 + i, t = r / a.group, g = r - t * a.group;
+        const int r = ty + 8 * i, t = r / a.group, g = r - t * a.group;
         const float f = l[i] != 0.f ? 1.f / l[i] : 0.f;
         bool finite = true;
         float *out = reinterpret_cast<float *>(a.out + (it.x.q0 + it.t0 + t) * a.o_row + (it.kh * a.group + g) * a.o_head);
@@ -452,19 +472,19 @@ __global__ void __launch_bounds__(kThreads32) k_window32(const __grid_constant__
         for (int d = 0; d < kVecs; ++d)
 #pragma unroll
             for (int e = 0; e < kVec; e += 2) {
-                const float2 x = make_float2(o[i][d * kVec + e] * f, o[i][d * kVec + e + 1] * f);
+                const float2 y = o[i][(d * kVec + e) / 2], x = make_float2(y.x * f, y.y * f);
                 const int dim = d * 16 * kVec + tx * kVec + e;
                 finite &= fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY;
                 if (t < per && t < it.count && dim < a.dim) *reinterpret_cast<float2 *>(out + dim) = x;
             }
         if (!finite && t < per && t < it.count) again |= 1u << i;
     }
-    // the warp's rows ty * 8 .. of both its halves, as any lane of a half says
+    // the rows of both halves of the warp, as any lane of a half says
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) again |= __shfl_xor_sync(0xffffffffu, again, w);
     for (int half = 0; half < 2; ++half)
         for (uint32_t left = __shfl_sync(0xffffffffu, again, half * 16); left; left &= left - 1) {
-            const int r = (tid / 32 * 2 + half) * 8 + __ffs(left) - 1, t = r / a.group;
+            const int r = tid / 32 * 2 + half + 8 * (__ffs(left) - 1), t = r / a.group;
             row_alone<float>(a, it.x, it.t0 + t, it.kh * a.group + r - t * a.group);
         }
 }
@@ -826,19 +846,27 @@ int launch_rows(mr_context *ctx, const WindowArgs &a) {
     return MR_OK;
 }
 
-template <int DP>
+template <int DP, int ROWS>
 int launch32(mr_context *ctx, const WindowArgs &a) {
-    const int per = kRows32 / a.group;
+    using Shared = Shared32<DP, ROWS>;
+    const int per = ROWS / a.group;
     const int64_t items = (a.tokens / per + static_cast<int64_t>(a.batch)) * a.kv_heads;
     MR_REQUIRE(items <= INT32_MAX, "too many rows and heads for one call");
     static std::atomic<uint64_t> allowed{0};
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window32<DP>), sizeof(Shared32<DP>), allowed));
-    k_window32<DP><<<static_cast<unsigned>(items), kThreads32, sizeof(Shared32<DP>), ctx->stream>>>(a);
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window32<DP, ROWS>), sizeof(Shared), allowed));
+    k_window32<DP, ROWS><<<static_cast<unsigned>(items), kThreads32, sizeof(Shared), ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     return MR_OK;
 }
+template <int DP>
+int launch32(mr_context *ctx, const WindowArgs &a) {
+    // fewer than two CTAs of 64 rows an SM: the smaller ones (short flashnano-1.5 prompts, 745
+    // tokens in 53 or 106 CTAs: 12.1 us against 17.3)
+    const bool few = static_cast<int64_t>(a.tokens) * a.heads < int64_t(2) * 64 * ctx->sm_count;
+    return a.group <= 32 && few ? launch32<DP, 32>(ctx, a) : launch32<DP, 64>(ctx, a);
+}
 int launch32(mr_context *ctx, WindowArgs &a) {
-    if (a.group > kRows32) return launch_rows<float>(ctx, a);
+    if (a.group > 64) return launch_rows<float>(ctx, a);
     return a.dim <= 32 ? launch32<32>(ctx, a) : a.dim <= 64 ? launch32<64>(ctx, a) : launch32<128>(ctx, a);
 }
 
