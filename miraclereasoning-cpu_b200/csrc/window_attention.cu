@@ -11,15 +11,21 @@
 // over the 128-key tiles that any of their rows sees; tiles between the sinks and
 // the window are skipped.  Warp roles: warps 0-3 and 4-7 the softmax of one query
 // tile each (a thread a row, so a row's maximum and sum need no exchange), warp 8
-// the TMA loads, warp 9 the products.  S = Q K^T and O += P V accumulate in TMEM
-// (S of both tiles 2 x 128 columns, O of both behind); P, rounded to the operands'
-// type, goes back to TMEM over its own S and is the first operand of the second
-// product, V the second one as it lies in memory (MN-major).  While one tile is in
-// softmax the other is in the products.  The two exponentials and products of a
-// 128 x 128 tile (head dim 128) cost 1024 cycles each on an SM, so both units bound
-// the kernel together.  O is rescaled only where a row's maximum grows by more than
-// 2^8: until then the weights are taken against the old maximum, which the sum
-// shares, so nothing is lost but headroom.
+// the TMA loads, warps 9 and 10 the products of one query tile each.  S = Q K^T and
+// O += P V accumulate in TMEM (S of both tiles 2 x 128 columns, O of both behind); P,
+// rounded to the operands' type, goes back to TMEM over its own S and is the first
+// operand of the second product, V the second one as it lies in memory (MN-major).
+// O is rescaled only where a row's maximum grows by more than 2^8: until then the
+// weights are taken against the old maximum, which the sum shares, so nothing is lost
+// but headroom.
+//
+// What bounds it: a 128 x 128 tile's exponentials (head dim 128) take the special-function
+// unit 1024 cycles, its two products the tensor cores as many.  One tile's softmax runs
+// beside the other's products; with two softmax warps a scheduler, each unit is busy 57% of
+// the time (ncu, flashlite's 8192-token context: 228 us, 1.2 PFLOP/s).  Measured and left out:
+// a quarter of the exponentials by polynomials (no faster at head dim 64, 15% slower at 128),
+// key tiles of 64 with the next scores worked out ahead (290 us), two threads a row (314 us),
+// P beside S where TMEM has room (head dim 64: no difference).
 //
 // A weight is 0 where the mask hides a key, but 0 x NaN is NaN: a row whose values are
 // not all finite at the end is worked out again from the visible keys alone
