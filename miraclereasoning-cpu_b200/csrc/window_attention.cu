@@ -137,20 +137,21 @@ struct Maps {
 
 // Shared memory behind the tiles.
 struct Barriers {
-    uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
+    uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
     uint32_t tmem;
     int stop;  // a wait gave up: every role leaves
 };
 
-// A bounded wait; false when it gives up, or another role has.
-__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up) {
+// A bounded wait; false when it gives up, or another role has.  (Two seconds, and what a warp may take
+// to work 32 rows out again alone: `limit`.)
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up, uint64_t limit) {
     if (tc::try_wait(bar, parity)) return true;
     const uint64_t start = tc::now();
     for (unsigned spin = 1;; ++spin) {
         if (tc::try_wait(bar, parity)) return true;
         if (spin % 64 == 0) {
             if (*reinterpret_cast<volatile int *>(&b->stop)) return false;
-            if (tc::now() - start > tc::kWaitNs) {
+            if (tc::now() - start > limit) {
                 *reinterpret_cast<volatile int *>(&b->stop) = 1;
                 *reinterpret_cast<volatile int *>(gave_up) = 1;
                 return false;
@@ -281,48 +282,67 @@ struct Item {
     int front, first, tiles;   // tiles 0 .. front - 1, then first ..
     __device__ __forceinline__ int tile(int j) const { return j < front ? j : first + j - front; }
 };
-// Items in falling order of their tiles' numbers, so that the longest of a causal prompt start first.
+// The items of a call, in falling order of their tiles' numbers, so that the longest of a
+// causal prompt start first; `most` queries each.  Whole warps.
 template <int KEYS>
-__device__ bool item_of(const WindowArgs &a, int most, Item &it) {
-    const int lane = threadIdx.x % 32;
-    int total = 0;
-    for (int s = lane; s < a.batch; s += 32) total += (span_of(a, s).n + most - 1) / most;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(total) * a.kv_heads) return false;
-    const int pair = total - 1 - static_cast<int>(blockIdx.x) / a.kv_heads;
-    it.kh = static_cast<int>(blockIdx.x) % a.kv_heads;
-    int base = 0, s = -1;
-    for (int s0 = 0; s0 < a.batch; s0 += 32) {
-        const int mine = s0 + lane < a.batch ? (span_of(a, s0 + lane).n + most - 1) / most : 0;
-        int sum = mine;
+struct Items {
+    int most, pairs;   // items of one KV head
+    int64_t total;
+    int mine, sum;     // of sequence `lane`, and of those up to it (32 sequences at most; else found again for each item)
+    __device__ __forceinline__ int of(const WindowArgs &a, int s) const {
+        return s < a.batch ? (span_of(a, s).n + most - 1) / most : 0;
+    }
+    static __device__ __forceinline__ int scan(int x) {
+        const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int below = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += below;
+            const int below = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += below;
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, base + sum > pair);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            s = s0 + l;
-            base += __shfl_sync(0xffffffffu, sum - mine, l);
-            break;
-        }
-        base += __shfl_sync(0xffffffffu, sum, 31);
+        return x;
     }
-    if (s < 0) return false;  // offsets that overlap so far that their sum wraps
-    it.x = span_of(a, s);
-    it.t0 = (pair - base) * most;
-    it.count = min(most, it.x.n - it.t0);
-    const int low = it.x.m - it.x.n + it.t0, high = low + it.count - 1;  // their positions
-    it.front = it.first = it.tiles = 0;
-    if (high < 0) return true;
-    const int start = a.window ? max(0, low - a.window + 1) : 0;  // the first key in a window
-    it.first = start / KEYS;
-    it.front = min(it.first, (min(a.sinks, start) + KEYS - 1) / KEYS);
-    it.tiles = it.front + high / KEYS - it.first + 1;
-    return true;
-}
+    __device__ __forceinline__ void init(const WindowArgs &a, int queries) {
+        const int lane = threadIdx.x % 32;
+        most = queries;
+        mine = of(a, lane);
+        pairs = mine;
+        for (int s = lane + 32; s < a.batch; s += 32) pairs += of(a, s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
+        total = static_cast<int64_t>(max(pairs, 0)) * a.kv_heads;
+        sum = scan(mine);
+    }
+    __device__ __forceinline__ bool get(const WindowArgs &a, int64_t index, Item &it) const {
+        if (index >= total) return false;
+        const int lane = threadIdx.x % 32;
+        const int pair = pairs - 1 - static_cast<int>(index / a.kv_heads);
+        it.kh = static_cast<int>(index % a.kv_heads);
+        int base = 0, s = -1;
+        for (int s0 = 0; s0 < a.batch; s0 += 32) {
+            const int here = a.batch <= 32 ? mine : of(a, s0 + lane), upto = a.batch <= 32 ? sum : scan(here);
+            const uint32_t past = __ballot_sync(0xffffffffu, base + upto > pair);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                s = s0 + l;
+                base += __shfl_sync(0xffffffffu, upto - here, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (s < 0) return false;  // offsets that overlap so far that their sum wraps
+        it.x = span_of(a, s);
+        it.t0 = (pair - base) * most;
+        it.count = min(most, it.x.n - it.t0);
+        const int low = it.x.m - it.x.n + it.t0, high = low + it.count - 1;  // their positions
+        it.front = it.first = it.tiles = 0;
+        if (high < 0) return true;
+        const int start = a.window ? max(0, low - a.window + 1) : 0;  // the first key in a window
+        it.first = start / KEYS;
+        it.front = min(it.first, (min(a.sinks, start) + KEYS - 1) / KEYS);
+        it.tiles = it.front + high / KEYS - it.first + 1;
+        return true;
+    }
+};
 
 // ---- float32 ------------------------------------------------------------------------
 // On the CUDA cores, in float32 throughout (the tensor cores would need three parts of
@@ -354,8 +374,10 @@ __global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constan
     constexpr int kVec = DP >= 64 ? 4 : 2, kVecs = DP / 16 / kVec;  // a thread's dims: kVecs pieces of kVec
     const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
     const int per = ROWS / a.group;
+    Items<kKeys32> items;
+    items.init(a, per);
     Item it;
-    if (!item_of<kKeys32>(a, per, it)) return;
+    if (!items.get(a, blockIdx.x, it)) return;
     auto rows_in = [&](auto &to, const char *base, int64_t stride, int tile) {  // a tile's keys or values; zeros past the end
         for (int e = tid; e < kKeys32 * DP / 4; e += kThreads32) {
             const int r = e / (DP / 4), c = e % (DP / 4), row = it.tile(tile) * kKeys32 + r;
@@ -495,7 +517,15 @@ __global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constan
         }
 }
 
-template <typename T, int DP>
+// A CTA's items: one of each round of as many as there are CTAs, forwards and backwards in
+// turn, so that who has a round's longest has the next one's shortest.
+__device__ __forceinline__ int64_t item_of(int round) {
+    return static_cast<int64_t>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// kRounds: a CTA takes items of several rounds; else one.  (A body of its own: the loop around
+// everything cost 6% where items are long.)
+template <typename T, int DP, bool kRounds>
 __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant__ WindowArgs a,
                                                           const __grid_constant__ Maps maps) {
     using S = Shape<DP>;
@@ -509,6 +539,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc::saddr(bar)), "r"(count) : "memory");
         };
         init(&b->q_full, 1);
+        init(&b->q_empty, 2);
         for (int i = 0; i < S::kStages; ++i) {
             init(&b->kv_full[i], 1);
             init(&b->kv_empty[i], 2);
@@ -529,42 +560,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
     }
     if (warp == kLoadWarp && lane < 3)
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
-    Item it = {};
-    const bool work = item_of<kKeys>(a, 2 * per, it);
-    if (!work) it.tiles = it.count = 0;
+    Items<kKeys> items;
+    items.init(a, 2 * per);
+    const uint64_t limit = tc::kWaitNs + 4000ull * a.rows;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = b->tmem, q_tiles = tc::saddr(tiles), stages = q_tiles + 2 * S::kQBytes;
-    const int n = it.tiles;
+    Item it;
+    bool ok = true;
     // 384 threads start with 168 registers each; a softmax thread holds a row of 128 scores
     // and takes 216, of what the third warpgroup gives: 2 x 216 + 72 = 3 x 168.
     if (warp >= kLoadWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kLoadWarp) {
-        if (lane == 0 && n > 0) {
-            expect(&b->q_full, 2 * S::kHalves * per * a.group * 128);
-            for (int w = 0; w < 2; ++w)
-                for (int h = 0; h < S::kHalves; ++h)
-                    load_box(q_tiles + w * S::kQBytes + h * kHalfQ, &maps.q, h * 64, it.kh * a.group,
-                             it.x.q0 + it.t0 + w * per, &b->q_full);
-            // K0, V0, K1, V1, ... through the stages
-            int issued = 0;
-            auto load = [&](const CUtensorMap *map, int j) {
-                const int st = issued % S::kStages, use = issued / S::kStages;
-                if (use > 0 && !wait_for(&b->kv_empty[st], (use - 1) & 1, b, a.gave_up)) return false;
-                expect(&b->kv_full[st], S::kStageBytes);
-                for (int h = 0; h < S::kHalves; ++h)
-                    load_box(stages + st * S::kStageBytes + h * kHalfK, map, h * 64, it.kh, it.x.k0 + it.tile(j) * kKeys,
-                             &b->kv_full[st]);
-                ++issued;
-                return true;
-            };
-            for (int j = 0; j < n; ++j)
-                if (!load(&maps.k, j) || !load(&maps.v, j)) break;
+        int issued = 0, count = 0;  // stages and items with tiles so far
+        for (int round = 0; (kRounds || round == 0) && ok && items.get(a, item_of(round), it); ++round) {
+            if (it.tiles == 0) continue;
+            if (lane == 0) {
+                // Q once the last item's products with it are done
+                ok = count == 0 || wait_for(&b->q_empty, (count - 1) & 1, b, a.gave_up, limit);
+                if (ok) {
+                    expect(&b->q_full, 2 * S::kHalves * per * a.group * 128);
+                    for (int w = 0; w < 2; ++w)
+                        for (int h = 0; h < S::kHalves; ++h)
+                            load_box(q_tiles + w * S::kQBytes + h * kHalfQ, &maps.q, h * 64, it.kh * a.group,
+                                     it.x.q0 + it.t0 + w * per, &b->q_full);
+                    ++count;
+                }
+                // K0, V0, K1, V1, ... through the stages
+                auto load = [&](const CUtensorMap *map, int j) {
+                    const int st = issued % S::kStages, use = issued / S::kStages;
+                    if (use > 0 && !wait_for(&b->kv_empty[st], (use - 1) & 1, b, a.gave_up, limit)) return false;
+                    expect(&b->kv_full[st], S::kStageBytes);
+                    for (int h = 0; h < S::kHalves; ++h)
+                        load_box(stages + st * S::kStageBytes + h * kHalfK, map, h * 64, it.kh,
+                                 it.x.k0 + it.tile(j) * kKeys, &b->kv_full[st]);
+                    ++issued;
+                    return true;
+                };
+                for (int j = 0; j < it.tiles && ok; ++j) ok = load(&maps.k, j) && load(&maps.v, j);
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        if (lane == 0) {
             // no copy may land after the CTA has left (the last stages; those before were waited for by the products)
             const uint64_t start = tc::now();
-            while (!tc::try_wait(&b->q_full, 0) && tc::now() - start < tc::kWaitNs) {
-            }
+            if (count > 0)
+                while (!tc::try_wait(&b->q_full, (count - 1) & 1) && tc::now() - start < tc::kWaitNs) {
+                }
             for (int i = max(0, issued - S::kStages); i < issued; ++i)
                 while (!tc::try_wait(&b->kv_full[i % S::kStages], (i / S::kStages) & 1) && tc::now() - start < tc::kWaitNs) {
                 }
@@ -573,16 +616,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         // A warp for each query tile, so that one's waits do not hold up the other's products.
         // All of it walks through them and one lane issues: descriptors stay in uniform
         // registers, where the instruction wants them.
-        if (n > 0) {
+        {
             constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
             const uint32_t qk = mma_desc(kBf16, kKeys, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
             const int w = warp - kMathWarp;
             const uint64_t q = tc::sw128_desc(q_tiles + w * S::kQBytes), k_desc = tc::sw128_desc(stages), v_desc = mn_desc(stages);
             const uint32_t s_at = tmem + w * kTile, o_at = tmem + S::kO + w * DP;
             const bool leader = elect();
-            int st = 0, round = 0;  // the next stage, and the parity of its fill
+            int st = 0, fill = 0;  // the next stage, and the parity of its fill
             auto take = [&] {
-                if (!wait_for(&b->kv_full[st], round, b, a.gave_up)) return false;
+                if (!wait_for(&b->kv_full[st], fill, b, a.gave_up, limit)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return true;
             };
@@ -591,7 +634,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 __syncwarp();
                 if (++st == S::kStages) {
                     st = 0;
-                    round ^= 1;
+                    fill ^= 1;
                 }
             };
             auto scores = [&] {
@@ -605,39 +648,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 }
                 __syncwarp();
             };
-            bool ok = wait_for(&b->q_full, 0, b, a.gave_up) && take();
-            if (ok) {
-                scores();
-                leave();
-            }
-            for (int j = 0; j < n && ok; ++j) {
-                ok = take();
-                const uint64_t v = v_desc + st * (S::kStageBytes >> 4);
-                // P comes in two halves; the first is multiplied while the second is worked out
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    ok = ok && wait_for(half ? &b->p_full[w] : &b->p_half[w], j & 1, b, a.gave_up);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (leader) {
-#pragma unroll
-                        for (int i = half * kKeys / 32; i < (half + 1) * kKeys / 32; ++i)
-                            mma_ts(o_at, s_at + i * 8, v + i * 128, pv, j > 0 || i > 0);
-                        if (half) tc::commit(&b->o_done[w]);
-                    }
-                    __syncwarp();
-                }
-                leave();
-                if (ok && j + 1 < n) {
-                    ok = take();
-                    if (ok) scores();
+            int count = 0, g = 0;  // items and steps so far
+            for (int round = 0; (kRounds || round == 0) && ok && items.get(a, item_of(round), it); ++round) {
+                const int n = it.tiles;
+                if (n == 0) continue;
+                ok = wait_for(&b->q_full, count++ & 1, b, a.gave_up, limit) && take();
+                if (ok) {
+                    scores();
+                    if (n == 1 && leader) tc::commit(&b->q_empty);
                     leave();
+                }
+                for (int j = 0; j < n && ok; ++j, ++g) {
+                    ok = take();
+                    const uint64_t v = v_desc + st * (S::kStageBytes >> 4);
+                    // P comes in two halves; the first is multiplied while the second is worked out
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        ok = ok && wait_for(half ? &b->p_full[w] : &b->p_half[w], g & 1, b, a.gave_up, limit);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (leader) {
+#pragma unroll
+                            for (int i = half * kKeys / 32; i < (half + 1) * kKeys / 32; ++i)
+                                mma_ts(o_at, s_at + i * 8, v + i * 128, pv, j > 0 || i > 0);
+                            if (half) tc::commit(&b->o_done[w]);
+                        }
+                        __syncwarp();
+                    }
+                    leave();
+                    if (ok && j + 1 < n) {
+                        ok = take();
+                        if (ok) scores();
+                        if (j + 2 == n && leader) tc::commit(&b->q_empty);
+                        leave();
+                    }
                 }
             }
         }
     } else if (warp < kLoadWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int w = warp / 4, r = (warp & 3) * 32 + lane, tt = r / a.group, g = r - tt * a.group;
+        int done = 0;  // steps so far
+        for (int round = 0; (kRounds || round == 0) && ok && items.get(a, item_of(round), it); ++round) {
+        const int n = it.tiles;
         const int i = it.t0 + w * per + tt;  // query of the sequence
         const bool live = tt < per && w * per + tt < it.count;
         const int p = live ? it.x.m - it.x.n + i : -1;
@@ -652,7 +705,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         // the warp sees are left out.  Two bodies: the scores of either stay in registers of its own.
         auto step = [&](int j, auto hides) {
             constexpr bool kHides = decltype(hides)::value;
-            if (!__all_sync(0xffffffffu, wait_for(&b->s_full[w], j & 1, b, a.gave_up))) return false;
+            if (!__all_sync(0xffffffffu, wait_for(&b->s_full[w], done & 1, b, a.gave_up, limit))) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             uint32_t s[kKeys];
 #pragma unroll
@@ -683,7 +736,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 const float grown = max_nan(m, top);
                 if (j > 0) {
                     // done already, since the scores came behind it
-                    if (!__all_sync(0xffffffffu, wait_for(&b->o_done[w], (j - 1) & 1, b, a.gave_up))) return false;
+                    if (!__all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit))) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const float c = m == grown ? 1.f : pow2((m - grown) * scale);
                     l *= c;
@@ -703,7 +756,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             // The two tiles take the special-function unit in turns, a quarter overlapping; otherwise both
             // settle into doing their exponentials, and then their products, at the same time
             // (chunked flashnano-1.7 prompts 35.1 us without, 34.0 with).
-            if ((w == 1 || j > 0) && !__all_sync(0xffffffffu, wait_for(&b->turn[w], (w == 1 ? j : j - 1) & 1, b, a.gave_up)))
+            if ((w == 1 || done > 0) && !__all_sync(0xffffffffu, wait_for(&b->turn[w], (w == 1 ? done : done - 1) & 1, b, a.gave_up, limit)))
                 return false;
             float2 sum[2] = {};
             // The weights, rounded to the operands' type: half a step each, at random, of sums
@@ -747,14 +800,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             if (lane == 0) arrive(&b->p_full[w]);
             return true;
         };
-        bool ok = true;
-        for (int j = 0; j < n && ok; ++j) {
+        for (int j = 0; j < n && ok; ++j, ++done) {
             const int kb = it.tile(j) * kKeys;
             ok = kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)
                      ? step(j, std::true_type())
                      : step(j, std::false_type());
         }
-        if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (n - 1) & 1, b, a.gave_up));
+        if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit));
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int h = it.kh * a.group + g;
@@ -785,6 +837,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 const int from = __ffs(again) - 1;
                 row_alone<T>(a, it.x, __shfl_sync(0xffffffffu, i, from), __shfl_sync(0xffffffffu, h, from));
             }
+        }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
@@ -834,11 +887,19 @@ int launch(mr_context *ctx, WindowArgs &a) {
     MR_CHECK(encode(&maps.q, a.q, kBf16, a.dim, a.heads, a.tokens, a.q_head, a.q_row, a.group, per));
     MR_CHECK(encode(&maps.k, a.k, kBf16, a.dim, a.kv_heads, a.rows, a.k_head, a.k_row, 1, kKeys));
     MR_CHECK(encode(&maps.v, a.v, kBf16, a.dim, a.kv_heads, a.rows, a.v_head, a.v_row, 1, kKeys));
-    static std::atomic<uint64_t> allowed{0};
-    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_window<T, DP>), S::kSmem, allowed));
     const int64_t pairs = a.tokens / (2 * per) + static_cast<int64_t>(a.batch);  // no sequence has more than one that is not full
-    MR_REQUIRE(pairs * a.kv_heads <= INT32_MAX, "too many rows and heads for one call");
-    k_window<T, DP><<<static_cast<unsigned>(pairs * a.kv_heads), kTcThreads, S::kSmem, ctx->stream>>>(a, maps);
+    const int64_t items = pairs * a.kv_heads;
+    MR_REQUIRE(items <= INT32_MAX, "too many rows and heads for one call");
+    // Short items: a CTA an SM that loads the next while it finishes one (40 prompts of 100 tokens:
+    // 23.0 us, 28.5 with a CTA each).  Long ones: a CTA each, whose order the GPU balances as they end
+    // (one flashlite context: 229 us, 239 in fixed rounds).
+    const int64_t keys = std::min<int64_t>(a.rows / a.batch, a.window ? static_cast<int64_t>(a.window) + a.sinks : a.rows);
+    const bool rounds = keys <= 1024;
+    const auto kernel = rounds ? k_window<T, DP, true> : k_window<T, DP, false>;
+    static std::atomic<uint64_t> allowed[2] = {};
+    MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(kernel), S::kSmem, allowed[rounds]));
+    const int64_t grid = rounds ? std::min<int64_t>(items, ctx->sm_count) : items;
+    kernel<<<static_cast<unsigned>(grid), kTcThreads, S::kSmem, ctx->stream>>>(a, maps);
     MR_CUDA_TRY(cudaGetLastError());
     return MR_OK;
 }

@@ -272,6 +272,16 @@ def test_window_attention(served, dtype, heads, kv, dim, new, earlier, window, s
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_many_short_and_one_long_prompt(served, dtype):
+    # more pieces than the GPU has SMs, several to each; and a prompt whose pieces go one to an SM
+    rng = np.random.default_rng(12)
+    new = [int(n) for n in rng.integers(0, 30, 50)]
+    check_window(served, dtype, 4, 4, 64, new[:-1] + [0], [0] * 50, None, 0)
+    check_window(served, dtype, 4, 4, 72, new, [int(n) for n in rng.integers(0, 9, 50)], 7, 2)
+    check_window(served, dtype, 2, 1, 64, [1090], [0], None, 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_more_queries_than_keys(served, dtype):
     # the first queries stand before the first key: they see nothing and give zeros
     import torch
