@@ -660,33 +660,51 @@ __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk
     }
 }
 
-// A unit's weights: rows i = from + first, + step, .. of those seen.
-template <int H>
-__device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
-                                            int to, int first, int step, const float (&lse)[H]) {
+// A unit's weights: rows i = from + first, + step, .. of those seen; N heads' scores a row.
+template <int N, int H>
+__device__ __forceinline__ void add_rows(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
+                                         int to, int first, int step, const float (&lse)[H]) {
     constexpr int kRows = 4;  // in flight
     float *weights = a.weights + walk.s * a.w_batch + kh * a.w_head;
+#pragma unroll 1
     for (int i0 = from + first; i0 < to; i0 += step * kRows) {
-        float sum[kRows], was[kRows];
+        alignas(16) float2 x[kRows][N / 2];
+        float was[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            const int i = i0 + r * step;
-            sum[r] = 0.f;
-            was[r] = i < to ? weights[walk.seen.at(i)] : 0.f;
+            const int i = min(i0 + r * step, to - 1);
+            was[r] = weights[walk.seen.at(i)];
+            const float *row = scores + static_cast<int64_t>(i) * N;
+            if constexpr (N % 4 == 0) {
 #pragma unroll
-            for (int h = 0; h < H; h += 2) {
-                if (h >= a.heads2 || i >= to) continue;
-                const float2 x = __ldcg(reinterpret_cast<const float2 *>(scores + static_cast<int64_t>(i) * a.heads2 + h));
-                // a hidden row's score is -inf, and adds nothing whatever the sum is
-                sum[r] += x.x == -INFINITY ? 0.f : ex2(x.x - lse[h]);
-                sum[r] += x.y == -INFINITY ? 0.f : ex2(x.y - lse[h + 1]);
+                for (int h = 0; h < N / 2; h += 2)
+                    *reinterpret_cast<float4 *>(&x[r][h]) = __ldcg(reinterpret_cast<const float4 *>(row + 2 * h));
+            } else {
+#pragma unroll
+                for (int h = 0; h < N / 2; ++h) x[r][h] = __ldcg(reinterpret_cast<const float2 *>(row + 2 * h));
             }
         }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const int i = i0 + r * step;
-            if (i < to) weights[walk.seen.at(i)] = was[r] + sum[r];
+            // a hidden row's score is -inf, and adds nothing whatever the sum is
+#pragma unroll
+            for (int h = 0; h < N / 2; ++h) {
+                was[r] += x[r][h].x == -INFINITY ? 0.f : ex2(x[r][h].x - lse[2 * h]);
+                was[r] += x[r][h].y == -INFINITY ? 0.f : ex2(x[r][h].y - lse[2 * h + 1]);
+            }
+            if (i < to) weights[walk.seen.at(i)] = was[r];
         }
+    }
+}
+template <int H>
+__device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, const float *scores, int kh, int from,
+                                            int to, int first, int step, const float (&lse)[H]) {
+    if (a.heads2 == 2) return add_rows<2, H>(a, walk, scores, kh, from, to, first, step, lse);
+    if (a.heads2 == 4) return add_rows<4, H>(a, walk, scores, kh, from, to, first, step, lse);
+    if constexpr (H == 8) {
+        if (a.heads2 == 6) return add_rows<6, H>(a, walk, scores, kh, from, to, first, step, lse);
+        add_rows<8, H>(a, walk, scores, kh, from, to, first, step, lse);
     }
 }
 
@@ -927,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
         for (int b = part.b0 + lane; b <= b1; b += 32) {
             float2 x[H];
 #pragma unroll
-            for (int h = 0; h < H; ++h) x[h] = sums_of(part, b, h);
+            for (int h = 0; h < H; ++h) x[h] = h < a.heads2 ? sums_of(part, b, h) : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int h = 0; h < H; ++h) {
                 const float t = fmaxf(top[h], x[h].x), ref = t == -INFINITY ? 0.f : t;
@@ -937,6 +955,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
         }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
+            if (h >= a.heads2) continue;
             const float t = warp_max(top[h]), ref = t == -INFINITY ? 0.f : t;
             sum[h] = warp_sum(sum[h] * ex2(top[h] - ref));
             top[h] = t;
