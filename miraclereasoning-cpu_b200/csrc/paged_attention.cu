@@ -708,7 +708,7 @@ __device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &wal
     }
 }
 
-// Works through pieces; `done(math, piece, q, heads, kh, h0)` takes each one's results.
+// Works through pieces; `done(math, piece, q, unit, heads, kh, h0)` takes each one's results.
 template <typename T, typename M, typename Next, typename Done>
 __device__ __forceinline__ void work_through(const PagedArgs &a, uint32_t ring, const Next &start, const Done &done) {
     using R = typename M::R;

@@ -142,8 +142,8 @@ struct Barriers {
     int stop;  // a wait gave up: every role leaves
 };
 
-// A bounded wait; false when it gives up, or another role has.  (Two seconds, and what a warp may take
-// to work 32 rows out again alone: `limit`.)
+// A bounded wait; false when it gives up, or another role has.  (`limit`: two seconds, and what a warp may
+// take to work 32 rows out again alone.)
 __device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up, uint64_t limit) {
     if (tc::try_wait(bar, parity)) return true;
     const uint64_t start = tc::now();
@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constan
     // the rows of both halves of the warp, as any lane of a half says
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) again |= __shfl_xor_sync(0xffffffffu, again, w);
+    __syncwarp();  // the rows' first stores come before their second ones, which other lanes make
     for (int half = 0; half < 2; ++half)
         for (uint32_t left = __shfl_sync(0xffffffffu, again, half * 16); left; left &= left - 1) {
             const int r = tid / 32 * 2 + half + 8 * (__ffs(left) - 1), t = r / a.group;
@@ -562,7 +563,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
     Items<kKeys> items;
     items.init(a, 2 * per);
-    const uint64_t limit = tc::kWaitNs + 4000ull * a.rows;
+    const uint64_t limit = tc::kWaitNs + min(4000ull * a.rows, 8 * tc::kWaitNs);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -690,154 +691,155 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         const int w = warp / 4, r = (warp & 3) * 32 + lane, tt = r / a.group, g = r - tt * a.group;
         int done = 0;  // steps so far
         for (int round = 0; (kRounds || round == 0) && ok && items.get(a, item_of(round), it); ++round) {
-        const int n = it.tiles;
-        const int i = it.t0 + w * per + tt;  // query of the sequence
-        const bool live = tt < per && w * per + tt < it.count;
-        const int p = live ? it.x.m - it.x.n + i : -1;
-        // every row's position of this tile, for the tiles that need no mask
-        const int p_low = it.x.m - it.x.n + it.t0 + w * per, p_high = p_low + min(per, it.count - w * per) - 1;
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + w * kTile, o_at = tmem + lanes + S::kO + w * DP;
-        const float scale = fabsf(a.scale) * 1.4426950408889634f;
-        constexpr float kNone = -3.4028235e38f;  // no key seen yet
-        float m = kNone, l = 0.f;
-        // A tile's step; where the mask hides some of its keys, its quarters of 32 keys that no row of
-        // the warp sees are left out.  Two bodies: the scores of either stay in registers of its own.
-        auto step = [&](int j, auto hides) {
-            constexpr bool kHides = decltype(hides)::value;
-            if (!__all_sync(0xffffffffu, wait_for(&b->s_full[w], done & 1, b, a.gave_up, limit))) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[kKeys];
+            const int n = it.tiles;
+            const int i = it.t0 + w * per + tt;  // query of the sequence
+            const bool live = tt < per && w * per + tt < it.count;
+            const int p = live ? it.x.m - it.x.n + i : -1;
+            // every row's position of this tile, for the tiles that need no mask
+            const int p_low = it.x.m - it.x.n + it.t0 + w * per, p_high = p_low + min(per, it.count - w * per) - 1;
+            const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+            const uint32_t s_at = tmem + lanes + w * kTile, o_at = tmem + lanes + S::kO + w * DP;
+            const float scale = fabsf(a.scale) * 1.4426950408889634f;
+            constexpr float kNone = -3.4028235e38f;  // no key seen yet
+            float m = kNone, l = 0.f;
+            // A tile's step; where the mask hides some of its keys, its quarters of 32 keys that no row of
+            // the warp sees are left out.  Two bodies: the scores of either stay in registers of its own.
+            auto step = [&](int j, auto hides) {
+                constexpr bool kHides = decltype(hides)::value;
+                if (!__all_sync(0xffffffffu, wait_for(&b->s_full[w], done & 1, b, a.gave_up, limit))) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t s[kKeys];
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 32) tmem_get(s_at + c, s + c);
-            settle(s);
-            uint32_t used = 0;  // the quarters to work on
-            if (kHides) {
-                const int kb = it.tile(j) * kKeys;
-                const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
+                for (int c = 0; c < kKeys; c += 32) tmem_get(s_at + c, s + c);
+                settle(s);
+                uint32_t used = 0;  // the quarters to work on
+                if (kHides) {
+                    const int kb = it.tile(j) * kKeys;
+                    const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 32) {
-                    // a bit for each key that is seen: up to `high`, and from `low` on or in the sinks
-                    const uint32_t seen = below(high + 1 - c) & (~below(low - c) | below(front - c));
-                    if (__any_sync(0xffffffffu, seen)) used |= 1u << (c / 32);
+                    for (int c = 0; c < kKeys; c += 32) {
+                        // a bit for each key that is seen: up to `high`, and from `low` on or in the sinks
+                        const uint32_t seen = below(high + 1 - c) & (~below(low - c) | below(front - c));
+                        if (__any_sync(0xffffffffu, seen)) used |= 1u << (c / 32);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!(seen & (1u << e))) s[c + e] = 0xff800000u;
-                }
-            }
-            float tops[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) tops[c] = __uint_as_float(s[c]);
-#pragma unroll
-            for (int c = 8; c < kKeys; ++c) tops[c % 8] = max_nan(tops[c % 8], __uint_as_float(s[c]));
-            const float top = max_nan(max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])),
-                                      max_nan(max_nan(tops[4], tops[5]), max_nan(tops[6], tops[7])));
-            if (__any_sync(0xffffffffu, !((top - m) * scale <= 8.f))) {  // a NaN goes into the maximum, and so everywhere
-                const float grown = max_nan(m, top);
-                if (j > 0) {
-                    // done already, since the scores came behind it
-                    if (!__all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit))) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const float c = m == grown ? 1.f : pow2((m - grown) * scale);
-                    l *= c;
-#pragma unroll
-                    for (int d = 0; d < DP; d += 16) {
-                        uint32_t o[16];
-                        tmem_get16(o_at + d, o);
-                        settle(o);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
-                        tmem_put16(o_at + d, o);
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen & (1u << e))) s[c + e] = 0xff800000u;
                     }
                 }
-                m = grown;
-            }
-            const float shift = m == kNone ? 0.f : -m * scale;
-            // The two tiles take the special-function unit in turns, a quarter overlapping; otherwise both
-            // settle into doing their exponentials, and then their products, at the same time
-            // (chunked flashnano-1.7 prompts 35.1 us without, 34.0 with).
-            if ((w == 1 || done > 0) && !__all_sync(0xffffffffu, wait_for(&b->turn[w], (w == 1 ? done : done - 1) & 1, b, a.gave_up, limit)))
-                return false;
-            float2 sum[2] = {};
-            // The weights, rounded to the operands' type: half a step each, at random, of sums
-            // whose result is rounded to that type again.  The sum takes them unrounded.
-            auto weigh = [&](int c) {
-                float2 x = fma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(scale, scale),
-                                make_float2(shift, shift));
-                x.x = pow2(x.x);
-                x.y = pow2(x.y);
-                sum[c / 2 % 2] = add2(sum[c / 2 % 2], x);
-                s[c / 2] = pair_of(x.x, x.y, T());
-            };
-            auto hand_half = [&] {
-                tmem_put(s_at, s);
+                float tops[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) tops[c] = __uint_as_float(s[c]);
+#pragma unroll
+                for (int c = 8; c < kKeys; ++c) tops[c % 8] = max_nan(tops[c % 8], __uint_as_float(s[c]));
+                const float top = max_nan(max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])),
+                                          max_nan(max_nan(tops[4], tops[5]), max_nan(tops[6], tops[7])));
+                if (__any_sync(0xffffffffu, !((top - m) * scale <= 8.f))) {  // a NaN goes into the maximum, and so everywhere
+                    const float grown = max_nan(m, top);
+                    if (j > 0) {
+                        // done already, since the scores came behind it
+                        if (!__all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit))) return false;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const float c = m == grown ? 1.f : pow2((m - grown) * scale);
+                        l *= c;
+#pragma unroll
+                        for (int d = 0; d < DP; d += 16) {
+                            uint32_t o[16];
+                            tmem_get16(o_at + d, o);
+                            settle(o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * c);
+                            tmem_put16(o_at + d, o);
+                        }
+                    }
+                    m = grown;
+                }
+                const float shift = m == kNone ? 0.f : -m * scale;
+                // The two tiles take the special-function unit in turns, a quarter overlapping; otherwise both
+                // settle into doing their exponentials, and then their products, at the same time
+                // (chunked flashnano-1.7 prompts 35.1 us without, 34.0 with).
+                if ((w == 1 || done > 0) && !__all_sync(0xffffffffu, wait_for(&b->turn[w], (w == 1 ? done : done - 1) & 1, b, a.gave_up, limit)))
+                    return false;
+                float2 sum[2] = {};
+                // The weights, rounded to the operands' type: half a step each, at random, of sums
+                // whose result is rounded to that type again.  The sum takes them unrounded.
+                auto weigh = [&](int c) {
+                    float2 x = fma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), make_float2(scale, scale),
+                                    make_float2(shift, shift));
+                    x.x = pow2(x.x);
+                    x.y = pow2(x.y);
+                    sum[c / 2 % 2] = add2(sum[c / 2 % 2], x);
+                    s[c / 2] = pair_of(x.x, x.y, T());
+                };
+                auto hand_half = [&] {
+                    tmem_put(s_at, s);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive(&b->p_half[w]);
+                };
+#pragma unroll
+                for (int c0 = 0; c0 < kKeys; c0 += 32) {
+                    if (!kHides || used & (1u << (c0 / 32))) {
+#pragma unroll
+                        for (int c = c0; c < c0 + 32; c += 2) weigh(c);
+                    } else {
+#pragma unroll
+                        for (int c = c0; c < c0 + 32; c += 2) s[c / 2] = 0;
+                    }
+                    if (c0 + 32 == kKeys / 2) hand_half();
+                    if (c0 + 32 == kKeys * 3 / 4) {
+                        __syncwarp();
+                        if (lane == 0) arrive(&b->turn[w ^ 1]);
+                    }
+                }
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
+                tmem_put(s_at + kKeys / 4, s + kKeys / 4);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) arrive(&b->p_half[w]);
+                if (lane == 0) arrive(&b->p_full[w]);
+                return true;
             };
-#pragma unroll
-            for (int c0 = 0; c0 < kKeys; c0 += 32) {
-                if (!kHides || used & (1u << (c0 / 32))) {
-#pragma unroll
-                    for (int c = c0; c < c0 + 32; c += 2) weigh(c);
-                } else {
-#pragma unroll
-                    for (int c = c0; c < c0 + 32; c += 2) s[c / 2] = 0;
-                }
-                if (c0 + 32 == kKeys / 2) hand_half();
-                if (c0 + 32 == kKeys * 3 / 4) {
-                    __syncwarp();
-                    if (lane == 0) arrive(&b->turn[w ^ 1]);
-                }
+            for (int j = 0; j < n && ok; ++j, ++done) {
+                const int kb = it.tile(j) * kKeys;
+                ok = kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)
+                         ? step(j, std::true_type())
+                         : step(j, std::false_type());
             }
-            sum[0] = add2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
-            tmem_put(s_at + kKeys / 4, s + kKeys / 4);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) arrive(&b->p_full[w]);
-            return true;
-        };
-        for (int j = 0; j < n && ok; ++j, ++done) {
-            const int kb = it.tile(j) * kKeys;
-            ok = kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)
-                     ? step(j, std::true_type())
-                     : step(j, std::false_type());
-        }
-        if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit));
-        if (ok) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int h = it.kh * a.group + g;
-            char *out = a.out + (it.x.q0 + i) * a.o_row + h * a.o_head;
-            const float f = m == kNone ? 0.f : 1.f / l;
-            bool finite = true;
+            if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit));
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const int h = it.kh * a.group + g;
+                char *out = a.out + (it.x.q0 + i) * a.o_row + h * a.o_head;
+                const float f = m == kNone ? 0.f : 1.f / l;
+                bool finite = true;
 #pragma unroll
-            for (int d = 0; d < DP; d += 32) {
-                uint32_t o[32] = {};
-                if (n > 0) {
-                    tmem_get(o_at + d, o);
-                    settle(o);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint4 x;
-                    uint32_t *y = &x.x;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float u = __uint_as_float(o[e + 2 * c]) * f, v = __uint_as_float(o[e + 2 * c + 1]) * f;
-                        finite &= fabsf(u) < INFINITY && fabsf(v) < INFINITY;
-                        y[c] = pair_of(u, v, T());
+                for (int d = 0; d < DP; d += 32) {
+                    uint32_t o[32] = {};
+                    if (n > 0) {
+                        tmem_get(o_at + d, o);
+                        settle(o);
                     }
-                    if (live && d + e < a.dim) *reinterpret_cast<uint4 *>(out + (d + e) * 2) = x;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 x;
+                        uint32_t *y = &x.x;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float u = __uint_as_float(o[e + 2 * c]) * f, v = __uint_as_float(o[e + 2 * c + 1]) * f;
+                            finite &= fabsf(u) < INFINITY && fabsf(v) < INFINITY;
+                            y[c] = pair_of(u, v, T());
+                        }
+                        if (live && d + e < a.dim) *reinterpret_cast<uint4 *>(out + (d + e) * 2) = x;
+                    }
+                }
+                __syncwarp();  // the rows' first stores come before their second ones, which other lanes make
+                for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1) {
+                    const int from = __ffs(again) - 1;
+                    row_alone<T>(a, it.x, __shfl_sync(0xffffffffu, i, from), __shfl_sync(0xffffffffu, h, from));
                 }
             }
-            for (uint32_t again = __ballot_sync(0xffffffffu, live && !finite); again; again &= again - 1) {
-                const int from = __ffs(again) - 1;
-                row_alone<T>(a, it.x, __shfl_sync(0xffffffffu, i, from), __shfl_sync(0xffffffffu, h, from));
-            }
-        }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }

@@ -73,6 +73,8 @@ def test_valid_arguments_reach_the_context():
     (dict(scale=float("nan")), "scale must be finite"),
     (dict(value_pages=Fake((10, 16, 4, 64), F16)), "of one floating type"),
     (dict(value_pages=Fake((9, 16, 4, 64))), "differ in shape"),
+    (dict(key_pages=Fake((10, 16, 4, 64), stride=(1 << 32, 256, 64, 1))), "stride 0 passes 4 GB"),
+    (dict(key_pages=Fake((10, 16, 4, 64), stride=(1 << 60, 256, 64, 1))), "stride 0 is out of range"),
     (dict(key_pages=Fake((10, 16, 4, 60)), value_pages=Fake((10, 16, 4, 60))), "whole 16-byte pieces"),
     (dict(key_pages=Fake((10, 16, 4, 136)), value_pages=Fake((10, 16, 4, 136))), "at most 128 values"),
 ])
