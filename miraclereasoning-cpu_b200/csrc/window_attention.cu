@@ -8,8 +8,8 @@
 // 16-bit types run on the 5th-generation tensor cores (k_window).  A CTA works on
 // two tiles of 128 query rows (128 / group tokens x the group's heads: the heads
 // share their keys, and a tile of few tokens wastes little at the mask's edges)
-// over the 128-key tiles that any of their rows sees; tiles between the sinks and
-// the window are skipped.  Warp roles: warps 0-3 and 4-7 the softmax of one query
+// over the 128-key tiles that any of their rows sees; keys between the sinks and
+// the windows are skipped.  Warp roles: warps 0-3 and 4-7 the softmax of one query
 // tile each (a thread a row, so a row's maximum and sum need no exchange), warp 8
 // the TMA loads, warps 9 and 10 the products of one query tile each.  S = Q K^T and
 // O += P V accumulate in TMEM (S of both tiles 2 x 128 columns, O of both behind); P,
@@ -275,12 +275,17 @@ __device__ __forceinline__ uint32_t pair_of(float x, float y, __half) {
     return *reinterpret_cast<const uint32_t *>(&p);
 }
 
-// A CTA's work: queries t0 .. of sequence `x`, KV head `kh`, and the tiles of KEYS keys they see.
+// A CTA's work: queries t0 .. of sequence `x`, KV head `kh`, and the tiles of KEYS keys they see:
+// `front` tiles of the sinks, keys 0 .. edge - 1, and from key `first` on, where their windows
+// begin (no tile boundary: a window of 512 over 64 queries is five tiles of 128 wherever it lies).
+template <int KEYS>
 struct Item {
     Span x;
     int kh, t0, count;         // first query, queries
-    int front, first, tiles;   // tiles 0 .. front - 1, then first ..
-    __device__ __forceinline__ int tile(int j) const { return j < front ? j : first + j - front; }
+    int front, edge, first, tiles;
+    __device__ __forceinline__ int key(int j) const { return j < front ? j * KEYS : first + (j - front) * KEYS; }
+    // Past the last key of tile j that any query may see there.
+    __device__ __forceinline__ int past(int j) const { return j < front ? edge : INT32_MAX; }
 };
 // The items of a call, in falling order of their tiles' numbers, so that the longest of a
 // causal prompt start first; `most` queries each.  Whole warps.
@@ -312,7 +317,7 @@ struct Items {
         total = static_cast<int64_t>(max(pairs, 0)) * a.kv_heads;
         sum = scan(mine);
     }
-    __device__ __forceinline__ bool get(const WindowArgs &a, int64_t index, Item &it) const {
+    __device__ __forceinline__ bool get(const WindowArgs &a, int64_t index, Item<KEYS> &it) const {
         if (index >= total) return false;
         const int lane = threadIdx.x % 32;
         const int pair = pairs - 1 - static_cast<int>(index / a.kv_heads);
@@ -334,12 +339,15 @@ struct Items {
         it.t0 = (pair - base) * most;
         it.count = min(most, it.x.n - it.t0);
         const int low = it.x.m - it.x.n + it.t0, high = low + it.count - 1;  // their positions
-        it.front = it.first = it.tiles = 0;
+        it.front = it.edge = it.first = it.tiles = 0;
         if (high < 0) return true;
         const int start = a.window ? max(0, low - a.window + 1) : 0;  // the first key in a window
-        it.first = start / KEYS;
-        it.front = min(it.first, (min(a.sinks, start) + KEYS - 1) / KEYS);
-        it.tiles = it.front + high / KEYS - it.first + 1;
+        if (a.sinks < start) {  // keys between that no query sees
+            it.edge = a.sinks;
+            it.front = (a.sinks + KEYS - 1) / KEYS;
+            it.first = start;
+        }
+        it.tiles = it.front + (high - it.first) / KEYS + 1;
         return true;
     }
 };
@@ -376,11 +384,11 @@ __global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constan
     const int per = ROWS / a.group;
     Items<kKeys32> items;
     items.init(a, per);
-    Item it;
+    Item<kKeys32> it;
     if (!items.get(a, blockIdx.x, it)) return;
     auto rows_in = [&](auto &to, const char *base, int64_t stride, int tile) {  // a tile's keys or values; zeros past the end
         for (int e = tid; e < kKeys32 * DP / 4; e += kThreads32) {
-            const int r = e / (DP / 4), c = e % (DP / 4), row = it.tile(tile) * kKeys32 + r;
+            const int r = e / (DP / 4), c = e % (DP / 4), row = it.key(tile) + r;
             const bool live = row < it.x.m && 4 * c < a.dim;
             copy16(&to[r][4 * c], live ? base + (it.x.k0 + row) * stride + c * 16 : base, live);
         }
@@ -432,14 +440,14 @@ __global__ void __launch_bounds__(kThreads32, 3) k_window32(const __grid_constan
             }
         }
         float s[kMine][2];
-        const int first = it.tile(j) * kKeys32 + tx;
+        const int first = it.key(j) + tx, past = it.past(j);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             float top = -INFINITY;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 const int key = first + 16 * y;
-                const bool seen = key <= pos[i] && (a.window == 0 || pos[i] - key < a.window || key < a.sinks);
+                const bool seen = key <= pos[i] && key < past && (a.window == 0 || pos[i] - key < a.window || key < a.sinks);
                 s[i][y] = seen ? (dot[i][y].x + dot[i][y].y) * scale : -INFINITY;
                 top = fmaxf(top, s[i][y]);
             }
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = b->tmem, q_tiles = tc::saddr(tiles), stages = q_tiles + 2 * S::kQBytes;
-    Item it;
+    Item<kKeys> it;
     bool ok = true;
     // 384 threads start with 168 registers each; a softmax thread holds a row of 128 scores
     // and takes 216, of what the third warpgroup gives: 2 x 216 + 72 = 3 x 168.
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                     expect(&b->kv_full[st], S::kStageBytes);
                     for (int h = 0; h < S::kHalves; ++h)
                         load_box(stages + st * S::kStageBytes + h * kHalfK, map, h * 64, it.kh,
-                                 it.x.k0 + it.tile(j) * kKeys, &b->kv_full[st]);
+                                 it.x.k0 + it.key(j), &b->kv_full[st]);
                     ++issued;
                     return true;
                 };
@@ -714,8 +722,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 settle(s);
                 uint32_t used = 0;  // the quarters to work on
                 if (kHides) {
-                    const int kb = it.tile(j) * kKeys;
-                    const int high = p - kb, low = a.window ? high - a.window + 1 : 0, front = a.sinks - kb;
+                    const int kb = it.key(j), low = a.window ? p - kb - a.window + 1 : 0, front = a.sinks - kb;
+                    const int high = min(p, it.past(j) - 1) - kb;
 #pragma unroll
                     for (int c = 0; c < kKeys; c += 32) {
                         // a bit for each key that is seen: up to `high`, and from `low` on or in the sinks
@@ -802,8 +810,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 return true;
             };
             for (int j = 0; j < n && ok; ++j, ++done) {
-                const int kb = it.tile(j) * kKeys;
-                ok = kb + kKeys - 1 > p_low || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)
+                const int kb = it.key(j);
+                ok = kb + kKeys - 1 > min(p_low, it.past(j) - 1) || (a.window && kb <= p_high - a.window && kb + kKeys > a.sinks)
                          ? step(j, std::true_type())
                          : step(j, std::false_type());
             }
