@@ -31,6 +31,7 @@ struct AppendArgs {
     const int *lengths, *offsets;
     int64_t length_stride, offset_stride;
     int tokens, batch, heads, pieces;  // pieces: 16-byte pieces of a row
+    int team, share;  // warps that work together, and their tokens
 };
 
 // The sequence that owns packed row i: the last s with offsets[s] <= i; -1 if its
@@ -45,40 +46,57 @@ __device__ int sequence_of(const int *offsets, int64_t stride, int batch, int i)
     return lo >= 0 && __ldg(offsets + (lo + 1) * stride) > i ? lo : -1;
 }
 
-// One warp per token: its place is found once, then its heads' pieces are copied, four of the
-// keys and four of the values in flight a lane.
-__global__ void __launch_bounds__(256) k_append(AppendArgs a) {
-    const int token = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (token >= a.tokens) return;
-    int s = token, behind = 1;  // rows from this one to the sequence's end
-    if (a.offsets) {
-        s = sequence_of(a.offsets, a.offset_stride, a.batch, token);
-        if (s < 0) return;
-        behind = __ldg(a.offsets + (s + 1) * a.offset_stride) - token;
+// `team` warps take `share` tokens (kOne: one), few where rows are long: a lane finds one token's
+// place, then all copy the rows' pieces, four of the keys and four of the values in flight a lane.
+template <bool kOne>
+__global__ void __launch_bounds__(256, 4) k_append(const __grid_constant__ AppendArgs a) {
+    const int lane = threadIdx.x % 32, warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int first = warp / a.team * a.share;
+    const int mine = first + lane, n = a.heads * a.pieces;
+    if (first >= a.tokens) return;
+    int64_t kr = -1, vr = -1;
+    if (lane < a.share && mine < a.tokens) {
+        int s = mine, behind = 1;  // rows from this one to the sequence's end
+        if (a.offsets) {
+            s = sequence_of(a.offsets, a.offset_stride, a.batch, mine);
+            if (s >= 0) behind = __ldg(a.offsets + (s + 1) * a.offset_stride) - mine;
+        }
+        const int t = s >= 0 ? __ldg(a.lengths + s * a.length_stride) - behind : -1;
+        if (t >= 0) {
+            kr = a.pages.row(s, t, a.k.page, a.k.row);
+            vr = a.pages.row(s, t, a.v.page, a.v.row);
+        }
     }
-    const int t = __ldg(a.lengths + s * a.length_stride) - behind;
-    if (t < 0) return;
-    const int64_t kr = a.pages.row(s, t, a.k.page, a.k.row), vr = a.pages.row(s, t, a.v.page, a.v.row);
-    if (kr < 0) return;
-    const int n = a.heads * a.pieces;
     constexpr int kFlight = 4;
-    const char *keys = a.keys + token * a.key_token, *values = a.values + token * a.value_token;
-    for (int i0 = lane; i0 < n; i0 += 32 * kFlight) {
+    const int all = min(a.share, a.tokens - first) * n;
+    if (kOne) {
+        kr = __shfl_sync(0xffffffffu, kr, 0);
+        vr = __shfl_sync(0xffffffffu, vr, 0);
+        if (kr < 0) return;
+    }
+    for (int e0 = lane + warp % a.team * 32 * kFlight; e0 - lane < all; e0 += 32 * kFlight * a.team) {
         uint4 x[kFlight], y[kFlight];
-        int64_t at[kFlight];
+        char *to_k[kFlight], *to_v[kFlight];
 #pragma unroll
-        for (int e = 0; e < kFlight; ++e) {
-            const int i = min(i0 + 32 * e, n - 1), h = i / a.pieces, c = (i - h * a.pieces) * 16;
-            x[e] = *reinterpret_cast<const uint4 *>(keys + h * a.key_head + c);
-            y[e] = *reinterpret_cast<const uint4 *>(values + h * a.value_head + c);
-            at[e] = static_cast<int64_t>(h) << 32 | c;
+        for (int f = 0; f < kFlight; ++f) {
+            const int e = min(e0 + 32 * f, all - 1), token = kOne ? 0 : e / n, i = e - token * n;
+            const int h = i / a.pieces, c = (i - h * a.pieces) * 16;
+            const int64_t k = kOne ? kr : __shfl_sync(0xffffffffu, kr, token);
+            const int64_t v = kOne ? vr : __shfl_sync(0xffffffffu, vr, token);
+            const bool there = k >= 0 && e0 + 32 * f < all;
+            to_k[f] = there ? a.k.base + k + h * a.k.head + c : nullptr;
+            to_v[f] = a.v.base + v + h * a.v.head + c;
+            x[f] = y[f] = make_uint4(0, 0, 0, 0);
+            if (there) {
+                x[f] = *reinterpret_cast<const uint4 *>(a.keys + (first + token) * a.key_token + h * a.key_head + c);
+                y[f] = *reinterpret_cast<const uint4 *>(a.values + (first + token) * a.value_token + h * a.value_head + c);
+            }
         }
 #pragma unroll
-        for (int e = 0; e < kFlight; ++e)
-            if (i0 + 32 * e < n) {
-                const int64_t h = at[e] >> 32, c = at[e] & 0xffffffff;
-                *reinterpret_cast<uint4 *>(a.k.base + kr + h * a.k.head + c) = x[e];
-                *reinterpret_cast<uint4 *>(a.v.base + vr + h * a.v.head + c) = y[e];
+        for (int f = 0; f < kFlight; ++f)
+            if (to_k[f]) {
+                *reinterpret_cast<uint4 *>(to_k[f]) = x[f];
+                *reinterpret_cast<uint4 *>(to_v[f]) = y[f];
             }
     }
 }
@@ -393,8 +411,14 @@ extern "C" int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_a
     a.batch = static_cast<int>(batch);
     a.heads = static_cast<int>(keys->shape[1]);
     a.pieces = static_cast<int>(keys->shape[2] * size / 16);
-    const int warps = a.tokens < 4 * ctx->sm_count ? 1 : 8;  // few tokens: a CTA each, over all SMs
-    k_append<<<(a.tokens - 1) / warps + 1, warps * 32, 0, ctx->stream>>>(a);
+    // Few tokens: a CTA each, its warps sharing the row.  Else as many to a warp as make about 128
+    // pieces of each pool (79000 tokens of 18 pieces: 19 us, 62 with one each).
+    const int pieces = a.heads * a.pieces;
+    const bool few = a.tokens < 4 * ctx->sm_count;
+    a.share = few ? 1 : std::max(1, std::min(32, 128 / pieces));
+    a.team = few ? std::max(1, std::min(8, pieces / 128)) : 1;
+    const int warps = few ? a.team : 8, each = warps / a.team * a.share;
+    (a.share == 1 ? k_append<true> : k_append<false>)<<<(a.tokens - 1) / each + 1, warps * 32, 0, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
     return MR_OK;
 }

@@ -395,6 +395,32 @@ def test_append_pages(served, dtype, kv, dim, page):
         assert torch.equal(pool, was)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kv, dim, page", [(3, 24, 16), (1, 8, 5), (6, 64, 32)])
+def test_append_many_rows(served, dtype, kv, dim, page):
+    import torch
+    total, counts = [410, 0, 520, 3, 90], [410, 0, 407, 3, 0]
+    cache = Cache(total, page, kv, dim, dtype, garbage=7.0)
+    want = cache.keys.clone(), cache.values.clone()
+    for s, (n, c) in enumerate(zip(total, counts)):
+        for t in range(n - c, n):
+            for pool in (cache.keys, cache.values):
+                pool[int(cache.table[s, t // page]), t % page] = 7.0
+    new = [torch.cat([r[i][len(r[i]) - c:] for r, c in zip(cache.rows, counts)] + [cache.rows[0][i][:40] * NAN])
+           for i in range(2)]
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    cache.table[2, 200 // page] = 1 << 29   # a bad page: its rows are passed over
+    bad = slice(200 // page * page, 200 // page * page + page)
+    served.append_pages(*new, cache.keys, cache.values, cache.table, cache.lengths, offsets)
+    first = 520 - 407
+    for pool, was, r in zip((cache.keys, cache.values), want, cache.rows[2]):
+        hidden = [t for t in range(bad.start, bad.stop) if t >= first]
+        same = (pool == was).all(-1).all(-1)
+        assert int((~same).sum()) == len(hidden)          # the rows of the bad page's own place alone
+        assert (pool[~same] == 7.0).all()
+        assert torch.equal(was[~same], r[hidden])
+
+
 # ---- eviction -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kv, dim, page, lengths, budget, sinks, recent", [
