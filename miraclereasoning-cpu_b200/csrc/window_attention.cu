@@ -22,7 +22,7 @@
 // What bounds it: a 128 x 128 tile's exponentials (head dim 128) take the special-function
 // unit 1024 cycles, its two products the tensor cores as many.  One tile's softmax runs
 // beside the other's products; with two softmax warps a scheduler, each unit is busy 57% of
-// the time (ncu, flashlite's 8192-token context: 228 us, 1.2 PFLOP/s).  Measured and left out:
+// the time (ncu, flashlite's 8192-token context: 232 us, 1.2 PFLOP/s).  Measured and left out:
 // a quarter of the exponentials by polynomials (no faster at head dim 64, 15% slower at 128),
 // key tiles of 64 with the next scores worked out ahead (290 us), two threads a row (314 us),
 // P beside S where TMEM has room (head dim 64: no difference).
