@@ -119,8 +119,14 @@ struct EvictArgs {
 // Weights in rising order as unsigned numbers; both zeros equal, NaN the lowest.
 __device__ __forceinline__ uint32_t rank_key(float w) {
     if (w != w) return 0;
-    const uint32_t bits = __float_as_uint(w == 0.f ? 0.f : w);
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    const uint32_t bits = __float_as_uint(w + 0.f);  // -0 becomes 0
+    return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
+}
+
+__device__ __forceinline__ void cp_async4(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from)
+                 : "memory");
 }
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048, kCached = 48 << 10;
@@ -129,15 +135,17 @@ constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins =
 // the `budget` largest stay: the value of the last of them is found digit by digit, 11, 11
 // and 10 bits of the weights' order: counts of a digit among the rows that match the digits
 // found so far, and the highest digit that has the wanted row.  (The first 11 bits are sign,
-// exponent and two bits of the fraction, so that weights of all sizes fall on many counters; 128
-// rows that all fall on one, as after a reset, are counted at once.)  Rows above that value
-// stay, and the first few equal to it.  Then each warp counts its own stretch of the rows,
+// exponent and two bits of the fraction, so that weights of all sizes fall on many counters; a
+// warp's rows that all fall on one, as after a reset, are counted at once.)  Rows above that
+// value stay, and the first few equal to it.  Then each warp counts its own stretch of the rows,
 // and writes its kept rows in order behind those of the warps before it.
 //
-// The weights' order is kept in shared memory after the first read where it fits, four rows a
-// lane and access.  Every instruction here runs a few times at most, and a warp waits hundreds of
-// cycles for code that it meets first: the loops stay rolled (unrolled by eight, 12000 weights
-// took 40 us).
+// The weights come to shared memory where they fit, by asynchronous copies, and are their order
+// from the first count on.  20000 weights are 625 issues of the SM for each instruction that is
+// written once a weight: 4.0 us until they are there, 7.6 for the digits, 1.3 for the stretches'
+// counts, 4.2 for their rows and 1.4 for the kept weights.  What runs only a few times costs the
+// fetch of its code, hundreds of cycles a line: the loops stay rolled (loads unrolled by eight
+// took 6.0 us instead of the 4.0, and by eight everywhere 12000 weights took 40).
 __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant__ EvictArgs a) {
     __shared__ int counts[kBins];
     __shared__ int above[kSelectWarps], equal[kSelectWarps];
@@ -148,47 +156,47 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int n = sequence_rows(a.lengths, a.length_stride, s, a.capacity);
+    for (int i = tid; i < kBins; i += kSelectThreads) counts[i] = 0;
     const float *w = a.weights + s * a.w_batch + h * a.w_head;
     int *kept = a.kept + s * a.kept_batch + h * a.kept_head;
     float *nw = a.new_weights + s * a.nw_batch + h * a.nw_head;
     const int total = min(n, a.budget);
     if (tid == 0 && h == 0) a.new_lengths[s * a.new_length_stride] = total;
-    auto order = [&](int t, float x) {  // rows past the end: 0, and told apart by their number
-        return t >= n ? 0u : t < a.sinks || t >= n - a.recent ? 0xffffffffu : rank_key(x);
-    };
-    auto read = [&](int t) { return t < n ? order(t, __ldg(w + t)) : 0u; };
     const bool in_shared = a.capacity <= kCached;
+    const uint32_t ranked = max(n - a.recent, a.sinks) - a.sinks;  // rows behind the sinks, before the recent ones
+    auto order = [&](int t, float x) { return static_cast<uint32_t>(t - a.sinks) < ranked ? rank_key(x) : 0xffffffffu; };
+    // rows past the end: 0, and told apart by their number
+    auto read = [&](int t) { return t < n ? order(t, __ldg(w + t)) : 0u; };
+    auto one_of = [&](int t) { return in_shared ? cached[t] : read(t); };
     auto four = [&](int t) {
         return in_shared ? *reinterpret_cast<const uint4 *>(cached + t)
                          : make_uint4(read(t), read(t + 1), read(t + 2), read(t + 3));
     };
-    if (in_shared) {
-        const int end = (n + 3) & ~3;
-        constexpr int kFlight = 8;
+    if (in_shared && n > a.budget) {
 #pragma unroll 1
-        for (int t = tid; t < end; t += kSelectThreads * kFlight) {
-            float x[kFlight];
-#pragma unroll
-            for (int i = 0; i < kFlight; ++i) x[i] = __ldg(w + min(t + i * kSelectThreads, n - 1));
-#pragma unroll
-            for (int i = 0; i < kFlight; ++i)
-                if (t + i * kSelectThreads < end) cached[t + i * kSelectThreads] = order(t + i * kSelectThreads, x[i]);
-        }
-        __syncthreads();
+        for (int t = tid; t < n; t += kSelectThreads) cp_async4(cached + t, w + t);
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    uint32_t cut = 0;  // rows of a larger key stay, and `ties` of those equal to it
-    int ties = n;
+    __syncthreads();
     if (n > a.budget) {
+        uint32_t cut = 0;  // rows of a larger key stay, and `need` of those equal to it
         int need = a.budget;
 #pragma unroll 1
         for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
             const int bits = shift ? 11 : 10, bins = 1 << bits;
-            for (int i = tid; i < bins; i += kSelectThreads) counts[i] = 0;
-            __syncthreads();
+            if (shift != 21) {
+                for (int i = tid; i < bins; i += kSelectThreads) counts[i] = 0;
+                __syncthreads();
+            }
 #pragma unroll 1
             for (int t = 4 * tid; t - 4 * lane < n; t += 4 * kSelectThreads) {
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (t < n) x = four(t);
+                if (shift == 21 && in_shared && t < n) {  // weights as they came: their order from here on
+                    auto key_of = [&](int i, uint32_t raw) { return t + i < n ? order(t + i, __uint_as_float(raw)) : 0u; };
+                    x = make_uint4(key_of(0, x.x), key_of(1, x.y), key_of(2, x.z), key_of(3, x.w));
+                    *reinterpret_cast<uint4 *>(cached + t) = x;
+                }
                 const uint32_t key[4] = {x.x, x.y, x.z, x.w};
                 const uint32_t one = __shfl_sync(0xffffffffu, x.x >> shift, 0);
                 if (__all_sync(0xffffffffu, t + 3 < n && x.x >> shift == one && x.y >> shift == one &&
@@ -236,59 +244,47 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
             cut = cut << bits | s_digit;
             need = s_need;
         }
-        ties = need;
-    }
-    // a warp's stretch: rows to keep, and rows equal to the cut (in the upper half of a count), four a lane
-    auto marks = [&](int t, uint4 &x) {
-        x = t < n ? four(t) : make_uint4(0, 0, 0, 0);
-        const uint32_t key[4] = {x.x, x.y, x.z, x.w};
-        int count = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) count += (key[i] > cut ? 1 : 0) + (key[i] == cut && t + i < n ? 1 << 16 : 0);
-        return count;
-    };
-    const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 127) & ~127, lo = warp * stretch, hi = min(lo + stretch, n);
-    int kept_before = 0, equal_before = 0;
+        // a warp's stretch: rows to keep, and rows equal to the cut
+        const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 127) & ~127, lo = warp * stretch, hi = min(lo + stretch, n);
+        int kept_before = 0, equal_before = 0;
 #pragma unroll 1
-    for (int t = lo + 4 * lane; t < hi; t += 128) {
-        uint4 x;
-        const int count = marks(t, x);
-        kept_before += count & 0xffff;
-        equal_before += count >> 16;
-    }
-    kept_before = __reduce_add_sync(0xffffffffu, kept_before);
-    equal_before = __reduce_add_sync(0xffffffffu, equal_before);
-    __syncthreads();  // above[] of the last digit has been read
-    if (lane == 0) {
-        above[warp] = kept_before;
-        equal[warp] = equal_before;
-    }
-    __syncthreads();
-    kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
-    equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
+        for (int t = lo + 4 * lane; t < hi; t += 128) {
+            const uint4 x = four(t);
+            const uint32_t key[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                kept_before += key[i] > cut;
+                equal_before += key[i] == cut && t + i < n;
+            }
+        }
+        kept_before = __reduce_add_sync(0xffffffffu, kept_before);
+        equal_before = __reduce_add_sync(0xffffffffu, equal_before);
+        __syncthreads();  // above[] of the last digit has been read
+        if (lane == 0) {
+            above[warp] = kept_before;
+            equal[warp] = equal_before;
+        }
+        __syncthreads();
+        kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
+        equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
+        const uint32_t below = (1u << lane) - 1;
+        int base = kept_before + min(equal_before, need);
 #pragma unroll 1
-    for (int t = lo + 4 * lane; t - 4 * lane < hi; t += 128) {
-        uint4 x;
-        const int count = marks(t, x);
-        int sum = count;  // of the lanes up to this one
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int below = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += below;
+        for (int t = lo + lane; t - lane < hi; t += 32) {
+            const uint32_t key = t < hi ? one_of(t) : 0u;
+            bool stays = key > cut;
+            const uint32_t sames = __ballot_sync(0xffffffffu, key == cut && t < hi);
+            if (sames) {
+                stays = stays || (key == cut && t < hi && equal_before + __popc(sames & below) < need);
+                equal_before += __popc(sames);
+            }
+            const uint32_t all = __ballot_sync(0xffffffffu, stays);
+            const int at = base + __popc(all & below);
+            if (stays && at < a.budget) kept[at] = t;
+            base += __popc(all);
         }
-        int over = kept_before + ((sum - count) & 0xffff), eq = equal_before + ((sum - count) >> 16);
-        const uint32_t key[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool same = key[i] == cut && t + i < n, more = key[i] > cut;
-            const int at = over + min(eq, ties);
-            if ((more || (same && eq < ties)) && at < a.budget) kept[at] = t + i;
-            over += more;
-            eq += same;
-        }
-        const int all = __shfl_sync(0xffffffffu, sum, 31);
-        kept_before += all & 0xffff;
-        equal_before += all >> 16;
+    } else {
+        for (int i = tid; i < n; i += kSelectThreads) kept[i] = i;
     }
 #pragma unroll 1
     for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
