@@ -123,13 +123,15 @@ __device__ __forceinline__ uint32_t rank_key(float w) {
     return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ void cp_async4(void *to, const void *from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
-                 "l"(from)
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from), "n"(BYTES)
                  : "memory");
 }
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins = 2048, kCached = 48 << 10;
+constexpr int kMarked = 28;  // rows that a thread marks at once
 
 // CTA = (sequence, head).  The sinks and the recent rows take part as the largest of all, so
 // the `budget` largest stay: the value of the last of them is found digit by digit, 11, 11
@@ -137,18 +139,19 @@ constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32, kBins =
 // found so far, and the highest digit that has the wanted row.  (The first 11 bits are sign,
 // exponent and two bits of the fraction, so that weights of all sizes fall on many counters; a
 // warp's rows that all fall on one, as after a reset, are counted at once.)  Rows above that
-// value stay, and the first few equal to it.  Then each warp counts its own stretch of the rows,
-// and writes its kept rows in order behind those of the warps before it.
+// value stay, and the first few equal to it.  Then each thread marks a few rows of its own, and
+// the kept ones go in order behind those of the threads before it.
 //
 // The weights come to shared memory where they fit, by asynchronous copies, and are their order
 // from the first count on.  20000 weights are 625 issues of the SM for each instruction that is
-// written once a weight: 4.0 us until they are there, 7.6 for the digits, 1.3 for the stretches'
-// counts, 4.2 for their rows and 1.4 for the kept weights.  What runs only a few times costs the
-// fetch of its code, hundreds of cycles a line: the loops stay rolled (loads unrolled by eight
-// took 6.0 us instead of the 4.0, and by eight everywhere 12000 weights took 40).
+// written once a weight: 3.1 us until they are there, 7.5 for the digits, 3.2 for the rows that
+// stay and 1.5 for their weights.  (Votes and counts of bits for every 32 rows in turn took 5.4 us
+// instead of the 3.2, whether the rows were stored one by one or in lines.)  What runs only a few
+// times costs the fetch of its code, hundreds of cycles a line: the loops stay rolled (loads
+// unrolled by eight took 6.0 us instead of 3.1, and by eight everywhere 12000 weights took 40).
 __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant__ EvictArgs a) {
     __shared__ int counts[kBins];
-    __shared__ int above[kSelectWarps], equal[kSelectWarps];
+    __shared__ int above[kSelectWarps];
     __shared__ uint32_t s_digit;
     __shared__ int s_need;
     extern __shared__ __align__(16) uint32_t cached[];
@@ -167,14 +170,16 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
     auto order = [&](int t, float x) { return static_cast<uint32_t>(t - a.sinks) < ranked ? rank_key(x) : 0xffffffffu; };
     // rows past the end: 0, and told apart by their number
     auto read = [&](int t) { return t < n ? order(t, __ldg(w + t)) : 0u; };
-    auto one_of = [&](int t) { return in_shared ? cached[t] : read(t); };
     auto four = [&](int t) {
         return in_shared ? *reinterpret_cast<const uint4 *>(cached + t)
                          : make_uint4(read(t), read(t + 1), read(t + 2), read(t + 3));
     };
     if (in_shared && n > a.budget) {
+        const int fours = reinterpret_cast<uintptr_t>(w) % 16 ? 0 : n & ~3;
 #pragma unroll 1
-        for (int t = tid; t < n; t += kSelectThreads) cp_async4(cached + t, w + t);
+        for (int t = 4 * tid; t < fours; t += 4 * kSelectThreads) cp_async<16>(cached + t, w + t);
+#pragma unroll 1
+        for (int t = fours + tid; t < n; t += kSelectThreads) cp_async<4>(cached + t, w + t);
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
     __syncthreads();
@@ -244,44 +249,58 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
             cut = cut << bits | s_digit;
             need = s_need;
         }
-        // a warp's stretch: rows to keep, and rows equal to the cut
-        const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 127) & ~127, lo = warp * stretch, hi = min(lo + stretch, n);
+        // Rows that stay, in order: a thread's own few rows become two masks, larger than the cut and
+        // equal to it, whose counts (below 2^15 in a part of the rows) are added up over the CTA in
+        // the halves of one number.  From shared memory, a warp's kept rows are gathered where its
+        // keys were, and stored in whole lines.
         int kept_before = 0, equal_before = 0;
 #pragma unroll 1
-        for (int t = lo + 4 * lane; t < hi; t += 128) {
-            const uint4 x = four(t);
-            const uint32_t key[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                kept_before += key[i] > cut;
-                equal_before += key[i] == cut && t + i < n;
-            }
-        }
-        kept_before = __reduce_add_sync(0xffffffffu, kept_before);
-        equal_before = __reduce_add_sync(0xffffffffu, equal_before);
-        __syncthreads();  // above[] of the last digit has been read
-        if (lane == 0) {
-            above[warp] = kept_before;
-            equal[warp] = equal_before;
-        }
-        __syncthreads();
-        kept_before = __reduce_add_sync(0xffffffffu, lane < warp ? above[lane] : 0);
-        equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? equal[lane] : 0);
-        const uint32_t below = (1u << lane) - 1;
-        int base = kept_before + min(equal_before, need);
+        for (int part = 0; part < n; part += kSelectThreads * kMarked) {
+            // vectors of four a thread: an odd number, so that eight threads' meet all banks
+            const int mine = min(((n - part + kSelectThreads - 1) / kSelectThreads + 3) / 4 | 1, kMarked / 4) * 4;
+            const int lo = part + warp * 32 * mine, from = lo + lane * mine;
+            uint32_t stay = 0, same = 0;
 #pragma unroll 1
-        for (int t = lo + lane; t - lane < hi; t += 32) {
-            const uint32_t key = t < hi ? one_of(t) : 0u;
-            bool stays = key > cut;
-            const uint32_t sames = __ballot_sync(0xffffffffu, key == cut && t < hi);
-            if (sames) {
-                stays = stays || (key == cut && t < hi && equal_before + __popc(sames & below) < need);
-                equal_before += __popc(sames);
+            for (int i = 0; i < mine && from + i < n; i += 4) {
+                const uint4 x = four(from + i);
+                const uint32_t key[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    stay |= (key[e] > cut ? 1u << e : 0u) << i;
+                    same |= (key[e] == cut && from + i + e < n ? 1u << e : 0u) << i;
+                }
             }
-            const uint32_t all = __ballot_sync(0xffffffffu, stays);
-            const int at = base + __popc(all & below);
-            if (stays && at < a.budget) kept[at] = t;
-            base += __popc(all);
+            const int count = __popc(stay) + (__popc(same) << 16);
+            int sum = count;  // of the lanes up to this one
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int under = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += under;
+            }
+            __syncthreads();  // above[] of the part before, or of the last digit, has been read
+            if (lane == 31) above[warp] = sum;
+            __syncthreads();
+            const int warps = above[lane], under = __reduce_add_sync(0xffffffffu, lane < warp ? warps : 0);
+            const int all = __reduce_add_sync(0xffffffffu, warps);
+            const int first = kept_before + (under & 0xffff) + min(equal_before + (under >> 16), need);
+            sum += under - count;
+            const int equals = equal_before + (sum >> 16);  // rows equal to the cut before this thread's
+            int at = kept_before + (sum & 0xffff) + min(equals, need);
+            for (int room = need - equals; same && room > 0; same &= same - 1, --room) stay |= same & -same;
+            kept_before += all & 0xffff;
+            equal_before += all >> 16;
+#pragma unroll 1
+            for (; stay; stay &= stay - 1, ++at) {
+                const int row = from + __ffs(stay) - 1;
+                if (in_shared) cached[lo + at - first] = row;
+                else if (at < a.budget) kept[at] = row;
+            }
+            if (in_shared) {
+                at = __shfl_sync(0xffffffffu, at, 31);
+                __syncwarp();
+#pragma unroll 1
+                for (int i = first + lane; i < min(at, a.budget); i += 32) kept[i] = static_cast<int>(cached[lo + i - first]);
+            }
         }
     } else {
         for (int i = tid; i < n; i += kSelectThreads) kept[i] = i;

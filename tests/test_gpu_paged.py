@@ -462,6 +462,43 @@ def test_evict_pages(served, dtype, kv, dim, page, lengths, budget, sinks, recen
                 assert (moved[len(rows):] == 7.0).all()
 
 
+@pytest.mark.parametrize("rows,lengths,budget,sinks,recent,skew", [
+    (40000, [40000, 28672, 28673, 4097], 20000, 4, 300, 0),   # more rows than the CTA marks at once
+    (49152, [49152, 49151, 1], 49000, 0, 0, 0),               # the most that shared memory takes
+    (60000, [60000, 57345, 33, 0], 31, 1, 2, 0),              # more than it takes
+    (60000, [60000, 40001], 59000, 0, 1, 1),
+    (5001, [5001, 3999, 2], 1000, 0, 0, 1),                   # weights on no 16-byte boundary, odd lengths
+    (5001, [5001, 129], 5000, 2500, 2500, 3),
+])
+def test_eviction_chooses_among_many_rows(served, rows, lengths, budget, sinks, recent, skew):
+    """Which rows are kept, with ties over all threads, weights alike in a whole head and strided rows of weights."""
+    import torch
+    heads, page = 3, 8
+    pages = -(-rows // page)
+    rng = np.random.default_rng(7)
+    weights = (rng.random((len(lengths), heads, pages * page)) ** 4).astype(np.float32)
+    weights[:, 0] = np.round(weights[:, 0] * 16) / 16
+    weights[:, 1] = 0.0
+    held = torch.zeros(len(lengths), heads, pages * page + skew, device="cuda")
+    held[:, :, skew:] = torch.tensor(weights)
+    keys = torch.zeros(pages, page, heads, 8, device="cuda", dtype=torch.bfloat16)
+    room = -(-budget // page)
+    target = torch.arange(len(lengths) * room, dtype=torch.int32, device="cuda").view(len(lengths), room)
+    pools = [torch.empty(len(lengths) * room, page, heads, 8, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(len(lengths), 1)
+    kept, new_lengths, new_weights = served.evict_pages(
+        keys, keys, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), held[:, :, skew:], target, budget=budget,
+        sinks=sinks, recent=recent, target_keys=pools[0], target_values=pools[1])
+    kept, new_weights = kept.cpu().numpy(), new_weights.cpu().numpy()
+    assert new_lengths.tolist() == [min(n, budget) for n in lengths]
+    for s, n in enumerate(lengths):
+        for h in range(heads):
+            want = ref.evict(weights[s, h], n, budget, sinks, recent)
+            assert kept[s, h].tolist() == want + [-1] * (budget - len(want))
+            np.testing.assert_array_equal(new_weights[s, h, :len(want)], weights[s, h, want])
+            assert not new_weights[s, h, len(want):].any()
+
+
 def test_eviction_within_one_pool_and_past_bad_pages(served):
     import torch
     cache = Cache([60, 50], 8, 2, 32, "float16", extra=8)
