@@ -285,10 +285,15 @@ def _plain_evict(s):
 
 # ---- the framework's calls ----------------------------------------------------------------------------------------
 @functools.cache
-def _backend():
-    """The program's backend, on the stream that torch works on."""
+def _backend_on(device, stream):
     package = importlib.import_module("miraclereasoning-cpu_b200")
-    return package.CUDABackend(stream=torch.cuda.current_stream().cuda_stream)
+    return package.CUDABackend(device_index=device, stream=stream)
+
+
+def _backend():
+    """The program's backend of the device and the stream that torch works on at this call."""
+    stream = torch.cuda.current_stream()
+    return _backend_on(stream.device_index, stream.cuda_stream)
 
 
 def _own_paged(s):
