@@ -330,7 +330,12 @@ __global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_cons
     const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % 32;
     const int at = (blockIdx.x * kCopyWarps + threadIdx.x / 32) * 32 + lane;
     const int total = min(sequence_rows(a.lengths, a.length_stride, s, a.capacity), min(a.budget, a.target_rows));
-    if (at - lane >= total) return;
+    if (at - lane >= total) {
+        // waits too: with no rows anywhere, this grid would end, and what is queued behind it start,
+        // while the selection still writes
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     // the target's page is found before the selection is waited for
     int64_t to_k = -1, to_v = -1, k = -1, v = -1;
     if (at < total) {

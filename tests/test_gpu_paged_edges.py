@@ -1,0 +1,39 @@
+"""The paged cache's operators at the edges of what their description allows: empty batches, extreme scalars, small
+weights, infinities in visible rows, waits that give up."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+from conftest import submodule
+from test_gpu_paged import TYPES, Cache, check_paged, check_window, queries, served, wide  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(*values):
+    import torch
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ---- eviction -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lengths", [0, -3])
+def test_an_eviction_of_empty_sequences_is_over_before_what_follows_it(served, lengths):
+    """No row is copied, so that nothing of the copying kernel has work; what it was launched behind still has to end
+    before the next kernels of the stream read its outputs."""
+    import torch
+    batch, heads, page, budget, room = 16, 64, 8, 4096, 1024
+    pool = torch.zeros(4, page, heads, 8, device="cuda", dtype=torch.bfloat16)
+    table = torch.zeros(batch, budget // page, dtype=torch.int32, device="cuda")
+    target = torch.zeros(batch, room, dtype=torch.int32, device="cuda")
+    weights = torch.ones(batch, heads, budget, device="cuda")
+    empty = torch.full((batch,), lengths, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        kept = torch.full((batch, heads, budget), 7, dtype=torch.int32, device="cuda")
+        new_lengths = torch.full((batch,), 7, dtype=torch.int32, device="cuda")
+        new_weights = torch.full((batch, heads, room * page), 7.0, device="cuda")
+        served.evict_pages(pool, pool.clone(), table, empty, weights, target, budget=budget, sinks=2, recent=3,
+                           target_keys=pool.clone(), target_values=pool.clone(), kept=kept, new_lengths=new_lengths,
+                           new_weights=new_weights)
+        # read back to front: the selection's last writes first
+        read = new_weights.flip(0).clone(), kept.flip(0).clone(), new_lengths.clone()
+        assert not read[0].any() and (read[1] == -1).all() and not read[2].any()
