@@ -1017,7 +1017,9 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     a.kv_heads = static_cast<int>(kv_heads);
     a.group = static_cast<int>(heads / kv_heads);
     a.dim = static_cast<int>(query->shape[2]);
-    a.window = window;
+    // A window of all rows hides nothing; a shorter one is below 2^30, as positions are in size, so that
+    // their differences stay within 32 bits.
+    a.window = window < keys->shape[0] ? window : 0;
     a.sinks = sinks;
     // a scale of 0 weighs all visible keys alike, and must leave the hidden ones' -inf alone
     a.scale = scale == 0.f ? 1e-30f : scale;

@@ -37,3 +37,23 @@ def test_an_eviction_of_empty_sequences_is_over_before_what_follows_it(served, l
         # read back to front: the selection's last writes first
         read = new_weights.flip(0).clone(), kept.flip(0).clone(), new_lengths.clone()
         assert not read[0].any() and (read[1] == -1).all() and not read[2].any()
+
+
+# ---- prompts ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8, 12, 11])
+def test_windows_up_to_the_largest_number(served, dtype, window):
+    # more queries than keys (positions below 0), as many, fewer; windows of more, all and all but one of the keys
+    new, keys = [19, 10, 4, 300], [12, 10, 9, 0]
+    q, k, v = (queries(n, h, 64, dtype, seed=n) for n, h in ((sum(new), 4), (sum(keys), 2), (sum(keys) + 1, 2)))
+    qo, ko = (ints(0, *np.cumsum(x).tolist()) for x in (new, keys))
+    got = served.window_attention(q, k, v[:-1], qo, ko, window=window, sinks=1)
+    served.finish()
+    for s in range(4):
+        a, b, c, d = sum(new[:s]), sum(new[:s + 1]), sum(keys[:s]), sum(keys[:s + 1])
+        if c == d:
+            assert not got[a:b].any()
+            continue
+        want, _, mixed, reach = ref.attend(wide(q[a:b]), wide(k[c:d]), wide(v[c:d]), range(d - c - b + a, d - c), 0.125,
+                                           window, 1)
+        assert np.all(np.abs(wide(got[a:b]) - want) <= ref.output_bound(want, mixed, reach, 64, 12, dtype, True))
