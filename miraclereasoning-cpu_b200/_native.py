@@ -59,6 +59,8 @@ SIGNATURES = {
     "mr_context_create_on_stream": (_I, [_I, _P, C.POINTER(_P)]),
     "mr_context_destroy": (_I, [_P]),
     "mr_context_finish": (_I, [_P]),
+    "mr_context_set_wait_limit": (_I, [_P, C.c_uint64]),
+    "mr_context_inject_fault": (_I, [_P, _I]),
     "mr_buffer_alloc": (_I, [_P, _SZ, C.POINTER(_P)]),
     "mr_buffer_free": (_I, [_P]),
     "mr_buffer_count": (_I, [_P, C.POINTER(_SZ)]),

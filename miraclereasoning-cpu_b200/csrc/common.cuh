@@ -48,6 +48,8 @@ struct mr_context {
     void *scratch = nullptr;  // of the calls queued outside a capture, in stream order (context_scratch)
     size_t scratch_bytes = 0;
     int *wait_error = nullptr;  // host word that kernels set when a bounded wait gave up (check_waits)
+    uint64_t wait_limit = 2000000000;  // nanoseconds (mr_context_set_wait_limit)
+    bool withhold = false;    // fault injection for tests (mr_context_inject_fault)
     std::atomic<int> refs{1};
 };
 

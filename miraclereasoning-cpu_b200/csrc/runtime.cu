@@ -144,6 +144,19 @@ int mr_context_finish(mr_context *ctx) {
     return mr::check_waits(ctx);
 }
 
+int mr_context_set_wait_limit(mr_context *ctx, uint64_t nanoseconds) {
+    MR_REQUIRE(ctx, "ctx is NULL");
+    MR_REQUIRE(nanoseconds >= 1000000, "a wait limit below 1 ms");
+    ctx->wait_limit = nanoseconds;
+    return MR_OK;
+}
+
+int mr_context_inject_fault(mr_context *ctx, int on) {
+    MR_REQUIRE(ctx, "ctx is NULL");
+    ctx->withhold = on != 0;
+    return MR_OK;
+}
+
 int mr_buffer_alloc(mr_context *ctx, size_t count, mr_buffer **out) {
     MR_REQUIRE(ctx && out, "NULL argument");
     MR_REQUIRE(count > 0, "invalid buffer size 0");

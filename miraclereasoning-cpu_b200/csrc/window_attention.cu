@@ -52,6 +52,8 @@ struct WindowArgs {
     int tokens, rows, batch, heads, kv_heads, group, dim, window, sinks;
     float scale;
     int *gave_up;    // host word of the context
+    uint64_t limit;  // of a wait: the context's, and what a warp may take to work 32 rows out again alone
+    int withhold;    // fault injection: no values are loaded
 };
 
 // Where sequence s lies, cut to the arrays: first query, queries, first key, keys.
@@ -137,13 +139,12 @@ struct Maps {
 
 // Shared memory behind the tiles.
 struct Barriers {
-    uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
+    uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_done[2], turn[2], drained[2];
     uint32_t tmem;
     int stop;  // a wait gave up: every role leaves
 };
 
-// A bounded wait; false when it gives up, or another role has.  (`limit`: two seconds, and what a warp may
-// take to work 32 rows out again alone.)
+// A bounded wait; false when it gives up, or another role has.
 __device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up, uint64_t limit) {
     if (tc::try_wait(bar, parity)) return true;
     const uint64_t start = tc::now();
@@ -157,6 +158,15 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, int parity, Barriers *b,
                 return false;
             }
         }
+    }
+}
+// The same by a whole warp, which goes on or gives up together.
+__device__ __forceinline__ bool warp_wait_for(uint64_t *bar, int parity, Barriers *b, int *gave_up, uint64_t limit) {
+    return __all_sync(0xffffffffu, wait_for(bar, parity, b, gave_up, limit));
+}
+// A bounded wait for what is in flight, whoever has given up; `unless`: where it may not come.
+__device__ __forceinline__ void wait_in_flight(uint64_t *bar, int parity, uint64_t start, volatile int *unless = nullptr) {
+    while (!tc::try_wait(bar, parity) && !(unless && *unless) && tc::now() - start < tc::kWaitNs) {
     }
 }
 // One lane of a converged warp.
@@ -559,6 +569,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             init(&b->p_full[i], 4);
             init(&b->o_done[i], 1);
             init(&b->turn[i], 4);
+            init(&b->drained[i], 1);
         }
         b->stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -571,7 +582,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v) : "memory");
     Items<kKeys> items;
     items.init(a, 2 * per);
-    const uint64_t limit = tc::kWaitNs + min(4000ull * a.rows, 8 * tc::kWaitNs);
+    const uint64_t limit = a.limit;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -607,24 +618,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                     ++issued;
                     return true;
                 };
-                for (int j = 0; j < it.tiles && ok; ++j) ok = load(&maps.k, j) && load(&maps.v, j);
+                for (int j = 0; j < it.tiles && ok; ++j) ok = load(&maps.k, j) && !a.withhold && load(&maps.v, j);
             }
             ok = __shfl_sync(0xffffffffu, ok, 0);
         }
         if (lane == 0) {
-            // no copy may land after the CTA has left (the last stages; those before were waited for by the products)
+            // no copy may land after the CTA has left (the last stages; those before were waited for by the products),
+            // and no arrival of the products
             const uint64_t start = tc::now();
-            if (count > 0)
-                while (!tc::try_wait(&b->q_full, (count - 1) & 1) && tc::now() - start < tc::kWaitNs) {
-                }
+            if (count > 0) wait_in_flight(&b->q_full, (count - 1) & 1, start);
             for (int i = max(0, issued - S::kStages); i < issued; ++i)
-                while (!tc::try_wait(&b->kv_full[i % S::kStages], (i / S::kStages) & 1) && tc::now() - start < tc::kWaitNs) {
-                }
+                wait_in_flight(&b->kv_full[i % S::kStages], (i / S::kStages) & 1, start);
+            if (count > 0) wait_in_flight(&b->q_empty, (count - 1) & 1, start, &b->stop);
+            for (int i = max(0, issued - S::kStages); i < issued; ++i)
+                wait_in_flight(&b->kv_empty[i % S::kStages], (i / S::kStages) & 1, start, &b->stop);
         }
     } else if (warp == kMathWarp || warp == kMathWarp + 1) {
         // A warp for each query tile, so that one's waits do not hold up the other's products.
         // All of it walks through them and one lane issues: descriptors stay in uniform
-        // registers, where the instruction wants them.
+        // registers, where the instruction wants them.  A lane whose wait gave up issues nothing more
+        // but walks on; the warp leaves together, by a vote once a step (a vote a wait: 1.5% slower).
         {
             constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
             const uint32_t qk = mma_desc(kBf16, kKeys, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
@@ -633,10 +646,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             const uint32_t s_at = tmem + w * kTile, o_at = tmem + S::kO + w * DP;
             const bool leader = elect();
             int st = 0, fill = 0;  // the next stage, and the parity of its fill
+            bool mine = true;      // none of this lane's waits gave up
             auto take = [&] {
-                if (!wait_for(&b->kv_full[st], fill, b, a.gave_up, limit)) return false;
+                mine = mine && wait_for(&b->kv_full[st], fill, b, a.gave_up, limit);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                return true;
             };
             auto leave = [&] {
                 if (leader) tc::commit(&b->kv_empty[st]);
@@ -648,7 +661,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             };
             auto scores = [&] {
                 const uint64_t k = k_desc + st * (S::kStageBytes >> 4);
-                if (leader) {
+                if (leader && mine) {
 #pragma unroll
                     for (int i = 0; i < DP / 16; ++i)
                         tc::mma(s_at, q + ((i / 4) * kHalfQ + (i % 4) * 32) / 16, k + ((i / 4) * kHalfK + (i % 4) * 32) / 16, qk,
@@ -661,22 +674,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             for (int round = 0; (kRounds || round == 0) && ok && items.get(a, item_of(round), it); ++round) {
                 const int n = it.tiles;
                 if (n == 0) continue;
-                ok = wait_for(&b->q_full, count++ & 1, b, a.gave_up, limit) && take();
-                if (ok) {
-                    scores();
-                    if (n == 1 && leader) tc::commit(&b->q_empty);
-                    leave();
-                }
+                mine = mine && wait_for(&b->q_full, count++ & 1, b, a.gave_up, limit);
+                take();
+                scores();
+                if (n == 1 && leader) tc::commit(&b->q_empty);
+                leave();
                 for (int j = 0; j < n && ok; ++j, ++g) {
-                    ok = take();
+                    take();
                     const uint64_t v = v_desc + st * (S::kStageBytes >> 4);
                     // P comes in two halves; the first is multiplied while the second is worked out
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        ok = ok && wait_for(half ? &b->p_full[w] : &b->p_half[w], g & 1, b, a.gave_up, limit);
-                        if (!ok) break;
+                        mine = mine && wait_for(half ? &b->p_full[w] : &b->p_half[w], g & 1, b, a.gave_up, limit);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        if (leader) {
+                        if (leader && mine) {
 #pragma unroll
                             for (int i = half * kKeys / 32; i < (half + 1) * kKeys / 32; ++i)
                                 mma_ts(o_at, s_at + i * 8, v + i * 128, pv, j > 0 || i > 0);
@@ -685,14 +696,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                         __syncwarp();
                     }
                     leave();
-                    if (ok && j + 1 < n) {
-                        ok = take();
-                        if (ok) scores();
+                    if (j + 1 < n) {
+                        take();
+                        scores();
                         if (j + 2 == n && leader) tc::commit(&b->q_empty);
                         leave();
                     }
+                    ok = __all_sync(0xffffffffu, mine);
                 }
             }
+            // no product may still run when the CTA gives its memory back, whatever made the warp leave
+            if (leader) tc::commit(&b->drained[w]);
+            __syncwarp();
+            wait_in_flight(&b->drained[w], 0, tc::now());
+            __syncwarp();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
     } else if (warp < kLoadWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -714,7 +732,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             // the warp sees are left out.  Two bodies: the scores of either stay in registers of its own.
             auto step = [&](int j, auto hides) {
                 constexpr bool kHides = decltype(hides)::value;
-                if (!__all_sync(0xffffffffu, wait_for(&b->s_full[w], done & 1, b, a.gave_up, limit))) return false;
+                if (!warp_wait_for(&b->s_full[w], done & 1, b, a.gave_up, limit)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t s[kKeys];
 #pragma unroll
@@ -745,7 +763,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                     const float grown = max_nan(m, top);
                     if (j > 0) {
                         // done already, since the scores came behind it
-                        if (!__all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit))) return false;
+                        if (!warp_wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit)) return false;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const float c = m == grown ? 1.f : pow2((m - grown) * scale);
                         l *= c;
@@ -765,7 +783,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 // The two tiles take the special-function unit in turns, a quarter overlapping; otherwise both
                 // settle into doing their exponentials, and then their products, at the same time
                 // (chunked flashnano-1.7 prompts 35.1 us without, 34.0 with).
-                if ((w == 1 || done > 0) && !__all_sync(0xffffffffu, wait_for(&b->turn[w], (w == 1 ? done : done - 1) & 1, b, a.gave_up, limit)))
+                if ((w == 1 || done > 0) && !warp_wait_for(&b->turn[w], (w == 1 ? done : done - 1) & 1, b, a.gave_up, limit))
                     return false;
                 float2 sum[2] = {};
                 // The weights, rounded to the operands' type: half a step each, at random, of sums
@@ -815,7 +833,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                          ? step(j, std::true_type())
                          : step(j, std::false_type());
             }
-            if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit));
+            if (n > 0 && ok) ok = warp_wait_for(&b->o_done[w], (done - 1) & 1, b, a.gave_up, limit);
             if (ok) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int h = it.kh * a.group + g;
@@ -1024,6 +1042,8 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     // a scale of 0 weighs all visible keys alike, and must leave the hidden ones' -inf alone
     a.scale = scale == 0.f ? 1e-30f : scale;
     a.gave_up = ctx->wait_error;
+    a.limit = ctx->wait_limit + std::min<uint64_t>(uint64_t(4000) * a.rows, 8 * mr::tc::kWaitNs);
+    a.withhold = ctx->withhold;
     return query->dtype == MR_DTYPE_F32   ? launch32(ctx, a)
            : query->dtype == MR_DTYPE_F16 ? launch16<__half>(ctx, a)
                                           : launch16<__nv_bfloat16>(ctx, a);

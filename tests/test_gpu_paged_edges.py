@@ -57,3 +57,53 @@ def test_windows_up_to_the_largest_number(served, dtype, window):
         want, _, mixed, reach = ref.attend(wide(q[a:b]), wide(k[c:d]), wide(v[c:d]), range(d - c - b + a, d - c), 0.125,
                                            window, 1)
         assert np.all(np.abs(wide(got[a:b]) - want) <= ref.output_bound(want, mixed, reach, 64, 12, dtype, True))
+
+
+# ---- waits that give up -------------------------------------------------------------------------------------------
+LIMIT_NS = 20_000_000
+
+
+@pytest.fixture
+def faulty(pkg):
+    """A backend whose prompt attention can be told not to load its values: those who wait for them give up."""
+    import torch
+    native = submodule("_native")
+    backend = pkg.CUDABackend(stream=torch.cuda.current_stream().cuda_stream)
+    native.call("mr_context_set_wait_limit", backend.context, LIMIT_NS)
+
+    def fault(on):
+        native.call("mr_context_inject_fault", backend.context, int(on))
+    backend.fault = fault
+    return backend
+
+
+@pytest.mark.parametrize("heads, kv, dim, new", [
+    (4, 2, 64, [60]),            # one tile of keys
+    (4, 2, 128, [300, 0, 9]),
+    (5, 1, 128, [1400]),         # long: a CTA for each piece
+    (8, 8, 64, [40] * 60),       # several pieces to a CTA
+])
+def test_a_prompt_whose_waits_give_up_ends_and_says_so(pkg, faulty, heads, kv, dim, new):
+    import time
+    import torch
+    q, k, v = (queries(sum(new), h, dim, "bfloat16", seed=h) for h in (heads, kv, kv))
+    offsets = ints(0, *np.cumsum(new).tolist())
+    want = faulty.window_attention(q, k, v, offsets)
+    faulty.finish()
+    for _ in range(2):
+        faulty.fault(True)
+        begin = time.perf_counter()
+        faulty.window_attention(q, k, v, offsets)
+        with pytest.raises(pkg.CUDAError, match="gave up") as failure:
+            faulty.finish()
+        assert failure.value.code == submodule("_native").MR_ERR_TIMEOUT
+        assert time.perf_counter() - begin < 10
+        faulty.finish()   # told once
+        faulty.fault(False)
+        assert torch.equal(faulty.window_attention(q, k, v, offsets), want)
+        faulty.finish()
+
+
+def test_wait_limits_have_a_least_value(pkg, faulty):
+    with pytest.raises(pkg.CUDAError, match="below 1 ms"):
+        submodule("_native").call("mr_context_set_wait_limit", faulty.context, 999_999)
