@@ -390,7 +390,10 @@ MR_API int mr_attention_static_scratch(mr_context *ctx, const float *q, const fl
  * is cut to the table's rows (an append drops the rows past them), a negative
  * one is 0.
  * Calls queue work on the context's stream and return; they can be captured
- * into a CUDA graph.  Scratch memory: calls outside a capture share the
+ * into a CUDA graph.  A wait inside a kernel that gave up leaves results that
+ * are not valid: the next of these calls, mr_context_finish or
+ * mr_buffer_download returns MR_ERR_TIMEOUT, once (a download has copied the
+ * values all the same; one of these calls has queued nothing).  Scratch memory: calls outside a capture share the
  * context's, in stream order; a captured call's belongs to its graph.  So two
  * contexts, or two graphs, may run at the same time. */
 typedef struct {

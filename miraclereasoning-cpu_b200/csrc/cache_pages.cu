@@ -410,6 +410,7 @@ extern "C" int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_a
                    static_cast<long long>(batch));
     }
     MR_REQUIRE(ctx, "ctx is NULL");
+    MR_CHECK(mr::check_waits(ctx));
     if (!keys->shape[0] || !batch || !key_pages->shape[0] || !page_table->shape[1]) return MR_OK;
     DeviceGuard guard(ctx->device);
     const int64_t size = dtype_bytes(keys->dtype);
@@ -478,6 +479,7 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     MR_REQUIRE(batch <= 65535, "more than 65535 sequences");
     MR_REQUIRE(heads <= 65535 && batch * heads <= INT32_MAX, "too many heads");
     MR_REQUIRE(ctx, "ctx is NULL");
+    MR_CHECK(mr::check_waits(ctx));
     if (!batch) return MR_OK;
     DeviceGuard guard(ctx->device);
     EvictArgs a;

@@ -1071,6 +1071,7 @@ extern "C" int mr_paged_attention(mr_context *ctx, const mr_array *query, const 
                        "the pages' stride %d passes 4 GB", i);
     if (weights) MR_CHECK(check_weights(weights, "weights", batch, kv_heads, capacity, true));
     MR_REQUIRE(ctx, "ctx is NULL");
+    MR_CHECK(mr::check_waits(ctx));
     if (!batch) return MR_OK;
     DeviceGuard guard(ctx->device);
     const int64_t size = dtype_bytes(query->dtype);

@@ -213,7 +213,7 @@ int mr_buffer_download(const mr_buffer *buf, size_t offset, float *host, size_t 
     MR_CUDA_TRY(cudaMemcpyAsync(host, buf->ptr + offset, count * sizeof(float), cudaMemcpyDeviceToHost,
                                 buf->ctx->stream));
     MR_CUDA_TRY(cudaStreamSynchronize(buf->ctx->stream));
-    return MR_OK;
+    return mr::check_waits(buf->ctx);
 }
 
 int mr_buffer_copy(const mr_buffer *src, mr_buffer *dst, size_t src_offset, size_t dst_offset,

@@ -107,3 +107,36 @@ def test_a_prompt_whose_waits_give_up_ends_and_says_so(pkg, faulty, heads, kv, d
 def test_wait_limits_have_a_least_value(pkg, faulty):
     with pytest.raises(pkg.CUDAError, match="below 1 ms"):
         submodule("_native").call("mr_context_set_wait_limit", faulty.context, 999_999)
+
+
+def test_a_wait_that_gave_up_is_reported_where_its_results_are_read_or_used(pkg, faulty):
+    import torch
+    native = submodule("_native")
+    rng = np.random.default_rng(3)
+    q, k, v = (faulty.upload_array(rng.normal(size=(40, h, 64)), "bfloat16") for h in (4, 2, 2))
+    offsets = faulty.upload_array([0, 40], "int32")
+    want = faulty.read_array(faulty.window_attention(q, k, v, offsets))
+    cache = Cache([40], 16, 2, 64, "bfloat16", extra=6)
+    target, weights = ints(*cache.spare[:1])[None], torch.rand(1, 2, 48, device="cuda")
+    one, row = queries(1, 4, 64, "bfloat16"), queries(1, 2, 64, "bfloat16")
+    calls = [lambda: faulty.paged_attention(one, cache.keys, cache.values, cache.table, cache.lengths),
+             lambda: faulty.append_pages(row, row, cache.keys, cache.values, cache.table, cache.lengths),
+             lambda: faulty.evict_pages(cache.keys, cache.values, cache.table, cache.lengths, weights, target, budget=16),
+             lambda: faulty.window_attention(q, k, v, offsets),
+             lambda: faulty.read_array(q)]
+    for call in calls:
+        faulty.fault(True)
+        bad = faulty.window_attention(q, k, v, offsets)
+        faulty.fault(False)
+        torch.cuda.synchronize()
+        with pytest.raises(pkg.CUDAError, match="gave up") as failure:
+            call()
+        assert failure.value.code == native.MR_ERR_TIMEOUT
+        call()   # told once
+        assert np.array_equal(faulty.read_array(faulty.window_attention(q, k, v, offsets)), want)
+    faulty.fault(True)
+    bad = faulty.window_attention(q, k, v, offsets)
+    with pytest.raises(pkg.CUDAError, match="gave up"):   # not waited for before
+        faulty.read_array(bad)
+    faulty.fault(False)
+    faulty.finish()
