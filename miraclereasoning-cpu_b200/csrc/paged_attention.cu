@@ -687,11 +687,15 @@ __device__ __forceinline__ void add_rows(const PagedArgs &a, const Piece &walk, 
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const int i = i0 + r * step;
-            // a hidden row's score is -inf, and adds nothing whatever the sum is
+            // A hidden row's score is -inf, and adds nothing whatever the sum is; nor does a head past the
+            // group (lse infinite), whatever its score is: of an infinite key, 0 x inf.
+            auto share = [&](float score, int h) {
+                return score == -INFINITY || lse[h] == INFINITY ? 0.f : ex2(score - lse[h]);
+            };
 #pragma unroll
             for (int h = 0; h < N / 2; ++h) {
-                was[r] += x[r][h].x == -INFINITY ? 0.f : ex2(x[r][h].x - lse[2 * h]);
-                was[r] += x[r][h].y == -INFINITY ? 0.f : ex2(x[r][h].y - lse[2 * h + 1]);
+                was[r] += share(x[r][h].x, 2 * h);
+                was[r] += share(x[r][h].y, 2 * h + 1);
             }
             if (i < to) weights[walk.seen.at(i)] = was[r];
         }

@@ -140,3 +140,23 @@ def test_a_wait_that_gave_up_is_reported_where_its_results_are_read_or_used(pkg,
         faulty.read_array(bad)
     faulty.fault(False)
     faulty.finish()
+
+
+# ---- one token ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv, lengths", [
+    (3, 3, [40, 9]), (10, 1, [40]), (5, 1, [33, 200]), (18, 2, [70]),   # groups that blocks of heads leave room in
+    (3, 3, [2600, 900]), (10, 1, [1500]), (9, 3, [3000]), (8, 2, [1500]),   # sequences cut between warps
+])
+def test_an_infinite_visible_key_and_weights(served, dtype, heads, kv, lengths):
+    """A key of -inf where all queries are positive: a score of -inf, a weight of 0, and nothing else about the row."""
+    cache = Cache(lengths, 16, kv, 64, dtype)
+    q = queries(len(lengths), heads, 64, dtype)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.25
+    rows = [{3}, {3, 8}][:len(lengths)]
+    for s, hidden in enumerate(rows):
+        for t in hidden:
+            cache.keys[int(cache.table[s, t // 16]), t % 16, :, 7] = float("-inf")
+            cache.rows[s][0][t, :, 7] = float("-inf")
+    check_paged(served, cache, q, dtype, weighted=True, hidden=rows)
+    check_paged(served, cache, q, dtype, 30, 9, weighted=True, hidden=rows)
