@@ -28,6 +28,7 @@
 // (cp.async, 16 bytes a lane, page ids looked up a step ahead), which runs on
 // from one unit into the next, and its own running softmax.
 #include <cmath>
+#include <type_traits>
 
 #include "cache_ops.cuh"
 
@@ -281,9 +282,13 @@ template <typename T, int DP_>
 struct Math16 {
     static constexpr int DP = DP_, kHeads = 8, STEP = DP == 128 ? 16 : 32, STAGES = DP == 32 ? 6 : 3;
     using R = Ring<T, DP, STEP, STAGES>;
+    // Weights are taken against the maximum / 2^kLift, so that the largest is 2^kLift: float16 ends at 2^-25
+    // below, and what is less than 2^-40 of the largest weight is lost instead of 2^-25 (32768 rows of
+    // 2^-25.2 beside one: 8e-4 of the sum).  All statistics of a warp are of that reference.
+    static constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
     uint32_t qf[DP / 16][2];   // Q^T fragments: head lane / 4
     float o[DP / 16][4];       // O^T: dims 16 b + lane / 4 (+ 8), heads 2 (lane % 4) and + 1
-    float m[2], l[2];          // heads 2 (lane % 4), + 1; l only of this lane's rows
+    float m[2], l[2];          // heads 2 (lane % 4), + 1: maximum - kLift, sum; l only of this lane's rows
 
     __device__ __forceinline__ void begin(const PagedArgs &a, const char *q, int heads) {
         const int lane = threadIdx.x % 32, h = lane / 4;
@@ -340,7 +345,7 @@ struct Math16 {
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], i));
-            top[h] = fmaxf(top[h], m[h]);
+            top[h] = fmaxf(top[h] - kLift, m[h]);
             grown |= top[h] > m[h];
             ref[h] = top[h] == -INFINITY ? 0.f : top[h];
         }

@@ -160,3 +160,44 @@ def test_an_infinite_visible_key_and_weights(served, dtype, heads, kv, lengths):
             cache.rows[s][0][t, :, 7] = float("-inf")
     check_paged(served, cache, q, dtype, weighted=True, hidden=rows)
     check_paged(served, cache, q, dtype, 30, 9, weighted=True, hidden=rows)
+
+
+def one_above_many(n, kv, dim, dtype, at=0, above=17.5):
+    """n rows of scores 0 and values 1 but for row `at`, whose score is `above` (queries of it alone, scale 1) and whose
+    values are 0; and the weight of each of the others, the outputs and row `at`'s weight in 64 bits."""
+    import torch
+    kind = getattr(torch, dtype)
+    keys = torch.zeros(n, kv, dim, device="cuda", dtype=kind)
+    values = torch.ones_like(keys)
+    keys[at, :, 0], values[at] = 1, 0
+    small = np.exp(-np.float64(above))
+    total = 1 + (n - 1) * small
+    return keys, values, small / total, (n - 1) * small / total, 1 / total
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, batch, heads, kv, dim", [
+    (1000, 2, 8, 2, 64), (1000, 1, 3, 3, 32), (500, 1, 8, 1, 128),   # a quarter of the rows each warp's
+    (4096, 40, 40, 40, 64), (2048, 24, 80, 80, 128), (32769, 3, 8, 4, 64),   # many rows a warp, cut and whole
+])
+def test_many_small_weights_beside_a_large_one(served, dtype, n, batch, heads, kv, dim):
+    import torch
+    page = 64
+    pages = -(-n // page)
+    for at in (0, n - 1):
+        rows = one_above_many(n, kv, dim, dtype, at)
+        keys, values = (torch.zeros(pages * page, kv, dim, device="cuda", dtype=rows[0].dtype) for _ in range(2))
+        keys[:n], values[:n] = rows[0], rows[1]
+        small, want, large = rows[2:]
+        q = torch.zeros(batch, heads, dim, device="cuda", dtype=keys.dtype)
+        q[:, :, 0] = 17.5
+        weights = torch.zeros(batch, kv, pages * page, device="cuda")
+        table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)   # all sequences share the pages
+        got = served.paged_attention(q, keys.view(pages, page, kv, dim), values.view(pages, page, kv, dim), table,
+                                     ints(*[n] * batch), scale=1.0, weights=weights)
+        bound = ref.output_bound(want, want, 17.5, dim, n, dtype, False)
+        assert np.abs(wide(got) - want).max() <= bound, (wide(got).min(), wide(got).max(), want, bound)
+        error = 2 * ref.score_error(17.5, dim) + 2 * (n + heads) * 2.0 ** -24
+        spent = np.full(pages * page, small)
+        spent[at], spent[n:] = large, 0
+        assert np.all(np.abs(wide(weights) * kv / heads - spent) <= (error + 2.0 ** -23) * spent)
