@@ -17,7 +17,7 @@
 // operand of the second product, V the second one as it lies in memory (MN-major).
 // O is rescaled only where a row's maximum grows by more than 2^8: until then the
 // weights are taken against the old maximum, which the sum shares, so nothing is lost
-// but headroom.
+// but headroom (Headroom: float16 has less of it).
 //
 // What bounds it: a 128 x 128 tile's exponentials (head dim 128) take the special-function
 // unit 1024 cycles, its two products the tensor cores as many.  One tile's softmax runs
@@ -119,6 +119,17 @@ __global__ void __launch_bounds__(128) k_rows(const __grid_constant__ WindowArgs
 }
 
 // ---- tensor cores -----------------------------------------------------------------
+// Powers of two: how far a weight may pass its reference, and the reference below the maximum
+// that it was taken from.  A float16 weight ends at 2^16, and half its smallest step is
+// 2^-25: against a reference of 2^-11 of the maximum, small weights are off by 2^-36 of the largest
+// (2^-25 without: 8192 rows of 2^-25.2 beside one, 2e-4 of the sum, were lost).  The less a weight may
+// grow, the more often O is rescaled: flashlite's 8192 tokens take 246.7 us with 2^8 and 2^7, 250.8
+// with 2^4 and 2^11, 263.3 with 2^2 and 2^13.
+template <typename T>
+struct Headroom {
+    static constexpr float kGrows = std::is_same<T, __half>::value ? 4.f : 8.f;
+    static constexpr float kLift = std::is_same<T, __half>::value ? 11.f : 0.f;
+};
 constexpr int kTile = 128, kKeys = 128;  // query rows and keys of a tile
 constexpr int kLoadWarp = 8, kMathWarp = 9, kTcThreads = 384;  // warp 11 fills the third warpgroup
 // bytes of 64 dims of a tile's queries, and of its keys
@@ -759,7 +770,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 for (int c = 8; c < kKeys; ++c) tops[c % 8] = max_nan(tops[c % 8], __uint_as_float(s[c]));
                 const float top = max_nan(max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])),
                                           max_nan(max_nan(tops[4], tops[5]), max_nan(tops[6], tops[7])));
-                if (__any_sync(0xffffffffu, !((top - m) * scale <= 8.f))) {  // a NaN goes into the maximum, and so everywhere
+                if (__any_sync(0xffffffffu, !((top - m) * scale <= Headroom<T>::kGrows))) {  // a NaN goes into the maximum, and so everywhere
                     const float grown = max_nan(m, top);
                     if (j > 0) {
                         // done already, since the scores came behind it
@@ -779,7 +790,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                     }
                     m = grown;
                 }
-                const float shift = m == kNone ? 0.f : -m * scale;
+                const float shift = m == kNone ? 0.f : fmaf(-m, scale, Headroom<T>::kLift);
                 // The two tiles take the special-function unit in turns, a quarter overlapping; otherwise both
                 // settle into doing their exponentials, and then their products, at the same time
                 // (chunked flashnano-1.7 prompts 35.1 us without, 34.0 with).

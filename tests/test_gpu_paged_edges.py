@@ -201,3 +201,40 @@ def test_many_small_weights_beside_a_large_one(served, dtype, n, batch, heads, k
         spent = np.full(pages * page, small)
         spent[at], spent[n:] = large, 0
         assert np.all(np.abs(wide(weights) * kv / heads - spent) <= (error + 2.0 ** -23) * spent)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, heads, kv, dim", [(8193, 4, 1, 64), (8193, 8, 8, 128), (1000, 6, 2, 128), (700, 130, 1, 16)])
+def test_many_small_weights_in_a_prompt(served, dtype, n, heads, kv, dim):
+    """The last queries of a prompt, each with one key far above all others."""
+    import torch
+    for at in (0, 300, n - 9):
+        new = 9 if n > 1000 else n
+        keys, values = one_above_many(n, kv, dim, dtype, at)[:2]
+        q = torch.zeros(new, heads, dim, device="cuda", dtype=keys.dtype)
+        q[:, :, 0] = 17.5
+        got = wide(served.window_attention(q, keys, values, ints(0, new), ints(0, n), scale=1.0))
+        small = np.exp(-np.float64(17.5))
+        for i in range(new):
+            seen = n - new + i + 1
+            want = 1.0 if seen <= at else (seen - 1) * small / (1 + (seen - 1) * small)
+            bound = ref.output_bound(want, want, 17.5, dim, seen, dtype, True)
+            assert np.abs(got[i] - want).max() <= bound, (at, i, got[i].min(), got[i].max(), want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("step", [0.9, 1.9, 2.1, 7.9, 8.1])
+def test_scores_that_grow_from_tile_to_tile(served, dtype, step):
+    """The maximum of every 128 keys `step` powers of two above that of those before: weights at the end of their range."""
+    import torch
+    rng = np.random.default_rng(2)
+    kind = getattr(torch, dtype)
+    n, heads, dim = 900, 4, 64
+    q = torch.zeros(200, heads, dim, device="cuda", dtype=kind)
+    q[:, :, 0] = 1
+    k = torch.zeros(n, heads, dim, device="cuda", dtype=kind)
+    k[:, :, 0] = (torch.arange(n, device="cuda") // 128 * (step * np.log(2))).to(kind)[:, None]
+    v = torch.tensor(rng.normal(size=(n, heads, dim))).to(kind).cuda()
+    got = served.window_attention(q, k, v, ints(0, 200), ints(0, n), scale=1.0)
+    want, _, mixed, reach = ref.attend(wide(q), wide(k), wide(v), range(n - 200, n), 1.0)
+    assert np.all(np.abs(wide(got) - want) <= ref.output_bound(want, mixed, reach, dim, n, dtype, True))
