@@ -738,7 +738,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
             const uint32_t s_at = tmem + lanes + w * kTile, o_at = tmem + lanes + S::kO + w * DP;
             const float scale = fabsf(a.scale) * 1.4426950408889634f;
             constexpr float kNone = -3.4028235e38f;  // no key seen yet
-            float m = kNone, l = 0.f;
+            // Rows of no query of the sequence (another's, or what shared memory held) have no say in when the
+            // others' values are rescaled, and so rounded anew: their maximum cannot grow.
+            float m = live ? kNone : INFINITY, l = 0.f;
             // A tile's step; where the mask hides some of its keys, its quarters of 32 keys that no row of
             // the warp sees are left out.  Two bodies: the scores of either stay in registers of its own.
             auto step = [&](int j, auto hides) {
@@ -770,7 +772,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 for (int c = 8; c < kKeys; ++c) tops[c % 8] = max_nan(tops[c % 8], __uint_as_float(s[c]));
                 const float top = max_nan(max_nan(max_nan(tops[0], tops[1]), max_nan(tops[2], tops[3])),
                                           max_nan(max_nan(tops[4], tops[5]), max_nan(tops[6], tops[7])));
-                if (__any_sync(0xffffffffu, !((top - m) * scale <= Headroom<T>::kGrows))) {  // a NaN goes into the maximum, and so everywhere
+                // (never of a NaN, whose row's values all become NaN)
+                if (__any_sync(0xffffffffu, (top - m) * scale > Headroom<T>::kGrows)) {
                     const float grown = max_nan(m, top);
                     if (j > 0) {
                         // done already, since the scores came behind it

@@ -238,3 +238,29 @@ def test_scores_that_grow_from_tile_to_tile(served, dtype, step):
     got = served.window_attention(q, k, v, ints(0, 200), ints(0, n), scale=1.0)
     want, _, mixed, reach = ref.attend(wide(q), wide(k), wide(v), range(n - 200, n), 1.0)
     assert np.all(np.abs(wide(got) - want) <= ref.output_bound(want, mixed, reach, dim, n, dtype, True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, dim", [(5, 64), (9, 128), (3, 104)])
+def test_a_prompt_repeats_bit_for_bit_whatever_ran_before_it(served, dtype, heads, dim):
+    """Groups that leave rows of a tile over: those hold what the kernel before left there."""
+    q, k, v = (queries(n, h, dim, dtype, seed=n) for n, h in ((400, heads), (1500, 1), (1499, 1)))
+    k = k[:1499]
+    before = [queries(12000, h, dim, dtype, seed=h) for h in (4, 1, 1)]
+    got = []
+    for size in (0.0, 3000.0, 0.0, 1.0):
+        served.window_attention(before[0] * size, *before[1:], ints(0, 12000), window=200)
+        got.append(wide(served.window_attention(q, k, v, ints(0, 400), ints(0, 1499))))
+    assert all(np.array_equal(got[0], x) for x in got[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_sequence_does_not_see_its_neighbours_queries(served, dtype):
+    import torch
+    q, k, v = (queries(n, h, 64, dtype, seed=n) for n, h in ((60, 8), (1060, 2), (1061, 2)))
+    v = v[:1060]
+    got = []
+    for factor in (1, 100, float("nan")):
+        other = torch.cat([q[:10], q[10:] * factor])
+        got.append(wide(served.window_attention(other, k, v, ints(0, 10, 60), ints(0, 1000, 1060))[:10]))
+    assert all(np.array_equal(got[0], x) for x in got[1:])
