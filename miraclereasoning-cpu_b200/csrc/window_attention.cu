@@ -981,8 +981,13 @@ int launch32(mr_context *ctx, WindowArgs &a) {
 
 template <typename T>
 int launch16(mr_context *ctx, WindowArgs &a) {
-    // a tile holds whole groups; a group of more heads than it has rows goes by rows, as no rows of keys do
-    if (a.group > kTile || a.rows == 0) return launch_rows<T>(ctx, a);
+    // Under the smallest scales a tile's maximum would not leave `none seen`, and 0 would not leave the hidden
+    // keys' -inf alone.  Float16 scores are below 2^40, and a scale of 2^-100 weighs them all alike as 0 does.
+    constexpr float kLeast = 1e-36f;
+    if (a.scale == 0.f && std::is_same<T, __half>::value) a.scale = 0x1p-100f;
+    // A tile holds whole groups; a group of more heads than it has rows goes by rows, as no rows of keys do,
+    // and those scales.
+    if (a.group > kTile || a.rows == 0 || fabsf(a.scale) < kLeast) return launch_rows<T>(ctx, a);
     return a.dim <= 64 ? launch<T, 64>(ctx, a) : launch<T, 128>(ctx, a);
 }
 
@@ -1053,8 +1058,7 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     // their differences stay within 32 bits.
     a.window = window < keys->shape[0] ? window : 0;
     a.sinks = sinks;
-    // a scale of 0 weighs all visible keys alike, and must leave the hidden ones' -inf alone
-    a.scale = scale == 0.f ? 1e-30f : scale;
+    a.scale = scale;
     a.gave_up = ctx->wait_error;
     a.limit = ctx->wait_limit + std::min<uint64_t>(uint64_t(4000) * a.rows, 8 * mr::tc::kWaitNs);
     a.withhold = ctx->withhold;

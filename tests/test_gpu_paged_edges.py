@@ -264,3 +264,17 @@ def test_a_sequence_does_not_see_its_neighbours_queries(served, dtype):
         other = torch.cat([q[:10], q[10:] * factor])
         got.append(wide(served.window_attention(other, k, v, ints(0, 10, 60), ints(0, 1000, 1060))[:10]))
     assert all(np.array_equal(got[0], x) for x in got[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-36, -9e-37, 1e-38, -1e-39, 1e-45, 1e-50])
+def test_prompts_of_the_smallest_scales(served, dtype, scale):
+    # down to float32's smallest number, and what it rounds to 0: all visible keys weigh alike
+    check_window(served, dtype, 4, 2, 64, [70, 3], [0, 140], scale=scale)
+    check_window(served, dtype, 3, 3, 40, [20], [200], window=33, sinks=2, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("scale", [1e-36, 1e-37, 0.0])
+def test_small_scales_of_large_scores(served, dtype, scale):
+    check_window(served, dtype, 4, 2, 64, [70], [60], scale=scale, size=2.0 ** 115)
