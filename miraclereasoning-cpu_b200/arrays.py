@@ -8,8 +8,11 @@ have.  The owner keeps the memory alive until the queued work is done.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import math
 import struct
+from pathlib import Path
 
 import numpy as np
 
@@ -40,26 +43,46 @@ def described(array, name, device):
     return struct.pack("<Qii8q", array.data_ptr(), code, len(shape), *shape, *pad, *array.stride(), *pad)
 
 
-try:
-    from . import _pycall
-except ImportError as missing:
-    raise _native.CUDAError(f"{_native.LIBRARY_PATH.with_name('_pycall.so')} is missing or unusable ({missing}): build it "
-                            f"with 'python miraclereasoning-cpu_b200/build.py'") from None
-_pycall.types(_CODES, described)
-describe = _pycall.describe
-APPEND, PAGED, WINDOW, EVICT = _pycall.APPEND, _pycall.PAGED, _pycall.WINDOW, _pycall.EVICT
+# the operators in csrc/pycall.c's order
+APPEND, PAGED, WINDOW, EVICT = range(4)
 _NAMES = ("mr_append_pages", "mr_paged_attention", "mr_window_attention", "mr_evict_pages")
+# this interpreter's own build of csrc/pycall.c
+PYCALL = Path(__file__).resolve().with_name("_pycall" + importlib.machinery.EXTENSION_SUFFIXES[0])
+_module = None   # the module, once a call has needed it
+_call = None     # its call(), once the library's operators are handed over to it
 
 
-def bind():
-    """Hands the library's operators over to ``invoke``."""
-    lib = _native.library()
-    _pycall.bind(*[C.cast(getattr(lib, name), C.c_void_p).value for name in _NAMES])
+def _pycall():
+    global _module
+    if _module is None:
+        try:
+            spec = importlib.util.spec_from_file_location(f"{__package__}._pycall", PYCALL)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as missing:
+            raise _native.CUDAError(f"{PYCALL} is missing or unusable ({missing}): build it with "
+                                    f"'python miraclereasoning-cpu_b200/build.py'") from None
+        module.types(_CODES, described)
+        _module = module
+    return _module
+
+
+def describe(array, name, device):
+    """An operator's argument as mr_array, in bytes."""
+    return _pycall().describe(array, name, device)
+
+
+def _bound():
+    global _call
+    lib, module = _native.library(), _pycall()
+    module.bind(*[C.cast(getattr(lib, name), C.c_void_p).value for name in _NAMES])
+    _call = module.call
+    return _call
 
 
 def invoke(which, *args):
     """An operator: its context's address, the device, arrays (None: left out) and scalars."""
-    status = _pycall.call(which, *args)
+    status = (_call or _bound())(which, *args)
     if status:
         _native.check(status, _NAMES[which])
 

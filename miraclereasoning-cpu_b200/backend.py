@@ -130,7 +130,6 @@ class CUDABackend:
             call("mr_context_create_on_stream", device_index, stream, C.byref(handle))
         self.context = handle
         self._where = handle.value, device_index   # of every array operator's call
-        arrays.bind()
 
     def __del__(self):
         ctx = getattr(self, "context", None)

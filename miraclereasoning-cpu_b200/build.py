@@ -10,6 +10,7 @@ The build is incremental on source timestamps.  No GPU is needed to build.
 from __future__ import annotations
 
 import argparse
+import importlib.machinery
 import os
 import shutil
 import subprocess
@@ -20,7 +21,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 SRC = HERE / "csrc"
 OUT = HERE / "libmiracle_cuda.so"
-PYCALL = HERE / "_pycall.so"
+PYCALL = HERE / f"_pycall{importlib.machinery.EXTENSION_SUFFIXES[0]}"   # of the interpreter that builds it
 OBJ = HERE / "_build"
 HEADER = HERE.parent / "include" / "miracle_cuda.h"
 
@@ -71,7 +72,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
 def build_pycall(force: bool = False, verbose: bool = False) -> Path:
     src = SRC / "pycall.c"
     if force or _stale(PYCALL, [src, HEADER]):
-        tmp = PYCALL.with_suffix(".so.tmp")
+        tmp = PYCALL.with_name(PYCALL.name + ".tmp")
         cmd = [shutil.which("gcc") or "cc", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
                f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(tmp)]
         if verbose:

@@ -18,7 +18,7 @@
 
 #define MOST 11
 
-enum { APPEND, PAGED, WINDOW, EVICT, CALLS };
+enum { APPEND, PAGED, WINDOW, EVICT, CALLS };  /* arrays.py has the same order */
 static const struct {
     int arrays, scalars;
     const char *names[MOST];
@@ -170,10 +170,7 @@ PyMODINIT_FUNC PyInit__pycall(void) {
     stride = PyUnicode_InternFromString("stride");
     dtype = PyUnicode_InternFromString("dtype");
     data_ptr = PyUnicode_InternFromString("data_ptr");
-    if (m && get_device && shape && stride && dtype && data_ptr && PyModule_AddIntConstant(m, "APPEND", APPEND) == 0 &&
-        PyModule_AddIntConstant(m, "PAGED", PAGED) == 0 && PyModule_AddIntConstant(m, "WINDOW", WINDOW) == 0 &&
-        PyModule_AddIntConstant(m, "EVICT", EVICT) == 0)
-        return m;
+    if (m && get_device && shape && stride && dtype && data_ptr) return m;
     Py_XDECREF(m);
     return NULL;
 }
