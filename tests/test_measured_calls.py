@@ -26,6 +26,7 @@ def test_a_backend_for_each_stream_and_device(measured, monkeypatch):
     now = SimpleNamespace(device_index=0, cuda_stream=11)
     monkeypatch.setitem(sys.modules, PACKAGE, SimpleNamespace(CUDABackend=backend))
     monkeypatch.setattr(measured.torch.cuda, "current_stream", lambda *a: now)
+    monkeypatch.setattr(measured.torch.accelerator, "current_stream", lambda *a: (now.device_index, now.cuda_stream))
     first = measured._backend()
     assert (first.device_index, first.stream) == (0, 11)
     now = SimpleNamespace(device_index=0, cuda_stream=12)
