@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256, 4) k_append(const __grid_constant__ Appen
             s = sequence_of(a.offsets, a.offset_stride, a.batch, mine);
             if (s >= 0) behind = __ldg(a.offsets + (s + 1) * a.offset_stride) - mine;
         }
-        const int t = s >= 0 ? __ldg(a.lengths + s * a.length_stride) - behind : -1;
+        const int t = s >= 0 ? max(0, __ldg(a.lengths + s * a.length_stride)) - behind : -1;
         if (t >= 0) {
             kr = a.pages.row(s, t, a.k.page, a.k.row);
             vr = a.pages.row(s, t, a.v.page, a.v.row);

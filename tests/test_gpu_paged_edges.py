@@ -278,3 +278,14 @@ def test_prompts_of_the_smallest_scales(served, dtype, scale):
 @pytest.mark.parametrize("scale", [1e-36, 1e-37, 0.0])
 def test_small_scales_of_large_scores(served, dtype, scale):
     check_window(served, dtype, 4, 2, 64, [70], [60], scale=scale, size=2.0 ** 115)
+
+
+# ---- append -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("length, end", [(-2 ** 31, 2 ** 31 - 1), (-2 ** 31, 2), (-1, 2 ** 31 - 1), (0, 2)])
+def test_appending_to_a_length_of_none_writes_nothing(served, length, end):
+    # a negative length is 0, whatever the offsets are: no row of the sequence is one of its last
+    import torch
+    pools = [torch.zeros(3, 8, 2, 64, device="cuda") for _ in range(2)]
+    rows = [torch.ones(2, 2, 64, device="cuda") for _ in range(2)]
+    served.append_pages(*rows, *pools, ints([0, 1, 2]), ints(length), ints(0, end))
+    assert not pools[0].any() and not pools[1].any()
