@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
         for (int i = tid; i < n; i += kSelectThreads) kept[i] = i;
     }
 #pragma unroll 1
-    for (int i = total + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    for (uint32_t i = total + tid; i < static_cast<uint32_t>(a.budget); i += kSelectThreads) kept[i] = -1;  // to 2^31 - 1
     __syncthreads();
     constexpr int kFlight = 4;
 #pragma unroll 1

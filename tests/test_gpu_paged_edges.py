@@ -289,3 +289,15 @@ def test_appending_to_a_length_of_none_writes_nothing(served, length, end):
     rows = [torch.ones(2, 2, 64, device="cuda") for _ in range(2)]
     served.append_pages(*rows, *pools, ints([0, 1, 2]), ints(length), ints(0, end))
     assert not pools[0].any() and not pools[1].any()
+
+
+def test_a_budget_of_the_largest_number_keeps_all_rows(served):
+    # 8 GB of places for kept rows, all but 20 of them empty
+    import torch
+    cache = Cache([20], 16, 1, 8, "bfloat16", extra=4)
+    kept, lengths, weights = served.evict_pages(cache.keys, cache.values, cache.table, cache.lengths,
+                                                torch.rand(1, 1, 32, device="cuda"), ints(*cache.spare[:2])[None],
+                                                budget=2 ** 31 - 1, sinks=2 ** 30, recent=2 ** 30 - 1)
+    served.finish()
+    assert kept.shape == (1, 1, 2 ** 31 - 1) and kept[0, 0, :20].tolist() == list(range(20)) and lengths.tolist() == [20]
+    assert int(kept[0, 0, 20:].amax()) == -1 and int(kept[0, 0, 20:].amin()) == -1
