@@ -1070,7 +1070,7 @@ extern "C" int mr_paged_attention(mr_context *ctx, const mr_array *query, const 
     MR_CHECK(check_ints(lengths, "lengths", 1));
     MR_REQUIRE(lengths->shape[0] == batch, "lengths must have %lld values", static_cast<long long>(batch));
     MR_CHECK(check_table(page_table, "page_table", batch, key_pages->shape[1]));
-    MR_REQUIRE(batch * heads <= INT32_MAX / 2, "too many heads");
+    MR_REQUIRE(batch * heads <= INT32_MAX / 2 && heads * query->shape[2] <= INT32_MAX, "too many heads");
     MR_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
     MR_REQUIRE(std::isfinite(scale), "scale must be finite");
     const int64_t capacity = page_table->shape[1] * key_pages->shape[1];
