@@ -407,8 +407,11 @@ typedef struct {
 /* Copies new rows keys / values [tokens, kv heads, dim] into their pages.
  * offsets [batch + 1] I32: sequence s owns the rows offsets[s] .. offsets[s + 1]
  * - 1, which become the last of its lengths[s] rows; NULL: one row per sequence
- * (tokens = batch).  Rows in no sequence are not read.  Two rows given the same
- * place leave one of the two there. */
+ * (tokens = batch).  Rows in no sequence are not read.  Two rows of one call
+ * must not be given the same place (sequences that share a page they append
+ * to): pieces of 16 bytes of either may stay there, and one's key beside the
+ * other's value.  A sequence's rows before its first (more new rows than its
+ * length) are dropped. */
 MR_API int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_array *values, const mr_array *key_pages,
                            const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
                            const mr_array *offsets);
@@ -419,7 +422,10 @@ MR_API int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_array
  * rows are visible; 0: all.  Scores are scaled by `scale`.  A sequence that sees
  * no row gives zeros.  weights (NULL, or F32 [batch, kv heads, table rows]):
  * row t's softmax weight, summed over the query heads of its key / value head,
- * is added to weights[s][kv head][t]. */
+ * is added to weights[s][kv head][t].  With weights the call's scratch memory
+ * holds a float32 score for each query head and each row that the table and
+ * the window let a sequence have, whatever the lengths are (8 GB for 32
+ * sequences of 32 heads in tables of 2 M rows); the context keeps the largest. */
 MR_API int mr_paged_attention(mr_context *ctx, const mr_array *query, const mr_array *key_pages,
                               const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
                               const mr_array *weights, const mr_array *out, int window, int sinks, float scale);
@@ -430,7 +436,10 @@ MR_API int mr_paged_attention(mr_context *ctx, const mr_array *query, const mr_a
  * (I32 [batch + 1], rising, cut to the arrays).  The last query stands at the
  * last key: query i of n over m keys at position p = m - n + i sees key j if
  * j <= p and (window is 0, or p - j < window, or j < sinks).  A query that sees
- * none gives zeros.  Rows of out that belong to no sequence stay as they were. */
+ * none gives zeros.  Rows of out that belong to no sequence stay as they were.
+ * In 16 bits each weight is rounded to that type before it meets the values
+ * (F16: those under 2^-25 of the largest with an error of 2^-36 of it); scores,
+ * their sums and the values' mix are float32. */
 MR_API int mr_window_attention(mr_context *ctx, const mr_array *query, const mr_array *keys, const mr_array *values,
                                const mr_array *query_offsets, const mr_array *key_offsets, const mr_array *out,
                                int window, int sinks, float scale);

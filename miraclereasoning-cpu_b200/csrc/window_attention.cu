@@ -22,7 +22,7 @@
 // What bounds it: a 128 x 128 tile's exponentials (head dim 128) take the special-function
 // unit 1024 cycles, its two products the tensor cores as many.  One tile's softmax runs
 // beside the other's products; with two softmax warps a scheduler, each unit is busy 57% of
-// the time (ncu, flashlite's 8192-token context: 232 us, 1.2 PFLOP/s).  Measured and left out:
+// the time (ncu, flashlite's 8192-token context; 239 us in a CUDA graph, 1.15 PFLOP/s).  Measured and left out:
 // a quarter of the exponentials by polynomials (no faster at head dim 64, 15% slower at 128),
 // key tiles of 64 with the next scores worked out ahead (290 us), two threads a row (314 us),
 // P beside S where TMEM has room (head dim 64: no difference).
@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(128) k_rows(const __grid_constant__ WindowArgs
 // that it was taken from.  A float16 weight ends at 2^16, and half its smallest step is
 // 2^-25: against a reference of 2^-11 of the maximum, small weights are off by 2^-36 of the largest
 // (2^-25 without: 8192 rows of 2^-25.2 beside one, 2e-4 of the sum, were lost).  The less a weight may
-// grow, the more often O is rescaled: flashlite's 8192 tokens take 246.7 us with 2^8 and 2^7, 250.8
-// with 2^4 and 2^11, 263.3 with 2^2 and 2^13.
+// grow, the more often O is rescaled: flashlite's 8192 tokens take 242.9 us with 2^8 and 2^7, 246.8
+// with 2^4 and 2^11, 258.7 with 2^2 and 2^13.
 template <typename T>
 struct Headroom {
     static constexpr float kGrows = std::is_same<T, __half>::value ? 4.f : 8.f;
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
         // A warp for each query tile, so that one's waits do not hold up the other's products.
         // All of it walks through them and one lane issues: descriptors stay in uniform
         // registers, where the instruction wants them.  A lane whose wait gave up issues nothing more
-        // but walks on; the warp leaves together, by a vote once a step (a vote a wait: 1.5% slower).
+        // but walks on; the warp leaves together, by a vote once a step (0.3% of the time; a vote a wait: 1.5%).
         {
             constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
             const uint32_t qk = mma_desc(kBf16, kKeys, a.scale < 0.f, false), pv = mma_desc(kBf16, DP, false, true);
