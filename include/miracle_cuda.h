@@ -97,8 +97,8 @@ MR_API int mr_context_destroy(mr_context *ctx);
 /* OpenCLBackend.finish (opencl.py:302-303) */
 MR_API int mr_context_finish(mr_context *ctx);
 /* How long a wait inside a kernel queued on the context (prompt attention's
- * copies and products) may last before it gives up (default 2 s, at least 1 ms; a
- * few microseconds for each key row are added), and fault injection for tests
+ * copies and products) may last before it gives up (default 2 s, 1 ms to 10 minutes;
+ * a few microseconds for each key row are added), and fault injection for tests
  * of that path, on the host's side: with `on` the prompt kernel loads no values,
  * so that those who wait for them give up.  No GPU fault is involved.  Both
  * hold for calls made from then on.  No reference counterpart. */

@@ -147,6 +147,7 @@ int mr_context_finish(mr_context *ctx) {
 int mr_context_set_wait_limit(mr_context *ctx, uint64_t nanoseconds) {
     MR_REQUIRE(ctx, "ctx is NULL");
     MR_REQUIRE(nanoseconds >= 1000000, "a wait limit below 1 ms");
+    MR_REQUIRE(nanoseconds <= 600000000000, "a wait limit above 10 minutes");
     ctx->wait_limit = nanoseconds;
     return MR_OK;
 }

@@ -301,3 +301,9 @@ def test_a_budget_of_the_largest_number_keeps_all_rows(served):
     served.finish()
     assert kept.shape == (1, 1, 2 ** 31 - 1) and kept[0, 0, :20].tolist() == list(range(20)) and lengths.tolist() == [20]
     assert int(kept[0, 0, 20:].amax()) == -1 and int(kept[0, 0, 20:].amin()) == -1
+
+
+@pytest.mark.parametrize("nanoseconds", [600_000_000_001, 2 ** 64 - 1])
+def test_wait_limits_have_an_end(pkg, faulty, nanoseconds):
+    with pytest.raises(pkg.CUDAError, match="above 10 minutes"):
+        submodule("_native").call("mr_context_set_wait_limit", faulty.context, nanoseconds)
