@@ -853,7 +853,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_window(const __grid_constant_
                 const int h = it.kh * a.group + g;
                 char *out = a.out + (it.x.q0 + i) * a.o_row + h * a.o_head;
                 const float f = m == kNone ? 0.f : 1.f / l;
-                bool finite = true;
+                // (The maximum's own weight is 2^kLift, but for how far m * scale was rounded: by powers of two where scores
+                // pass 2^25.  Float16 loses its bits where that made it small; such rows are worked out again too.)
+                bool finite = !std::is_same<T, __half>::value || m == kNone || l >= 0x1p10f;
+                static_assert(!std::is_same<T, __half>::value || Headroom<T>::kLift > 10.f, "a usual sum is above that");
 #pragma unroll
                 for (int d = 0; d < DP; d += 32) {
                     uint32_t o[32] = {};

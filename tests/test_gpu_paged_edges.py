@@ -307,3 +307,51 @@ def test_a_budget_of_the_largest_number_keeps_all_rows(served):
 def test_wait_limits_have_an_end(pkg, faulty, nanoseconds):
     with pytest.raises(pkg.CUDAError, match="above 10 minutes"):
         submodule("_native").call("mr_context_set_wait_limit", faulty.context, nanoseconds)
+
+
+# ---- values that take the slow way -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths, heads, kv", [([3000], 2, 1), ([1700, 40, 900], 6, 2), ([500], 10, 1)])
+def test_an_infinite_value_leaves_the_other_dims_alone(served, dtype, lengths, heads, kv):
+    """One part of a cut sequence is worked out again by rows, and joined with parts that are not."""
+    import torch
+    cache = Cache(lengths, 16, kv, 64, dtype)
+    q = queries(len(lengths), heads, 64, dtype)
+    for s, n in enumerate(lengths):
+        t = n // 3
+        cache.values[int(cache.table[s, t // 16]), t % 16, :, 5] = float("inf")
+    weights = torch.zeros(len(lengths), kv, cache.table.shape[1] * 16, device="cuda")
+    got = served.paged_attention(q, cache.keys, cache.values, cache.table, cache.lengths, weights=weights)
+    rest = [d for d in range(64) if d != 5]
+    for s, (k, v) in enumerate(cache.rows):
+        n = len(k)
+        want, w, mixed, reach = ref.attend(wide(q[s:s + 1]), wide(k), wide(v), [n - 1], 0.125)
+        bound = ref.output_bound(want, mixed, reach, 64, n, dtype, False)[0]
+        assert np.isinf(wide(got[s])[:, 5]).all()
+        assert np.all(np.abs(wide(got[s]) - want[0])[:, rest] <= bound[:, rest])
+        spent = w[0].reshape(kv, heads // kv, n).sum(1)
+        error = 2 * ref.score_error(reach.max(), 64) + 2 * (n + heads) * 2.0 ** -24 + 2.0 ** -23
+        assert np.all(np.abs(wide(weights[s, :, :n]) - spent) <= error * spent + 1e-30)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [300.0, 3000.0, 12000.0])
+def test_scores_of_many_millions(served, dtype, size):
+    """Scores whose neighbouring 32-bit numbers are further apart than a weight's range: the largest takes all."""
+    cache = Cache([700, 90], 16, 2, 64, dtype, scale=size)
+    q = queries(2, 8, 64, dtype, scale=size)
+    # One weight w is left: w v / w.  The output is rounded; in 16-bit prompts w as well, over the sum of it unrounded.
+    step = ref.HALF_STEP[dtype]
+    bounds = step, step if dtype == "float32" else (1 + step) ** 2 - 1
+    got = wide(served.paged_attention(q, cache.keys, cache.values, cache.table, cache.lengths, scale=1.0))
+    prompt = [wide(served.window_attention(q[s:s + 1], *cache.rows[s], ints(0, 1), ints(0, n), scale=1.0)[0])
+              for s, n in enumerate((700, 90))]
+    for s in range(2):
+        k, v, x = wide(cache.rows[s][0]), wide(cache.rows[s][1]), wide(q[s])
+        for h in range(8):
+            scores = k[:, h // 4] @ x[h]
+            order = np.argsort(scores)
+            reach = (np.abs(k[:, h // 4]) @ np.abs(x[h])).max()
+            assert scores[order[-1]] - scores[order[-2]] > 200 * 2.0 ** -23 * reach + 100   # no two within the scores' error
+            for out, bound in zip((got[s][h], prompt[s][h]), bounds):
+                assert np.all(np.abs(out - v[order[-1], h // 4]) <= bound * np.abs(v[order[-1], h // 4]))
