@@ -355,3 +355,26 @@ def test_scores_of_many_millions(served, dtype, size):
             assert scores[order[-1]] - scores[order[-2]] > 200 * 2.0 ** -23 * reach + 100   # no two within the scores' error
             for out, bound in zip((got[s][h], prompt[s][h]), bounds):
                 assert np.all(np.abs(out - v[order[-1], h // 4]) <= bound * np.abs(v[order[-1], h // 4]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv, lengths", [
+    (4, 1, [900, 30]), (8, 2, [400]), (7, 1, [1800]), (16, 1, [926, 3]), (34, 2, [700, 1]), (130, 1, [1200]),
+    (51, 3, [20]), (72, 8, [2300, 64]),
+])
+def test_many_small_weights_added_to_large_ones(served, dtype, heads, kv, lengths):
+    """What the heads add to a row is added up before it meets the 100 or so that are there: one rounding of the two."""
+    import torch
+    cache = Cache(lengths, 16, kv, 64, dtype)
+    q = queries(len(lengths), heads, 64, dtype)
+    was = torch.tensor(np.random.default_rng(9).uniform(50, 120, (len(lengths), kv, cache.table.shape[1] * 16))).float().cuda()
+    weights = was.clone()
+    served.paged_attention(q, cache.keys, cache.values, cache.table, cache.lengths, weights=weights)
+    for s, (k, v) in enumerate(cache.rows):
+        n = len(k)
+        _, w, _, reach = ref.attend(wide(q[s:s + 1]), wide(k), wide(v), [n - 1], 0.125)
+        spent = w[0].reshape(kv, heads // kv, n).sum(1)
+        error = 2 * ref.score_error(reach.max(), 64) + 2 * (n + heads) * 2.0 ** -24
+        before, after = wide(was[s]), wide(weights[s])
+        assert np.all(np.abs(after[:, :n] - before[:, :n] - spent) <= error * spent + 2.0 ** -24 * (before[:, :n] + 2 * spent))
+        assert np.array_equal(after[:, n:], before[:, n:])
