@@ -665,70 +665,66 @@ __device__ __noinline__ void piece_by_rows(const PagedArgs &a, const Piece &walk
     }
 }
 
-// A head's weights: rows i = from + first, + step, .. of those seen; N query heads' scores a row and block
-// of heads.  A row's shares are added up before they meet what is there, which may be so much larger
-// that each alone would be lost in its rounding.  lse: of one block; of several (kBlocks) they are read
-// from a.lse, of unit `unit` on.
+// The shares of a block of heads in a head's weights: rows i = from + first, + step, .. of those seen; N
+// query heads' scores a row.  A row's shares are added up before they meet what is there, which may be
+// so much larger that each alone would be lost in its rounding: of several blocks (kBlocks), block b
+// leaves the sum so far where the first one's first score was, and the last adds it to the weight.
 template <int N, int H, bool kBlocks>
 __device__ __forceinline__ void add_rows(const PagedArgs &a, const Piece &walk, int64_t unit, int kh, int from, int to,
-                                         int first, int step, const float (&lse)[H]) {
+                                         int first, int step, const float (&lse)[H], int b) {
     constexpr int kRows = 4;  // in flight
+    const bool last = !kBlocks || b == a.blocks - 1;
     float *weights = a.weights + walk.s * a.w_batch + kh * a.w_head;
+    float *scores = a.scores + unit * a.seen_max * N;
+    const int64_t block = b * a.seen_max * N;
 #pragma unroll 1
     for (int i0 = from + first; i0 < to; i0 += step * kRows) {
+        alignas(16) float2 x[kRows][N / 2];
         float was[kRows], sum[kRows];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            was[r] = weights[walk.seen.at(min(i0 + r * step, to - 1))];
-            sum[r] = 0.f;
-        }
-#pragma unroll 1
-        for (int b = 0; b < (kBlocks ? a.blocks : 1); ++b) {
-            const float *scores = a.scores + (unit + b) * a.seen_max * N;
-            alignas(16) float2 x[kRows][N / 2];
+            const int i = min(i0 + r * step, to - 1);
+            float *row = scores + static_cast<int64_t>(i) * N;
+            was[r] = last ? weights[walk.seen.at(i)] : 0.f;
+            sum[r] = kBlocks && b ? __ldcg(row) : 0.f;
+            if (kBlocks) row += block;
+            if constexpr (N % 4 == 0) {
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                const float *row = scores + static_cast<int64_t>(min(i0 + r * step, to - 1)) * N;
-                if constexpr (N % 4 == 0) {
+                for (int h = 0; h < N / 2; h += 2)
+                    *reinterpret_cast<float4 *>(&x[r][h]) = __ldcg(reinterpret_cast<const float4 *>(row + 2 * h));
+            } else {
 #pragma unroll
-                    for (int h = 0; h < N / 2; h += 2)
-                        *reinterpret_cast<float4 *>(&x[r][h]) = __ldcg(reinterpret_cast<const float4 *>(row + 2 * h));
-                } else {
-#pragma unroll
-                    for (int h = 0; h < N / 2; ++h) x[r][h] = __ldcg(reinterpret_cast<const float2 *>(row + 2 * h));
-                }
+                for (int h = 0; h < N / 2; ++h) x[r][h] = __ldcg(reinterpret_cast<const float2 *>(row + 2 * h));
             }
-            float of[N];
-#pragma unroll
-            for (int h = 0; h < N; ++h)
-                of[h] = !kBlocks ? lse[h] : b * H + h < a.group ? __ldcg(a.lse + (unit + b) * H + h) : INFINITY;
-            // A hidden row's score is -inf, and adds nothing whatever the sum is; nor does a head past the
-            // group (lse infinite), whatever its score is: of an infinite key, 0 x inf.
-            auto share = [&](float score, int h) {
-                return score == -INFINITY || of[h] == INFINITY ? 0.f : ex2(score - of[h]);
-            };
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-#pragma unroll
-                for (int h = 0; h < N / 2; ++h) {
-                    sum[r] += share(x[r][h].x, 2 * h);
-                    sum[r] += share(x[r][h].y, 2 * h + 1);
-                }
         }
+        // A hidden row's score is -inf, and adds nothing whatever the sum is; nor does a head past the
+        // group (lse infinite), whatever its score is: of an infinite key, 0 x inf.
+        auto share = [&](float score, int h) {
+            return score == -INFINITY || lse[h] == INFINITY ? 0.f : ex2(score - lse[h]);
+        };
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
-            if (i0 + r * step < to) weights[walk.seen.at(i0 + r * step)] = was[r] + sum[r];
+        for (int r = 0; r < kRows; ++r) {
+            const int i = i0 + r * step;
+#pragma unroll
+            for (int h = 0; h < N / 2; ++h) {
+                sum[r] += share(x[r][h].x, 2 * h);
+                sum[r] += share(x[r][h].y, 2 * h + 1);
+            }
+            if (i >= to) continue;
+            if (last) weights[walk.seen.at(i)] = was[r] + sum[r];
+            else scores[static_cast<int64_t>(i) * N] = sum[r];
+        }
     }
 }
 template <int H>
 __device__ __forceinline__ void add_weights(const PagedArgs &a, const Piece &walk, int64_t unit, int kh, int from, int to,
                                             int first, int step, const float (&lse)[H]) {
-    if (a.heads2 == 2) return add_rows<2, H, false>(a, walk, unit, kh, from, to, first, step, lse);
+    if (a.heads2 == 2) return add_rows<2, H, false>(a, walk, unit, kh, from, to, first, step, lse, 0);
     if constexpr (H == 8) {
-        if (a.heads2 == 4) return add_rows<4, H, false>(a, walk, unit, kh, from, to, first, step, lse);
-        if (a.heads2 == 6) return add_rows<6, H, false>(a, walk, unit, kh, from, to, first, step, lse);
+        if (a.heads2 == 4) return add_rows<4, H, false>(a, walk, unit, kh, from, to, first, step, lse, 0);
+        if (a.heads2 == 6) return add_rows<6, H, false>(a, walk, unit, kh, from, to, first, step, lse, 0);
     }
-    add_rows<H, H, false>(a, walk, unit, kh, from, to, first, step, lse);
+    add_rows<H, H, false>(a, walk, unit, kh, from, to, first, step, lse, 0);
 }
 
 // Works through pieces; `done(math, piece, q, unit, heads, kh, h0)` takes each one's results.
@@ -865,7 +861,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_paged_few(const __grid
 // own stretch's rows.
 constexpr int kJoin = 2;  // warps for each of k_paged's, to hide the latency of the little that each reads
 
-template <typename T, typename M>
+// kBlocks: with weights, and groups of several blocks of heads (in one kernel with the other case some of its
+// registers spill).
+template <typename T, typename M, bool kBlocks>
 __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ PagedArgs a) {
     constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
     constexpr int64_t kPart = H * DP;
@@ -989,24 +987,18 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
         const int lo = walk.t0 * STEP, rows = min(walk.t1 * STEP, walk.seen.rows) - lo;
         const int from = lo + rows * share / kJoin, to = lo + rows * (share + 1) / kJoin;
         const int64_t unit = static_cast<int64_t>(walk.s) * plan.units + walk.u;
-        float lse[H];
-        for (int b = 0; b < a.blocks; ++b) {
+        const int kh = walk.u / a.blocks;
+        for (int b = 0; b < (kBlocks ? a.blocks : 1); ++b) {
             const int start = walk.base + (walk.u + b) * walk.steps;
             const int b0 = plan.worker_of(start), b1 = plan.worker_of(start + walk.steps - 1);
-            float top[H], sum[H];
+            float top[H], sum[H], lse[H];
             if (b0 != b1) softmax_of({a.partial, b0, plan.start(b0) >= start ? 0 : 1}, b1, top, sum);
 #pragma unroll
             for (int h = 0; h < H; ++h)
                 lse[h] = h >= a.group - b * H ? INFINITY : b0 == b1 ? __ldcg(a.lse + (unit + b) * H + h) : log_sum(top[h], sum[h]);
-            // of several blocks, beside those of whole units: all warps of the unit leave the same there
-            if (a.blocks > 1 && b0 != b1 && lane == 0)
-#pragma unroll
-                for (int h = 0; h < H; ++h) a.lse[(unit + b) * H + h] = lse[h];
+            if constexpr (kBlocks) add_rows<H, H, true>(a, walk, unit, kh, from, to, lane, 32, lse, b);
+            else add_weights<H>(a, walk, unit, kh, from, to, lane, 32, lse);
         }
-        __syncwarp();
-        const int kh = walk.u / a.blocks;
-        if (a.blocks > 1) add_rows<H, H, true>(a, walk, unit, kh, from, to, lane, 32, lse);
-        else add_weights<H>(a, walk, unit, kh, from, to, lane, 32, lse);
     }
 }
 
@@ -1052,7 +1044,8 @@ int launch(mr_context *ctx, PagedArgs &a) {
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings, allowed));
     k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
-    MR_CHECK((launch_early(ctx, dim3(grid * kJoin), dim3(kThreads), k_join<T, M>, a)));
+    MR_CHECK(launch_early(ctx, dim3(grid * kJoin), dim3(kThreads),
+                          a.weights && a.blocks > 1 ? k_join<T, M, true> : k_join<T, M, false>, a));
     return MR_OK;
 }
 
