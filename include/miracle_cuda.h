@@ -48,7 +48,7 @@ enum mr_status {
     MR_ERR_NOMEM = 5      /* device allocation failed */
 };
 
-enum mr_dtype { MR_DTYPE_F32 = 0, MR_DTYPE_F16 = 1, MR_DTYPE_BF16 = 2, MR_DTYPE_I32 = 3 };
+enum mr_dtype { MR_DTYPE_F32 = 0, MR_DTYPE_F16 = 1, MR_DTYPE_BF16 = 2, MR_DTYPE_I32 = 3, MR_DTYPE_U8 = 4 };
 
 /* config.py:9-10 FAMILIES, in order */
 enum mr_family {
@@ -460,6 +460,56 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
                           const mr_array *target_keys, const mr_array *target_values, const mr_array *target_table,
                           const mr_array *kept, const mr_array *new_lengths, const mr_array *new_weights, int budget,
                           int sinks, int recent);
+
+/* ---- pages of 4 bits a value ---------------------------------------------------
+ * mr_append_pages, mr_append_rotated, mr_read_pages, mr_paged_attention and
+ * mr_evict_pages also take pools of U8 [pages, page rows, kv heads, 5 dim / 8], for
+ * head dims 32, 64, 96 and 128; each row starts on a boundary of 4 bytes (dims 32
+ * and 96), 8 (64) or 16 (128), in address and strides.  A row is dim / 2 bytes of codes, the even dim in a
+ * byte's low half, then for each 32 dims two little-endian IEEE float16 numbers, a
+ * step s and a base z: code c stands for s (64 + c) + z, rounded to float16.
+ * Writing a row: s = (max - min) / 15 of the 32 values and z = min - 64 s, each
+ * rounded to float16, c the nearest of 0 .. 15; 32 values of which one is not finite
+ * or which are too far apart for float16 (from about +-13 000 on) read as NaN.
+ * What is written depends on the values alone. */
+
+/* mr_append_pages with a rotation on the way: the first 2 n dims of each query
+ * [tokens, heads, dim] and key are turned by position * frequencies[p] (F32 [n],
+ * n <= dim / 2; NULL: none) for pair p, which is the dims 2 p and 2 p + 1, or with
+ * split_half p and p + n (kernels.cl:30-44).  A token's position is positions[i]
+ * (I32 [tokens]), or its row of the sequence where positions is NULL.  The angle is
+ * the exact product, its sine and cosine are rounded to float32 once (mr_op_rope
+ * rounds the product too), and so is each product and sum of a turn; the result is
+ * rounded to the type, or to 4 bits.  Turned queries go to out [tokens, heads, dim]
+ * (query and out may both be NULL); those of tokens in no sequence stay as they
+ * were.  All of query, keys, values and out are of one type, the pages of the same
+ * or of 4 bits. */
+MR_API int mr_append_rotated(mr_context *ctx, const mr_array *query, const mr_array *keys, const mr_array *values,
+                             const mr_array *key_pages, const mr_array *value_pages, const mr_array *page_table,
+                             const mr_array *lengths, const mr_array *offsets, const mr_array *frequencies,
+                             const mr_array *positions, const mr_array *out, int split_half);
+
+/* The way back of mr_append_pages: sequence s's last offsets[s + 1] - offsets[s]
+ * rows (NULL: its newest row) go to keys and values [tokens, kv heads, dim] at
+ * offsets[s] ..; from 4-bit pages as any floating type, from others as their own.  A row that
+ * the pages do not hold (a bad page, past the table, before the first) is zeros;
+ * rows of keys and values in no sequence stay as they were. */
+MR_API int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const mr_array *value_pages,
+                         const mr_array *page_table, const mr_array *lengths, const mr_array *offsets,
+                         const mr_array *keys, const mr_array *values);
+
+/* ---- log probabilities ------------------------------------------------------------
+ * Of rows of logits [rows, vocabulary] (F32, F16 or BF16): the log probability of
+ * each of the given tokens (I32 [rows] or [rows, n]; one outside the vocabulary, as
+ * padding is, gives 0) in logprobs F32 of the same shape; the entropy in nats in
+ * F32 [rows]; and the most likely tokens, falling, the lower one of equals first
+ * (NaN counts as the lowest), in top_tokens I32 and top_logprobs F32 [rows, top],
+ * top at most 128 and the vocabulary.  tokens and logprobs, and the last two, may be
+ * NULL together; entropy too.  A logit of -inf has probability 0 and adds nothing; a row of
+ * them alone has log probabilities -inf and entropy 0; a NaN or +inf in a row makes its
+ * log probabilities and its entropy NaN.  Sums are float32. */
+MR_API int mr_log_probabilities(mr_context *ctx, const mr_array *logits, const mr_array *tokens, const mr_array *logprobs,
+                                const mr_array *entropy, const mr_array *top_tokens, const mr_array *top_logprobs);
 
 #ifdef __cplusplus
 }

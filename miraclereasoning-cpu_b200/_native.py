@@ -112,6 +112,9 @@ SIGNATURES = {
     "mr_paged_attention": (_I, [_P] * 8 + [_I, _I, _F]),
     "mr_window_attention": (_I, [_P] * 7 + [_I, _I, _F]),
     "mr_evict_pages": (_I, [_P] * 12 + [_I, _I, _I]),
+    "mr_append_rotated": (_I, [_P] * 12 + [_I]),
+    "mr_read_pages": (_I, [_P] * 8),
+    "mr_log_probabilities": (_I, [_P] * 7),
     "mr_model_set_wait_limit": (_I, [_P, C.c_uint64]),
     "mr_model_load_file": (_I, [_P, C.c_char_p, _I, _I, C.POINTER(C.c_int64), C.c_char_p, C.c_uint64]),
     "mr_model_inject_fault": (_I, [_P, _I]),

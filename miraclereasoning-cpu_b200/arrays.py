@@ -2,8 +2,9 @@
 
 An operator argument is a backend ``Tensor`` (float32), a ``DeviceArray`` made by ``CUDABackend.upload_array`` /
 ``empty_array``, or any object with the same accessors on the backend's GPU: ``data_ptr()``, ``shape``, ``stride()``,
-``dtype`` (named float32, float16, bfloat16 or int32), ``get_device()`` and ``new_empty(shape)``, as torch tensors
-have.  The owner keeps the memory alive until the queued work is done.
+``dtype`` (named float32, float16, bfloat16, int32 or uint8), ``get_device()`` and ``new_empty(shape)``, with a
+``dtype`` too where outputs are of another type than the inputs, as torch tensors have.  The owner keeps the memory alive
+until the queued work is done.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import importlib.machinery
 import importlib.util
 import math
 import struct
+import sys
 from pathlib import Path
 
 import numpy as np
@@ -19,8 +21,8 @@ import numpy as np
 from . import _native
 from .weights import float32_to_bf16_bits
 
-TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 3}   # enum mr_dtype
-_ITEM = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4}
+TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int32": 3, "uint8": 4}   # enum mr_dtype
+_ITEM = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "uint8": 1}
 _CODES = {}    # a dtype object -> its code, as its name says
 
 
@@ -37,15 +39,16 @@ def described(array, name, device):
         raise ValueError(f"{name} must have 1 to 4 dimensions, not {len(shape)}")
     code = TYPES.get(str(dtype).rsplit(".", 1)[-1])
     if code is None:
-        raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16 or int32 is needed")
+        raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16, int32 or uint8 is needed")
     _CODES[dtype] = code
     pad = (0,) * (4 - len(shape))
     return struct.pack("<Qii8q", array.data_ptr(), code, len(shape), *shape, *pad, *array.stride(), *pad)
 
 
 # the operators in csrc/pycall.c's order
-APPEND, PAGED, WINDOW, EVICT = range(4)
-_NAMES = ("mr_append_pages", "mr_paged_attention", "mr_window_attention", "mr_evict_pages")
+APPEND, PAGED, WINDOW, EVICT, ROTATED, READ, SCORE = range(7)
+_NAMES = ("mr_append_pages", "mr_paged_attention", "mr_window_attention", "mr_evict_pages", "mr_append_rotated",
+          "mr_read_pages", "mr_log_probabilities")
 # this interpreter's own build of csrc/pycall.c
 PYCALL = Path(__file__).resolve().with_name("_pycall" + importlib.machinery.EXTENSION_SUFFIXES[0])
 _module = None   # the module, once a call has needed it
@@ -95,7 +98,7 @@ class DeviceArray:
         if not shape or any(not isinstance(n, int) or n < 0 for n in shape):
             raise ValueError(f"invalid array shape: {shape}")
         if dtype not in TYPES:
-            raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16 or int32 is needed")
+            raise ValueError(f"unsupported array type {dtype}: float32, float16, bfloat16, int32 or uint8 is needed")
         self.backend, self.shape, self.dtype = backend, shape, dtype
         self.size = math.prod(shape)
         self.words = max(1, -(-self.size * _ITEM[dtype] // 4))   # the buffer's float32 elements
@@ -124,8 +127,18 @@ class DeviceArray:
             step *= max(n, 1)
         return tuple(reversed(strides))
 
-    def new_empty(self, shape):
-        return DeviceArray(self.backend, shape, self.dtype)
+    def new_empty(self, shape, dtype=None):
+        return DeviceArray(self.backend, shape, dtype or self.dtype)
+
+
+def empty_like(array, shape, dtype):
+    """An array of another type by the owner of `array`: its library's type of that name."""
+    kind = array.dtype
+    if str(kind).rsplit(".", 1)[-1] == dtype:
+        return array.new_empty(shape)
+    if not isinstance(kind, str):
+        dtype = getattr(sys.modules[type(kind).__module__], dtype)
+    return array.new_empty(shape, dtype=dtype)
 
 
 def stored(array, dtype):

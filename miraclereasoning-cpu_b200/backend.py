@@ -9,8 +9,10 @@ dispatches to the kernel's ``mr_op_*`` entry point.  There is no host fallback:
 a missing library or device raises ``CUDAError``.
 
 Beyond the reference: a paged key / value cache for serving several sequences
-(``append_pages``, ``paged_attention``, ``window_attention``, ``evict_pages``),
-on arrays of any owner in float32, float16 or bfloat16 (``arrays.py``).
+(``append_pages``, ``append_rotated``, ``read_pages``, ``paged_attention``,
+``window_attention``, ``evict_pages``), and ``log_probabilities`` of its logits,
+on arrays of any owner in float32, float16 or bfloat16 (``arrays.py``); the cache
+may be held in 4 bits a value.
 """
 from __future__ import annotations
 
@@ -22,7 +24,7 @@ import numpy as np
 
 from . import _native, arrays
 from ._native import CUDAError, call
-from .arrays import DeviceArray, host_type, invoke, stored, widened
+from .arrays import DeviceArray, empty_like, host_type, invoke, stored, widened
 
 # kernel name -> (NDRange rank, argument kinds) in kernels.cl order
 _KERNELS = {
@@ -85,8 +87,8 @@ class Tensor:
         call("mr_buffer_pointer", self.handle, C.byref(pointer))
         return pointer.value
 
-    def new_empty(self, shape):
-        return self.backend.empty(shape)
+    def new_empty(self, shape, dtype="float32"):
+        return self.backend.empty(shape) if dtype == "float32" and all(shape) else DeviceArray(self.backend, shape, dtype)
 
 
 def _count(value, name, least=0):
@@ -289,11 +291,35 @@ class CUDABackend:
     # paged key / value cache (include/miracle_cuda.h: mr_array and what follows) -----
     # Pools are [pages, page rows, kv heads, dim], page_table [batch, table pages] and lengths
     # [batch] int32; row t of sequence s is row t % page rows of page page_table[s, t // page rows].
+    # Pools of uint8 [pages, page rows, kv heads, 5 dim / 8] hold 4 bits a value, for head dims 32, 64, 96 and 128:
+    # a step and a base for 32 values (the header has the format).  append_pages, append_rotated, read_pages,
+    # paged_attention and evict_pages take them.
 
     def append_pages(self, keys, values, key_pages, value_pages, page_table, lengths, offsets=None):
         """New rows [tokens, kv heads, dim] into their pages.  ``lengths`` counts them already; sequence s's
         new rows are offsets[s] .. offsets[s + 1] - 1 (``offsets`` None: one row per sequence)."""
         invoke(arrays.APPEND, *self._where, keys, values, key_pages, value_pages, page_table, lengths, offsets)
+
+    def append_rotated(self, keys, values, key_pages, value_pages, page_table, lengths, frequencies, offsets=None, *,
+                       positions=None, query=None, out=None, split_half=False):
+        """``append_pages`` with the position rotation on the way: the first 2 n dims of ``keys``, and of ``query``
+        [tokens, heads, dim], are turned by position * ``frequencies`` [n] (float32), in pairs of neighbours or with
+        ``split_half`` of dims p and p + n (as ``rotate`` does).  ``positions`` int32 [tokens]; None: a token's row of
+        its sequence.  Returns the turned query, ``out`` (an array like the query; rows of no sequence are not
+        written), or None without one."""
+        if query is not None and out is None:
+            out = _like(query, "query")
+        invoke(arrays.ROTATED, *self._where, query, keys, values, key_pages, value_pages, page_table, lengths, offsets,
+               frequencies, positions, out, 1 if split_half else 0)
+        return out
+
+    def read_pages(self, key_pages, value_pages, page_table, lengths, offsets, keys, values):
+        """The way back of ``append_pages``: each sequence's last rows from their pages to ``keys`` and ``values``
+        [tokens, kv heads, dim], sequence s's to offsets[s] .. offsets[s + 1] - 1 (``offsets`` None: its newest row
+        alone).  From 4-bit pages as any floating type, so that ``window_attention`` can take a prompt's later part.
+        Rows that no page holds are zeros.  Returns (keys, values)."""
+        invoke(arrays.READ, *self._where, key_pages, value_pages, page_table, lengths, offsets, keys, values)
+        return keys, values
 
     def paged_attention(self, query, key_pages, value_pages, page_table, lengths, *, window=None, sinks=0, scale=None,
                         weights=None, out=None):
@@ -347,6 +373,31 @@ class CUDABackend:
         invoke(arrays.EVICT, *self._where, key_pages, value_pages, page_table, lengths, weights, target_keys, target_values,
                target_table, kept, new_lengths, new_weights, budget, sinks, recent)
         return kept, new_lengths, new_weights
+
+    # logits (include/miracle_cuda.h: mr_log_probabilities) ----------------------------
+    def log_probabilities(self, logits, tokens=None, *, top=0, logprobs=None, entropy=None, top_tokens=None,
+                          top_logprobs=None):
+        """Of rows of ``logits`` [rows, vocabulary]: (logprobs, entropy, top_tokens, top_logprobs).  ``logprobs`` are
+        the log probabilities of ``tokens`` (int32 [rows] or [rows, n]; one outside the vocabulary gives 0), None
+        without them; ``entropy`` [rows] in nats; the ``top`` most likely tokens (at most 128) and their log
+        probabilities [rows, top], falling, the lower token first where they are equal."""
+        top = _count(top, "top")
+        if len(getattr(logits, "shape", ())) != 2:
+            raise ValueError("logits must be an array [rows, vocabulary]")
+        rows = logits.shape[0]
+        if tokens is not None and logprobs is None:
+            logprobs = empty_like(logits, tuple(tokens.shape), "float32")
+        if entropy is None:
+            entropy = empty_like(logits, (rows,), "float32")
+        if top_tokens is None:
+            top_tokens = empty_like(logits, (rows, top), "int32")
+        if top_logprobs is None:
+            top_logprobs = empty_like(logits, (rows, top), "float32")
+        if tuple(top_tokens.shape) != (rows, top):
+            raise ValueError(f"top_tokens must be [{rows}, {top}]")
+        best = (top_tokens, top_logprobs) if top else (None, None)
+        invoke(arrays.SCORE, *self._where, logits, tokens, logprobs, entropy, *best)
+        return logprobs, entropy, top_tokens, top_logprobs
 
     def finish(self):
         call("mr_context_finish", self.context)

@@ -13,7 +13,10 @@ namespace cache {
 
 constexpr int kMaxDim = 128;
 
-inline int dtype_bytes(int dtype) { return dtype == MR_DTYPE_F16 || dtype == MR_DTYPE_BF16 ? 2 : 4; }
+inline int dtype_bytes(int dtype) {
+    return dtype == MR_DTYPE_F16 || dtype == MR_DTYPE_BF16 ? 2 : dtype == MR_DTYPE_U8 ? 1 : 4;
+}
+inline bool is_float(int dtype) { return dtype == MR_DTYPE_F32 || dtype == MR_DTYPE_F16 || dtype == MR_DTYPE_BF16; }
 
 // One array argument: its shape, type and strides are usable by the kernels.
 // rows: the last dimension is read in 16-byte pieces.  Sets the error and
@@ -21,7 +24,7 @@ inline int dtype_bytes(int dtype) { return dtype == MR_DTYPE_F16 || dtype == MR_
 inline int check_array(const mr_array *a, const char *name, int ndim, bool rows, bool written) {
     MR_REQUIRE(a, "%s is missing", name);
     MR_REQUIRE(a->ndim == ndim, "%s must have %d dimensions, not %d", name, ndim, a->ndim);
-    MR_REQUIRE(a->dtype >= MR_DTYPE_F32 && a->dtype <= MR_DTYPE_I32, "%s has an unknown type", name);
+    MR_REQUIRE(a->dtype >= MR_DTYPE_F32 && a->dtype <= MR_DTYPE_U8, "%s has an unknown type", name);
     const int64_t size = dtype_bytes(a->dtype), most = int64_t(1) << 46;
     bool empty = false;
     for (int i = 0; i < ndim; ++i) {
@@ -84,7 +87,7 @@ inline int check_weights(const mr_array *a, const char *name, int64_t batch, int
 inline int check_pools(const mr_array *k, const mr_array *v, const char *kn, const char *vn, bool written) {
     MR_CHECK(check_array(k, kn, 4, true, written));
     MR_CHECK(check_array(v, vn, 4, true, written));
-    MR_REQUIRE(k->dtype != MR_DTYPE_I32 && k->dtype == v->dtype, "%s and %s must be of one floating type", kn, vn);
+    MR_REQUIRE(is_float(k->dtype) && k->dtype == v->dtype, "%s and %s must be of one floating type", kn, vn);
     for (int i = 0; i < 4; ++i) MR_REQUIRE(k->shape[i] == v->shape[i], "%s and %s differ in shape", kn, vn);
     MR_REQUIRE(k->shape[1] > 0 && k->shape[2] > 0 && k->shape[3] > 0, "%s: an empty page row", kn);
     return MR_OK;

@@ -389,6 +389,9 @@ using namespace mr::cache;
 extern "C" int mr_append_pages(mr_context *ctx, const mr_array *keys, const mr_array *values, const mr_array *key_pages,
                                const mr_array *value_pages, const mr_array *page_table, const mr_array *lengths,
                                const mr_array *offsets) {
+    if (key_pages && key_pages->dtype == MR_DTYPE_U8)
+        return mr_append_rotated(ctx, nullptr, keys, values, key_pages, value_pages, page_table, lengths, offsets, nullptr,
+                                 nullptr, nullptr, 0);
     MR_CHECK(check_array(keys, "keys", 3, true, false));
     MR_CHECK(check_array(values, "values", 3, true, false));
     MR_CHECK(check_pools(key_pages, value_pages, "key_pages", "value_pages", true));

@@ -19,7 +19,7 @@
 
 #define MOST 11
 
-enum { APPEND, PAGED, WINDOW, EVICT, CALLS };  /* arrays.py has the same order */
+enum { APPEND, PAGED, WINDOW, EVICT, ROTATED, READ, SCORE, CALLS };  /* arrays.py has the same order */
 static const struct {
     int arrays, scalars;
     const char *names[MOST];
@@ -29,6 +29,10 @@ static const struct {
     {6, 3, {"query", "keys", "values", "query_offsets", "key_offsets", "out"}},
     {11, 3, {"key_pages", "value_pages", "page_table", "lengths", "weights", "target_keys", "target_values",
              "target_table", "kept", "new_lengths", "new_weights"}},
+    {11, 1, {"query", "keys", "values", "key_pages", "value_pages", "page_table", "lengths", "offsets", "frequencies",
+             "positions", "out"}},
+    {7, 0, {"key_pages", "value_pages", "page_table", "lengths", "offsets", "keys", "values"}},
+    {6, 0, {"logits", "tokens", "logprobs", "entropy", "top_tokens", "top_logprobs"}},
 };
 static void *functions[CALLS];
 static PyObject *codes;      /* dtype -> enum mr_dtype, of the types met */
@@ -129,14 +133,21 @@ static PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n) {
     else if (which == WINDOW)
         status = ((int (*)(mr_context *, A, A, A, A, A, A, int, int, float))f)(ctx, a[0], a[1], a[2], a[3], a[4], a[5], x[0],
                                                                              x[1], scale);
-    else
+    else if (which == EVICT)
         status = ((int (*)(mr_context *, A, A, A, A, A, A, A, A, A, A, A, int, int, int))f)(
             ctx, a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], x[0], x[1], x[2]);
+    else if (which == ROTATED)
+        status = ((int (*)(mr_context *, A, A, A, A, A, A, A, A, A, A, A, int))f)(
+            ctx, a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], x[0]);
+    else if (which == READ)
+        status = ((int (*)(mr_context *, A, A, A, A, A, A, A))f)(ctx, a[0], a[1], a[2], a[3], a[4], a[5], a[6]);
+    else
+        status = ((int (*)(mr_context *, A, A, A, A, A, A))f)(ctx, a[0], a[1], a[2], a[3], a[4], a[5]);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(status);
 }
 
-/* bind(addresses): of mr_append_pages, mr_paged_attention, mr_window_attention, mr_evict_pages */
+/* bind(addresses): of the library's functions, in that order */
 static PyObject *bind(PyObject *self, PyObject *const *args, Py_ssize_t n) {
     (void)self;
     if (n != CALLS) return PyErr_Format(PyExc_TypeError, "bind takes %d addresses, not %zd", CALLS, n);

@@ -1007,7 +1007,7 @@ extern "C" int mr_window_attention(mr_context *ctx, const mr_array *query, const
     MR_CHECK(check_array(keys, "keys", 3, true, false));
     MR_CHECK(check_array(values, "values", 3, true, false));
     MR_CHECK(check_array(out, "out", 3, true, true));
-    MR_REQUIRE(query->dtype != MR_DTYPE_I32 && keys->dtype == query->dtype && values->dtype == query->dtype &&
+    MR_REQUIRE(is_float(query->dtype) && keys->dtype == query->dtype && values->dtype == query->dtype &&
                    out->dtype == query->dtype,
                "query, keys, values and out must be of one floating type");
     for (int i = 0; i < 3; ++i) {
