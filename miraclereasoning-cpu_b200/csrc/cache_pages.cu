@@ -6,7 +6,7 @@
 // writes the kept rows.  Rows move as 16-byte pieces, consecutive threads taking
 // consecutive pieces of a row and then the next key / value head, so that both
 // sides touch whole 32-byte sectors whatever the head dim.
-#include "cache_ops.cuh"
+#include "packed.cuh"
 
 namespace mr {
 namespace cache {
@@ -324,8 +324,10 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
 }
 
 // Kept rows to their target pages: a warp takes 32 rows of a head, a lane looks up one row's two
-// places, and all copy the rows piece by piece, four loads of each pool in flight a lane.
+// places, and all copy the rows piece by piece (16 bytes, or what rows of 4-bit values are whole
+// multiples of), four loads of each pool in flight a lane.
 constexpr int kCopyWarps = 4;
+template <typename Bytes>
 __global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_constant__ EvictArgs a) {
     const int s = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % 32;
     const int at = (blockIdx.x * kCopyWarps + threadIdx.x / 32) * 32 + lane;
@@ -353,19 +355,19 @@ __global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_cons
     const int n = 32 * a.pieces;
     constexpr int kFlight = 4;
     for (int e0 = lane; e0 < n; e0 += 32 * kFlight) {
-        uint4 x[kFlight], y[kFlight];
+        Bytes x[kFlight], y[kFlight];
         int64_t tks[kFlight], tvs[kFlight];
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
-            const int e = min(e0 + 32 * i, n - 1), r = e / a.pieces, c = (e - r * a.pieces) * 16;
+            const int e = min(e0 + 32 * i, n - 1), r = e / a.pieces, c = (e - r * a.pieces) * static_cast<int>(sizeof(Bytes));
             const int64_t from_k = __shfl_sync(0xffffffffu, k, r), from_v = __shfl_sync(0xffffffffu, v, r);
             tks[i] = __shfl_sync(0xffffffffu, to_k, r);
             tvs[i] = __shfl_sync(0xffffffffu, to_v, r);
             if (e0 + 32 * i >= n) tks[i] = -1;
-            x[i] = y[i] = make_uint4(0, 0, 0, 0);
+            x[i] = y[i] = Bytes{};
             if (from_k >= 0 && tks[i] >= 0) {
-                x[i] = __ldcs(reinterpret_cast<const uint4 *>(kb + from_k + c));
-                y[i] = __ldcs(reinterpret_cast<const uint4 *>(vb + from_v + c));
+                x[i] = __ldcs(reinterpret_cast<const Bytes *>(kb + from_k + c));
+                y[i] = __ldcs(reinterpret_cast<const Bytes *>(vb + from_v + c));
             }
             tks[i] += c;
             tvs[i] += c;
@@ -374,8 +376,8 @@ __global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_cons
 #pragma unroll
         for (int i = 0; i < kFlight; ++i)
             if (tks[i] >= 0) {
-                *reinterpret_cast<uint4 *>(tk + tks[i]) = x[i];
-                *reinterpret_cast<uint4 *>(tv + tvs[i]) = y[i];
+                *reinterpret_cast<Bytes *>(tk + tks[i]) = x[i];
+                *reinterpret_cast<Bytes *>(tv + tvs[i]) = y[i];
             }
     }
 }
@@ -452,8 +454,14 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
                               const mr_array *target_keys, const mr_array *target_values, const mr_array *target_table,
                               const mr_array *kept, const mr_array *new_lengths, const mr_array *new_weights,
                               int budget, int sinks, int recent) {
-    MR_CHECK(check_pools(key_pages, value_pages, "key_pages", "value_pages", false));
-    MR_CHECK(check_pools(target_keys, target_values, "target_keys", "target_values", true));
+    const bool packed = key_pages && key_pages->dtype == MR_DTYPE_U8;
+    if (packed) {
+        MR_CHECK(check_packed(key_pages, value_pages, "key_pages", "value_pages", false));
+        MR_CHECK(check_packed(target_keys, target_values, "target_keys", "target_values", true));
+    } else {
+        MR_CHECK(check_pools(key_pages, value_pages, "key_pages", "value_pages", false));
+        MR_CHECK(check_pools(target_keys, target_values, "target_keys", "target_values", true));
+    }
     MR_REQUIRE(target_keys->dtype == key_pages->dtype, "the target pages must be of the pages' type");
     for (int i = 1; i < 4; ++i)
         MR_REQUIRE(target_keys->shape[i] == key_pages->shape[i],
@@ -512,7 +520,8 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     a.budget = budget;
     a.sinks = sinks;
     a.recent = recent;
-    a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / 16);
+    const int unit = packed ? packed_unit(key_pages->shape[3]) : 16;
+    a.pieces = static_cast<int>(key_pages->shape[3] * dtype_bytes(key_pages->dtype) / unit);
     static std::atomic<uint64_t> allowed{0};
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_select), kCached * 4, allowed));
     const int cached = capacity <= kCached ? (static_cast<int>(capacity) + 3) / 4 * 16 : 0;
@@ -521,7 +530,8 @@ extern "C" int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const 
     const int64_t rows = std::min<int64_t>(budget, capacity);
     if (rows) {
         const dim3 grid(static_cast<unsigned>((rows - 1) / (32 * kCopyWarps) + 1), a.heads, a.batch);
-        MR_CHECK(launch_early(ctx, grid, dim3(kCopyWarps * 32), k_copy_kept, a));
+        MR_CHECK(launch_early(ctx, grid, dim3(kCopyWarps * 32),
+                              unit == 16 ? k_copy_kept<uint4> : unit == 8 ? k_copy_kept<uint2> : k_copy_kept<uint32_t>, a));
     }
     return MR_OK;
 }

@@ -24,7 +24,7 @@ inline int packed_unit(int64_t bytes) { return static_cast<int>(std::min<int64_t
 inline int check_packed(const mr_array *k, const mr_array *v, const char *kn, const char *vn, bool written) {
     MR_CHECK(check_array(k, kn, 4, false, written));
     MR_CHECK(check_array(v, vn, 4, false, written));
-    MR_REQUIRE(k->dtype == v->dtype, "%s and %s must be of one type", kn, vn);
+    MR_REQUIRE(k->dtype == MR_DTYPE_U8 && v->dtype == MR_DTYPE_U8, "%s and %s must be of one type", kn, vn);
     for (int i = 0; i < 4; ++i) MR_REQUIRE(k->shape[i] == v->shape[i], "%s and %s differ in shape", kn, vn);
     MR_REQUIRE(k->shape[1] > 0 && k->shape[2] > 0, "%s: an empty page row", kn);
     const int64_t bytes = k->shape[3];

@@ -177,3 +177,18 @@ def test_arrays_of_bytes():
     import torch
     made = arrays.empty_like(torch.zeros(2, dtype=torch.bfloat16), (4, 1), "float32")
     assert made.dtype == torch.float32 and made.shape == (4, 1)
+
+
+def test_attention_and_eviction_of_4_bits_are_checked():
+    k, v = bytes_of(64)
+    both = dict(key_pages=k, value_pages=v)
+    assert paged(**both) == "ctx is NULL"
+    assert paged(query=Fake((3, 8, 64), F32), out=Fake((3, 8, 64), F32, pointer=1 << 28), **both) == "ctx is NULL"
+    assert "of one floating type" in paged(out=Fake((3, 8, 64), F32, pointer=1 << 28), **both)
+    assert "of one floating type" in paged(query=Fake((3, 8, 64), I32), out=Fake((3, 8, 64), I32, pointer=1 << 28), **both)
+    assert "of one type" in paged(key_pages=k)
+    assert "32 values a head, the pages 64" in paged(query=Fake((3, 8, 32)), out=Fake((3, 8, 32), pointer=1 << 28), **both)
+    far = bytes_of(64, stride=(1 << 32, 160, 40, 1))
+    assert "stride 0 passes 4 GB" in paged(key_pages=far[0], value_pages=far[1])
+    assert evict(target_keys=k, target_values=v, **both) == "ctx is NULL"
+    assert "target_keys and target_values must be of one type" in evict(**both)
