@@ -48,6 +48,13 @@ __device__ __forceinline__ uint32_t codes64(uint32_t word) {
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x54005400, 0xea;" : "=r"(x) : "r"(word));
     return x;
 }
+// All eight codes of a word, those n and n + 4 of the natural order in c[n].
+__device__ __forceinline__ void word_codes(uint32_t word, uint32_t (&c)[4]) {
+    c[0] = codes64(word << 4);
+    c[1] = codes64(word);
+    c[2] = codes64(word >> 4);
+    c[3] = codes64(word >> 8);
+}
 // s (64 + c) + z of two codes.
 __device__ __forceinline__ uint32_t fma2(uint32_t codes, __half2 s, __half2 z) {
     const __half2 x = __hfma2(*reinterpret_cast<const __half2 *>(&codes), s, z);

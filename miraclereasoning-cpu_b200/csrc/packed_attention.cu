@@ -10,6 +10,15 @@
 // ldmatrix transposes 16-bit units (four codes) of eight rows, so that each register
 // holds the same four dims of two rows, and the four results of a word go to rows of
 // different product tiles.
+//
+// A step of 32 rows of 128 dims is 665 instructions: 210 and 220 for the two products' operands and issue, 95
+// for the softmax, 120 for the copies of two steps on.  32 sequences ragged to 32768 rows at 8 heads of 128
+// (668 MB): 145 us, of which 20 are the start, the uneven end and the join; the copies alone take 113.
+// Logical operations and float16 multiply-adds each issue every other cycle, and 1.5 cycles each when
+// mixed, so that moving work between the two gains nothing (shifts as additions: 166 and 167 us at the time);
+// 8-bit floating-point products of the codes as they stand (e4m3 0 .. 15 are linear) need fewer masks, but that
+// type is widened in software here: 790 instructions a step, 175 us.  Four CTAs an SM spill (150); of
+// all 16 warps' stretches joined in shared memory first, one long sequence gains 1 us and the batch loses 8.
 #include "packed.cuh"
 #include "paged_core.cuh"
 
@@ -24,6 +33,10 @@ struct Ring4 {
     static constexpr int kRowBytes = DP <= 64 ? 48 : 80;  // odd multiples of 16: eight rows' pieces lie in different banks
     static __device__ __forceinline__ int pieces(const PagedArgs &) { return kPieces; }
     static __device__ __forceinline__ uint32_t offset(int row, int piece) { return row * kRowBytes + piece * kUnit; }
+    // of piece e of a step's rows
+    static __device__ __forceinline__ uint32_t place(int e) {
+        return kRowBytes == kRow ? e * kUnit : offset(e / kPieces, e % kPieces);
+    }
 };
 
 __device__ __forceinline__ void ldmatrix2(uint32_t (&r)[4], uint32_t address) {
@@ -53,16 +66,26 @@ struct Math4 : Heads8<__half, DP_ / 16> {
     using Base::o;
     using Base::m;
     using Base::l;
-    static constexpr bool kAgain = false;  // what is not finite here is NaN, and stays it
+    static constexpr bool kRuns = true, kAgain = false;  // what is not finite here is NaN, and stays it
     static constexpr int kCtas = 3, DP = DP_, G = DP / kShared, kHeads = 8, STEP = 32;
-    // Queries of 16 bits are one float16 operand, those of 32 two, scaled by a power of 2 for each head so that
-    // the largest value is below 2^15: what float16 loses is below 2^-39 of it, or 2^-22 of the value itself.
-    static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+    // CTAs of an SM.  Three have more steps under way, two leave room for the joining kernel's CTAs to start beside
+    // them and fewer partials to join: from about 24 steps a warp on (by the tables; with weights, which the joining
+    // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128: 1 sequence 23.2 with two, 27.4 with
+    // three; 4 sequences 49.6, 49.8; 16 sequences 158, 146).
+    static int ctas(int64_t steps, int sms, bool weights) {
+        return steps >= (weights ? 48 : 24) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
+    }
+    // Weights in one float16 part are off by 2^-12, an eighth of a bfloat16 result's rounding; other results
+    // get a second part.
+    static constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
     struct R : Ring4<DP> {
         static constexpr int kBytes = 2 * STEP * Ring4<DP>::kRowBytes;
         static constexpr int kWarpBytes = kBytes * 3;
     };
     static constexpr int STAGES = 3;
+    // Queries of 16 bits are one float16 operand, those of 32 two, scaled by a power of 2 for each head so that
+    // the largest is in [2^14, 2^15): what is lost is below 2^-39 of it, or 2^-22 of the value itself.
+    static constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
     uint32_t qf[kParts][G][2][2];
     float f[2];  // of heads 2 (lane % 4), + 1: products to scores
 
@@ -81,7 +104,7 @@ struct Math4 : Heads8<__half, DP_ / 16> {
         // 2^n: 14 less the exponent of the largest; 1 where that is 0 or not finite
         const int exponent = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 127);
         const int n = most > 0.f && most < INFINITY ? 14 - exponent : 0;
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + n) << 23);      // n: -113 .. 114
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + n) << 23);  // n: -113 .. 114
         const float down = __uint_as_float(static_cast<uint32_t>(127 - n) << 23);
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -89,7 +112,7 @@ struct Math4 : Heads8<__half, DP_ / 16> {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    // codes 2 j + e of the word's two halves
+                    // codes 2 j + e of a word's two halves
                     const float u = x[g][2 * j + e] * up, w = x[g][4 + 2 * j + e] * up;
                     qf[0][g][j][e] = pack2(u, w, __half());
                     if constexpr (kParts == 2) {
@@ -102,47 +125,51 @@ struct Math4 : Heads8<__half, DP_ / 16> {
         this->clear();
     }
 
+    // S^T of 16 rows at `tile`.
+    __device__ __forceinline__ void products(float (&s)[4], uint32_t tile) const {
+        const int lane = threadIdx.x % 32, r = lane / 4;
+        const uint32_t part = (lane % 16) * R::kRowBytes + lane / 16 * 16;
+        s[0] = s[1] = s[2] = s[3] = 0.f;
+        uint32_t p0[G], p1[G];
+        load_pairs<G>(p0, tile + r * R::kRowBytes + DP / 2);
+        load_pairs<G>(p1, tile + (r + 8) * R::kRowBytes + DP / 2);
+#pragma unroll
+        for (int g = 0; g < G; g += 2) {
+            uint32_t w[4];
+            if (g + 1 < G) ldmatrix(w, tile + part + g * 16);
+            else ldmatrix2(w, tile + part + g * 16 - lane / 16 * 16);
+#pragma unroll
+            for (int i = 0; i < (g + 1 < G ? 2 : 1); ++i) {
+                const __half2 s0 = __low2half2(halves(p0[g + i])), z0 = __high2half2(halves(p0[g + i]));
+                const __half2 s1 = __low2half2(halves(p1[g + i])), z1 = __high2half2(halves(p1[g + i]));
+                uint32_t u[4], v[4];
+                word_codes(w[2 * i], u);
+                word_codes(w[2 * i + 1], v);
+                const uint32_t k0[4] = {fma2(u[0], s0, z0), fma2(v[0], s1, z1), fma2(u[1], s0, z0), fma2(v[1], s1, z1)};
+                const uint32_t k1[4] = {fma2(u[2], s0, z0), fma2(v[2], s1, z1), fma2(u[3], s0, z0), fma2(v[3], s1, z1)};
+#pragma unroll
+                for (int part_of = kParts - 1; part_of >= 0; --part_of) {
+                    mma16(s, k0, qf[part_of][g + i][0][0], qf[part_of][g + i][0][1], __half());
+                    mma16(s, k1, qf[part_of][g + i][1][0], qf[part_of][g + i][1][1], __half());
+                }
+            }
+        }
+    }
+
     __device__ __forceinline__ void step(const PagedArgs &a, uint32_t stage, uint32_t live, int rows, float *scores) {
-        const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+        const int lane = threadIdx.x % 32, c = lane % 4;
         constexpr int S = STEP / 16;
         // this lane's row and piece for ldmatrix: 16 rows of two groups' codes
         const uint32_t part = (lane % 16) * R::kRowBytes + lane / 16 * 16;
         float s[S][4];
 #pragma unroll
-        for (int x = 0; x < S; ++x) {
-            s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-            const uint32_t tile = stage + x * 16 * R::kRowBytes;
-            uint32_t p0[G], p1[G];
-            load_pairs<G>(p0, tile + r * R::kRowBytes + DP / 2);
-            load_pairs<G>(p1, tile + (r + 8) * R::kRowBytes + DP / 2);
-#pragma unroll
-            for (int g = 0; g < G; g += 2) {
-                uint32_t w[4];
-                if (g + 1 < G) ldmatrix(w, tile + part + g * 16);
-                else ldmatrix2(w, tile + part + g * 16 - lane / 16 * 16);
-#pragma unroll
-                for (int i = 0; i < (g + 1 < G ? 2 : 1); ++i) {
-                    const __half2 s0 = __low2half2(halves(p0[g + i])), z0 = __high2half2(halves(p0[g + i]));
-                    const __half2 s1 = __low2half2(halves(p1[g + i])), z1 = __high2half2(halves(p1[g + i]));
-                    const uint32_t u = w[2 * i], v = w[2 * i + 1];
-                    const uint32_t k0[4] = {fma2(codes64(u << 4), s0, z0), fma2(codes64(v << 4), s1, z1),
-                                            fma2(codes64(u), s0, z0), fma2(codes64(v), s1, z1)};
-                    const uint32_t k1[4] = {fma2(codes64(u >> 4), s0, z0), fma2(codes64(v >> 4), s1, z1),
-                                            fma2(codes64(u >> 8), s0, z0), fma2(codes64(v >> 8), s1, z1)};
-#pragma unroll
-                    for (int part_of = kParts - 1; part_of >= 0; --part_of) {
-                        mma16(s[x], k0, qf[part_of][g + i][0][0], qf[part_of][g + i][0][1], __half());
-                        mma16(s[x], k1, qf[part_of][g + i][1][0], qf[part_of][g + i][1][1], __half());
-                    }
-                }
-            }
-        }
+        for (int x = 0; x < S; ++x) products(s[x], stage + x * 16 * R::kRowBytes);
         float ref[2];
-        this->settle(a, s, f[0], f[1], live, rows, scores, ref);
+        this->template settle<true>(a, s, f[0], f[1], live, rows, scores, ref);
 #pragma unroll
         for (int x = 0; x < S; ++x) {
-            uint32_t b0, b1, c0, c1;
-            this->weigh(s[x], ref, b0, b1, c0, c1);
+            uint32_t b0, b1, c0 = 0, c1 = 0;
+            this->template weigh<kTwo>(s[x], ref, b0, b1, c0, c1);
             const uint32_t tile = stage + (STEP + x * 16) * R::kRowBytes;
             uint32_t p[4][G];  // of rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
@@ -159,14 +186,15 @@ struct Math4 : Heads8<__half, DP_ / 16> {
                     const __half2 s1 = halves(__byte_perm(p[2][g + i], p[3][g + i], 0x5410));
                     const __half2 z1 = halves(__byte_perm(p[2][g + i], p[3][g + i], 0x7632));
                     const uint32_t u = w[2 * i], v = w[2 * i + 1];
-                    const uint32_t v0[4] = {fma2(codes64(u << 4), s0, z0), fma2(codes64(u), s0, z0),
-                                            fma2(codes64(v << 4), s1, z1), fma2(codes64(v), s1, z1)};
-                    const uint32_t v1[4] = {fma2(codes64(u >> 4), s0, z0), fma2(codes64(u >> 8), s0, z0),
-                                            fma2(codes64(v >> 4), s1, z1), fma2(codes64(v >> 8), s1, z1)};
+                    uint32_t uc[4], vc[4];
+                    word_codes(u, uc);
+                    word_codes(v, vc);
+                    const uint32_t v0[4] = {fma2(uc[0], s0, z0), fma2(uc[1], s0, z0), fma2(vc[0], s1, z1), fma2(vc[1], s1, z1)};
+                    const uint32_t v1[4] = {fma2(uc[2], s0, z0), fma2(uc[3], s0, z0), fma2(vc[2], s1, z1), fma2(vc[3], s1, z1)};
                     mma16(o[2 * (g + i)], v0, b0, b1, __half());
-                    mma16(o[2 * (g + i)], v0, c0, c1, __half());
+                    if (kTwo) mma16(o[2 * (g + i)], v0, c0, c1, __half());
                     mma16(o[2 * (g + i) + 1], v1, b0, b1, __half());
-                    mma16(o[2 * (g + i) + 1], v1, c0, c1, __half());
+                    if (kTwo) mma16(o[2 * (g + i) + 1], v1, c0, c1, __half());
                 }
             }
         }

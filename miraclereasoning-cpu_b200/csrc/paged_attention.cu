@@ -19,7 +19,8 @@ struct Math16 : Heads8<T, DP_ / 16> {
     using Heads8<T, DP_ / 16>::o;
     using Heads8<T, DP_ / 16>::m;
     using Heads8<T, DP_ / 16>::l;
-    static constexpr bool kAgain = true;
+    static constexpr bool kAgain = true, kRuns = false;
+    static int ctas(int64_t, int, bool) { return kCtas; }
     static constexpr int kCtas = 2, DP = DP_, kHeads = 8, STEP = DP == 128 ? 16 : 32, STAGES = DP == 32 ? 6 : 3;
     using R = Ring<T, DP, STEP, STAGES>;
     uint32_t qf[DP / 16][2];   // Q^T fragments: head lane / 4
@@ -53,11 +54,11 @@ struct Math16 : Heads8<T, DP_ / 16> {
             }
         }
         float ref[2];
-        this->settle(a, s, a.scale, a.scale, live, rows, scores, ref);
+        this->template settle<false>(a, s, a.scale, a.scale, live, rows, scores, ref);
 #pragma unroll
         for (int x = 0; x < S; ++x) {
             uint32_t b0, b1, c0, c1;
-            this->weigh(s[x], ref, b0, b1, c0, c1);
+            this->template weigh<true>(s[x], ref, b0, b1, c0, c1);
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) {
                 uint32_t v[4];
@@ -107,7 +108,8 @@ struct Math16 : Heads8<T, DP_ / 16> {
 // 8 rows x 4 heads of a step give 32 sums, folded so that each lane ends with one.
 template <int DP_>
 struct Math32 {
-    static constexpr bool kAgain = true;
+    static constexpr bool kAgain = true, kRuns = false;
+    static int ctas(int64_t, int, bool) { return kCtas; }
     static constexpr int kCtas = 2, DP = DP_, kHeads = 4, STEP = 8, STAGES = DP == 128 ? 3 : DP == 64 ? 6 : 8;
     static constexpr int kLanes = DP / 4, kRows = 32 / kLanes, kEach = STEP / kRows;  // lanes a row, rows at a time
     using R = Ring<float, DP, STEP, STAGES>;

@@ -59,6 +59,7 @@ struct PagedArgs {
     int64_t seen_max;
     int warps;       // of k_paged
     int heads2;      // query heads of a block, rounded up to even
+    int page_shift;  // log2 of the page's rows, -1 if they are no power of 2
 };
 
 
@@ -305,9 +306,10 @@ struct Heads8 {
         l[0] = l[1] = 0.f;
     }
 
-    // The products of S x 16 rows: scaled (f0, f1: of the lane's two heads), hidden ones taken out, kept
-    // for the weights; the maxima raised and what is there rescaled.  ref: what weights are taken against.
-    template <int S>
+    // The products of S x 16 rows: scaled (f0, f1: of the lane's two heads), hidden ones taken out (kAllSeen: after
+    // a look whether there are any), kept for the weights; the maxima raised and what is there rescaled.  ref:
+    // what weights are taken against.
+    template <bool kAllSeen, int S>
     __device__ __forceinline__ void settle(const PagedArgs &a, float (&s)[S][4], float f0, float f1, uint32_t live, int rows,
                                            float *scores, float (&ref)[2]) {
         const int lane = threadIdx.x % 32;
@@ -316,10 +318,26 @@ struct Heads8 {
         for (int x = 0; x < S; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool seen = (live >> (x * 16 + lane / 4 + (e >> 1) * 8)) & 1u;
-                s[x][e] = seen ? s[x][e] * (e & 1 ? f1 : f0) : -INFINITY;
-                top[e & 1] = fmaxf(top[e & 1], s[x][e]);
+                s[x][e] *= e & 1 ? f1 : f0;
+                if constexpr (!kAllSeen) {
+                    const bool seen = (live >> (x * 16 + lane / 4 + (e >> 1) * 8)) & 1u;
+                    s[x][e] = seen ? s[x][e] : -INFINITY;
+                    top[e & 1] = fmaxf(top[e & 1], s[x][e]);
+                }
             }
+        if constexpr (kAllSeen) {
+            if (live != 0xffffffffu >> (32 - 16 * S)) {
+#pragma unroll
+                for (int x = 0; x < S; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!((live >> (x * 16 + lane / 4 + (e >> 1) * 8)) & 1u)) s[x][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int x = 0; x < S; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[x][e]);
+        }
         if (scores) {
             const int h = 2 * (lane % 4);
 #pragma unroll
@@ -353,7 +371,8 @@ struct Heads8 {
             m[1] = top[1];
         }
     }
-    // The weights of 16 rows as the 16-bit operand P^T: its first part b0, b1 and the rest c0, c1.
+    // The weights of 16 rows as the 16-bit operand P^T: its first part b0, b1 and (TWO) the rest c0, c1.
+    template <bool TWO>
     __device__ __forceinline__ void weigh(const float (&s)[4], const float (&ref)[2], uint32_t &b0, uint32_t &b1, uint32_t &c0,
                                           uint32_t &c1) {
         float p[4];
@@ -362,14 +381,16 @@ struct Heads8 {
             p[e] = ex2(s[e] - ref[e & 1]);
             l[e & 1] += p[e];
         }
-        // the weights as the 16-bit operand, and what that rounding left (a second
-        // product): one part alone would add as much error again as the output's rounding
         const uint32_t h0 = pack2(p[0], p[1], T()), h1 = pack2(p[2], p[3], T());
-        const float2 r0 = unpack2(h0, T()), r1 = unpack2(h1, T());
         b0 = transposed(h0);
         b1 = transposed(h1);
-        c0 = transposed(pack2(p[0] - r0.x, p[1] - r0.y, T()));
-        c1 = transposed(pack2(p[2] - r1.x, p[3] - r1.y, T()));
+        if constexpr (TWO) {
+            // what that rounding left (a second product): one part alone would add as much
+            // error again as the output's rounding
+            const float2 r0 = unpack2(h0, T()), r1 = unpack2(h1, T());
+            c0 = transposed(pack2(p[0] - r0.x, p[1] - r0.y, T()));
+            c1 = transposed(pack2(p[2] - r1.x, p[3] - r1.y, T()));
+        }
     }
 
     // Sums over the warp; false if a value is not finite.
@@ -429,24 +450,116 @@ struct Feed {
     // Queues the copies of the step looked up into `stage` and looks up the next.
     // Returns the rows that are seen, a bit each.
     __device__ __forceinline__ uint32_t issue(const PagedArgs &a, uint32_t stage) {
-        const int lane = threadIdx.x % 32;
         const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
         if (more) {
-            const int pieces = R::pieces(a);
-            const char *kb = a.k + k, *vb = a.v + v;
-#pragma unroll
-            for (int c = 0; c < kCopies; ++c) {
-                const int e = c * 32 + lane, r = e / R::kPieces, p = e % R::kPieces;
-                const int page = __shfl_sync(0xffffffffu, id, r), at = __shfl_sync(0xffffffffu, row, r);
-                const bool there = page >= 0 && p < pieces;
-                const uint64_t n = there ? page : 0, t = there ? at : 0;
-                const int q = there ? p : 0;
-                const uint32_t to_shared = stage + R::offset(r, p);
-                copy_piece<R::kUnit>(to_shared, kb + (n * a.k_page + t * a.k_row + q * R::kUnit), there);
-                copy_piece<R::kUnit>(to_shared + STEP * R::kRowBytes, vb + (n * a.v_page + t * a.v_row + q * R::kUnit), there);
-            }
+            each(a, stage);
             i += STEP;
             if (i >= to) piece();
+            look(a);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return live;
+    }
+    // The step's copies, with every row's own place.
+    __device__ __forceinline__ void each(const PagedArgs &a, uint32_t stage) const {
+        const int lane = threadIdx.x % 32;
+        const int pieces = R::pieces(a);
+        const char *kb = a.k + k, *vb = a.v + v;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            const int e = c * 32 + lane, r = e / R::kPieces, p = e % R::kPieces;
+            const int page = __shfl_sync(0xffffffffu, id, r), at = __shfl_sync(0xffffffffu, row, r);
+            const bool there = page >= 0 && p < pieces;
+            const uint64_t n = there ? page : 0, t = there ? at : 0;
+            const int q = there ? p : 0;
+            const uint32_t to_shared = stage + R::offset(r, p);
+            copy_piece<R::kUnit>(to_shared, kb + (n * a.k_page + t * a.k_row + q * R::kUnit), there);
+            copy_piece<R::kUnit>(to_shared + STEP * R::kRowBytes, vb + (n * a.v_page + t * a.v_row + q * R::kUnit), there);
+        }
+    }
+};
+
+// The same for steps of 32 short rows, where looking up and addressing each 16 bytes would cost as much as the
+// products (227 instructions a step of 760 in all): most steps' rows lie one after the other in one page, or on both sides
+// of one border between two pages.  Then the first and the last row's addresses do for all, and where rows follow
+// each other without gaps (heads before rows in a page) the copies' addresses differ by constants.
+template <typename M, typename Next>
+struct RunFeed : Feed<M, Next> {
+    using Base = Feed<M, Next>;
+    using R = typename M::R;
+    using Base::STEP, Base::kCopies, Base::next, Base::i, Base::to, Base::more, Base::id, Base::row;
+    static_assert(STEP == 32, "a row a lane");
+    const char *kb, *vb;  // the piece's head in the pools
+    const int *table;     // its sequence's pages
+    __device__ __forceinline__ explicit RunFeed(const Next &n) : Base(n) {}
+    __device__ __forceinline__ void begin(const PagedArgs &a) {
+        if (!more) return;
+        const int kh = next.walk.u / a.blocks;
+        kb = a.k + kh * a.k_head;
+        vb = a.v + kh * a.v_head;
+        table = a.pages.table + next.walk.s * a.pages.table_stride;
+    }
+    __device__ __forceinline__ void look(const PagedArgs &a) {
+        const int at = i + static_cast<int>(threadIdx.x % 32);
+        id = -1;
+        row = 0;
+        if (more && at < to) {
+            const int t = next.walk.seen.at(at), page = a.page_shift >= 0 ? t >> a.page_shift : a.pages.page.div(t);
+            const int found = __ldg(table + page);
+            row = t - page * a.pages.page.d;
+            id = static_cast<unsigned>(found) < static_cast<unsigned>(a.pages.pages) ? found : -1;
+        }
+    }
+    static __device__ __forceinline__ const char *place(const char *base, uint32_t page, uint32_t stride, int n, int r) {
+        return base + static_cast<uint64_t>(static_cast<uint32_t>(n)) * page + static_cast<int64_t>(r) * stride;
+    }
+    __device__ __forceinline__ bool runs(const PagedArgs &a, uint32_t stage, uint32_t live) const {
+        if (live != 0xffffffffu) return false;
+        const int lane = threadIdx.x % 32, first = row - lane;
+        const int id0 = __shfl_sync(0xffffffffu, id, 0), row0 = __shfl_sync(0xffffffffu, first, 0);
+        const uint32_t begin = __ballot_sync(0xffffffffu, id == id0 && first == row0);
+        const bool tight = a.k_row == R::kRow && a.v_row == R::kRow;
+        const char *k0 = place(kb, a.k_page, a.k_row, id0, row0), *v0 = place(vb, a.v_page, a.v_row, id0, row0);
+        if (begin == live && tight) {
+            k0 += lane * R::kUnit;
+            v0 += lane * R::kUnit;
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+                const uint32_t to_shared = stage + R::place(c * 32 + lane);
+                copy_piece<R::kUnit>(to_shared, k0 + c * 32 * R::kUnit, true);
+                copy_piece<R::kUnit>(to_shared + STEP * R::kRowBytes, v0 + c * 32 * R::kUnit, true);
+            }
+            return true;
+        }
+        const int id1 = __shfl_sync(0xffffffffu, id, STEP - 1), row1 = __shfl_sync(0xffffffffu, first, STEP - 1);
+        const uint32_t end = __ballot_sync(0xffffffffu, id == id1 && first == row1);
+        // a prefix of the rows in the first run, all the others in the last
+        if ((begin & (begin + 1)) || (begin | end) != live) return false;
+        const char *k1 = place(kb, a.k_page, a.k_row, id1, row1), *v1 = place(vb, a.v_page, a.v_row, id1, row1);
+        const int border = __popc(begin);
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+            const int e = c * 32 + lane, r = e / R::kPieces, p = (e - r * R::kPieces) * R::kUnit;
+            const uint32_t to_shared = stage + R::place(e);
+            const bool low = r < border;
+            copy_piece<R::kUnit>(to_shared, (low ? k0 : k1) + (static_cast<uint64_t>(r) * a.k_row + p), true);
+            copy_piece<R::kUnit>(to_shared + STEP * R::kRowBytes, (low ? v0 : v1) + (static_cast<uint64_t>(r) * a.v_row + p), true);
+        }
+        return true;
+    }
+    __device__ __forceinline__ uint32_t issue(const PagedArgs &a, uint32_t stage) {
+        const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
+        if (more) {
+            if (!runs(a, stage, live)) {
+                this->k = kb - a.k;
+                this->v = vb - a.v;
+                this->each(a, stage);
+            }
+            i += STEP;
+            if (i >= to) {
+                this->piece();
+                begin(a);
+            }
             look(a);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -570,8 +683,9 @@ __device__ __forceinline__ void work_through(const PagedArgs &a, uint32_t ring, 
     using R = typename M::R;
     constexpr int H = M::kHeads, STEP = M::STEP, STAGES = M::STAGES;
     Next next(start);
-    Feed<M, Next> feed(start);
+    std::conditional_t<M::kRuns, RunFeed<M, Next>, Feed<M, Next>> feed(start);
     feed.piece();
+    if constexpr (M::kRuns) feed.begin(a);
     feed.look(a);
     uint32_t live[STAGES - 1];  // of the steps in flight, the oldest first
 #pragma unroll
@@ -585,6 +699,8 @@ __device__ __forceinline__ void work_through(const PagedArgs &a, uint32_t ring, 
         const int to = min(walk.t1 * STEP, walk.seen.rows);
         M math;
         math.begin(a, q, heads);
+        const int64_t score0 = unit * a.seen_max + walk.t0 * STEP;
+        float *scores = a.scores ? a.scores + score0 * a.heads2 : nullptr;  // of the step's first row
         for (int i = walk.t0 * STEP; i < to; i += STEP) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();  // every lane's copies of the step have landed, and all are done with the slot filled next
@@ -592,8 +708,8 @@ __device__ __forceinline__ void work_through(const PagedArgs &a, uint32_t ring, 
 #pragma unroll
             for (int j = 0; j + 1 < STAGES - 1; ++j) live[j] = live[j + 1];
             live[STAGES - 2] = feed.issue(a, ring + (slot == 0 ? STAGES - 1 : slot - 1) * R::kBytes);
-            math.step(a, ring + slot * R::kBytes, seen, to - i,
-                      a.scores ? a.scores + (unit * a.seen_max + i) * a.heads2 : nullptr);
+            math.step(a, ring + slot * R::kBytes, seen, to - i, scores);
+            if (scores) scores += STEP * a.heads2;
             slot = slot == STAGES - 1 ? 0 : slot + 1;
         }
         done(math, walk, q, unit, heads, kh, h0);
@@ -844,6 +960,9 @@ int launch(mr_context *ctx, PagedArgs &a) {
     constexpr int H = M::kHeads, STEP = M::STEP;
     a.blocks = (a.group - 1) / H + 1;
     a.heads2 = (std::min(a.group, H) + 1) / 2 * 2;
+    a.page_shift = -1;
+    for (int n = 0; n < 31; ++n)
+        if (a.pages.page.d == 1 << n) a.page_shift = n;
     // the most rows a token can see, and the most steps there can be
     a.seen_max = a.window ? std::min<int64_t>(a.capacity, static_cast<int64_t>(a.window) + a.sinks) : a.capacity;
     const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.blocks;
@@ -852,10 +971,10 @@ int launch(mr_context *ctx, PagedArgs &a) {
     // weights of a group in several blocks are added up by one warp, which only k_join can
     const bool few = steps <= kFewSteps && (!a.weights || a.blocks == 1);
     const int64_t ctas = few ? units : (units * steps + kWarps - 1) / kWarps;
-    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, M::kCtas * ctx->sm_count)));
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, M::ctas(units * steps, ctx->sm_count, a.weights) * ctx->sm_count)));
     a.warps = grid * kWarps;
-    const size_t partial = few ? 0 : sizeof(float) * 2 * kWarps * grid * H * M::DP;
-    const size_t sums = few ? 0 : sizeof(float2) * 2 * kWarps * grid * H;
+    const size_t partial = few ? 0 : sizeof(float) * 2 * a.warps * H * M::DP;
+    const size_t sums = few ? 0 : sizeof(float2) * 2 * a.warps * H;
     const size_t lse = a.weights && !few ? sizeof(float) * units * H : 0;
     const size_t scores = a.weights ? sizeof(float) * units * a.seen_max * a.heads2 : 0;
     auto up = [](size_t n) { return (n + 255) & ~size_t(255); };

@@ -28,6 +28,21 @@ class Cache4(Pages4):
             self.stored.append([packed.unpacked(x) for x in rows])
 
 
+def score_error(q, k, reach, factor, dtype):
+    """What a score is off by, beside 32-bit sums: queries in float16 parts, which lose 2^-39 of a head's largest value, or of
+    float32 2^-22 of a value."""
+    top = np.abs(k).max() if len(k) else 0.0
+    largest = np.abs(q).max(-1)[..., None] * top * abs(factor)
+    return 2.0 ** -39 * q.shape[-1] * largest + (2.0 ** -21 * reach if dtype == "float32" else 0.0)
+
+
+def operand_error(q, k, v, mixed, reach, factor, dtype):
+    """Scores' errors in a weight twice (numerator and sum); weights in two float16 parts (2^-22, and 2^-40 of the largest),
+    for bfloat16 in one."""
+    weights = 2.0 ** -11 if dtype == "bfloat16" else 2.0 ** -22
+    return (2 * score_error(q, k, reach, factor, dtype) + weights) * mixed + 2.0 ** -40 * len(v) * (np.abs(v).max() if len(v) else 0)
+
+
 def check(served, cache, q, dtype, window=None, sinks=0, weighted=False, scale=None, hidden=None, out=None):
     import torch
     batch, heads, dim = q.shape
@@ -40,15 +55,15 @@ def check(served, cache, q, dtype, window=None, sinks=0, weighted=False, scale=N
     for s, (k, v) in enumerate(cache.stored):
         n = len(k)
         want, w, mixed, reach = ref.attend(wide(q[s:s + 1]), k, v, [n - 1], factor, window, sinks, hidden[s] if hidden else ())
-        # queries and weights in two float16 parts: 2^-22 of each, and of a weight 2^-40 of the largest
-        parts = 2.0 ** -22 * (mixed + 2 * reach * mixed) + 2.0 ** -40 * n * (np.abs(v).max() if n else 0)
-        bound = ref.output_bound(want, mixed, reach, dim, n, dtype, False) + parts
+        bound = ref.output_bound(want, mixed, reach, dim, n, dtype, False)
+        bound = bound + operand_error(wide(q[s:s + 1]), k, v, mixed, reach, factor, dtype)
         assert np.all(np.abs(wide(got[s]) - want[0]) <= bound[0]), (s, np.abs(wide(got[s]) - want[0]).max(), bound.max())
         if weighted:
             grown = wide(weights[s]) - wide(before[s])
             spent = np.zeros((cache.kv, capacity))
             spent[:, :n] = w[0].reshape(cache.kv, heads // cache.kv, n).sum(1)
-            error = 2 * ref.score_error(reach.max(), dim) + 2.0 ** -21 * reach.max() + 2 * (n + heads) * 2.0 ** -24
+            error = 2 * (ref.score_error(reach.max(), dim) + score_error(wide(q[s:s + 1]), k, reach, factor, dtype).max())
+            error += 2 * (n + heads) * 2.0 ** -24
             assert np.all(np.abs(grown - spent) <= error * spent + 2.0 ** -23 * (1 + spent))
             assert torch.equal(weights[s, :, n:], before[s, :, n:])
     return got
@@ -246,7 +261,8 @@ def test_serving_from_4_bits(served, dtype, split):
         for s, n in enumerate(prompts):
             at = n + i
             want, w, mixed, reach = ref.attend(wide(q[s:s + 1]), held[s][0][:at + 1], held[s][1][:at + 1], [at], dim ** -0.5)
-            bound = ref.output_bound(want, mixed, reach, dim, at, dtype, False) + 2.0 ** -22 * mixed * (1 + 2 * reach) + 2.0 ** -33
+            bound = ref.output_bound(want, mixed, reach, dim, at, dtype, False)
+            bound = bound + operand_error(wide(q[s:s + 1]), held[s][0][:at + 1], held[s][1][:at + 1], mixed, reach, dim ** -0.5, dtype)
             assert np.all(np.abs(wide(out[s]) - want[0]) <= bound[0])
             spent[s][:, :at + 1] += w[0].reshape(kv, heads // kv, at + 1).sum(1)
     for s, n in enumerate(prompts):
@@ -261,7 +277,9 @@ def test_serving_from_4_bits(served, dtype, split):
             group = slice(h * heads // kv, (h + 1) * heads // kv)
             want, _, mixed, reach = ref.attend(wide(q[s:s + 1, group]), held[s][0][at, h:h + 1], held[s][1][at, h:h + 1], [40],
                                                dim ** -0.5)
-            bound = ref.output_bound(want, mixed, reach, dim, 41, dtype, False) + 2.0 ** -22 * mixed * (1 + 2 * reach) + 2.0 ** -33
+            bound = ref.output_bound(want, mixed, reach, dim, 41, dtype, False)
+            bound = bound + operand_error(wide(q[s:s + 1, group]), held[s][0][at, h:h + 1], held[s][1][at, h:h + 1], mixed, reach,
+                                          dim ** -0.5, dtype)
             assert np.all(np.abs(wide(out[s, group]) - want[0]) <= bound[0])
     logits = (out.reshape(2, -1).float() @ torch.tensor(rng.normal(size=(heads * dim, 500)), dtype=torch.float32, device="cuda"))
     logprobs, entropy, ids, best = served.log_probabilities(logits, logits.argmax(1).to(torch.int32), top=3)
