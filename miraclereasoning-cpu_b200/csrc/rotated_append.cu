@@ -8,6 +8,7 @@
 // are cheap.  They are worked out once a token and part of its rows, in the
 // registers of the warp that turns them.
 #include <cmath>
+#include <type_traits>
 
 #include "packed.cuh"
 
@@ -40,54 +41,71 @@ struct PlaceArgs {
     int batch;
 };
 
-// The sequence of packed token i (-1: of none) and its row there, which may lie before the first.
-__device__ __forceinline__ int place_of(const PlaceArgs &a, int i, int &row) {
-    int s = i, behind = 1;  // rows from this one to the sequence's end
-    if (a.offsets) {
-        int lo = -1, hi = a.batch;  // offsets[lo] <= i < offsets[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (__ldg(a.offsets + mid * a.offset_stride) <= i) lo = mid;
-            else hi = mid;
+// Where packed token i stands; the same in all lanes of a warp, which look for it together.
+struct Place {
+    int sequence;  // -1: of none
+    int begin, end;  // its tokens
+    int row;       // of token i there; may lie before the first
+    int rows;
+    // The last s with offsets[s] <= i, 32 at a time, if its end is behind i.
+    __device__ __forceinline__ void find(const PlaceArgs &a, int i) {
+        if (!a.offsets) {
+            sequence = begin = i;
+            end = i + 1;
+        } else {
+            const int lane = threadIdx.x % 32;
+            int lo = 0, n = a.batch + 1;  // it is among lo .. lo + n - 1
+            sequence = -1;
+            end = i;
+            do {
+                const int step = (n + 31) / 32, at = lane * step;
+                const bool under = at < n && __ldg(a.offsets + (lo + at) * a.offset_stride) <= i;
+                const uint32_t found = __ballot_sync(0xffffffffu, under);
+                if (!found) return;
+                const int k = 31 - __clz(found);
+                lo += k * step;
+                n = min(step, n - k * step);
+            } while (n > 1);
+            if (lo == a.batch) return;
+            const int last = __ldg(a.offsets + (lo + 1) * a.offset_stride);
+            if (last <= i) return;
+            sequence = lo;
+            begin = i;
+            end = last;
         }
-        if (lo < 0) return -1;
-        const int end = __ldg(a.offsets + (lo + 1) * a.offset_stride);
-        if (end <= i) return -1;
-        s = lo;
-        behind = end - i;
+        rows = max(0, __ldg(a.lengths + sequence * a.length_stride));
+        row = rows - (end - i);
     }
-    row = max(0, __ldg(a.lengths + s * a.length_stride)) - behind;
-    return s;
-}
+    // The same of a later token.
+    __device__ __forceinline__ void next(const PlaceArgs &a, int i) {
+        if (sequence >= 0 && i < end) row = rows - (end - i);
+        else find(a, i);
+    }
+};
 
-// Four values as float32.
-__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4 *>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-}
+// 16 bytes of a row: its values as float32, and back.
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, float (&x)[4]) {
-    union {
-        uint2 raw;
-        T v[4];
-    } u;
-    u.raw = *reinterpret_cast<const uint2 *>(p);
+struct Vector {
+    static constexpr int kValues = 16 / sizeof(T);
+    static __device__ __forceinline__ void widen(const uint4 &raw, float (&x)[kValues]) {
+        union {
+            uint4 raw;
+            T v[kValues];
+        } u;
+        u.raw = raw;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = widen(&u.v[j]);
-}
-__device__ __forceinline__ void store4(float *p, const float (&x)[4]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-template <typename T>
-__device__ __forceinline__ void store4(T *p, const float (&x)[4]) {
-    union {
-        uint2 raw;
-        T v[4];
-    } u;
+        for (int j = 0; j < kValues; ++j) x[j] = cache::widen(&u.v[j]);
+    }
+    static __device__ __forceinline__ uint4 narrow(const float (&x)[kValues]) {
+        union {
+            uint4 raw;
+            T v[kValues];
+        } u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) narrow(x[j], &u.v[j]);
-    *reinterpret_cast<uint2 *>(p) = u.raw;
-}
+        for (int j = 0; j < kValues; ++j) cache::narrow(x[j], &u.v[j]);
+        return u.raw;
+    }
+};
 
 __device__ __forceinline__ float min_nan(float a, float b) {
     float x;
@@ -98,6 +116,51 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     float x;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(a), "f"(b));
     return x;
+}
+
+// A lane's V values of a row as codes, and with the other lanes that have the same 32 their step and base (in
+// the low and the high half).  The code is rint((x - base) / step) - 64 of float32 operations: a product with
+// the step's inverse is off by 2^-16 of a step at most, and where that could round the other way the lane divides.
+template <int V>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[V], uint32_t &pair) {
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) {
+        lo = min_nan(lo, x[j]);
+        hi = max_nan(hi, x[j]);
+    }
+#pragma unroll
+    for (int o = 1; o < kShared / V; o <<= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const __half step = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
+    const float s = __half2float(step);
+    const __half zero = __float2half_rn(__fsub_rn(lo, __fmul_rn(64.f, s)));
+    const float z = __half2float(zero);
+    const bool held = fabsf(s) < INFINITY && fabsf(z) < INFINITY;
+    pair = held ? __half_as_ushort(step) | static_cast<uint32_t>(__half_as_ushort(zero)) << 16 : 0x7e007e00u;
+    if (!held || s == 0.f) return 0;
+    constexpr float kRound = 12582912.f;  // 1.5 x 2^23: added, it leaves a whole number in the low bits
+    const float inverse = __frcp_rn(s);
+    uint32_t codes = 0;
+    float worst = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], z), inverse), 64.f), 79.f);
+        const float n = __fadd_rn(q, kRound);
+        worst = fmaxf(worst, fabsf(q - (n - kRound)));
+        codes |= (__float_as_uint(n) & 15u) << (4 * j);
+    }
+    if (worst > 0.5f - 0x1p-12f) {
+        codes = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float n = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[j], z), s)), 64.f), 79.f);
+            codes |= (static_cast<uint32_t>(n) & 15u) << (4 * j);
+        }
+    }
+    return codes;
 }
 
 // sin and cos of position * frequency, each rounded to float32 once.  The product is kept in
@@ -143,176 +206,198 @@ struct RotateArgs {
     const int *positions;  // NULL: a token's row
     int64_t frequency_stride, position_stride;
     int tokens, heads, kv_heads, dim, half;  // half: pairs that turn
+    int wide;                                // lanes of a row, as a power of 2
+    int query_slots, kv_slots;               // slots of a token's queries, and of its keys or values
+    bool split;                              // pairs are p and p + half
     int team, share;                         // warps that share a token's rows, tokens of such a team
 };
 
-// How pairs lie: neighbours; p and p + half with four dims of a lane alike (half a multiple of
-// 4); the same, any half.
-enum { kNeighbours, kHalves, kAnyHalves };
+__device__ __forceinline__ uint4 shared16(uint32_t address) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(address) : "memory");
+    return x;
+}
 
-// A warp takes `share` tokens, or a part of one token's rows: of the queries, then keys, then
-// values.  A lane has the same four dims of every row (L lanes a row), so that a token's
-// angles stay in registers; kFlight rows a lane are under way.  Products and sums of a turn are
-// rounded one by one, so that a 4-bit code is the same wherever it is worked out.
+// How pairs lie: neighbours, or p and p + half, a lane's dims all turning alike (2 half, or half, a multiple of
+// their number); else either, looked at dim by dim.
+enum { kNeighbours, kHalves, kAny };
+
+
+// A CTA is a warp, so that what is the same in all lanes is worked out once, and 32 of them an SM have
+// the registers that they need.
+// A warp takes `share` tokens, or a part of one token's rows, in slots of as many rows of one kind (queries,
+// then keys, then values) as its lanes hold at 16 bytes each, copied to its ring in shared memory kDepth - 1
+// slots ahead, of later tokens too, whether or not they have a place.  A lane has the same dims of every row, so that a token's sines, worked out by the warp once, stay in
+// registers.  Products and sums of a turn are rounded one by one, so that a 4-bit code is the same wherever it
+// is worked out.
 template <typename T, int PAIRS, bool PACKED>
-__global__ void __launch_bounds__(256) k_append_rotated(const __grid_constant__ RotateArgs a) {
-    constexpr int kFlight = 4;
-    const int lane = threadIdx.x % 32, warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t first = static_cast<int64_t>(warp / a.team) * a.share;
-    const int part = warp % a.team;
+__global__ void __launch_bounds__(32, 32) k_append_rotated(const __grid_constant__ RotateArgs a) {
+    constexpr int V = Vector<T>::kValues, kDepth = 6, kTurns = PAIRS == kNeighbours ? V / 2 : V;
+    __shared__ float2 turns[kMaxDim / 2];
+    __shared__ uint4 ring_of[kDepth][32];
+    const int lane = threadIdx.x, warp = blockIdx.x;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_of));
+    const int unit = a.team == 1 ? warp : warp / a.team, part = warp - unit * a.team;
+    const int64_t first = static_cast<int64_t>(unit) * a.share;
     if (first >= a.tokens) return;
-    int64_t mine_k = -1, mine_v = -1;
-    int mine_position = 0;
-    bool mine_owned = false;
-    if (lane < a.share && first + lane < a.tokens) {
-        const int i = static_cast<int>(first) + lane;
-        int t = 0;
-        const int s = place_of(a.place, i, t);
-        mine_owned = s >= 0;
-        if (mine_owned) {
-            mine_position = a.positions ? __ldg(a.positions + i * a.position_stride) : t;
-            if (t >= 0) {
-                mine_k = a.pages.row(s, t, a.key_pool.page, a.key_pool.row);
-                mine_v = a.pages.row(s, t, a.value_pool.page, a.value_pool.row);
+    const int sub = lane >> a.wide, piece = lane - (sub << a.wide), d = piece * V, per = 32 >> a.wide, stride = per * a.team;
+    const bool inside = d < a.dim, low = d < a.half;
+    const bool turning = PAIRS == kAny ? a.half > 0 : d < 2 * a.half;  // this lane's dims
+    const int half_bytes = a.half / V * 16;                            // in the ring
+    const int lane_bytes = piece * 16;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(a.share), a.tokens - first));
+    // The slots of all kinds are dealt out to the team's warps in one row; the first row of each kind that is this warp's.
+    auto first_of = [&](int before) { return a.team == 1 ? 0 : (part + a.team - before % a.team) % a.team * per; };
+    const int query0 = part * per, key0 = first_of(a.query_slots), value0 = first_of(a.query_slots + a.kv_slots);
+    // Copies run through the same slots ahead: a kind's next row of this lane, how many rows are behind it, and where.
+    const char *copy_from = nullptr;
+    int64_t copy_step = 0;
+    int copy_rows = 0, copy_kind = -1, copy_token = static_cast<int>(first);
+    const int end_token = copy_token + tokens;
+    const uint32_t ring_lane = ring + lane * 16;
+    auto copy = [&](int at) {
+        while (copy_rows <= 0 && copy_token < end_token) {
+            if (++copy_kind == 3) {
+                copy_kind = 0;
+                if (++copy_token == end_token) break;
+            }
+            const Rows &rows = copy_kind == 0 ? a.q : copy_kind == 1 ? a.k : a.v;
+            const int row = copy_kind == 0 ? query0 : copy_kind == 1 ? key0 : value0;
+            copy_rows = (copy_kind == 0 ? a.heads : a.kv_heads) - row;
+            copy_from = rows.base + lane_bytes + copy_token * rows.token + (row + sub) * rows.head;
+            copy_step = stride * rows.head;
+        }
+        if (copy_rows > 0) {
+            // (an address behind the last row is not read)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring_lane + at * 512), "l"(copy_from),
+                         "r"(inside && sub < copy_rows ? 16 : 0)
+                         : "memory");
+            copy_from += copy_step;
+            copy_rows -= stride;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int f = 0; f < kDepth - 1; ++f) copy(f);
+    int at = 0;
+    Place place;
+#pragma unroll 1
+    for (int n = 0; n < tokens; ++n) {
+        const int token = static_cast<int>(first) + n;
+        // copies are under way while the place is looked up
+        if (n) place.next(a.place, token);
+        else place.find(a.place, token);
+        const bool owned = place.sequence >= 0;
+        const int position = !owned ? 0 : a.positions ? __ldg(a.positions + token * a.position_stride) : place.row;
+        char *to_k = nullptr, *to_v = nullptr;
+        if (owned && place.row >= 0) {
+            const int64_t rk = a.pages.row(place.sequence, place.row, a.key_pool.page, a.key_pool.row);
+            const int64_t rv = a.pages.row(place.sequence, place.row, a.value_pool.page, a.value_pool.row);
+            if (rk >= 0) {  // both or neither
+                to_k = a.key_pool.base + rk;
+                to_v = a.value_pool.base + rv;
             }
         }
-    }
-    int wide = 1;  // lanes a row
-    while (wide * 4 < a.dim) wide <<= 1;
-    const int sub = lane / wide, d = lane % wide * 4, rows = a.heads + 2 * a.kv_heads, each = 32 / wide * a.team;
-    const bool inside = d < a.dim;
-    const int dim0 = inside ? d : 0;
-    for (int n = 0; n < a.share && first + n < a.tokens; ++n) {
-        if (!__shfl_sync(0xffffffffu, mine_owned, n)) continue;
-        const int64_t to_k = __shfl_sync(0xffffffffu, mine_k, n), to_v = __shfl_sync(0xffffffffu, mine_v, n);
-        const int position = __shfl_sync(0xffffffffu, mine_position, n), token = static_cast<int>(first) + n;
-        // cos and sin of the pairs of the lane's dims; (1, 0) where they do not turn
-        float2 turn[4];
-        auto angle = [&](int p) {
-            return p < a.half ? turn_of(position, __ldg(a.frequencies + p * a.frequency_stride)) : make_float2(1.f, 0.f);
-        };
-        if (PAIRS == kNeighbours) {
-            turn[0] = turn[1] = angle(dim0 / 2);
-            turn[2] = turn[3] = angle(dim0 / 2 + 1);
-        } else if (PAIRS == kHalves) {
-            // each of the two lanes that meet the same four pairs works out two of them
-            const bool low = dim0 < a.half;
-            const int p = low ? dim0 : dim0 - a.half, there = lane + (low ? a.half : -a.half) / 4;
-            const float2 x = angle(p + (low ? 0 : 2)), y = angle(p + (low ? 1 : 3));
-            const int from = dim0 < 2 * a.half ? there : lane;
-            const float2 u = make_float2(__shfl_sync(0xffffffffu, x.x, from), __shfl_sync(0xffffffffu, x.y, from));
-            const float2 w = make_float2(__shfl_sync(0xffffffffu, y.x, from), __shfl_sync(0xffffffffu, y.y, from));
-            turn[0] = low ? x : u;
-            turn[1] = low ? y : w;
-            turn[2] = low ? u : x;
-            turn[3] = low ? w : y;
-        } else {
+        // the token's sines
+        __syncwarp();  // those of the token before have been read
+#pragma unroll 1
+        for (int p = lane; p < a.half; p += 32) turns[p] = turn_of(position, __ldg(a.frequencies + p * a.frequency_stride));
+        __syncwarp();
+        float2 turn[kTurns];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) turn[j] = angle(dim0 + j < a.half ? dim0 + j : dim0 + j - a.half);
+        for (int j = 0; j < kTurns; ++j) {
+            const int e = d + j, p = PAIRS == kNeighbours ? d / 2 + j : PAIRS == kAny && !a.split ? e / 2 : e < a.half ? e : e - a.half;
+            turn[j] = p < a.half ? turns[p] : make_float2(1.f, 0.f);
+            if (PAIRS == kHalves && low) turn[j].y = -turn[j].y;  // a cos - b sin as a sum, the same
         }
-        for (int base = part * (32 / wide); base < rows; base += each * kFlight) {
-            float x[kFlight][4], y[kFlight][4];  // the values, and with pairs of halves their partners
+        // one kind's slots: rows row0, + stride, .. of `count`, to `to` (not written where that is NULL)
+        auto work = [&](auto kind, int row0, int count, const Rows &from, char *to, int64_t head) {
+            constexpr int kKind = decltype(kind)::value;
+            char *dst = to + (row0 + sub) * head;
+            const int64_t step = stride * head;
+#pragma unroll 1
+            for (int rows = count - row0; rows > 0; rows -= stride, dst += step) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+                __syncwarp();  // every lane's copy of the slot has landed, and all are done with the one before it
+                copy(at == 0 ? kDepth - 1 : at - 1);
+                const uint32_t here = ring_lane + at * 512;
+                at = at == kDepth - 1 ? 0 : at + 1;
+                const bool there = to && inside && sub < rows;
+                float x[V];
+                Vector<T>::widen(shared16(here), x);
+                if (kKind < 2 && turning) {
+                    float y[V], z[V];
+                    if (PAIRS == kHalves) {
+                        Vector<T>::widen(shared16(low ? here + half_bytes : here - half_bytes), y);
+                    } else if (PAIRS == kAny) {
+                        const T *row = reinterpret_cast<const T *>(from.base + token * from.token + (count - rows + sub) * from.head);
 #pragma unroll
-            for (int f = 0; f < kFlight; ++f) {
-                const int i = base + sub + f * each;
-                const bool there = inside && i < rows;
-                const Rows &from = i < a.heads ? a.q : i < a.heads + a.kv_heads ? a.k : a.v;
-                const int h = i < a.heads ? i : i < a.heads + a.kv_heads ? i - a.heads : i - a.heads - a.kv_heads;
-                const T *row = reinterpret_cast<const T *>(from.base + token * from.token + h * from.head);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[f][j] = y[f][j] = 0.f;
-                if (there) load4(row + d, x[f]);
-                if (PAIRS == kHalves && there && i < a.heads + a.kv_heads && d < 2 * a.half)
-                    load4(row + (d < a.half ? d + a.half : d - a.half), y[f]);
-                if (PAIRS == kAnyHalves && there && i < a.heads + a.kv_heads) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int e = d + j;
-                        if (e < 2 * a.half) y[f][j] = widen(row + (e < a.half ? e + a.half : e - a.half));
-                    }
-                }
-            }
-#pragma unroll
-            for (int f = 0; f < kFlight; ++f) {
-                const int i = base + sub + f * each;
-                const bool query = i < a.heads, value = i >= a.heads + a.kv_heads, there = inside && i < rows;
-                const int h = query ? i : value ? i - a.heads - a.kv_heads : i - a.heads;
-                if (!value) {
-                    float z[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int e = d + j;
-                        const bool turns = e < 2 * a.half;
-                        const bool second = PAIRS == kNeighbours ? j & 1 : e >= a.half;
-                        const float other = PAIRS == kNeighbours ? x[f][j ^ 1] : y[f][j];
-                        const float p = __fmul_rn(x[f][j], turn[j].x), q = __fmul_rn(other, turn[j].y);
-                        z[j] = !turns ? x[f][j] : second ? __fadd_rn(p, q) : __fsub_rn(p, q);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[f][j] = z[j];
-                }
-                const int64_t place = value ? to_v : to_k;
-                const Pool &pool = value ? a.value_pool : a.key_pool;
-                char *to = pool.base + place + h * pool.head;
-                if (query) {
-                    if (there) store4(reinterpret_cast<T *>(a.out.base + token * a.out.token + h * a.out.head) + d, x[f]);
-                } else if (!PACKED) {
-                    if (there && place >= 0) store4(reinterpret_cast<T *>(to) + d, x[f]);
-                }
-                if (PACKED && __any_sync(0xffffffffu, there && !query)) {
-                    // 8 lanes share a step and a base
-                    float lo = min_nan(min_nan(x[f][0], x[f][1]), min_nan(x[f][2], x[f][3]));
-                    float hi = max_nan(max_nan(x[f][0], x[f][1]), max_nan(x[f][2], x[f][3]));
-#pragma unroll
-                    for (int o = 1; o < 8; o <<= 1) {
-                        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                    }
-                    const __half step = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
-                    const float s = __half2float(step);
-                    const __half zero = __float2half_rn(__fsub_rn(lo, __fmul_rn(64.f, s)));
-                    const float z = __half2float(zero);
-                    const bool held = fabsf(s) < INFINITY && fabsf(z) < INFINITY;
-                    uint32_t codes = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float c = rintf(__fdiv_rn(__fsub_rn(x[f][j], z), s)) - 64.f;
-                        const uint32_t code = held && s != 0.f ? static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) : 0u;
-                        codes |= code << (4 * j);
-                    }
-                    if (!query && there && place >= 0) {
-                        *reinterpret_cast<uint16_t *>(to + d / 2) = static_cast<uint16_t>(codes);
-                        if (d % kShared == 0) {
-                            const uint32_t nan = 0x7e007e00u;
-                            *reinterpret_cast<uint32_t *>(to + a.dim / 2 + d / kShared * 4) =
-                                held ? __half_as_ushort(step) | static_cast<uint32_t>(__half_as_ushort(zero)) << 16 : nan;
+                        for (int j = 0; j < V; ++j) {
+                            const int e = d + j, other = e < a.half ? e + a.half : e - a.half;
+                            y[j] = !a.split ? x[j ^ 1] : there && e < 2 * a.half ? widen(row + other) : 0.f;
                         }
                     }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float2 t = turn[PAIRS == kNeighbours ? j / 2 : j];
+                        const float p = __fmul_rn(x[j], t.x), q = __fmul_rn(PAIRS == kNeighbours ? x[j ^ 1] : y[j], t.y);
+                        const bool second = PAIRS == kAny && a.split ? d + j >= a.half : j & 1;
+                        z[j] = PAIRS == kHalves || second ? __fadd_rn(p, q) : __fsub_rn(p, q);
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (PAIRS != kAny || d + j < 2 * a.half) x[j] = z[j];
+                }
+                if (kKind == 0 || !PACKED) {
+                    if (there) *reinterpret_cast<uint4 *>(dst + lane_bytes) = Vector<T>::narrow(x);
+                } else {
+                    uint32_t pair;
+                    const uint32_t codes = quantise<V>(x, pair);
+                    if (there) {
+                        if (V == 8) *reinterpret_cast<uint32_t *>(dst + d / 2) = codes;
+                        else *reinterpret_cast<uint16_t *>(dst + d / 2) = static_cast<uint16_t>(codes);
+                        if (d % kShared == 0) *reinterpret_cast<uint32_t *>(dst + a.dim / 2 + d / kShared * 4) = pair;
+                    }
                 }
             }
-        }
+        };
+        work(std::integral_constant<int, 0>(), query0, a.heads, a.q, owned ? a.out.base + token * a.out.token : nullptr, a.out.head);
+        work(std::integral_constant<int, 1>(), key0, a.kv_heads, a.k, to_k, a.key_pool.head);
+        work(std::integral_constant<int, 2>(), value0, a.kv_heads, a.v, to_v, a.value_pool.head);
     }
 }
 
+// Lanes of a row of n 16-byte pieces, as a power of 2.
+int lanes_of(int64_t n) {
+    int wide = 0;
+    while (1 << wide < n) ++wide;
+    return wide;
+}
+
 template <typename T, bool PACKED>
-int launch_pairs(mr_context *ctx, const RotateArgs &a, bool split_half) {
-    // As many warps to a token as fill the GPU (16 to an SM) when tokens are few, one with several tokens when many.
-    const int rows = a.heads + 2 * a.kv_heads;
-    RotateArgs b = a;
+int launch_pairs(mr_context *ctx, RotateArgs &a, bool split_half) {
+    constexpr int V = Vector<T>::kValues;
+    // As many warps to a token as fill the GPU (16 to an SM) when tokens are few; one, with several tokens
+    // one after the other, when they are many.
+    a.wide = lanes_of(a.dim / V);
+    const int per = 32 >> a.wide;
+    a.query_slots = (a.heads + per - 1) / per;
+    a.kv_slots = (a.kv_heads + per - 1) / per;
+    const int slots = a.query_slots + 2 * a.kv_slots;
     const int64_t warps = 16 * static_cast<int64_t>(ctx->sm_count);
-    b.team = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, warps / std::max(a.tokens, 1))));
-    b.share = b.team > 1 ? 1 : static_cast<int>(std::min<int64_t>(4, (a.tokens + 2 * warps - 1) / (2 * warps)));
-    const int64_t all = (static_cast<int64_t>(a.tokens) + b.share - 1) / b.share * b.team;
-    constexpr int kWarps = 4;
-    const unsigned grid = static_cast<unsigned>((all + kWarps - 1) / kWarps);
-    if (!split_half) k_append_rotated<T, kNeighbours, PACKED><<<grid, kWarps * 32, 0, ctx->stream>>>(b);
-    else if (a.half % 4 == 0) k_append_rotated<T, kHalves, PACKED><<<grid, kWarps * 32, 0, ctx->stream>>>(b);
-    else k_append_rotated<T, kAnyHalves, PACKED><<<grid, kWarps * 32, 0, ctx->stream>>>(b);
+    a.team = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots, warps / a.tokens)));
+    a.share = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, a.tokens / (4 * warps))));
+    const int64_t all = (static_cast<int64_t>(a.tokens) + a.share - 1) / a.share * a.team;
+    auto run = [&](auto kernel) { kernel<<<static_cast<unsigned>(all), 32, 0, ctx->stream>>>(a); };
+    a.split = split_half;
+    if (!split_half && 2 * a.half % V == 0) run(k_append_rotated<T, kNeighbours, PACKED>);
+    else if (split_half && a.half % V == 0) run(k_append_rotated<T, kHalves, PACKED>);
+    else run(k_append_rotated<T, kAny, PACKED>);
     MR_CUDA_TRY(cudaGetLastError());
     return MR_OK;
 }
 template <typename T>
-int launch_rotated(mr_context *ctx, const RotateArgs &a, bool split_half, bool packed) {
+int launch_rotated(mr_context *ctx, RotateArgs &a, bool split_half, bool packed) {
     return packed ? launch_pairs<T, true>(ctx, a, split_half) : launch_pairs<T, false>(ctx, a, split_half);
 }
 
@@ -324,88 +409,103 @@ struct ReadArgs {
     PlaceArgs place;
     int tokens, heads, pieces;  // pieces: 16-byte pieces of a row of the results
     int code_bytes;             // of a 4-bit row
-    int team, share;            // warps that share a token's rows, tokens of such a team
+    int wide, team, share;      // as in RotateArgs
 };
 
 // 16 bytes of a result's row, from piece c of a pool's row.
 template <typename T, bool PACKED>
 struct Piece {
-    uint4 raw;         // PACKED: x: the codes, y: step and base
+    enum { V = 16 / sizeof(T) };
+    using Raw = std::conditional_t<PACKED, uint2, uint4>;  // PACKED: x: the codes, y: step and base
+    Raw raw;
     __device__ __forceinline__ void load(const char *row, int c, int code_bytes) {
-        constexpr int kValues = 16 / sizeof(T);
         if constexpr (!PACKED) {
             raw = *reinterpret_cast<const uint4 *>(row + 16 * c);
         } else {
-            raw.x = kValues == 8 ? *reinterpret_cast<const uint32_t *>(row + 4 * c) : *reinterpret_cast<const uint16_t *>(row + 2 * c);
-            raw.y = *reinterpret_cast<const uint32_t *>(row + code_bytes + c * kValues / kShared * 4);
+            raw.x = V == 8 ? *reinterpret_cast<const uint32_t *>(row + 4 * c) : *reinterpret_cast<const uint16_t *>(row + 2 * c);
+            raw.y = *reinterpret_cast<const uint32_t *>(row + code_bytes + c * V / kShared * 4);
         }
     }
     __device__ __forceinline__ uint4 value() const {
         if constexpr (!PACKED) {
             return raw;
         } else {
-            constexpr int kValues = 16 / sizeof(T);
             const __half2 pair = *reinterpret_cast<const __half2 *>(&raw.y);
             const __half2 s = __low2half2(pair), z = __high2half2(pair);
-            union {
-                uint4 all;
-                T v[kValues];
-            } u;
+            if constexpr (V == 8) {
+                uint32_t x[4];  // values j and j + 4
+                word_codes(raw.x, x);
 #pragma unroll
-            for (int j = 0; j < kValues; j += 2) {
-                // codes j and j + 1 into bits 4 .. 7 of the two halves
-                const uint32_t byte = raw.x >> (4 * j), two = (byte & 0xfu) << 4 | (byte & 0xf0u) << 16;
-                const uint32_t x = fma2(codes64(two), s, z);
+                for (int j = 0; j < 4; ++j) x[j] = fma2(x[j], s, z);
+                const uint4 y = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
+                                           __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
+                if constexpr (std::is_same<T, __half>::value) return y;
+                float f[8];
+                Vector<__half>::widen(y, f);
+                return Vector<T>::narrow(f);
+            } else {
+                // codes 0 and 1, 2 and 3 into bits 4 .. 7 of the two halves
+                const uint32_t low = (raw.x & 0xfu) << 4 | (raw.x & 0xf0u) << 16;
+                const uint32_t high = (raw.x & 0xf00u) >> 4 | (raw.x & 0xf000u) << 8;
+                const uint32_t x = fma2(codes64(low), s, z), y = fma2(codes64(high), s, z);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
-                narrow(f.x, &u.v[j]);
-                narrow(f.y, &u.v[j + 1]);
+                const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+                return make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(g.x), __float_as_uint(g.y));
             }
-            return u.all;
         }
     }
 };
 
+constexpr int kReadWarps = 4;
+
 template <typename T, bool PACKED>
-__global__ void __launch_bounds__(256) k_read_pages(const __grid_constant__ ReadArgs a) {
+__global__ void __launch_bounds__(kReadWarps * 32) k_read_pages(const __grid_constant__ ReadArgs a) {
     constexpr int kFlight = 4;
-    const int lane = threadIdx.x % 32, warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t first = static_cast<int64_t>(warp / a.team) * a.share;
+    const int lane = threadIdx.x % 32, warp = blockIdx.x * kReadWarps + threadIdx.x / 32;
+    const int unit = a.team == 1 ? warp : warp / a.team, part = warp - unit * a.team;
+    const int64_t first = static_cast<int64_t>(unit) * a.share;
     if (first >= a.tokens) return;
-    int64_t mine_k = -1, mine_v = -1;
-    bool mine_owned = false;
-    if (lane < a.share && first + lane < a.tokens) {
-        int t = 0;
-        const int s = place_of(a.place, static_cast<int>(first) + lane, t);
-        mine_owned = s >= 0;
-        if (s >= 0 && t >= 0) {
-            mine_k = a.pages.row(s, t, a.key_pool.page, a.key_pool.row);
-            mine_v = a.pages.row(s, t, a.value_pool.page, a.value_pool.row);
+    const int sub = lane >> a.wide, c = lane - (sub << a.wide), per = 32 >> a.wide, stride = per * a.team;
+    Place place;
+    place.find(a.place, static_cast<int>(first));
+    for (int n = 0; n < a.share && first + n < a.tokens; ++n) {
+        const int token = static_cast<int>(first) + n;
+        if (n) place.next(a.place, token);
+        if (place.sequence < 0) continue;
+        int64_t k = -1, v = -1;
+        if (place.row >= 0) {
+            k = a.pages.row(place.sequence, place.row, a.key_pool.page, a.key_pool.row);
+            v = a.pages.row(place.sequence, place.row, a.value_pool.page, a.value_pool.row);
         }
-    }
-    const int n = a.heads * a.pieces;
-    const int all = static_cast<int>(min(static_cast<int64_t>(a.share), a.tokens - first)) * n;
-    for (int e0 = lane + warp % a.team * 32 * kFlight; e0 - lane < all; e0 += 32 * kFlight * a.team) {
-        Piece<T, PACKED> x[kFlight], y[kFlight];
-        char *to_k[kFlight], *to_v[kFlight];
+        // this lane's next rows
+        int h = part * per + sub;
+        const char *from_k = a.key_pool.base + k + h * a.key_pool.head, *from_v = a.value_pool.base + v + h * a.value_pool.head;
+        char *to_k = a.k.base + token * a.k.token + 16 * c + h * a.k.head, *to_v = a.v.base + token * a.v.token + 16 * c + h * a.v.head;
+        if (c >= a.pieces) h = a.heads;
+#pragma unroll 1
+        while (__any_sync(0xffffffffu, h < a.heads)) {
+            Piece<T, PACKED> x[kFlight], y[kFlight];
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) {
-            const int e = min(e0 + 32 * f, all - 1), token = e / n, i = e - token * n, h = i / a.pieces, c = i - h * a.pieces;
-            const int64_t k = __shfl_sync(0xffffffffu, mine_k, token), v = __shfl_sync(0xffffffffu, mine_v, token);
-            const bool owned = __shfl_sync(0xffffffffu, mine_owned, token) && e0 + 32 * f < all;
-            to_k[f] = owned ? a.k.base + (first + token) * a.k.token + h * a.k.head + 16 * c : nullptr;
-            to_v[f] = a.v.base + (first + token) * a.v.token + h * a.v.head + 16 * c;
-            x[f].raw = y[f].raw = make_uint4(0, 0, 0, 0);  // a row that is not there: step and base 0, or zeros
-            if (owned && k >= 0) {
-                x[f].load(a.key_pool.base + k + h * a.key_pool.head, c, a.code_bytes);
-                y[f].load(a.value_pool.base + v + h * a.value_pool.head, c, a.code_bytes);
+            for (int f = 0; f < kFlight; ++f) {
+                x[f].raw = y[f].raw = typename Piece<T, PACKED>::Raw{};  // a row that is not there: zeros, or step and base 0
+                if (k >= 0 && h + f * stride < a.heads) {
+                    x[f].load(from_k, c, a.code_bytes);
+                    y[f].load(from_v, c, a.code_bytes);
+                }
+                from_k += stride * a.key_pool.head;
+                from_v += stride * a.value_pool.head;
             }
+#pragma unroll
+            for (int f = 0; f < kFlight; ++f) {
+                if (h + f * stride < a.heads) {
+                    *reinterpret_cast<uint4 *>(to_k) = x[f].value();
+                    *reinterpret_cast<uint4 *>(to_v) = y[f].value();
+                }
+                to_k += stride * a.k.head;
+                to_v += stride * a.v.head;
+            }
+            h += kFlight * stride;
         }
-#pragma unroll
-        for (int f = 0; f < kFlight; ++f)
-            if (to_k[f]) {
-                *reinterpret_cast<uint4 *>(to_k[f]) = x[f].value();
-                *reinterpret_cast<uint4 *>(to_v[f]) = y[f].value();
-            }
     }
 }
 
@@ -540,15 +640,15 @@ extern "C" int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const m
     a.heads = static_cast<int>(keys->shape[1]);
     a.pieces = static_cast<int>(keys->shape[2] * dtype_bytes(keys->dtype) / 16);
     a.code_bytes = static_cast<int>(keys->shape[2] / 2);
-    // Few tokens: warps share a row.  Else as many tokens to a warp as make about 128 pieces of each pool.
-    const int pieces = a.heads * a.pieces;
-    const bool few = a.tokens < 4 * ctx->sm_count;
-    a.team = few ? std::max(1, std::min(8, pieces / 128)) : 1;
-    a.share = few ? 1 : std::max(1, std::min(32, 128 / pieces));
+    // as the appends
+    a.wide = lanes_of(a.pieces);
+    const int per = 32 >> a.wide, slots = (a.heads + per - 1) / per;
+    const int64_t warps = 16 * static_cast<int64_t>(ctx->sm_count);
+    a.team = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(slots, warps / tokens)));
+    a.share = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, tokens / (2 * warps))));
     const int64_t all = (tokens + a.share - 1) / a.share * a.team;
-    constexpr int kWarps = 8;
-    const unsigned grid = static_cast<unsigned>((all + kWarps - 1) / kWarps);
-    auto run = [&](auto kernel) { kernel<<<grid, kWarps * 32, 0, ctx->stream>>>(a); };
+    const unsigned grid = static_cast<unsigned>((all + kReadWarps - 1) / kReadWarps);
+    auto run = [&](auto kernel) { kernel<<<grid, kReadWarps * 32, 0, ctx->stream>>>(a); };
     if (key_pages->dtype != MR_DTYPE_U8) run(k_read_pages<float, false>);  // 16-byte pieces of any type
     else if (keys->dtype == MR_DTYPE_F32) run(k_read_pages<float, true>);
     else if (keys->dtype == MR_DTYPE_F16) run(k_read_pages<__half, true>);
