@@ -6,19 +6,21 @@
 // (m: about the maximum; differences, so that logits far from 0 cost no digits).
 //
 // One pass: every logit is read once, at about seven operations, and each thread
-// keeps a running maximum, S and the entropy's sum of its own elements.  Bound by
-// memory where there are many rows; a row is one CTA's, or where rows are few a
-// cluster's of up to 8, whose sums and candidates meet in the first CTA's shared
-// memory.
+// keeps a running maximum, S and the entropy's sum of its own elements.  A row is a
+// team's: a CTA's; a warp's where rows are short; or where rows are few and long a
+// cluster's of up to 4 CTAs, whose sums and candidates meet in the first one's
+// shared memory.
 //
-// The most likely tokens come from the threads' maxima.  The k-th largest maximum T
-// is a lower bound of the k-th largest logit, and only a thread whose own maximum
-// reaches T can have such logits: about k threads' elements (of 256) are read again,
-// from L2, and the few that reach T are ranked by counting.  No work is added to the
-// pass, and none of it depends on the order of the logits.  Where very many logits
-// equal T (rows masked by -inf, constant rows), only larger ones are taken and the
-// rest filled with the first ones that equal it.
+// The most likely tokens come from maxima of 256 parts of the row (a CTA's threads; eight of a
+// warp's lane).  The k-th largest of them, T, is a lower bound of the k-th largest logit, and only a part
+// whose maximum reaches T can have such logits: about k parts' elements are read
+// again, from cache, and the few that reach T are ranked by counting.  No work is
+// added to the pass, and none of it depends on the order of the logits.  Where
+// very many logits equal T (rows masked by -inf, constant rows), only larger ones are
+// taken and the rest filled with the first ones that equal it.
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "cache_ops.cuh"
 
@@ -28,7 +30,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMostTop = 128, kRoom = 1024, kMostCtas = 8;
+constexpr int kMostTop = 128, kMostCtas = 4, kParts = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 // e^-kFar is 0 in float32: differences are cut there where they are factors, so that 0 x -inf is no NaN
 constexpr float kFar = 1e4f;
@@ -42,6 +44,7 @@ struct ScoreArgs {
     int *top_tokens;
     float *top_logprobs;
     int64_t top_token_row, top_logprob_row;
+    int64_t rows;
     int vocab, given, top, ctas;  // ctas: of a row
 };
 
@@ -50,6 +53,11 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0;
     const uint32_t bits = __float_as_uint(x + 0.f);
     return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
+}
+constexpr uint32_t kLowest = 0x007fffffu;  // of -inf
+// The logit of an order from kLowest on; NaN of 0.
+__device__ __forceinline__ float value_of(uint32_t order) {
+    return order ? __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order) : __uint_as_float(0x7fffffffu);
 }
 // The same with the token: larger is more likely, the lower token first; 0 is none.
 __device__ __forceinline__ uint64_t candidate(uint32_t order, int token) {
@@ -66,22 +74,33 @@ __device__ __forceinline__ float ex2(float x) {
 // Sums over elements x: s of e^(x - top), a of e^(x - top) (x - top).
 struct Sums {
     float top, s, a;  // no elements, or -inf alone: top -inf
-    __device__ __forceinline__ void add(const Sums &o) {
-        const float to = fmaxf(top, o.top);
-        auto moved = [&](const Sums &x, float &s2, float &a2) {
-            const float by = x.top - to, c = ex2(by * kLog2e);
-            const bool none = x.top == -INFINITY;  // nothing to move; s may be the NaN of a NaN
-            s2 = none ? x.s : x.s * c;
-            a2 = none ? x.a : c * fmaf(x.s, fmaxf(by, -kFar), x.a);
-        };
-        float s0, a0, s1, a1;
-        moved(*this, s0, a0);
-        moved(o, s1, a1);
-        top = to;
-        s = s0 + s1;
-        a = a0 + a1;
-    }
 };
+
+// Two float32 operations in one instruction.
+union Pair {
+    float2 f;
+    uint64_t bits;
+};
+__device__ __forceinline__ Pair both(float x) {
+    Pair p;
+    p.f = make_float2(x, x);
+    return p;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair c;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.bits) : "l"(a.bits), "l"(b.bits));
+    return c;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair c;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.bits) : "l"(a.bits), "l"(b.bits));
+    return c;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return d;
+}
 
 template <typename T>
 struct Vector {
@@ -91,6 +110,11 @@ struct Vector {
         T v[kValues];
     };
     __device__ __forceinline__ Vector() {}
+    // -inf everywhere, which adds nothing
+    __device__ __forceinline__ void clear() {
+        const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        raw = make_uint4(low, low, low, low);
+    }
     __device__ __forceinline__ float operator[](int i) const { return widen(&v[i]); }
 };
 
@@ -130,117 +154,163 @@ struct Slice {
     }
 };
 
+// P threads of a row (or of a CTA's share of it): a CTA or a warp.
+template <int P>
 struct Shared {
-    uint64_t found[kRoom];    // candidates
-    uint64_t best[kMostTop];  // of them the largest, falling; 0 behind
-    uint64_t all[kMostTop * kMostCtas];
-    uint32_t maxima[kThreads];
-    Sums sums[kWarps];
+    static constexpr int kWarps = P / 32, kRoom = P == 32 ? 256 : 1024, kLists = P == 32 ? 1 : kMostCtas;
+    uint64_t found[kRoom];           // candidates
+    uint64_t best[kMostTop];         // of them the largest, falling; 0 behind
+    uint64_t all[kMostTop * kLists - (P == 32) * (kMostTop - 1)];  // of the first CTA: every CTA's best
+    Sums parts[kWarps * kLists];     // and every warp's sums
+    Sums sums[kWarps];               // this team's
     Sums total;
+    uint32_t maxima[kParts];
+    uint8_t reaching[kParts];        // parts whose maximum reaches the bound; of a CTA, 32 of each warp
     uint32_t bound;
     int count;
     int tally[kWarps];
 };
+template <int P>
+__device__ __forceinline__ void team_sync() {
+    if (P == 32) __syncwarp();
+    else __syncthreads();
+}
 
 // Candidates of the slice: elements from `bound` on, or past it.
-template <typename T>
-__device__ __forceinline__ void collect(const Slice<T> &slice, Shared &sh, uint32_t bound, bool past) {
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+template <typename T, int P>
+__device__ __forceinline__ void collect(const Slice<T> &slice, Shared<P> &sh, int tid, uint32_t bound, bool past) {
+    constexpr int V = Slice<T>::V, kFlight = 4;
+    const int warp = tid / 32, lane = tid % 32;
+    const float limit = value_of(bound);
+    // as the orders compare; with 0, the order of NaN, all elements, or all others
+    auto reaches = [&](float x) { return past ? x > limit || (!bound && x == x) : x >= limit || !bound; };
     auto push = [&](int token, float x) {
-        const uint32_t o = order_of(x);
-        if (past ? o > bound : o >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kRoom) sh.found[at] = candidate(o, token);
-        }
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < Shared<P>::kRoom) sh.found[at] = candidate(order_of(x), token);
     };
-    slice.singles(tid, push);
-    uint32_t mask = __ballot_sync(0xffffffffu, sh.maxima[tid] >= bound);
-    while (mask) {
-        const int t = warp * 32 + __ffs(mask) - 1;
-        mask &= mask - 1;
-        for (int v = slice.v0 + t + lane * kThreads; v < slice.v1; v += 32 * kThreads) {
-            const Vector<T> x = slice.load(v);
+    slice.singles(tid, [&](int token, float x) {
+        if (reaches(x)) push(token, x);
+    });
+    // the elements of the warp's parts that reach the bound, read by all its lanes: 128 vectors at once
+    uint8_t *reaching = sh.reaching + warp * 32;
+    int parts = 0;
 #pragma unroll
-            for (int j = 0; j < Slice<T>::V; ++j) push(slice.head + v * Slice<T>::V + j, x[j]);
+    for (int i = 0; i < kParts / P; ++i) {
+        const int part = warp * 32 + i * P + lane;
+        const bool is = sh.maxima[part] >= bound;
+        const uint32_t mask = __ballot_sync(0xffffffffu, is);
+        if (is) reaching[parts + __popc(mask & ((1u << lane) - 1))] = static_cast<uint8_t>(part);
+        parts += __popc(mask);
+    }
+    __syncwarp();
+    const int each = (slice.v1 - slice.v0 + kParts - 1) / kParts, all = parts * each;
+    const float per = 1.f / static_cast<float>(each);
+#pragma unroll 1
+    for (int e0 = lane; e0 < all; e0 += 32 * kFlight) {
+        Vector<T> x[kFlight];
+        int v[kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            const int e = min(e0 + 32 * f, all - 1);
+            int t = min(static_cast<int>(static_cast<float>(e) * per), parts - 1);  // e / each, or one beside it
+            t -= t * each > e;
+            t += (t + 1) * each <= e;
+            v[f] = e0 + 32 * f < all ? slice.v0 + reaching[t] + (e - t * each) * kParts : slice.v1;
+            if (v[f] < slice.v1) x[f] = slice.load(v[f]);
+            else x[f].clear();
+        }
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            uint32_t hits = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) hits |= reaches(x[f][j]) ? 1u << j : 0u;
+            if (v[f] >= slice.v1) hits = 0;
+            for (; hits; hits &= hits - 1) {
+                const int token = slice.head + v[f] * V + __ffs(hits) - 1;
+                push(token, widen(slice.row + token));
+            }
         }
     }
 }
 
 // How many elements of the slice are from `bound` on; all threads have it.
-template <typename T>
-__device__ int count_from(const Slice<T> &slice, Shared &sh, uint32_t bound) {
-    const int tid = threadIdx.x;
+template <typename T, int P>
+__device__ int count_from(const Slice<T> &slice, Shared<P> &sh, int tid, uint32_t bound) {
     int n = 0;
     auto add = [&](int, float x) { n += order_of(x) >= bound; };
     slice.singles(tid, add);
-    for (int v = slice.v0 + tid; v < slice.v1; v += kThreads) {
+    for (int v = slice.v0 + tid; v < slice.v1; v += P) {
         const Vector<T> x = slice.load(v);
 #pragma unroll
         for (int j = 0; j < Slice<T>::V; ++j) add(0, x[j]);
     }
     n = __reduce_add_sync(0xffffffffu, n);
+    if (P == 32) return n;
     __syncthreads();
     if (tid % 32 == 0) sh.tally[tid / 32] = n;
     __syncthreads();
     n = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) n += sh.tally[w];
+    for (int w = 0; w < P / 32; ++w) n += sh.tally[w];
     return n;
 }
 
-// The slice's `want` largest elements into sh.best.
-template <typename T>
-__device__ __forceinline__ void choose(const Slice<T> &slice, Shared &sh, float largest, int want) {
-    constexpr int V = Slice<T>::V;
-    const int tid = threadIdx.x, lane = tid % 32;
-    const int mine = (tid < slice.head_count) + (tid < slice.tail_count) + (slice.v0 + tid < slice.v1);
-    sh.maxima[tid] = mine ? max(order_of(largest), 1u) : 0u;  // at least 1, of NaN alone too: has elements
+// The slice's `want` largest elements into sh.best.  largest: of the thread's parts.
+template <typename T, int P>
+__device__ __forceinline__ void choose(const Slice<T> &slice, Shared<P> &sh, int tid, const float (&largest)[kParts / P], int want) {
+    constexpr int V = Slice<T>::V, kKeys = kParts / 32, kRoom = Shared<P>::kRoom;
+    const int lane = tid % 32;
+#pragma unroll
+    for (int i = 0; i < kParts / P; ++i) {
+        const bool some = slice.v0 + tid + i * P < slice.v1 || (i == 0 && (tid < slice.head_count || tid < slice.tail_count));
+        sh.maxima[tid + i * P] = some ? max(order_of(largest[i]), 1u) : 0u;  // at least 1, of NaN alone too: has elements
+    }
     if (tid == 0) sh.count = 0;
-    __syncthreads();
+    team_sync<P>();
     if (tid < 32) {
         // the want-th largest of the maxima, or a number below it that not many more reach: halving
-        uint32_t key[kWarps], low = 0xffffffffu, high = 0;
+        uint32_t key[kKeys], low = 0xffffffffu, high = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kKeys; ++w) {
             key[w] = sh.maxima[w * 32 + lane];
             low = min(low, key[w]);
             high = max(high, key[w]);
         }
         low = __reduce_min_sync(0xffffffffu, low);
         high = __reduce_max_sync(0xffffffffu, high);
-        int reach = kThreads;
+        int reach = kParts;
         ++high;  // order_of(+inf) at most: does not wrap
-        while (high - low > 1 && reach > want + 8) {
+        while (high - low > 1 && reach > want + 4 + want / 4) {
             const uint32_t mid = low + (high - low) / 2;
             int n = 0;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) n += key[w] >= mid;
+            for (int w = 0; w < kKeys; ++w) n += key[w] >= mid;
             n = __reduce_add_sync(0xffffffffu, n);
             if (n >= want) low = mid, reach = n;
             else high = mid;
         }
-        // fewer threads with elements than wanted, or among them NaN alone: everything counts
-        if (lane == 0) sh.bound = low <= 1 ? 0u : low;
+        // fewer parts with elements than wanted, or among them NaN alone: everything counts
+        if (lane == 0) sh.bound = low <= 1 ? 0u : max(low, kLowest);
     }
-    __syncthreads();
+    team_sync<P>();
     uint32_t bound = sh.bound;
     auto collected = [&](bool past) {
-        collect(slice, sh, bound, past);
-        __syncthreads();
+        collect<T, P>(slice, sh, tid, bound, past);
+        team_sync<P>();
         const int n = sh.count;
-        __syncthreads();
+        team_sync<P>();
         if (tid == 0) sh.count = 0;
-        __syncthreads();
+        team_sync<P>();
         return n;
     };
     int n = collected(false);
-    bool enough = n >= want;  // from the bound on (threads of NaN alone have less than their maximum says)
+    bool enough = n >= want;  // from the bound on (parts of NaN alone have less than their maximum says)
     if (enough && n > kRoom) n = collected(true);
     if (!enough || n > kRoom) {
         // the want-th largest itself, bit by bit
         bound = 0;
         for (int bit = 31; bit >= 0; --bit)
-            if (count_from(slice, sh, bound | 1u << bit) >= want) bound |= 1u << bit;
+            if (count_from<T, P>(slice, sh, tid, bound | 1u << bit) >= want) bound |= 1u << bit;
         n = collected(true);
     }
     if (n < want) {
@@ -260,11 +330,13 @@ __device__ __forceinline__ void choose(const Slice<T> &slice, Shared &sh, float 
             fill(lane < slice.tail_count, slice.tail + lane);
         }
         n = want;
-        __syncthreads();
+        team_sync<P>();
     }
-    for (int i = tid; i < kMostTop; i += kThreads) sh.best[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
+    if (slice.count() < kMostTop) {  // a list of fewer than are asked for ends in zeros
+        for (int i = tid; i < kMostTop; i += P) sh.best[i] = 0;
+        team_sync<P>();
+    }
+    for (int i = tid; i < n; i += P) {
         const uint64_t c = sh.found[i];
         int above = 0;
         for (int j = 0; j < n; ++j) above += sh.found[j] > c;
@@ -272,15 +344,27 @@ __device__ __forceinline__ void choose(const Slice<T> &slice, Shared &sh, float 
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_log_probabilities(const __grid_constant__ ScoreArgs a) {
-    __shared__ Shared sh;
-    constexpr int V = Slice<T>::V, kFlight = sizeof(T) == 4 ? 4 : 2;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const int rank = a.ctas == 1 ? 0 : static_cast<int>(cg::this_cluster().block_rank());
-    const int64_t r = blockIdx.x / a.ctas;
+// All CTAs of the cluster have started: said at the start, waited for before their memory is written.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+template <typename T, int P>
+__global__ void __launch_bounds__(P == 32 ? 128 : P) k_log_probabilities(const __grid_constant__ ScoreArgs a) {
+    constexpr int V = Slice<T>::V, kEach = kParts / P, kWarps = P / 32, kTeams = P == 32 ? 4 : 1;
+    // vectors of a thread under way: one of each of its parts, or some of its only one
+    constexpr int kFlight = P == 32 ? kEach : sizeof(T) == 4 ? 4 : 2;
+    __shared__ Shared<P> teams[kTeams];
+    Shared<P> &sh = teams[P == 32 ? threadIdx.x / 32 : 0];
+    const int tid = P == 32 ? threadIdx.x % 32 : threadIdx.x, warp = tid / 32, lane = tid % 32;
+    if (P > 32 && a.ctas > 1) cluster_arrive();
+    const int rank = P == 32 || a.ctas == 1 ? 0 : static_cast<int>(cg::this_cluster().block_rank());
+    const int64_t r = P == 32 ? static_cast<int64_t>(blockIdx.x) * kTeams + threadIdx.x / 32 : blockIdx.x / a.ctas;
+    if (P == 32 && r >= a.rows) return;
     const Slice<T> slice(a, r, rank);
     Sums mine = {-INFINITY, 0.f, 0.f};
+    float largest[kEach];  // of the parts
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) largest[i] = -INFINITY;
     float from = 0.f;  // mine.top, 0 while that is -inf: -inf less 0 is no NaN
     auto grow = [&](float top) {
         if (top > mine.top) {
@@ -297,101 +381,151 @@ __global__ void __launch_bounds__(kThreads) k_log_probabilities(const __grid_con
         mine.s += e;
         mine.a = fmaf(e, fmaxf(d, -kFar), mine.a);
     };
+    // a group of vectors is under way while the one before it is worked on
+    Vector<T> now[kFlight];
+    auto load = [&](int v) {
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) {
+            if (v + f * P < slice.v1) now[f] = slice.load(v + f * P);
+            else now[f].clear();
+        }
+    };
+    load(slice.v0 + tid);
+    // the given tokens' logits come early too
+    int given = -1;
+    float given_logit = 0.f;
+    if (rank == 0 && tid < a.given) {
+        given = a.tokens[r * a.token_row + tid];
+        if (static_cast<unsigned>(given) < static_cast<unsigned>(a.vocab)) given_logit = widen(slice.row + given);
+    }
     slice.singles(tid, [&](int, float x) {
+        largest[0] = fmaxf(largest[0], x);
         grow(x);
         add(x);
     });
-    for (int v = slice.v0 + tid; v < slice.v1; v += kFlight * kThreads) {
+#pragma unroll 1
+    for (int v = slice.v0 + tid; v - tid < slice.v1; v += kFlight * P) {
         Vector<T> x[kFlight];
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f)
-            if (v + f * kThreads < slice.v1) x[f] = slice.load(v + f * kThreads);
-            else x[f].raw = make_uint4(0, 0, 0, 0);
-        float top = -INFINITY;
+        for (int f = 0; f < kFlight; ++f) x[f].raw = now[f].raw;
+        load(v + kFlight * P);
+        float all = -INFINITY;
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f)
-            if (v + f * kThreads < slice.v1)
+        for (int f = 0; f < kFlight; ++f) {
+            float top = x[f][0];
 #pragma unroll
-                for (int j = 0; j < V; ++j) top = fmaxf(top, x[f][j]);
-        grow(top);
-#pragma unroll
-        for (int f = 0; f < kFlight; ++f)
-            if (v + f * kThreads < slice.v1)
-#pragma unroll
-                for (int j = 0; j < V; ++j) add(x[f][j]);
-    }
-    // the row's sums
-    Sums sum = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Sums other = {__shfl_xor_sync(0xffffffffu, sum.top, o), __shfl_xor_sync(0xffffffffu, sum.s, o),
-                            __shfl_xor_sync(0xffffffffu, sum.a, o)};
-        sum.add(other);
-    }
-    if (lane == 0) sh.sums[warp] = sum;
-    __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) sum.add(sh.sums[w]);
-        sh.total = sum;
-    }
-    if (a.top) choose(slice, sh, mine.top, min(a.top, slice.count()));
-    if (a.ctas > 1) {
-        cg::this_cluster().sync();
-        if (rank == 0) {
-            if (tid == 0) {
-                for (int c = 1; c < a.ctas; ++c) sum.add(cg::this_cluster().map_shared_rank(&sh, c)->total);
-                sh.total = sum;
-            }
-            const int n = a.ctas * a.top;
-            for (int i = tid; i < n; i += kThreads)
-                sh.all[i] = cg::this_cluster().map_shared_rank(&sh, i / a.top)->best[i % a.top];
+            for (int j = 1; j < V; ++j) top = fmaxf(top, x[f][j]);
+            if (kEach > 1) largest[f % kEach] = fmaxf(largest[f % kEach], top);
+            all = fmaxf(all, top);
         }
-        cg::this_cluster().sync();  // the others' memory has been read
+        grow(all);
+        Pair s = {make_float2(mine.s, 0.f)}, sa = {make_float2(mine.a, 0.f)};
+        const Pair minus = both(-from), log2e = both(kLog2e);
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                Pair d = add2({make_float2(x[f][j], x[f][j + 1])}, minus), e = mul2(d, log2e);
+                e.f = make_float2(ex2(e.f.x), ex2(e.f.y));
+                s = add2(s, e);
+                d.f = make_float2(fmaxf(d.f.x, -kFar), fmaxf(d.f.y, -kFar));
+                sa = fma2(e, d, sa);
+            }
+        mine.s = s.f.x + s.f.y;
+        mine.a = sa.f.x + sa.f.y;
+    }
+    if (kEach == 1) largest[0] = mine.top;
+    // the row's sums: of a warp, all against its maximum
+    auto reduce = [](Sums &x) {
+        const float top = warp_max(x.top), by = x.top - top, c = ex2(by * kLog2e);
+        const bool none = x.top == -INFINITY;  // nothing to move; s may be the NaN of a NaN
+        x.a = warp_sum(none ? x.a : c * fmaf(x.s, fmaxf(by, -kFar), x.a));
+        x.s = warp_sum(none ? x.s : x.s * c);
+        x.top = top;
+    };
+    reduce(mine);
+    if (lane == 0) sh.sums[warp] = mine;
+    if (a.top) choose<T, P>(slice, sh, tid, largest, min(a.top, slice.count()));
+    team_sync<P>();
+    Sums *parts = sh.sums;
+    if (P > 32 && a.ctas > 1) {
+        // every CTA's results to the first one's memory; all have started
+        cluster_wait();
+        Shared<P> *root = cg::this_cluster().map_shared_rank(&sh, 0);
+        for (int i = tid; i < a.top; i += P) root->all[rank * a.top + i] = sh.best[i];
+        if (tid < kWarps) root->parts[rank * kWarps + tid] = sh.sums[tid];
+        cg::this_cluster().sync();
         if (rank) return;
-        const int n = a.ctas * a.top;
-        for (int i = tid; i < n; i += kThreads) {
+        parts = sh.parts;
+        // the place of each among all: how many of each falling list are larger, by halving, all lists at once
+        int widest = 1;
+        while (widest * 2 <= a.top) widest *= 2;
+        for (int i = tid; i < a.ctas * a.top; i += P) {
             const uint64_t c = sh.all[i];
+            int larger[kMostCtas] = {};
+            for (int w = widest; w; w >>= 1)
+#pragma unroll
+                for (int l = 0; l < kMostCtas; ++l)
+                    if (l < a.ctas && larger[l] + w <= a.top && sh.all[l * a.top + larger[l] + w - 1] > c) larger[l] += w;
             int above = 0;
-            for (int j = 0; j < n; ++j) above += sh.all[j] > c;
+#pragma unroll
+            for (int l = 0; l < kMostCtas; ++l) above += larger[l];
             if (c && above < a.top) sh.best[above] = c;
         }
     }
-    __syncthreads();
-    const Sums all = sh.total;
+    if (warp == kWarps - 1 && P > 32) {
+        static_assert(kWarps * kMostCtas <= 32, "a sum a lane");
+        Sums x = {-INFINITY, 0.f, 0.f};
+        if (lane < kWarps * a.ctas) x = parts[lane];
+        reduce(x);
+        if (lane == 0) sh.total = x;
+    }
+    team_sync<P>();
+    const Sums all = P == 32 ? mine : sh.total;
     const float log_s = logf(all.s);
     // a row of -inf alone: -inf, and no entropy
-    auto log_p = [&](int token) { return all.s == 0.f ? -INFINITY : widen(slice.row + token) - all.top - log_s; };
+    auto log_p = [&](float x) { return all.s == 0.f ? -INFINITY : x - all.top - log_s; };
     if (a.entropy && tid == 0) a.entropy[r * a.entropy_row] = all.s == 0.f ? 0.f : log_s - all.a / all.s;
-    for (int i = tid; i < a.given; i += kThreads) {
+    auto put = [&](int i, int token, float x) {
+        a.logprobs[r * a.logprob_row + i] = static_cast<unsigned>(token) < static_cast<unsigned>(a.vocab) ? log_p(x) : 0.f;
+    };
+    if (tid < a.given) put(tid, given, given_logit);
+    for (int i = tid + P; i < a.given; i += P) {
         const int t = a.tokens[r * a.token_row + i];
-        a.logprobs[r * a.logprob_row + i] = static_cast<unsigned>(t) < static_cast<unsigned>(a.vocab) ? log_p(t) : 0.f;
+        put(i, t, static_cast<unsigned>(t) < static_cast<unsigned>(a.vocab) ? widen(slice.row + t) : 0.f);
     }
-    for (int i = tid; i < a.top; i += kThreads) {
-        const int t = token_of(sh.best[i]);
-        a.top_tokens[r * a.top_token_row + i] = t;
-        a.top_logprobs[r * a.top_logprob_row + i] = log_p(t);
+    for (int i = tid; i < a.top; i += P) {
+        const uint64_t c = sh.best[i];
+        a.top_tokens[r * a.top_token_row + i] = token_of(c);
+        a.top_logprobs[r * a.top_logprob_row + i] = log_p(value_of(static_cast<uint32_t>(c >> 32)));
     }
 }
 
 template <typename T>
-int launch(mr_context *ctx, ScoreArgs &a, int64_t rows) {
-    // CTAs of a row: as many as give the GPU four an SM, each with two vectors a thread at least
+int launch(mr_context *ctx, ScoreArgs &a) {
+    // Short rows are a warp's, and where there are more than four an SM those of up to 64 KB (4096 rows of 2000 float32
+    // 16 us, a CTA each 43; of 16000 bfloat16 41 and 63; but 1000 of 64000 51 and 45).  A longer one's CTAs: as many as
+    // give the GPU four an SM, each with two vectors a thread at least.
     a.ctas = 1;
-    while (a.ctas < kMostCtas && rows * a.ctas * 2 <= 4 * ctx->sm_count &&
-           a.vocab / Slice<T>::V >= 2 * kThreads * a.ctas * 2)
+    if (a.vocab <= 1024 || (a.rows > 4 * ctx->sm_count && a.vocab * static_cast<int64_t>(sizeof(T)) <= 64 << 10)) {
+        k_log_probabilities<T, 32><<<static_cast<unsigned>((a.rows + 3) / 4), 128, 0, ctx->stream>>>(a);
+        MR_CUDA_TRY(cudaGetLastError());
+        return MR_OK;
+    }
+    while (a.ctas < kMostCtas && a.rows * a.ctas * 2 <= 4 * ctx->sm_count &&
+           a.vocab / Slice<T>::V >= 2 * kParts * a.ctas * 2)
         a.ctas *= 2;
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = a.ctas;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(rows * a.ctas));
-    config.blockDim = dim3(kThreads);
+    config.gridDim = dim3(static_cast<unsigned>(a.rows * a.ctas));
+    config.blockDim = dim3(256);
     config.stream = ctx->stream;
     config.attrs = &cluster;
     config.numAttrs = a.ctas > 1;
-    MR_CUDA_TRY(cudaLaunchKernelEx(&config, k_log_probabilities<T>, a));
+    MR_CUDA_TRY(cudaLaunchKernelEx(&config, k_log_probabilities<T, 256>, a));
     return MR_OK;
 }
 
@@ -465,7 +599,8 @@ extern "C" int mr_log_probabilities(mr_context *ctx, const mr_array *logits, con
     a.logits = static_cast<const char *>(logits->data);
     a.row_bytes = logits->stride[0] * dtype_bytes(logits->dtype);
     a.vocab = static_cast<int>(vocab);
-    return logits->dtype == MR_DTYPE_F32   ? launch<float>(ctx, a, rows)
-           : logits->dtype == MR_DTYPE_F16 ? launch<__half>(ctx, a, rows)
-                                           : launch<__nv_bfloat16>(ctx, a, rows);
+    a.rows = rows;
+    return logits->dtype == MR_DTYPE_F32   ? launch<float>(ctx, a)
+           : logits->dtype == MR_DTYPE_F16 ? launch<__half>(ctx, a)
+                                           : launch<__nv_bfloat16>(ctx, a);
 }
