@@ -469,9 +469,13 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * byte's low half, then for each 32 dims two little-endian IEEE float16 numbers, a
  * step s and a base z: code c stands for s (64 + c) + z, rounded to float16.
  * Writing a row: s = (max - min) / 15 of the 32 values and z = min - 64 s, each
- * rounded to float16, c the nearest of 0 .. 15; 32 values of which one is not finite
- * or which are too far apart for float16 (from about +-13 000 on) read as NaN.
- * What is written depends on the values alone. */
+ * rounded to float16, c the nearest of 0 .. 15.  32 values of which one is not finite
+ * or whose base passes float16 (values from -6870 to 6870, say) read as NaN.  What
+ * is written depends on the values alone.
+ * Attention's queries and results are of any floating type.  Each weight meets the
+ * values in float16 (BF16: one part, an error of 2^-12 of it; F16 and F32: two,
+ * 2^-22), with errors of 2^-40 of a row's largest weight.  An infinite step or base,
+ * which no call writes, gives infinities or NaN. */
 
 /* mr_append_pages with a rotation on the way: the first 2 n dims of each query
  * [tokens, heads, dim] and key are turned by position * frequencies[p] (F32 [n],
@@ -483,7 +487,8 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * rounded to the type, or to 4 bits.  Turned queries go to out [tokens, heads, dim]
  * (query and out may both be NULL); those of tokens in no sequence stay as they
  * were.  All of query, keys, values and out are of one type, the pages of the same
- * or of 4 bits. */
+ * or of 4 bits; out must not overlap the inputs.  What mr_append_pages says of
+ * places, dropped rows and offsets holds here. */
 MR_API int mr_append_rotated(mr_context *ctx, const mr_array *query, const mr_array *keys, const mr_array *values,
                              const mr_array *key_pages, const mr_array *value_pages, const mr_array *page_table,
                              const mr_array *lengths, const mr_array *offsets, const mr_array *frequencies,

@@ -131,14 +131,19 @@ class DeviceArray:
         return DeviceArray(self.backend, shape, dtype or self.dtype)
 
 
+_KINDS = {}    # (a dtype object, a type's name) -> its library's dtype object of that name, None if it is that already
+
+
 def empty_like(array, shape, dtype):
-    """An array of another type by the owner of `array`: its library's type of that name."""
+    """An array of a named type by the owner of `array`."""
     kind = array.dtype
-    if str(kind).rsplit(".", 1)[-1] == dtype:
-        return array.new_empty(shape)
-    if not isinstance(kind, str):
-        dtype = getattr(sys.modules[type(kind).__module__], dtype)
-    return array.new_empty(shape, dtype=dtype)
+    try:
+        found = _KINDS[kind, dtype]
+    except KeyError:
+        same = str(kind).rsplit(".", 1)[-1] == dtype
+        found = None if same else dtype if isinstance(kind, str) else getattr(sys.modules[type(kind).__module__], dtype)
+        _KINDS[kind, dtype] = found
+    return array.new_empty(shape) if found is None else array.new_empty(shape, dtype=found)
 
 
 def stored(array, dtype):

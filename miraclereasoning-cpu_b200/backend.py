@@ -386,15 +386,15 @@ class CUDABackend:
             raise ValueError("logits must be an array [rows, vocabulary]")
         rows = logits.shape[0]
         if tokens is not None and logprobs is None:
-            logprobs = empty_like(logits, tuple(tokens.shape), "float32")
+            logprobs = empty_like(logits, tokens.shape, "float32")
         if entropy is None:
             entropy = empty_like(logits, (rows,), "float32")
         if top_tokens is None:
             top_tokens = empty_like(logits, (rows, top), "int32")
+        elif tuple(top_tokens.shape) != (rows, top):
+            raise ValueError(f"top_tokens must be [{rows}, {top}]")
         if top_logprobs is None:
             top_logprobs = empty_like(logits, (rows, top), "float32")
-        if tuple(top_tokens.shape) != (rows, top):
-            raise ValueError(f"top_tokens must be [{rows}, {top}]")
         best = (top_tokens, top_logprobs) if top else (None, None)
         invoke(arrays.SCORE, *self._where, logits, tokens, logprobs, entropy, *best)
         return logprobs, entropy, top_tokens, top_logprobs

@@ -71,15 +71,17 @@ def test_appends_to_pages_of_4_bits_are_checked():
 def read(**changes):
     k, v = bytes_of(64)
     args = dict(key_pages=k, value_pages=v, table=Fake((3, 5), I32), lengths=Fake((3,), I32), offsets=Fake((4,), I32),
-                keys=Fake((90, 4, 64)), values=Fake((90, 4, 64), pointer=1 << 28))
+                keys=Fake((90, 4, 64), pointer=1 << 27), values=Fake((90, 4, 64), pointer=1 << 28))
     args.update(changes)
     return refused("mr_read_pages", list(args.values()))
 
 
 @pytest.mark.parametrize("changes, message", [
     (dict(), "ctx is NULL"),
-    (dict(keys=Fake((90, 4, 64), F32), values=Fake((90, 4, 64), F32, pointer=1 << 28)), "ctx is NULL"),
-    (dict(values=Fake((90, 4, 64))), "must not share memory"),
+    (dict(keys=Fake((90, 4, 64), F32, pointer=1 << 27), values=Fake((90, 4, 64), F32, pointer=1 << 28)), "ctx is NULL"),
+    (dict(values=Fake((90, 4, 64), pointer=1 << 27)), "keys and values must not share memory"),
+    (dict(keys=Fake((90, 4, 64))), "keys and the pages must not share memory"),
+    (dict(values=Fake((90, 4, 64), pointer=1 << 24)), "values and the pages must not share memory"),
     (dict(keys=Fake((90, 4, 64), stride=(0, 64, 1))), "must not overlap itself"),
     (dict(keys=Fake((90, 4, 64), U8)), "of one floating type"),
     (dict(keys=Fake((90, 2, 64)), values=Fake((90, 2, 64), pointer=1 << 28)), "\\[tokens, 4, 64\\]"),
