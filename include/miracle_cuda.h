@@ -465,15 +465,16 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * mr_append_pages, mr_append_rotated, mr_read_pages, mr_paged_attention and
  * mr_evict_pages also take pools of U8 [pages, page rows, kv heads, 5 dim / 8], for
  * head dims 32, 64, 96 and 128; each row starts on a boundary of 4 bytes (dims 32
- * and 96), 8 (64) or 16 (128), in address and strides.  A row is dim / 2 bytes of codes, the even dim in a
- * byte's low half, then for each 32 dims two little-endian IEEE float16 numbers, a
- * step s and a base z: code c stands for s (64 + c) + z, rounded to float16.
+ * and 96), 8 (64) or 16 (128), in address and strides.  A row is dim / 2 bytes of
+ * codes, the even dim in a byte's low half, then for each 32 dims two little-endian
+ * IEEE float16 numbers, a step s and a base z: code c stands for s (64 + c) + z,
+ * rounded to float16.
  * Writing a row: s = (max - min) / 15 of the 32 values and z = min - 64 s, each
  * rounded to float16, c the nearest of 0 .. 15.  32 values of which one is not finite
  * or whose base passes float16 (values from -6870 to 6870, say) read as NaN.  What
  * is written depends on the values alone.
  * Attention's queries and results are of any floating type.  Each weight meets the
- * values in float16 (BF16: one part, an error of 2^-12 of it; F16 and F32: two,
+ * values in float16 (BF16: one part, an error of 2^-11 of it; F16 and F32: two,
  * 2^-22), with errors of 2^-40 of a row's largest weight.  An infinite step or base,
  * which no call writes, gives infinities or NaN. */
 
@@ -496,8 +497,8 @@ MR_API int mr_append_rotated(mr_context *ctx, const mr_array *query, const mr_ar
 
 /* The way back of mr_append_pages: sequence s's last offsets[s + 1] - offsets[s]
  * rows (NULL: its newest row) go to keys and values [tokens, kv heads, dim] at
- * offsets[s] ..; from 4-bit pages as any floating type, from others as their own.  A row that
- * the pages do not hold (a bad page, past the table, before the first) is zeros;
+ * offsets[s] ..; from 4-bit pages as any floating type, from others as their own.
+ * A row that the pages do not hold (a bad page, past the table, before the first) is zeros;
  * rows of keys and values in no sequence stay as they were. */
 MR_API int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const mr_array *value_pages,
                          const mr_array *page_table, const mr_array *lengths, const mr_array *offsets,
@@ -510,9 +511,9 @@ MR_API int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const mr_ar
  * F32 [rows]; and the most likely tokens, falling, the lower one of equals first
  * (NaN counts as the lowest), in top_tokens I32 and top_logprobs F32 [rows, top],
  * top at most 128 and the vocabulary.  tokens and logprobs, and the last two, may be
- * NULL together; entropy too.  A logit of -inf has probability 0 and adds nothing; a row of
- * them alone has log probabilities -inf and entropy 0; a NaN or +inf in a row makes its
- * log probabilities and its entropy NaN.  Sums are float32. */
+ * NULL together; entropy too.  A logit of -inf has probability 0 and adds nothing; a
+ * row of them alone has log probabilities -inf and entropy 0; a NaN or +inf in a row
+ * makes its log probabilities and its entropy NaN.  Sums are float32. */
 MR_API int mr_log_probabilities(mr_context *ctx, const mr_array *logits, const mr_array *tokens, const mr_array *logprobs,
                                 const mr_array *entropy, const mr_array *top_tokens, const mr_array *top_logprobs);
 

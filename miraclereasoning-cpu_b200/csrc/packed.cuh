@@ -4,9 +4,10 @@
 // codes, the even dim in a byte's low half, and behind them two float16 numbers for
 // each 32 dims, a step s and a base z.  Code c stands for s (64 + c) + z, rounded to
 // float16 once.  The base is that of code -64, not of code 0, because a code ored
-// into the fraction of float16's 64 is the number 64 + c: half of a word's codes
-// become operands of one fused multiply-add without a shift.  (The base's own rounding,
-// at most 2^-12 of 4.8 ranges of the 32 values, moves a value by 2% of a step.)
+// into the fraction of float16's 64 is the number 64 + c: a pair of a word's codes becomes
+// an operand of one fused multiply-add by a logical operation, behind a shift for
+// three pairs of the four.  (The base's own rounding,
+// 2^-11 of about 4.8 times the spread of the 32 values, moves a value by 4% of a step.)
 #pragma once
 
 #include "cache_ops.cuh"

@@ -75,7 +75,7 @@ struct Math4 : Heads8<__half, DP_ / 16> {
     static int ctas(int64_t steps, int sms, bool weights) {
         return steps >= (weights ? 48 : 24) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
     }
-    // Weights in one float16 part are off by 2^-12, an eighth of a bfloat16 result's rounding; other results
+    // Weights in one float16 part are off by 2^-11, an eighth of a bfloat16 result's rounding; other results
     // get a second part.
     static constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
     struct R : Ring4<DP> {

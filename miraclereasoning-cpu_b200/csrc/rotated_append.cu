@@ -44,13 +44,13 @@ struct PlaceArgs {
 // Where packed token i stands; the same in all lanes of a warp, which look for it together.
 struct Place {
     int sequence;  // -1: of none
-    int begin, end;  // its tokens
+    int end;       // behind its last token
     int row;       // of token i there; may lie before the first
     int rows;
     // The last s with offsets[s] <= i, 32 at a time, if its end is behind i.
     __device__ __forceinline__ void find(const PlaceArgs &a, int i) {
         if (!a.offsets) {
-            sequence = begin = i;
+            sequence = i;
             end = i + 1;
         } else {
             const int lane = threadIdx.x % 32;
@@ -70,7 +70,6 @@ struct Place {
             const int last = __ldg(a.offsets + (lo + 1) * a.offset_stride);
             if (last <= i) return;
             sequence = lo;
-            begin = i;
             end = last;
         }
         rows = max(0, __ldg(a.lengths + sequence * a.length_stride));
@@ -512,7 +511,7 @@ __global__ void __launch_bounds__(kReadWarps * 32) k_read_pages(const __grid_con
     }
 }
 
-// Checks that the three operators share: rows of keys and values that stand for pages' rows.
+// Checks that both operators share: rows of keys and values that stand for pages' rows.
 int check_rows(const mr_array *keys, const mr_array *values, const mr_array *key_pages, const mr_array *value_pages,
                const mr_array *page_table, const mr_array *lengths, const mr_array *offsets, bool read) {
     MR_CHECK(check_array(keys, "keys", 3, true, read));
