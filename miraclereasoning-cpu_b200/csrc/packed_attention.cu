@@ -13,7 +13,7 @@
 //
 // A step of 32 rows of 128 dims is 665 instructions: 210 and 220 for the two products' operands and issue, 95
 // for the softmax, 120 for the copies of two steps on.  32 sequences ragged to 32768 rows at 8 heads of 128
-// (668 MB): 145 us, of which 20 are the start, the uneven end and the join; the copies alone take 113.
+// (668 MB): 145 us, of which about 20 are the start, the uneven end and the join; the copies alone take 113.
 // Logical operations and float16 multiply-adds each issue every other cycle, and 1.5 cycles each when
 // mixed, so that moving work between the two gains nothing (shifts as additions: 166 and 167 us at the time);
 // 8-bit floating-point products of the codes as they stand (e4m3 0 .. 15 are linear) need fewer masks, but that
@@ -71,7 +71,7 @@ struct Math4 : Heads8<__half, DP_ / 16> {
     // CTAs of an SM.  Three have more steps under way, two leave room for the joining kernel's CTAs to start beside
     // them and fewer partials to join: from about 24 steps a warp on (by the tables; with weights, which the joining
     // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128: 1 sequence 23.2 with two, 27.4 with
-    // three; 4 sequences 49.6, 49.8; 16 sequences 158, 146).
+    // three; 4 sequences 49.6, 49.8; 16 sequences 158, 146; a quicker join has since taken 3 us off each).
     static int ctas(int64_t steps, int sms, bool weights) {
         return steps >= (weights ? 48 : 24) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
     }

@@ -809,25 +809,42 @@ __global__ void __launch_bounds__(kThreads, M::kCtas) k_paged_few(const __grid_c
     });
 }
 
+// Whether there are weights to add, and for groups of several blocks of heads (in one kernel with the other case
+// some of its registers spill).
+enum { kNoWeights, kWeights, kBlockWeights };
+// Warps for each of k_paged's, to hide the latency of the little that each reads.  One is enough for the short way
+// there is without weights over pages of 4 bits (one sequence of 32768 rows: 20.7 us, with two 22.3; with weights,
+// 24 sequences to 8192 rows: 37.8 and 36.0).
+template <typename M, int MODE>
+constexpr int kJoiners = M::kRuns && MODE == kNoWeights ? 1 : 2;
+
 // Joins the units that were cut: the warps whose stretch starts inside a unit
 // share its columns, four at a time.  With weights, every warp then adds up its
-// own stretch's rows.
-constexpr int kJoin = 2;  // warps for each of k_paged's, to hide the latency of the little that each reads
-
-// kBlocks: with weights, and groups of several blocks of heads (in one kernel with the other case some of its
-// registers spill).
-template <typename T, typename M, bool kBlocks>
+// own stretch's rows.  All of it is latency: what needs no partials (whose columns, in whole-number divisions;
+// the weights on their way to L2) comes before the wait, and loads of a kind are issued together.
+template <typename T, typename M, int MODE>
 __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ PagedArgs a) {
     constexpr int H = M::kHeads, DP = M::DP, STEP = M::STEP;
     constexpr int64_t kPart = H * DP;
+    constexpr int kJoin = kJoiners<M, MODE>;
+    constexpr bool kBlocks = MODE == kBlockWeights;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int id = blockIdx.x * kWarps + warp, worker = id / kJoin, share = id % kJoin;
     Plan<STEP> plan;
     plan.init(a);
     Walk walk = {};
     const bool work = walk.init(a, plan, worker);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!work) return;
+    if (MODE != kNoWeights && work) {
+        // the weights that this warp adds to, which k_paged leaves alone, into L2
+        Walk ahead = walk;
+        while (ahead.next(a, plan)) {
+            const int rows = min(ahead.t1 * STEP, ahead.seen.rows) - ahead.t0 * STEP;
+            const int from = ahead.t0 * STEP + rows * share / kJoin, to = ahead.t0 * STEP + rows * (share + 1) / kJoin;
+            const float *weights = a.weights + ahead.s * a.w_batch + ahead.u / a.blocks * a.w_head;
+            for (int i = from + 32 * lane; i < to + 31; i += 32 * 32)
+                if (to > from) asm volatile("prefetch.global.L2 [%0];" ::"l"(weights + ahead.seen.at(min(i, to - 1))));
+        }
+    }
     // The partials of a unit cut between workers b0 ..: a worker's first piece is in its
     // slot 0, so only b0's may be its last one, in slot 1.
     struct Parts {
@@ -841,19 +858,33 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
     auto sums_of = [&](const Parts &part, int b, int h) {
         return __ldcg(a.sums + ((b == part.b0 ? part.slot0 : 0) * H + h) * warps + b);
     };
-    const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
-    if (first < walk.x) {
-        const int b0 = plan.worker_of(first), b1 = plan.worker_of(first + walk.steps - 1), n = b1 - b0 + 1;
-        const Parts part = {a.partial, b0, plan.start(b0) >= first ? 0 : 1};
-        const int kh = cut / a.blocks, h0 = cut % a.blocks * H, heads = min(H, a.group - h0);
-        const int columns = heads * (DP / 4), sharers = (n - 1) * kJoin, me = (worker - b0 - 1) * kJoin + share;
-        const int c0 = columns * me / sharers, c1 = columns * (me + 1) / sharers;
+    // this warp's columns of a unit that its stretch starts in
+    int kh = 0, h0 = 0, n = 0, c0 = 0, c1 = 0;
+    Parts part = {a.partial, 0, 0};
+    if (work) {
+        const int cut = (walk.x - walk.base) / walk.steps, first = walk.base + cut * walk.steps;
+        if (first < walk.x) {
+            part.b0 = plan.worker_of(first);
+            part.slot0 = plan.start(part.b0) >= first ? 0 : 1;
+            n = plan.worker_of(first + walk.steps - 1) - part.b0 + 1;
+            kh = cut / a.blocks;
+            h0 = cut % a.blocks * H;
+            const int columns = min(H, a.group - h0) * (DP / 4), sharers = (n - 1) * kJoin;
+            const int me = (worker - part.b0 - 1) * kJoin + share;
+            c0 = columns * me / sharers;
+            c1 = columns * (me + 1) / sharers;
+        }
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!work) return;
+    if (c0 < c1) {
+        const int b0 = part.b0;
         // head by head of its columns
         for (int h = c0 / (DP / 4); h * (DP / 4) < c1; ++h) {
             const int lo = max(c0, h * (DP / 4)), hi = min(c1, (h + 1) * (DP / 4));
-            int wide = 1;  // lanes side by side over the columns, the rest over the partials
-            while (wide < 32 && wide < hi - lo) wide <<= 1;
-            const int step = 32 / wide;
+            // 2^shift lanes side by side over the columns, the rest over the partials
+            const int shift = hi - lo > 1 ? min(32 - __clz(hi - lo - 1), 5) : 0;
+            const int wide = 1 << shift, step = 32 >> shift, beside = lane & (wide - 1), behind = lane >> shift;
             constexpr int kFlight = 5;
             float4 v[kFlight];  // the first columns' values are under way while the softmax is worked out
             float top_of[kFlight];
@@ -862,25 +893,32 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
                 top_of[i] = b < n ? sums_of(part, b0 + b, h).x : -INFINITY;
             };
 #pragma unroll
-            for (int i = 0; i < kFlight; ++i) load(min(lo + lane % wide, hi - 1), i, lane / wide + i * step);
+            for (int i = 0; i < kFlight; ++i) load(min(lo + beside, hi - 1), i, behind + i * step);
             float top = -INFINITY, sum = 0.f;
-#pragma unroll 5
-            for (int b = lane; b < n; b += 32) {
-                const float2 x = sums_of(part, b0 + b, h);
-                const float t = fmaxf(top, x.x), ref = t == -INFINITY ? 0.f : t;
-                sum = fmaf(sum, ex2(top - ref), x.y * ex2(x.x - ref));
-                top = t;
+            for (int base = 0; base < n; base += 32 * kFlight) {
+                float2 x[kFlight];
+#pragma unroll
+                for (int i = 0; i < kFlight; ++i) {
+                    const int b = base + lane + 32 * i;
+                    x[i] = b < n ? sums_of(part, b0 + b, h) : make_float2(-INFINITY, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < kFlight; ++i) {
+                    const float t = fmaxf(top, x[i].x), ref = t == -INFINITY ? 0.f : t;
+                    sum = fmaf(sum, ex2(top - ref), x[i].y * ex2(x[i].x - ref));
+                    top = t;
+                }
             }
             const float most = warp_max(top), ref = most == -INFINITY ? 0.f : most;
             sum = warp_sum(sum * ex2(top - ref));
             const float f = sum != 0.f ? 1.f / sum : 0.f;
             for (int base = lo; base < hi; base += wide) {
-                const int c = min(base + lane % wide, hi - 1);
+                const int c = min(base + beside, hi - 1);
                 float4 x = {};
                 for (int b = 0; b < n; b += kFlight * step) {
                     if (base != lo || b)
 #pragma unroll
-                        for (int i = 0; i < kFlight; ++i) load(c, i, b + lane / wide + i * step);
+                        for (int i = 0; i < kFlight; ++i) load(c, i, b + behind + i * step);
 #pragma unroll
                     for (int i = 0; i < kFlight; ++i) {
                         const float w = ex2(top_of[i] - ref) * f;
@@ -907,7 +945,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
             }
         }
     }
-    if (!a.weights) return;
+    if (MODE == kNoWeights) return;
     // A cut unit's softmax over its partials: each head's maximum and sum, in every lane.
     auto softmax_of = [&](const Parts &part, int b1, float (&top)[H], float (&sum)[H]) {
 #pragma unroll
@@ -935,6 +973,26 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
             top[h] = t;
         }
     };
+    // Its logarithm, of head lane / each in a group of `each` lanes: all heads at once.
+    const int each = a.heads2 == 2 ? 16 : a.heads2 == 4 ? 8 : 4;
+    auto log_sum_of = [&](const Parts &part, int b1) {
+        const int h = lane / each;
+        float top = -INFINITY, sum = 0.f;
+        if (h < a.heads2) {
+#pragma unroll 4
+            for (int b = part.b0 + lane % each; b <= b1; b += each) {
+                const float2 x = sums_of(part, b, h);
+                const float t = fmaxf(top, x.x), ref = t == -INFINITY ? 0.f : t;
+                sum = fmaf(sum, ex2(top - ref), x.y * ex2(x.x - ref));
+                top = t;
+            }
+        }
+        float most = top;
+        for (int o = each / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        sum *= ex2(top - (most == -INFINITY ? 0.f : most));
+        for (int o = each / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        return log_sum(most, sum);
+    };
     while (walk.next(a, plan)) {
         if (walk.u % a.blocks) continue;  // the group's first block of heads adds up for all of them
         const int lo = walk.t0 * STEP, rows = min(walk.t1 * STEP, walk.seen.rows) - lo;
@@ -944,11 +1002,22 @@ __global__ void __launch_bounds__(kThreads, 5) k_join(const __grid_constant__ Pa
         for (int b = 0; b < (kBlocks ? a.blocks : 1); ++b) {
             const int start = walk.base + (walk.u + b) * walk.steps;
             const int b0 = plan.worker_of(start), b1 = plan.worker_of(start + walk.steps - 1);
-            float top[H], sum[H], lse[H];
-            if (b0 != b1) softmax_of({a.partial, b0, plan.start(b0) >= start ? 0 : 1}, b1, top, sum);
+            float lse[H];
+            const Parts part = {a.partial, b0, plan.start(b0) >= start ? 0 : 1};
+            if constexpr (M::kRuns) {
+                const float mine = b0 != b1 ? log_sum_of(part, b1) : 0.f;
 #pragma unroll
-            for (int h = 0; h < H; ++h)
-                lse[h] = h >= a.group - b * H ? INFINITY : b0 == b1 ? __ldcg(a.lse + (unit + b) * H + h) : log_sum(top[h], sum[h]);
+                for (int h = 0; h < H; ++h) {
+                    const float joined = __shfl_sync(0xffffffffu, mine, h * each % 32);
+                    lse[h] = h >= a.group - b * H ? INFINITY : b0 == b1 ? __ldcg(a.lse + (unit + b) * H + h) : joined;
+                }
+            } else {
+                float top[H], sum[H];
+                if (b0 != b1) softmax_of(part, b1, top, sum);
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+                    lse[h] = h >= a.group - b * H ? INFINITY : b0 == b1 ? __ldcg(a.lse + (unit + b) * H + h) : log_sum(top[h], sum[h]);
+            }
             if constexpr (kBlocks) add_rows<H, H, true>(a, walk, unit, kh, from, to, lane, 32, lse, b);
             else add_weights<H>(a, walk, unit, kh, from, to, lane, 32, lse);
         }
@@ -1000,9 +1069,13 @@ int launch(mr_context *ctx, PagedArgs &a) {
     MR_CHECK(allow_shared(ctx->device, reinterpret_cast<const void *>(k_paged<T, M>), kRings, allowed));
     k_paged<T, M><<<grid, kThreads, kRings, ctx->stream>>>(a);
     MR_CUDA_TRY(cudaGetLastError());
-    MR_CHECK(launch_early(ctx, dim3(grid * kJoin), dim3(kThreads),
-                          a.weights && a.blocks > 1 ? k_join<T, M, true> : k_join<T, M, false>, a));
-    return MR_OK;
+    auto join = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        return launch_early(ctx, dim3(grid * kJoiners<M, MODE>), dim3(kThreads), k_join<T, M, MODE>, a);
+    };
+    return !a.weights      ? join(std::integral_constant<int, kNoWeights>())
+           : a.blocks == 1 ? join(std::integral_constant<int, kWeights>())
+                           : join(std::integral_constant<int, kBlockWeights>());
 }
 
 }  // namespace
