@@ -69,11 +69,11 @@ struct Math4 : Heads8<__half, DP_ / 16> {
     static constexpr bool kRuns = true, kAgain = false;  // what is not finite here is NaN, and stays it
     static constexpr int kCtas = 3, DP = DP_, G = DP / kShared, kHeads = 8, STEP = 32;
     // CTAs of an SM.  Three have more steps under way, two leave room for the joining kernel's CTAs to start beside
-    // them and fewer partials to join: from about 24 steps a warp on (by the tables; with weights, which the joining
-    // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128: 1 sequence 23.2 with two, 27.4 with
-    // three; 4 sequences 49.6, 49.8; 16 sequences 158, 146; a quicker join has since taken 3 us off each).
+    // them and fewer partials to join: from about 9 steps a warp on (by the tables; with weights, which the joining
+    // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128, two and three: 1 sequence 19.7 and 21.3,
+    // 2 30.0 and 29.5, 4 48.2 and 46.7, 16 156 and 143; with weights 8 sequences 103 and 104, 16 191 and 184).
     static int ctas(int64_t steps, int sms, bool weights) {
-        return steps >= (weights ? 48 : 24) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
+        return steps >= (weights ? 48 : 9) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
     }
     // Weights in one float16 part are off by 2^-11, an eighth of a bfloat16 result's rounding; other results
     // get a second part.
