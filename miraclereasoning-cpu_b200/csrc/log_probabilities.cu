@@ -18,6 +18,15 @@
 // added to the pass, and none of it depends on the order of the logits.  Where
 // very many logits equal T (rows masked by -inf, constant rows), only larger ones are
 // taken and the rest filled with the first ones that equal it.
+//
+// 4096 rows of 32000 float32, 2 given tokens and 5 alternatives (525 MB): 92 us, 5.7 TB/s.  What a row costs once
+// (its sums joined, its list) leaves a CTA without loads under way, so that the start of a later row is fetched
+// to L2 meanwhile: 99.5 without it; 95 with 16 KB, 91 with 64, which other sizes lose again; all of each row ahead of its
+// loads 89, but 1000 rows 10% slower.  Rows through rings of asynchronous copies in shared memory took 8% more than
+// registers, CTAs of 128 or 512 threads 115 and 126 us.  16-bit rows are bound by their instructions and the
+// exponentials' unit (60% and 47% busy; 2000 rows of 64000 bfloat16 74 us, half of the copy rate); whole groups without
+// bounds checks and sums kept in pairs gained nothing there.  One row of 64000 takes 7.3 us: most of it is the list,
+// whose steps follow each other.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -31,6 +40,8 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMostTop = 128, kMostCtas = 4, kParts = 256;
+constexpr int kResident = 4;             // CTAs of an SM
+constexpr uint32_t kAhead = 32 << 10;    // bytes of a later row, fetched to L2
 constexpr float kLog2e = 1.4426950408889634f;
 // e^-kFar is 0 in float32: differences are cut there where they are factors, so that 0 x -inf is no NaN
 constexpr float kFar = 1e4f;
@@ -46,6 +57,7 @@ struct ScoreArgs {
     int64_t top_token_row, top_logprob_row;
     int64_t rows;
     int vocab, given, top, ctas;  // ctas: of a row
+    int ahead;                    // CTAs that run at once
 };
 
 // Logits in rising order as unsigned numbers; both zeros equal, NaN the lowest.
@@ -349,7 +361,7 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 template <typename T, int P>
-__global__ void __launch_bounds__(P == 32 ? 128 : P) k_log_probabilities(const __grid_constant__ ScoreArgs a) {
+__global__ void __launch_bounds__(P == 32 ? 128 : P, P == 32 ? 0 : kResident) k_log_probabilities(const __grid_constant__ ScoreArgs a) {
     constexpr int V = Slice<T>::V, kEach = kParts / P, kWarps = P / 32, kTeams = P == 32 ? 4 : 1;
     // vectors of a thread under way: one of each of its parts, or some of its only one
     constexpr int kFlight = P == 32 ? kEach : sizeof(T) == 4 ? 4 : 2;
@@ -435,6 +447,12 @@ __global__ void __launch_bounds__(P == 32 ? 128 : P) k_log_probabilities(const _
         mine.a = sa.f.x + sa.f.y;
     }
     if (kEach == 1) largest[0] = mine.top;
+    if (P > 32 && a.ctas == 1 && tid == 0 && r + a.ahead < a.rows) {
+        // the start of the row that the next CTA here will read, to L2 while this one's is worked out
+        const uintptr_t next = (reinterpret_cast<uintptr_t>(a.logits + (r + a.ahead) * a.row_bytes) + 15) / 16 * 16;
+        const uint32_t bytes = min(kAhead, (static_cast<uint32_t>(a.vocab) * static_cast<uint32_t>(sizeof(T)) - 15) / 16 * 16);
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(next), "r"(bytes) : "memory");
+    }
     // the row's sums: of a warp, all against its maximum
     auto reduce = [](Sums &x) {
         const float top = warp_max(x.top), by = x.top - top, c = ex2(by * kLog2e);
@@ -507,6 +525,7 @@ int launch(mr_context *ctx, ScoreArgs &a) {
     // 16 us, a CTA each 43; of 16000 bfloat16 41 and 63; but 1000 of 64000 51 and 45).  A longer one's CTAs: as many as
     // give the GPU four an SM, each with two vectors a thread at least.
     a.ctas = 1;
+    a.ahead = kResident * ctx->sm_count;
     if (a.vocab <= 1024 || (a.rows > 4 * ctx->sm_count && a.vocab * static_cast<int64_t>(sizeof(T)) <= 64 << 10)) {
         k_log_probabilities<T, 32><<<static_cast<unsigned>((a.rows + 3) / 4), 128, 0, ctx->stream>>>(a);
         MR_CUDA_TRY(cudaGetLastError());
