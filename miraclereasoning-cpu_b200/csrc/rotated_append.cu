@@ -230,7 +230,8 @@ enum { kNeighbours, kHalves, kAny };
 // A CTA is a warp: what is the same in all its lanes is worked out once, and 32 of them an SM have the
 // registers that they need.  Bound by memory and instructions alike: 9 ragged prompts of 16 / 4 heads of 128 (8290
 // tokens, 102 MB) 21.0 us, 4.9 TB/s; loads straight to registers, three slots ahead, took 30 whatever the
-// order, and divisions in place of the shifts 1.1 us.  24 sequences of 16 / 4 split-half heads of 64 (9200 tokens,
+// order, and divisions in place of the shifts 1.1 us; the sines are 1.8 us, two or more warps a token 7 us each more,
+// and turns and codes by two operations an instruction took 0.4 us more.  Issue slots are 70% busy.  24 sequences of 16 / 4 split-half heads of 64 (9200 tokens,
 // 57 MB) 18 us, where what a token costs once (its place, its sines) is a third of the instructions.
 template <typename T, int PAIRS, bool PACKED>
 __global__ void __launch_bounds__(32, 32) k_append_rotated(const __grid_constant__ RotateArgs a) {
@@ -460,6 +461,9 @@ struct Piece {
 
 constexpr int kReadWarps = 4;
 
+// A warp takes tokens, or a part of one token's heads, as in the append, with four rows of keys and of values a lane
+// under way.  Bound by memory: 6 ragged sequences of 33 400 rows of 8 heads of 128 from 4 bits to bfloat16 (176 MB)
+// 33.5 us, 5.3 TB/s.
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(kReadWarps * 32) k_read_pages(const __grid_constant__ ReadArgs a) {
     constexpr int kFlight = 4;
