@@ -5,8 +5,11 @@
  * Read in Python and passed through ctypes, that is most of a small call's time
  * (a one-token attention took the host 17.7 microseconds so, 13.3 through this
  * module); here the accessors are read into the structs and the library's
- * function is called directly.  Everything
- * else of the binding stays in ctypes (_native.py), which also hands over the
+ * function is called directly.  A type of arrays that offers DLPack's exchange of
+ * descriptions in C (version 1, __dlpack_c_exchange_api__, as torch's tensors do)
+ * is read by that, one call an array instead of five (an append of 64 rows with
+ * their rotation, ten arrays, 11.8 microseconds without and 9.0 so).
+ * Everything else of the binding stays in ctypes (_native.py), which also hands over the
  * functions' addresses, so that this module links to no library.
  */
 #define PY_SSIZE_T_CLEAN
@@ -51,6 +54,64 @@ static int numbers(PyObject *tuple, int64_t *to) {
     return (int)n;
 }
 
+/* Of DLPack 1: a description of an array, and the table of functions of which one fills it in (0: done). */
+typedef struct {
+    void *data;
+    int32_t device_type, device;
+    int32_t ndim;
+    uint8_t code, bits;
+    uint16_t lanes;
+    int64_t *shape, *strides;
+    uint64_t byte_offset;
+} dl_array;
+typedef struct {
+    uint32_t major, minor;
+    void *earlier, *allocate, *from_object, *to_object;
+    int (*describe)(void *object, dl_array *to);
+    void *stream;
+} dl_functions;
+enum { DL_CUDA = 2 };
+static PyTypeObject *met;                  /* the type of arrays met last, and its function or NULL */
+static int (*met_describe)(void *, dl_array *);
+static PyObject *exchange;
+
+/* The type's own function: an heir's accessors may say something else. */
+static void meet(PyTypeObject *type) {
+    PyObject *capsule = type->tp_dict ? PyDict_GetItemWithError(type->tp_dict, exchange) : NULL;
+    const dl_functions *f = NULL;
+    if (capsule && PyCapsule_IsValid(capsule, "dlpack_exchange_api")) f = PyCapsule_GetPointer(capsule, "dlpack_exchange_api");
+    met_describe = f && f->major == 1 ? f->describe : NULL;
+    Py_INCREF(type);
+    Py_XSETREF(met, type);
+    PyErr_Clear();
+}
+
+/* 1 if the object's type describes it as an array on the device by the exchange. */
+static int read_exchanged(PyObject *array, long device, mr_array *to) {
+    dl_array x;
+    if (Py_TYPE(array) != met) meet(Py_TYPE(array));
+    if (!met_describe) return 0;
+    if (met_describe(array, &x)) {
+        PyErr_Clear();
+        return 0;
+    }
+    const int bits = x.lanes == 1 ? x.code << 8 | x.bits : 0;
+    const int type = bits == (2 << 8 | 32)   ? MR_DTYPE_F32
+                     : bits == (2 << 8 | 16) ? MR_DTYPE_F16
+                     : bits == (4 << 8 | 16) ? MR_DTYPE_BF16
+                     : bits == (0 << 8 | 32) ? MR_DTYPE_I32
+                     : bits == (1 << 8 | 8)  ? MR_DTYPE_U8
+                                             : -1;
+    if (x.device_type != DL_CUDA || x.device != device || x.ndim < 1 || x.ndim > 4 || !x.strides || type < 0) return 0;
+    memset(to, 0, sizeof(*to));
+    to->data = x.data ? (char *)x.data + x.byte_offset : NULL;
+    to->dtype = type;
+    to->ndim = x.ndim;
+    memcpy(to->shape, x.shape, sizeof(int64_t) * (size_t)x.ndim);
+    memcpy(to->stride, x.strides, sizeof(int64_t) * (size_t)x.ndim);
+    return 1;
+}
+
 /* 1 if the object describes an array on the device in the usual way. */
 static int read_array(PyObject *array, long device, mr_array *to) {
     int ok = 0;
@@ -77,7 +138,7 @@ static int read_array(PyObject *array, long device, mr_array *to) {
 }
 
 static int describe_into(PyObject *array, const char *name, long device, mr_array *to) {
-    if (read_array(array, device, to)) return 1;
+    if (read_exchanged(array, device, to) || read_array(array, device, to)) return 1;
     PyObject *bytes = PyObject_CallFunction(slow, "Osl", array, name, device);
     if (!bytes) return 0;
     const int ok = PyBytes_Check(bytes) && PyBytes_GET_SIZE(bytes) == (Py_ssize_t)sizeof(*to);
@@ -182,7 +243,8 @@ PyMODINIT_FUNC PyInit__pycall(void) {
     stride = PyUnicode_InternFromString("stride");
     dtype = PyUnicode_InternFromString("dtype");
     data_ptr = PyUnicode_InternFromString("data_ptr");
-    if (m && get_device && shape && stride && dtype && data_ptr) return m;
+    exchange = PyUnicode_InternFromString("__dlpack_c_exchange_api__");
+    if (m && exchange && get_device && shape && stride && dtype && data_ptr) return m;
     Py_XDECREF(m);
     return NULL;
 }
