@@ -498,8 +498,8 @@ MR_API int mr_append_rotated(mr_context *ctx, const mr_array *query, const mr_ar
 /* The way back of mr_append_pages: sequence s's last offsets[s + 1] - offsets[s]
  * rows (NULL: its newest row) go to keys and values [tokens, kv heads, dim] at
  * offsets[s] ..; from 4-bit pages as any floating type, from others as their own.
- * A row that the pages do not hold (a bad page, past the table, before the first) is zeros;
- * rows of keys and values in no sequence stay as they were. */
+ * A row that the pages do not hold (a bad page, past the table, before the first) is
+ * zeros; rows of keys and values in no sequence stay as they were. */
 MR_API int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const mr_array *value_pages,
                          const mr_array *page_table, const mr_array *lengths, const mr_array *offsets,
                          const mr_array *keys, const mr_array *values);
