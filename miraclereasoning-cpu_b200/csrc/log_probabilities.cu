@@ -521,12 +521,14 @@ __global__ void __launch_bounds__(P == 32 ? 128 : P, P == 32 ? 0 : kResident) k_
 
 template <typename T>
 int launch(mr_context *ctx, ScoreArgs &a) {
-    // Short rows are a warp's, and where there are more than four an SM those of up to 64 KB (4096 rows of 2000 float32
-    // 16 us, a CTA each 43; of 16000 bfloat16 41 and 63; but 1000 of 64000 51 and 45).  A longer one's CTAs: as many as
-    // give the GPU four an SM, each with two vectors a thread at least.
+    // Short rows are a warp's, and where there are more than four an SM those of up to 64 KB, in float32 52, and 32 bytes
+    // for each row that there is (us of a warp and of a CTA each: 4096 rows of 4000 float32 23 and 41, of 12000 52 and 55, of
+    // 16000 69 and 64; of 32000 bfloat16 72 and 83; 1000 of 8000 float32 13.1 and 14.4, of 32000 bfloat16 28.2 and 25.5).
+    // A longer one's CTAs: as many as give the GPU four an SM, each with two vectors a thread at least.
     a.ctas = 1;
     a.ahead = kResident * ctx->sm_count;
-    if (a.vocab <= 1024 || (a.rows > 4 * ctx->sm_count && a.vocab * static_cast<int64_t>(sizeof(T)) <= 64 << 10)) {
+    const int64_t bytes = a.vocab * static_cast<int64_t>(sizeof(T)), most = (sizeof(T) == 4 ? 52 : 64) << 10;
+    if (a.vocab <= 1024 || (a.rows > 4 * ctx->sm_count && bytes <= std::min(most, 32 * a.rows))) {
         k_log_probabilities<T, 32><<<static_cast<unsigned>((a.rows + 3) / 4), 128, 0, ctx->stream>>>(a);
         MR_CUDA_TRY(cudaGetLastError());
         return MR_OK;

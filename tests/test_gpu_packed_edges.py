@@ -105,7 +105,7 @@ def test_chunk_after_chunk_reads_what_was_just_written(served, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows, vocab", [(593, 33_003), (1300, 16_500)])
+@pytest.mark.parametrize("rows, vocab", [(593, 33_003), (1300, 16_500), (1300, 7001), (4100, 1027)])
 def test_more_rows_than_run_at_once(served, dtype, rows, vocab):
     """Rows at odd addresses, of which later ones are fetched ahead up to the last: each as if it were alone."""
     import torch
