@@ -474,8 +474,8 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * or whose base passes float16 (values from -6870 to 6870, say) read as NaN.  What
  * is written depends on the values alone.
  * Attention's queries and results are of any floating type.  Each weight meets the
- * values in float16 (BF16: one part, an error of 2^-11 of it; F16 and F32: two,
- * 2^-22), with errors of 2^-40 of a row's largest weight.  An infinite step or base,
+ * values in two float16 parts (an error of 2^-22 of it, and of 2^-40 of a row's largest
+ * weight), F32 queries the keys in two (2^-22).  An infinite step or base,
  * which no call writes, gives infinities or NaN. */
 
 /* mr_append_pages with a rotation on the way: the first 2 n dims of each query

@@ -11,13 +11,15 @@
 // holds the same four dims of two rows, and the four results of a word go to rows of
 // different product tiles.
 //
-// A step of 32 rows of 128 dims is 665 instructions: 210 and 220 for the two products' operands and issue, 95
-// for the softmax, 120 for the copies of two steps on.  32 sequences ragged to 32768 rows at 8 heads of 128
-// (668 MB): 145 us, of which about 20 are the start, the uneven end and the join; the copies alone take 113.
+// A step of 32 rows of 128 dims is 706 instructions: 210 and 236 for the two products' operands and issue, 120
+// for the softmax and the weights' two parts, 120 for the copies of two steps on.  32 sequences ragged to 32768 rows
+// at 8 heads of 128 (668 MB): 157 us in bfloat16 and float16, 178 in float32, of which about 20 are the start, the uneven
+// end and the join; the copies alone take 113.  (Weights in one float16 part, off by 2^-11, took 142: they were as much as an
+// eighth of a bfloat16 result's rounding, which moved several results in a hundred to the next bfloat16 number.)
 // Logical operations and float16 multiply-adds each issue every other cycle, and 1.5 cycles each when
-// mixed, so that moving work between the two gains nothing (shifts as additions: 166 and 167 us at the time);
+// mixed, so that moving work between the two gains nothing.  Tried beside one part of each weight, at 145 us:
 // 8-bit floating-point products of the codes as they stand (e4m3 0 .. 15 are linear) need fewer masks, but that
-// type is widened in software here: 790 instructions a step, 175 us.  Four CTAs an SM spill (150); of
+// type is widened in software here, 790 instructions a step, 175 us; four CTAs an SM spill (150); of
 // all 16 warps' stretches joined in shared memory first, one long sequence gains 1 us and the batch loses 8.
 #include "packed.cuh"
 #include "paged_core.cuh"
@@ -70,14 +72,11 @@ struct Math4 : Heads8<__half, DP_ / 16> {
     static constexpr int kCtas = 3, DP = DP_, G = DP / kShared, kHeads = 8, STEP = 32;
     // CTAs of an SM.  Three have more steps under way, two leave room for the joining kernel's CTAs to start beside
     // them and fewer partials to join: from about 9 steps a warp on (by the tables; with weights, which the joining
-    // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128, two and three: 1 sequence 19.7 and 21.3,
-    // 2 30.0 and 29.5, 4 48.2 and 46.7, 16 156 and 143; with weights 8 sequences 103 and 104, 16 191 and 184).
+    // kernel adds up, 48) three are faster (us at 32768 rows of 8 heads of 128, two and three: 1 sequence 21.0 and 22.5,
+    // 2 31.9 and 31.4, 4 52.3 and 49.9, 16 171 and 157; with weights 8 sequences 111.3 and 111.4, 16 207 and 199).
     static int ctas(int64_t steps, int sms, bool weights) {
         return steps >= (weights ? 48 : 9) * static_cast<int64_t>(3 * kWarps) * sms ? 3 : 2;
     }
-    // Weights in one float16 part are off by 2^-11, an eighth of a bfloat16 result's rounding; other results
-    // get a second part.
-    static constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
     struct R : Ring4<DP> {
         static constexpr int kBytes = 2 * STEP * Ring4<DP>::kRowBytes;
         static constexpr int kWarpBytes = kBytes * 3;
@@ -168,8 +167,8 @@ struct Math4 : Heads8<__half, DP_ / 16> {
         this->template settle<true>(a, s, f[0], f[1], live, rows, scores, ref);
 #pragma unroll
         for (int x = 0; x < S; ++x) {
-            uint32_t b0, b1, c0 = 0, c1 = 0;
-            this->template weigh<kTwo>(s[x], ref, b0, b1, c0, c1);
+            uint32_t b0, b1, c0, c1;
+            this->weigh(s[x], ref, b0, b1, c0, c1);
             const uint32_t tile = stage + (STEP + x * 16) * R::kRowBytes;
             uint32_t p[4][G];  // of rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9
 #pragma unroll
@@ -192,9 +191,9 @@ struct Math4 : Heads8<__half, DP_ / 16> {
                     const uint32_t v0[4] = {fma2(uc[0], s0, z0), fma2(uc[1], s0, z0), fma2(vc[0], s1, z1), fma2(vc[1], s1, z1)};
                     const uint32_t v1[4] = {fma2(uc[2], s0, z0), fma2(uc[3], s0, z0), fma2(vc[2], s1, z1), fma2(vc[3], s1, z1)};
                     mma16(o[2 * (g + i)], v0, b0, b1, __half());
-                    if (kTwo) mma16(o[2 * (g + i)], v0, c0, c1, __half());
+                    mma16(o[2 * (g + i)], v0, c0, c1, __half());
                     mma16(o[2 * (g + i) + 1], v1, b0, b1, __half());
-                    if (kTwo) mma16(o[2 * (g + i) + 1], v1, c0, c1, __half());
+                    mma16(o[2 * (g + i) + 1], v1, c0, c1, __half());
                 }
             }
         }

@@ -58,7 +58,7 @@ struct Math16 : Heads8<T, DP_ / 16> {
 #pragma unroll
         for (int x = 0; x < S; ++x) {
             uint32_t b0, b1, c0, c1;
-            this->template weigh<true>(s[x], ref, b0, b1, c0, c1);
+            this->weigh(s[x], ref, b0, b1, c0, c1);
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) {
                 uint32_t v[4];

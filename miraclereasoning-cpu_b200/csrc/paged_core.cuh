@@ -371,8 +371,9 @@ struct Heads8 {
             m[1] = top[1];
         }
     }
-    // The weights of 16 rows as the 16-bit operand P^T: its first part b0, b1 and (TWO) the rest c0, c1.
-    template <bool TWO>
+    // The weights of 16 rows as two operands P^T, the first part b0, b1 and what its rounding left c0, c1 (a second
+    // product): one part alone would add as much error again as the output's rounding, and an eighth of it where
+    // float16 weights make bfloat16 results.
     __device__ __forceinline__ void weigh(const float (&s)[4], const float (&ref)[2], uint32_t &b0, uint32_t &b1, uint32_t &c0,
                                           uint32_t &c1) {
         float p[4];
@@ -384,13 +385,9 @@ struct Heads8 {
         const uint32_t h0 = pack2(p[0], p[1], T()), h1 = pack2(p[2], p[3], T());
         b0 = transposed(h0);
         b1 = transposed(h1);
-        if constexpr (TWO) {
-            // what that rounding left (a second product): one part alone would add as much
-            // error again as the output's rounding
-            const float2 r0 = unpack2(h0, T()), r1 = unpack2(h1, T());
-            c0 = transposed(pack2(p[0] - r0.x, p[1] - r0.y, T()));
-            c1 = transposed(pack2(p[2] - r1.x, p[3] - r1.y, T()));
-        }
+        const float2 r0 = unpack2(h0, T()), r1 = unpack2(h1, T());
+        c0 = transposed(pack2(p[0] - r0.x, p[1] - r0.y, T()));
+        c1 = transposed(pack2(p[2] - r1.x, p[3] - r1.y, T()));
     }
 
     // Sums over the warp; false if a value is not finite.
@@ -813,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, M::kCtas) k_paged_few(const __grid_c
 // some of its registers spill).
 enum { kNoWeights, kWeights, kBlockWeights };
 // Warps for each of k_paged's, to hide the latency of the little that each reads.  One is enough for the short way
-// there is without weights over pages of 4 bits (one sequence of 32768 rows: 20.7 us, with two 22.3; with weights,
+// there is without weights over pages of 4 bits (one sequence of 32768 rows: 1.6 us less than two; with weights,
 // 24 sequences to 8192 rows: 37.8 and 36.0).
 template <typename M, int MODE>
 constexpr int kJoiners = M::kRuns && MODE == kNoWeights ? 1 : 2;
