@@ -67,6 +67,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
 }
 constexpr uint32_t kLowest = 0x007fffffu;  // of -inf
+constexpr uint32_t kZero = 0x80000000u;    // of both zeros; no logit has the order below it, -0's by its bits
 // The logit of an order from kLowest on; NaN of 0.
 __device__ __forceinline__ float value_of(uint32_t order) {
     return order ? __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order) : __uint_as_float(0x7fffffffu);
@@ -301,8 +302,9 @@ __device__ __forceinline__ void choose(const Slice<T> &slice, Shared<P> &sh, int
             if (n >= want) low = mid, reach = n;
             else high = mid;
         }
-        // fewer parts with elements than wanted, or among them NaN alone: everything counts
-        if (lane == 0) sh.bound = low <= 1 ? 0u : max(low, kLowest);
+        // Fewer parts with elements than wanted, or among them NaN alone: everything counts.  Otherwise an order whose
+        // number compares alike: the one below zero's reads as -0, which zeros reach but do not pass.
+        if (lane == 0) sh.bound = low <= 1 ? 0u : low == kZero - 1 ? kZero : max(low, kLowest);
     }
     team_sync<P>();
     uint32_t bound = sh.bound;
