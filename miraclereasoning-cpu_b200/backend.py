@@ -305,8 +305,8 @@ class CUDABackend:
         """``append_pages`` with the position rotation on the way: the first 2 n dims of ``keys``, and of ``query``
         [tokens, heads, dim], are turned by position * ``frequencies`` [n] (float32), in pairs of neighbours or with
         ``split_half`` of dims p and p + n (as ``rotate`` does).  ``positions`` int32 [tokens]; None: a token's row of
-        its sequence.  Returns the turned query, ``out`` (an array like the query; rows of no sequence are not
-        written), or None without one."""
+        its sequence.  Returns the turned query, ``out`` (an array like the query, of memory that none of the others
+        has; rows of no sequence are not written), or None without one."""
         if query is not None and out is None:
             out = _like(query, "query")
         invoke(arrays.ROTATED, *self._where, query, keys, values, key_pages, value_pages, page_table, lengths, offsets,

@@ -581,7 +581,11 @@ extern "C" int mr_append_rotated(mr_context *ctx, const mr_array *query, const m
         MR_REQUIRE(query->shape[0] == tokens && query->shape[2] == dim, "query must be [%lld, heads, %lld], as keys",
                    static_cast<long long>(tokens), static_cast<long long>(dim));
         MR_REQUIRE(query->shape[1] * dim <= INT32_MAX / 4, "too many heads");
+        // rows of other tokens and kinds are read before and while turned queries are written
         MR_CHECK(check_apart(query, "query", out, "out"));
+        MR_CHECK(check_apart(keys, "keys", out, "out"));
+        MR_CHECK(check_apart(values, "values", out, "out"));
+        for (const mr_array *pool : {key_pages, value_pages}) MR_CHECK(check_apart(pool, "the pages", out, "out"));
     }
     if (frequencies) {
         MR_CHECK(check_array(frequencies, "frequencies", 1, false, false));
