@@ -99,11 +99,15 @@ def _count(value, name, least=0):
     raise ValueError(f"{name} must be a whole number from {least} on{', or None' if least else ''}: {value!r}")
 
 
+def _no_array(array, name):
+    return ValueError(f"{name} must be a device array, not {type(array).__name__}")
+
+
 def _like(array, name):
     try:
         return array.new_empty(array.shape)
     except AttributeError:
-        raise ValueError(f"{name} must be a device array, not {type(array).__name__}") from None
+        raise _no_array(array, name) from None
 
 
 class CUDABackend:
@@ -384,17 +388,26 @@ class CUDABackend:
         top = _count(top, "top")
         if len(getattr(logits, "shape", ())) != 2:
             raise ValueError("logits must be an array [rows, vocabulary]")
+        for array, name in ((tokens, "tokens"), (top_tokens, "top_tokens")):
+            if array is not None and not hasattr(array, "shape"):
+                raise _no_array(array, name)
+
+        def made(shape, dtype):
+            if not hasattr(logits, "new_empty"):
+                raise _no_array(logits, "logits")
+            return empty_like(logits, shape, dtype)
+
         rows = logits.shape[0]
         if tokens is not None and logprobs is None:
-            logprobs = empty_like(logits, tokens.shape, "float32")
+            logprobs = made(tokens.shape, "float32")
         if entropy is None:
-            entropy = empty_like(logits, (rows,), "float32")
+            entropy = made((rows,), "float32")
         if top_tokens is None:
-            top_tokens = empty_like(logits, (rows, top), "int32")
+            top_tokens = made((rows, top), "int32")
         elif tuple(top_tokens.shape) != (rows, top):
             raise ValueError(f"top_tokens must be [{rows}, {top}]")
         if top_logprobs is None:
-            top_logprobs = empty_like(logits, (rows, top), "float32")
+            top_logprobs = made((rows, top), "float32")
         best = (top_tokens, top_logprobs) if top else (None, None)
         invoke(arrays.SCORE, *self._where, logits, tokens, logprobs, entropy, *best)
         return logprobs, entropy, top_tokens, top_logprobs
