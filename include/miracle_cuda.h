@@ -483,8 +483,9 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * n <= dim / 2; NULL: none) for pair p, which is the dims 2 p and 2 p + 1, or with
  * split_half p and p + n (kernels.cl:30-44).  A token's position is positions[i]
  * (I32 [tokens]), or its row of the sequence where positions is NULL.  The angle is
- * the exact product, its sine and cosine are rounded to float32 once (mr_op_rope
- * rounds the product too), and so is each product and sum of a turn; the result is
+ * the exact product, of up to 2^50 (frequencies to 2^19 at any position); its sine and
+ * cosine are rounded to float32 once (mr_op_rope rounds the product too), and so is
+ * each product and sum of a turn; the result is
  * rounded to the type, or to 4 bits.  Turned queries go to out [tokens, heads, dim]
  * (query and out may both be NULL); those of tokens in no sequence stay as they
  * were.  All of query, keys, values and out are of one type, the pages of the same

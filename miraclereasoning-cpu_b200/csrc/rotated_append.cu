@@ -166,6 +166,8 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[V], uint32_t &pair
 // two parts and reduced by multiples of pi / 2 in 64 bits, so that far positions lose nothing
 // (2^31 radians leave 2^-70); what is left, at most pi / 4, goes through the Taylor series to
 // x^15 and x^16, whose next terms are below 5e-17.  One angle is about 25 64-bit operations.
+// Past 2^47 radians the product's second part shows in what is left: 1.1 at 2^50, where the series ends at
+// 8e-15, still far below a rounding; from 2^54 on results are wrong.
 __device__ __forceinline__ float2 turn_of(int position, float frequency) {
     const double p = position, f = frequency;
     const double a = p * f, rest = fma(p, f, -a);
