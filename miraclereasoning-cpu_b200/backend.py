@@ -388,26 +388,24 @@ class CUDABackend:
         top = _count(top, "top")
         if len(getattr(logits, "shape", ())) != 2:
             raise ValueError("logits must be an array [rows, vocabulary]")
-        for array, name in ((tokens, "tokens"), (top_tokens, "top_tokens")):
-            if array is not None and not hasattr(array, "shape"):
-                raise _no_array(array, name)
-
-        def made(shape, dtype):
-            if not hasattr(logits, "new_empty"):
-                raise _no_array(logits, "logits")
-            return empty_like(logits, shape, dtype)
-
         rows = logits.shape[0]
-        if tokens is not None and logprobs is None:
-            logprobs = made(tokens.shape, "float32")
-        if entropy is None:
-            entropy = made((rows,), "float32")
-        if top_tokens is None:
-            top_tokens = made((rows, top), "int32")
-        elif tuple(top_tokens.shape) != (rows, top):
-            raise ValueError(f"top_tokens must be [{rows}, {top}]")
-        if top_logprobs is None:
-            top_logprobs = made((rows, top), "float32")
+        try:
+            if tokens is not None and logprobs is None:
+                logprobs = empty_like(logits, tokens.shape, "float32")
+            if entropy is None:
+                entropy = empty_like(logits, (rows,), "float32")
+            if top_tokens is None:
+                top_tokens = empty_like(logits, (rows, top), "int32")
+            elif tuple(top_tokens.shape) != (rows, top):
+                raise ValueError(f"top_tokens must be [{rows}, {top}]")
+            if top_logprobs is None:
+                top_logprobs = empty_like(logits, (rows, top), "float32")
+        except AttributeError:   # found only here, so that arrays are not looked at twice
+            for array, name, accessor in ((logits, "logits", "new_empty"), (tokens, "tokens", "shape"),
+                                          (top_tokens, "top_tokens", "shape")):
+                if array is not None and not hasattr(array, accessor):
+                    raise _no_array(array, name) from None
+            raise
         best = (top_tokens, top_logprobs) if top else (None, None)
         invoke(arrays.SCORE, *self._where, logits, tokens, logprobs, entropy, *best)
         return logprobs, entropy, top_tokens, top_logprobs
