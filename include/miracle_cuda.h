@@ -471,12 +471,13 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * rounded to float16.
  * Writing a row: s = (max - min) / 15 of the 32 values and z = min - 64 s, each
  * rounded to float16, c the nearest of 0 .. 15.  32 values of which one is not finite
- * or whose base passes float16 (values from -6870 to 6870, say) read as NaN.  What
+ * or whose base passes float16 (values from -6870 to 6870, say) read as NaN; one whose
+ * nearest code stands for more than float16 holds (near 65504) reads as infinity.  What
  * is written depends on the values alone.
  * Attention's queries and results are of any floating type.  Each weight meets the
  * values in two float16 parts (an error of 2^-22 of it, and of 2^-40 of a row's largest
- * weight), F32 queries the keys in two (2^-22).  An infinite step or base,
- * which no call writes, gives infinities or NaN. */
+ * weight), F32 queries the keys in two (2^-22).  An infinite value, step
+ * or base (no call writes the last two) makes infinities or NaN of what it meets. */
 
 /* mr_append_pages with a rotation on the way: the first 2 n dims of each query
  * [tokens, heads, dim] and key are turned by position * frequencies[p] (F32 [n],
@@ -490,7 +491,9 @@ MR_API int mr_evict_pages(mr_context *ctx, const mr_array *key_pages, const mr_a
  * (query and out may both be NULL); those of tokens in no sequence stay as they
  * were.  All of query, keys, values and out are of one type, the pages of the same
  * or of 4 bits; out must not overlap the inputs.  What mr_append_pages says of
- * places, dropped rows and offsets holds here. */
+ * places, dropped rows and offsets holds here, but that rows in no sequence may be
+ * read (none of their values goes anywhere); so it does where that one's pages are of
+ * 4 bits. */
 MR_API int mr_append_rotated(mr_context *ctx, const mr_array *query, const mr_array *keys, const mr_array *values,
                              const mr_array *key_pages, const mr_array *value_pages, const mr_array *page_table,
                              const mr_array *lengths, const mr_array *offsets, const mr_array *frequencies,
@@ -514,7 +517,8 @@ MR_API int mr_read_pages(mr_context *ctx, const mr_array *key_pages, const mr_ar
  * top at most 128 and the vocabulary.  tokens and logprobs, and the last two, may be
  * NULL together; entropy too.  A logit of -inf has probability 0 and adds nothing; a
  * row of them alone has log probabilities -inf and entropy 0; a NaN or +inf in a row
- * makes its log probabilities and its entropy NaN.  Sums are float32. */
+ * makes its log probabilities and its entropy NaN.  Sums are float32.  Results must
+ * not overlap the inputs or each other. */
 MR_API int mr_log_probabilities(mr_context *ctx, const mr_array *logits, const mr_array *tokens, const mr_array *logprobs,
                                 const mr_array *entropy, const mr_array *top_tokens, const mr_array *top_logprobs);
 

@@ -325,7 +325,8 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(const __grid_constant
 
 // Kept rows to their target pages: a warp takes 32 rows of a head, a lane looks up one row's two
 // places, and all copy the rows piece by piece (16 bytes, or what rows of 4-bit values are whole
-// multiples of), four loads of each pool in flight a lane.
+// multiples of), four loads of each pool in flight a lane.  16 sequences of 8192 rows of 4 bits to 2048 with
+// their selection: 8 heads of 128 35 us, 10 of 96 45, 16 of 64 48, 32 of 32 72 (at the copy rate 13 to 17): pieces of 8 and 4 bytes.
 constexpr int kCopyWarps = 4;
 template <typename Bytes>
 __global__ void __launch_bounds__(kCopyWarps * 32) k_copy_kept(const __grid_constant__ EvictArgs a) {

@@ -15,18 +15,22 @@
 // warp's lane).  The k-th largest of them, T, is a lower bound of the k-th largest logit, and only a part
 // whose maximum reaches T can have such logits: about k parts' elements are read
 // again, from cache, and the few that reach T are ranked by counting.  No work is
-// added to the pass, and none of it depends on the order of the logits.  Where
-// very many logits equal T (rows masked by -inf, constant rows), only larger ones are
-// taken and the rest filled with the first ones that equal it.
+// added to the pass, and the list's does not depend on the order of the logits.  Where
+// more of them reach T than there is room for (rows that allow fewer tokens than are asked for beside
+// a mask of -inf, constant rows), the row is read once more for the larger ones alone, and the
+// rest filled with the first ones that equal T, looked for by one warp.  That is slow: 20 alternatives of rows that
+// allow 5 tokens take 25 us instead of 7.3 (1 row of 64000 float32), 27 instead of 9.1 (64 of 64000 bfloat16), 255
+// instead of 37 (4096 of 8000 float32, where a warp counts every masked logit).
 //
 // 4096 rows of 32000 float32, 2 given tokens and 5 alternatives (525 MB): 92 us, 5.7 TB/s.  What a row costs once
 // (its sums joined, its list) leaves a CTA without loads under way, so that the start of a later row is fetched
 // to L2 meanwhile: 99.5 without it; 95 with 16 KB, 91 with 64, which other sizes lose again; all of each row ahead of its
 // loads 89, but 1000 rows 10% slower.  Rows through rings of asynchronous copies in shared memory took 8% more than
 // registers, CTAs of 128 or 512 threads 115 and 126 us.  16-bit rows are bound by their instructions and the
-// exponentials' unit (60% and 47% busy; 2000 rows of 64000 bfloat16 74 us, half of the copy rate); whole groups without
-// bounds checks and sums kept in pairs gained nothing there.  One row of 64000 takes 7.3 us: most of it is the list,
-// whose steps follow each other.
+// exponentials' unit (60% and 47% busy; 2000 rows of 64000 bfloat16 66 us, 4096 of 32000 62, 60 to 66% of the copy
+// rate); whole groups without bounds checks and sums kept in pairs gained nothing there.  Short rows, a warp's, have nothing
+// fetched ahead: 4096 of 4000, 8000 and 12000 float32 20.6, 32.0 and 43.0 us where the copy rate has 10.2, 20.4 and 30.5.
+// One row of 64000 takes 7.3 us: most of it is the list, whose steps follow each other.
 #include <cooperative_groups.h>
 
 #include <type_traits>

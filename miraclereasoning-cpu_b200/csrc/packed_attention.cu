@@ -13,9 +13,12 @@
 //
 // A step of 32 rows of 128 dims is 706 instructions: 210 and 236 for the two products' operands and issue, 120
 // for the softmax and the weights' two parts, 120 for the copies of two steps on.  32 sequences ragged to 32768 rows
-// at 8 heads of 128 (668 MB): 157 us in bfloat16 and float16, 178 in float32, of which about 20 are the start, the uneven
+// at 8 heads of 128 (668 MB): 160 us in bfloat16 and float16, 178 in float32, of which about 20 are the start, the uneven
 // end and the join; the copies alone take 113.  (Weights in one float16 part, off by 2^-11, took 142: they were as much as an
 // eighth of a bfloat16 result's rounding, which moved several results in a hundred to the next bfloat16 number.)
+// Smaller dims have less of a row for what a step costs once, and copies of 4 or 8 bytes: 16 sequences ragged to 16384 rows,
+// four query heads each (170 MB): 8 heads of 128 62.5 us, 10 of 96 75.6, 16 of 64 83.6, 32 of 32 125; with rows before
+// heads in a page, where every 16 bytes have an address of their own, 70, 92, 95 and 152.
 // Logical operations and float16 multiply-adds each issue every other cycle, and 1.5 cycles each when
 // mixed, so that moving work between the two gains nothing.  Tried beside one part of each weight, at 145 us:
 // 8-bit floating-point products of the codes as they stand (e4m3 0 .. 15 are linear) need fewer masks, but that

@@ -1,4 +1,5 @@
-// One-token attention over rows of the query's type (paged_core.cuh has the rest).
+// One-token attention over rows of the query's type (paged_core.cuh has the rest): about one
+// multiplication a byte, so bound by memory.
 #include "packed.cuh"
 #include "paged_core.cuh"
 

@@ -5,15 +5,15 @@
 //   out = sum_t exp(s_t - max s) v_t / sum_t exp(s_t - max s),
 //
 // per query head; heads / kv heads query heads read the same key / value rows.
-// Every visible row is read once, with about one multiplication per byte, so
-// the kernel is bound by memory, and its work is to keep enough rows in flight
-// on every SM whatever the lengths are.
+// Every visible row is read once.  What bounds that is said with the ways to work
+// on a step; what they share is to keep enough rows in flight on every SM whatever
+// the lengths are.
 //
 // Work.  A unit is (sequence, key / value head, block of at most kHeads query
 // heads).  Its visible rows, numbered 0 .. without the gap between sinks and
 // window, form steps of STEP rows; the steps of all units, one after the other,
-// are cut into as many even stretches as the grid has warps (eight an SM, all
-// resident).  So a batch of any lengths is balanced to a step, one long sequence
+// are cut into as many even stretches as the grid has warps (four a CTA, of
+// which M::ctas() an SM are resident).  So a batch of any lengths is balanced to a step, one long sequence
 // runs on the whole GPU, and the host need not know the lengths.  A warp's
 // stretch holds the end of one unit, whole units, and the start of another: whole
 // units are written out, the two ends go to scratch as softmax partials (weighted
@@ -24,10 +24,14 @@
 // unit is a CTA's instead, a quarter of it each warp's: there is nothing to join
 // but the four warps' partials, in shared memory, and the second launch is saved
 // (flashnano-1.7's window of 516 rows in a batch of 48: 9.7 us, cut and joined 20.1).
+// The host goes by what the table could hold, so tables much longer than their sequences
+// lose that: 32 sequences of 500 rows (8 heads of 128 in 4 bits) 11.2 us, in tables for 32768 rows 16.3; with
+// weights 13.9 and 23.8.  From 1500 rows on there is little in it (27.3 and 27.9; 33.6 and 38.4).
 //
 // Rows.  Warps never wait for each other there: each has its own ring of row copies
-// (cp.async, 16 bytes a lane, page ids looked up a step ahead), which runs on
-// from one unit into the next, and its own running softmax.
+// (cp.async, R::kUnit bytes a lane: 16, for rows of 4 bits what they are whole
+// multiples of; page ids looked up a step ahead), which runs on from one unit into
+// the next, and its own running softmax.
 #pragma once
 
 #include <cmath>
